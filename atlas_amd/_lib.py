@@ -43,6 +43,18 @@ class SamplingC(C.Structure):
                 ("rng_seed", C.c_uint64)]
 
 
+class Kv4CacheC(C.Structure):
+    """atlas_kv4_cache"""
+    _fields_ = [("data", C.c_void_p), ("n_pages", C.c_int), ("page_len", C.c_int), ("n_kv", C.c_int),
+                ("head_dim", C.c_int)]
+
+
+class Kv4BatchC(C.Structure):
+    """atlas_kv4_batch"""
+    _fields_ = [("row_starts", C.c_void_p), ("kv_lens", C.c_void_p), ("block_table", C.c_void_p),
+                ("table_stride", C.c_int), ("n_seqs", C.c_int), ("n_rows", C.c_int), ("max_len", C.c_int)]
+
+
 HOOK_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c_int,
                       C.POINTER(C.c_float))
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
@@ -114,6 +126,14 @@ SIGNATURES = {
     "atlas_quantize_int4_dev": (I, [P, I, I64, I, P, P]),
     "atlas_quantize_int8_host": (I, [P, I64, I64, P, P]),
     "atlas_quantize_int4_host": (I, [P, I64, I64, I64, P, P]),
+    "atlas_quantize_mxfp4_dev": (I, [P, I, I64, I64, I64, P, P]),
+    "atlas_dequantize_mxfp4_dev": (I, [P, P, I64, I64, P, I64]),
+    "atlas_quantize_mxfp4_host": (I, [P, I64, I64, P, P]),
+    "atlas_gemm_mxfp4_f32": (I, [P, P, P, P, P, I, I, I, I64]),
+    "atlas_kv4_cache_bytes": (I64, [C.POINTER(Kv4CacheC)]),
+    "atlas_kv4_write_f32": (I, [C.POINTER(Kv4CacheC), C.POINTER(Kv4BatchC), P, P, I64]),
+    "atlas_kv4_read_f32": (I, [C.POINTER(Kv4CacheC), C.POINTER(Kv4BatchC), P, P, I64]),
+    "atlas_kv4_attention_f32": (I, [C.POINTER(Kv4CacheC), C.POINTER(Kv4BatchC), P, I64, I, F, I, P, I64]),
     "atlas_fill_random": (I, [I, P, I64, U64, F, F]),
     # engine (include/atlas_engine.h)
     "atlas_model_create": (P, [C.POINTER(ModelConfigC)]),

@@ -24,7 +24,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libatlas_kernels.so")
 
-SOURCES = ["gemv.hip", "skinny.hip", "prompt_gemm.hip", "attention.hip", "fused.hip", "errors.cpp", "runtime.cpp",
+SOURCES = ["gemv.hip", "skinny.hip", "prompt_gemm.hip", "attention.hip", "fused.hip", "mxfp4.hip", "kv4.hip",
+           "errors.cpp", "runtime.cpp",
            "capi.cpp", "engine.cpp", "st_format.cpp", "loader.cpp", "blas.cpp"]
 
 

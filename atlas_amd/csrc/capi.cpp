@@ -7,6 +7,7 @@
 #include "common.hpp"
 #include "fused.hpp"
 #include "gemv.hpp"
+#include "mxfp4.hpp"
 
 using namespace atlas;
 
@@ -291,6 +292,45 @@ ATLAS_API int atlas_quantize_int4_dev(const void* src, int src_is_bf16, int64_t 
     return quant_i4_launch(src, src_is_bf16, (long)n, block, data, scales, stream());
 }
 
+ATLAS_API int atlas_quantize_mxfp4_dev(const void* src, int src_is_bf16, int64_t rows, int64_t cols,
+                                       int64_t ld, uint8_t* data, uint8_t* scales) {
+    return mxfp4_quant_launch(src, src_is_bf16, (long)rows, (long)cols, (long)ld, data, scales, stream());
+}
+
+ATLAS_API int atlas_dequantize_mxfp4_dev(const uint8_t* data, const uint8_t* scales, int64_t rows,
+                                         int64_t cols, float* out, int64_t ld) {
+    return mxfp4_dequant_launch(data, scales, (long)rows, (long)cols, out, (long)ld, stream());
+}
+
+ATLAS_API int atlas_gemm_mxfp4_f32(const uint8_t* w, const uint8_t* w_scales, const uint8_t* x,
+                                   const uint8_t* x_scales, float* y, int m, int n, int k, int64_t ld) {
+    return mxfp4_gemm_launch(w, w_scales, x, x_scales, y, m, n, k, (long)ld, stream());
+}
+
+ATLAS_API int64_t atlas_kv4_cache_bytes(const atlas_kv4_cache* c) {
+    ATLAS_REQUIRE(c, "kv4_cache_bytes: null argument");
+    return kv4_cache_bytes(*c);
+}
+
+ATLAS_API int atlas_kv4_write_f32(const atlas_kv4_cache* c, const atlas_kv4_batch* b, const float* k,
+                                  const float* v, int64_t ld) {
+    ATLAS_REQUIRE(c && b, "kv4_write: null argument");
+    return kv4_write_launch(*c, *b, k, v, (long)ld, stream());
+}
+
+ATLAS_API int atlas_kv4_read_f32(const atlas_kv4_cache* c, const atlas_kv4_batch* b, float* k, float* v,
+                                 int64_t ld) {
+    ATLAS_REQUIRE(c && b, "kv4_read: null argument");
+    return kv4_read_launch(*c, *b, k, v, (long)ld, stream());
+}
+
+ATLAS_API int atlas_kv4_attention_f32(const atlas_kv4_cache* c, const atlas_kv4_batch* b, const float* q,
+                                      int64_t ld_q, int n_heads, float scale, int window, float* out,
+                                      int64_t ld_out) {
+    ATLAS_REQUIRE(c && b, "kv4_attention: null argument");
+    return kv4_attention_launch(*c, *b, q, (long)ld_q, n_heads, scale, window, out, (long)ld_out, stream());
+}
+
 ATLAS_API int atlas_fill_random(int kind, void* out, int64_t n, uint64_t seed, float a, float b) {
     ATLAS_REQUIRE(kind >= 0 && kind <= 2, "fill_random: kind %d", kind);
     return init_launch(kind, out, (long)n, (unsigned long long)seed, a, b, stream());
@@ -353,6 +393,42 @@ ATLAS_API int atlas_quantize_int4_host(const float* w, int64_t rows, int64_t col
             const uint8_t nib = (uint8_t)(q & 0x0F);
             if (i % 2 == 0) data[i / 2] = (uint8_t)((data[i / 2] & 0x0F) | (nib << 4));
             else data[i / 2] = (uint8_t)((data[i / 2] & 0xF0) | nib);
+        }
+    }
+    return ATLAS_OK;
+}
+
+// MXFP4 on the host, the rule of mxfp4.hpp
+ATLAS_API int atlas_quantize_mxfp4_host(const float* w, int64_t rows, int64_t cols, uint8_t* data,
+                                        uint8_t* scales) {
+    ATLAS_REQUIRE(w && data && scales && rows >= 0 && cols >= 0, "quantize_mxfp4_host: bad args");
+    const int64_t kb = (cols + kMxBlock - 1) / kMxBlock;
+    for (int64_t b = 0; b < rows * kb; ++b) {
+        const float* v = w + b / kb * cols + b % kb * kMxBlock;
+        const int64_t left = cols - b % kb * kMxBlock, n = left < kMxBlock ? left : kMxBlock;
+        float mx = 0.0f;
+        bool finite = true;
+        for (int64_t i = 0; i < n; ++i) {
+            finite = finite && std::isfinite(v[i]);
+            mx = std::fmax(mx, std::fabs(v[i]));
+        }
+        uint32_t bits;
+        std::memcpy(&bits, &mx, 4);
+        const int e = (int)(bits >> 23), byte = !finite ? kMxNan : mx == 0.0f ? 127 : e > 2 ? e - 2 : 0;
+        scales[b] = (uint8_t)byte;
+        bits = (uint32_t)(254 - byte) << 23;              // 2^(127 - byte), unused for kMxNan
+        float inv;
+        std::memcpy(&inv, &bits, 4);
+        uint8_t* out = data + b * (kMxBlock / 2);
+        for (int64_t i = 0; i < kMxBlock; ++i) {
+            uint8_t code = 0;
+            if (i < n && byte != kMxNan) {
+                // the midpoints between neighbours, each to the even code
+                const float a = std::fabs(v[i]) * inv;
+                code = (uint8_t)((a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f));
+                if (std::signbit(v[i])) code |= 8;
+            }
+            out[i / 2] = (uint8_t)(i % 2 == 0 ? code : out[i / 2] | code << 4);
         }
     }
     return ATLAS_OK;

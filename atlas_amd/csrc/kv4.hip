@@ -1,0 +1,627 @@
+// kv4.hip -- the 4-bit KV cache: writing and reading tokens, and attention over it.
+//
+// K and V rows are MXFP4 along the head dimension (mxfp4.hpp), in pages of
+// page_len tokens that a block table strings together for each sequence.  A page
+// holds for each KV head, one after the other,
+//   K codes   [page_len][hd/2 bytes]          a token's elements in order
+//   K scales  [page_len/8][hd/32][8 tokens]
+//   V codes   [page_len/8][16][8 tokens][hd/32 bytes]
+//   V scales  [page_len/8][hd/32][8 tokens]
+// V's elements are cut into 16 groups of hd/16, a group of eight tokens side by
+// side, because the product P V contracts over tokens: a lane of the matrix
+// instruction has eight tokens of the same elements, and so finds them in one
+// piece.  A token still fills whole bytes, so that writing one touches no other.
+#include <algorithm>
+
+#include "mfma.hpp"
+#include "mxfp4.hpp"
+
+namespace atlas {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// what the kernels take of a cache and a batch
+struct Kv4Args {
+    uint8_t* cache;
+    int n_pages, n_kv, page_shift;      // page_len = 1 << page_shift
+    const int* starts;                  // [n_seqs + 1] or null: one row to a sequence
+    const int* lens;
+    const int* table;
+    int table_stride, n_seqs, n_rows;
+    int cap;                            // tokens that the table can hold
+};
+
+template <int HD>
+struct Kv4Layout {
+    static constexpr int KB = HD / 32;                  // blocks of a token
+    // offsets of the parts within a (page, head)'s bytes
+    __device__ static long k_scales(int page_len) { return (long)page_len * (HD / 2); }
+    __device__ static long v_codes(int page_len) { return (long)page_len * (HD / 2 + KB); }
+    __device__ static long v_scales(int page_len) { return (long)page_len * (HD + KB); }
+    __device__ static long bytes(int page_len) { return (long)page_len * (HD + 2 * KB); }
+};
+
+// Sequence and position of a batch's row; false: behind the last sequence.
+// The starts are the caller's: whatever they hold, s stays within [0, n_seqs).
+__device__ __forceinline__ bool kv4_row(const Kv4Args& a, int row, int& s, int& pos) {
+    if (!a.starts) {
+        s = row;
+        pos = max(a.lens[row], 0) - 1;
+        return row < a.n_seqs;
+    }
+    int lo = 0, hi = a.n_seqs;          // the last s with starts[s] <= row
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.starts[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    s = lo;
+    const int end = a.starts[lo + 1];
+    pos = max(a.lens[lo], 0) - (end - row);
+    return row < end && row >= a.starts[lo];
+}
+
+// the page of a position, or -1: outside the table, or an entry that is no page
+__device__ __forceinline__ int kv4_page(const Kv4Args& a, int s, int pos) {
+    if (pos < 0 || pos >= a.cap) return -1;
+    const int page = a.table[(long)s * a.table_stride + (pos >> a.page_shift)];
+    return page >= 0 && page < a.n_pages ? page : -1;
+}
+
+// ---- writing and reading ----------------------------------------------------------
+
+// A thread has 8 elements of a row of K (blockIdx.z 0) or V; four lanes a block.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Args a, const float* __restrict__ k,
+                                                        const float* __restrict__ v, long ld) {
+    typedef Kv4Layout<HD> L;
+    const int row = blockIdx.x, e = (blockIdx.y * 256 + threadIdx.x) * 8;
+    if (e >= a.n_kv * HD) return;                        // whole quads: n_kv * HD is a multiple of 32
+    int s, pos;
+    if (!kv4_row(a, row, s, pos)) return;
+    const int page = kv4_page(a, s, pos);
+    if (page < 0) return;
+    const f32x4* src = reinterpret_cast<const f32x4*>((blockIdx.z ? v : k) + row * ld + e);
+    const f32x4 p = src[0], q = src[1];
+    const float x[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, mx_mag(x[i]));
+    const int byte = mx_byte(quad_max(mx));
+    const uint32_t code = mx_encode8(x, byte);
+    const int plen = 1 << a.page_shift, head = e / HD, d = e % HD, at = pos & (plen - 1);
+    uint8_t* base = a.cache + ((long)page * a.n_kv + head) * L::bytes(plen);
+    const long sc = (long)(at >> 3) * (L::KB * 8) + (d / 32) * 8 + (at & 7);
+    if (blockIdx.z == 0) {
+        *reinterpret_cast<uint32_t*>(base + (long)at * (HD / 2) + d / 2) = code;
+        if (d % 32 == 0) base[L::k_scales(plen) + sc] = (uint8_t)byte;
+    } else {
+        // group of HD / 16 elements, [token % 8][KB bytes]
+        uint8_t* to = base + L::v_codes(plen) + (long)(at >> 3) * (HD * 4) + (d / (HD / 16)) * (8 * L::KB) + (at & 7) * L::KB;
+        if constexpr (HD == 64) {
+            *reinterpret_cast<uint16_t*>(to) = (uint16_t)code;
+            *reinterpret_cast<uint16_t*>(to + 8 * L::KB) = (uint16_t)(code >> 16);
+        } else {
+            *reinterpret_cast<uint32_t*>(to + (d % (HD / 16)) / 2) = code;
+        }
+        if (d % 32 == 0) base[L::v_scales(plen) + sc] = (uint8_t)byte;
+    }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, float* __restrict__ k, float* __restrict__ v,
+                                                       long ld) {
+    typedef Kv4Layout<HD> L;
+    const int row = blockIdx.x, e = (blockIdx.y * 256 + threadIdx.x) * 8;
+    if (e >= a.n_kv * HD) return;
+    int s, pos;
+    if (!kv4_row(a, row, s, pos)) return;
+    const int page = kv4_page(a, s, pos);
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (page >= 0) {
+        const int plen = 1 << a.page_shift, head = e / HD, d = e % HD, at = pos & (plen - 1);
+        const uint8_t* base = a.cache + ((long)page * a.n_kv + head) * L::bytes(plen);
+        const long sc = (long)(at >> 3) * (L::KB * 8) + (d / 32) * 8 + (at & 7);
+        uint32_t code;
+        int byte;
+        if (blockIdx.z == 0) {
+            code = *reinterpret_cast<const uint32_t*>(base + (long)at * (HD / 2) + d / 2);
+            byte = base[L::k_scales(plen) + sc];
+        } else {
+            const uint8_t* from = base + L::v_codes(plen) + (long)(at >> 3) * (HD * 4) + (d / (HD / 16)) * (8 * L::KB) + (at & 7) * L::KB;
+            if constexpr (HD == 64)
+                code = *reinterpret_cast<const uint16_t*>(from) |
+                       (uint32_t) * reinterpret_cast<const uint16_t*>(from + 8 * L::KB) << 16;
+            else
+                code = *reinterpret_cast<const uint32_t*>(from + (d % (HD / 16)) / 2);
+            byte = base[L::v_scales(plen) + sc];
+        }
+        mx_decode8(code, mx_scale(byte), x);
+    }
+    f32x4* to = reinterpret_cast<f32x4*>((blockIdx.z ? v : k) + row * ld + e);
+    to[0] = f32x4{x[0], x[1], x[2], x[3]};
+    to[1] = f32x4{x[4], x[5], x[6], x[7]};
+}
+
+// ---- attention --------------------------------------------------------------------
+//
+// A tile is up to 16 columns of (query row, head of the KV head's group), which
+// walk the cache in chunks of 32 tokens with a running maximum and sum.  Of a
+// chunk, with lane = 16 g + i and the token of a matrix row r of part t (0, 1)
+// being 2 r + t:
+//   S_t = K_t q       v_mfma_scale_f32_16x16x128_f8f6f4: K as it is stored (lane
+//                     (g, i): block g of token 2i + t), q as a sum of E4M3 parts
+//                     with falling scales.  Lane (g, i) gets tokens 8g .. 8g+7
+//                     of column i.
+//   O  += V^T P       v_mfma_f32_16x16x32_bf16: lane (g, i) gives tokens 8g ..
+//                     8g+7 of elements of group i of V, made bf16 exactly, and of
+//                     column i of P = exp2(S - m), which it has already, in two
+//                     bf16 parts.  It gets elements of groups 4g .. 4g+3 of
+//                     column i of O.
+// q in parts: the first is q / 2^e rounded to E4M3 (4 bits) with the row's
+// largest value in [128, 256) 2^e, each next one the remainder in units 16 times
+// smaller: after 5 parts 2^-20 of the row's largest value is left.
+// P in two parts: at most 2^-16 of each p is left (two roundings to 8 bits), beside
+// the 2^-2 to which the cache itself is rounded.
+// The maximum is raised only when a score passes it by more than 2^8 (p then
+// stays below 2^8, far from any overflow); most chunks need no rescaling.
+
+constexpr float kKv4Floor = -3.0e38f;  // running maximum of a row that has seen nothing
+constexpr float kKv4Lazy = 8.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Kv4AttnArgs {
+    Kv4Args c;
+    const float* q;
+    long ld_q;
+    float* out;
+    long ld_out;
+    int group;                          // heads of a KV head
+    int tokens;                         // rows of a tile: 16 / group
+    float scale;
+    int window;
+};
+
+// E4M3 parts of q: PARTS matrix instructions' operands and scale bytes.
+// HD 64: an instruction's 128 is two parts of the 64 (K's blocks given twice).
+// HD 256: part p's two halves are instructions 2p and 2p + 1.
+template <int HD>
+struct Kv4Query {
+    static constexpr int N = HD == 64 ? 3 : HD == 128 ? 5 : 10;
+    i32x8 q[N];
+    int byte[N];
+
+    // 8-bit operand: lane group g's first 16 bytes are elements 16g .. of the
+    // 128, the other 16 elements 64 + 16g ..; its scale is that of elements 32g ..
+    __device__ __forceinline__ void load(const float* row, float scale, int g) {
+        constexpr int H = HD == 256 ? 2 : 1, W = HD == 64 ? 16 : 32;
+        float x[H][W];
+        float mx = 0.f;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int j = 0; j < W / 4; ++j) {
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                if (row) v = *reinterpret_cast<const f32x4*>(row + h * 128 + (j >> 2) * 64 + g * 16 + (j & 3) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[h][4 * j + i] = v[i] * scale;
+                    mx = fmaxf(mx, mx_mag(x[h][4 * j + i]));
+                }
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const int top = max((int)(__float_as_uint(mx) >> 23) - 7, 0);
+        if constexpr (HD == 64) {
+#pragma unroll
+            for (int f = 0; f < N; ++f) {
+                const int b0 = max(top - 8 * f, 0), b1 = max(top - 8 * f - 4, 0);
+                split16(x[0], 0, mx_scale(b0), q[f], 0);
+                split16(x[0], 0, mx_scale(b1), q[f], 4);
+                byte[f] = g < 2 ? b0 : b1;
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < 5; ++p) {
+                const int b = max(top - 4 * p, 0);
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    split16(x[h], 0, mx_scale(b), q[p * H + h], 0);
+                    split16(x[h], 16, mx_scale(b), q[p * H + h], 4);
+                    byte[p * H + h] = b;
+                }
+            }
+        }
+    }
+
+    // 16 elements from `at` rounded to E4M3 into dwords w .. w+3, x keeps the rest
+    template <int W>
+    __device__ __forceinline__ static void split16(float (&x)[W], int at, float scale, i32x8& to, int w) {
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            float* e = x + at + 4 * d;
+            s16x2 c = {0, 0};
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, e[0], e[1], scale, false);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, e[2], e[3], scale, true);
+            const uint32_t u = __builtin_bit_cast(uint32_t, c);
+            const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u, scale, false);
+            const f32x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u, scale, true);
+            e[0] -= lo.x; e[1] -= lo.y; e[2] -= hi.x; e[3] -= hi.y;
+            to[w + d] = (int)u;
+        }
+    }
+};
+
+// a chunk's bytes in the registers of a wave
+template <int HD>
+struct Kv4Chunk {
+    typedef Kv4Layout<HD> L;
+    static constexpr int H = HD == 256 ? 2 : 1;          // K steps of 128 elements
+    static constexpr int VW = HD / 64 * 4;               // dwords of V
+    u32x4 k[H][2];                                       // [step][part t]
+    uint16_t ks[H];                                      // scale bytes of parts 0 and 1
+    uint32_t v[VW];
+    u32x2 vs;
+
+    // base: the (page, head)'s bytes; at: the chunk's first token in the page
+    __device__ __forceinline__ void load(const uint8_t* base, int at, int plen, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        const uint8_t* kp = base + (long)at * (HD / 2);
+        const uint8_t* ksp = base + L::k_scales(plen) + at * L::KB;
+        const uint8_t* vp = base + L::v_codes(plen) + (long)at * (HD / 2);
+        const uint8_t* vsp = base + L::v_scales(plen) + at * L::KB;
+        const int blk = HD == 64 ? g & 1 : g;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                k[h][t] = *reinterpret_cast<const u32x4*>(kp + (2 * i + t) * (HD / 2) + h * 64 + blk * 16);
+            ks[h] = *reinterpret_cast<const uint16_t*>(ksp + (i >> 2) * (8 * L::KB) + (4 * h + blk) * 8 + 2 * (i & 3));
+        }
+#pragma unroll
+        for (int w = 0; w < VW / 4; ++w) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(vp + (g * 16 + i) * (8 * L::KB) + 16 * w);
+            v[4 * w] = x.x; v[4 * w + 1] = x.y; v[4 * w + 2] = x.z; v[4 * w + 3] = x.w;
+        }
+        vs = *reinterpret_cast<const u32x2*>(vsp + (g * L::KB + i * (HD / 16) / 32) * 8);
+    }
+};
+
+// Blocks of V that read as NaN (scale bytes past kMxMaxByte), found in sc, the
+// scale bytes of the lane's eight tokens: returns sc without those bytes, so that
+// the product leaves the columns that do not see their tokens as they were, and
+// in z the rows 4g + r of O^T (bit r) that have to be NaN in the lane's column,
+// which sees [from, to].  Rare, so its loops stay rolled.
+template <int HD>
+__device__ __forceinline__ u32x4 kv4_nan_blocks(uint32_t s0, uint32_t s1, int first, int from, int to) {
+    constexpr int KB = HD / 32;
+    const int g = (threadIdx.x & 63) >> 4;
+    uint32_t rows = 0;
+#pragma unroll 1
+    for (int b = 0; b < KB; ++b)
+#pragma unroll 1
+        for (int j = 0; j < 32; ++j) {
+            // lane (j / 8, first group of block b) has token j's byte
+            const int lane = (j >> 3) * 16 + b * (16 / KB);
+            const uint32_t w0 = __shfl(s0, lane, 64), w1 = __shfl(s1, lane, 64);
+            const uint32_t byte = ((j & 4 ? w1 : w0) >> (8 * (j & 3))) & 255u;
+            const int key = first + j;
+            if ((int)byte <= kMxMaxByte || key < from || key > to) continue;
+            for (int r = 0; r < 4; ++r)
+                if ((4 * g + r) * (HD / 16) / 32 == b) rows |= 1u << r;
+        }
+    for (int j = 0; j < 4; ++j) {
+        if ((int)((s0 >> (8 * j)) & 255u) > kMxMaxByte) s0 &= ~(255u << (8 * j));
+        if ((int)((s1 >> (8 * j)) & 255u) > kMxMaxByte) s1 &= ~(255u << (8 * j));
+    }
+    return u32x4{s0, s1, rows, 0u};
+}
+
+template <int HD>
+struct Kv4State {
+    static constexpr int J = HD / 16;                    // elements of a group, and tiles of O
+    f32x4 o[J];
+    float m, l;
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < J; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m = kKv4Floor;
+        l = 0.f;
+    }
+
+    // V's code dword and byte of elements 2e, 2e+1 of token j
+    template <int J8, int E>
+    __device__ __forceinline__ static uint32_t v_pair(const Kv4Chunk<HD>& c, float s) {
+        constexpr int at = J8 * (HD / 32) + E;
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.v[at / 4], s, at % 4));
+    }
+
+    template <int E>
+    __device__ __forceinline__ void pv(const Kv4Chunk<HD>& c, const float (&s)[8], bf16x8 hi, bf16x8 lo) {
+        const uint32_t w[8] = {v_pair<0, E>(c, s[0]), v_pair<1, E>(c, s[1]), v_pair<2, E>(c, s[2]), v_pair<3, E>(c, s[3]),
+                               v_pair<4, E>(c, s[4]), v_pair<5, E>(c, s[5]), v_pair<6, E>(c, s[6]), v_pair<7, E>(c, s[7])};
+        u32x4 even, odd;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            even[p] = __builtin_amdgcn_perm(w[2 * p + 1], w[2 * p], 0x05040100u);
+            odd[p] = __builtin_amdgcn_perm(w[2 * p + 1], w[2 * p], 0x07060302u);
+        }
+        const bf16x8 a = __builtin_bit_cast(bf16x8, even), b = __builtin_bit_cast(bf16x8, odd);
+        o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, hi, o[2 * E], 0, 0, 0);
+        o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, hi, o[2 * E + 1], 0, 0, 0);
+        o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, lo, o[2 * E], 0, 0, 0);
+        o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, lo, o[2 * E + 1], 0, 0, 0);
+    }
+
+    // A chunk's tokens first .. first + 31.  masked: not every column sees all of
+    // them; the lane's column sees [from, to].  live: tokens of the chunk that
+    // the sequence has (the bytes of others are not looked at).
+    __device__ __forceinline__ void add(Kv4Chunk<HD>& c, const Kv4Query<HD>& q, int first, bool masked, int from,
+                                        int to, int live, int lane) {
+        const int g = lane >> 4;
+        f32x4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int f = 0; f < Kv4Query<HD>::N; ++f) {
+            const int h = HD == 256 ? f & 1 : 0;
+            const i32x8 k0 = {(int)c.k[h][0].x, (int)c.k[h][0].y, (int)c.k[h][0].z, (int)c.k[h][0].w, 0, 0, 0, 0};
+            const i32x8 k1 = {(int)c.k[h][1].x, (int)c.k[h][1].y, (int)c.k[h][1].z, (int)c.k[h][1].w, 0, 0, 0, 0};
+            // operand formats: 4 = E2M1, 0 = E4M3; the third argument picks the scale's byte
+            d[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k0, q.q[f], d[0], 4, 0, 0, c.ks[h], 0, q.byte[f]);
+            d[1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k1, q.q[f], d[1], 4, 0, 1, c.ks[h], 0, q.byte[f]);
+        }
+        float s[8];                                      // token first + 8 g + j
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = d[j & 1][j >> 1];
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = first + 8 * g + j;
+                if (key < from || key > to) s[j] = -__builtin_inff();
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
+        if (__any(top > m + kKv4Lazy)) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float to_m = fmaxf(m, top), down = __builtin_amdgcn_exp2f(m - to_m);
+            m = to_m;
+            l *= down;
+#pragma unroll
+            for (int j = 0; j < J; ++j) o[j] *= down;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const float a = __builtin_amdgcn_exp2f(s[2 * p] - m), b = __builtin_amdgcn_exp2f(s[2 * p + 1] - m);
+            l += a + b;
+            hi[p] = bf16_rne2(a, b);
+            lo[p] = bf16_rne2(a - bf16_lo(hi[p]), b - bf16_hi(hi[p]));
+        }
+        // tokens that are not there get the smallest scale: their p is zero, and
+        // whatever their bytes are the product is too
+        uint32_t sc[2] = {c.vs.x, c.vs.y};
+        if (live < 32) {
+            const int n = min(max(live - 8 * g, 0), 8);
+            sc[0] &= n >= 4 ? ~0u : (1u << (8 * n)) - 1u;
+            sc[1] &= n >= 8 ? ~0u : n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1u;
+        }
+        const uint32_t bad = (((~sc[0] - 0x03030303u) & sc[0]) | ((~sc[1] - 0x03030303u) & sc[1])) & 0x80808080u;
+        if (__any(bad != 0)) {
+            const u32x4 x = kv4_nan_blocks<HD>(sc[0], sc[1], first, from, to);
+            sc[0] = x.x;
+            sc[1] = x.y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (x.z >> r & 1u)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) o[j][r] = __builtin_nanf("");
+        }
+        float vsc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vsc[j] = mx_scale((sc[j >> 2] >> (8 * (j & 3))) & 255u);
+        const bf16x8 ph = __builtin_bit_cast(bf16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
+        const bf16x8 pl = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
+        pv<0>(c, vsc, ph, pl);
+        pv<1>(c, vsc, ph, pl);
+        if constexpr (HD >= 128) {
+            pv<2>(c, vsc, ph, pl);
+            pv<3>(c, vsc, ph, pl);
+        }
+        if constexpr (HD >= 256) {
+            pv<4>(c, vsc, ph, pl);
+            pv<5>(c, vsc, ph, pl);
+            pv<6>(c, vsc, ph, pl);
+            pv<7>(c, vsc, ph, pl);
+        }
+    }
+};
+
+// The tile u of a batch: its sequence, first row and rows; false: none.  Tiles
+// of sequence s begin at starts[s] / tokens + s, which leaves each sequence as
+// many as it needs, whatever the lengths.
+__device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int u, int& s, int& row, int& rows, int& pos) {
+    if (!a.c.starts) {
+        s = row = u;
+        rows = 1;
+        pos = max(a.c.lens[u], 0) - 1;
+        return true;
+    }
+    int lo = 0, hi = a.c.n_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.c.starts[mid] / a.tokens + mid <= u) lo = mid;
+        else hi = mid;
+    }
+    s = lo;
+    const int begin = max(a.c.starts[lo], 0), end = min(a.c.starts[lo + 1], a.c.n_rows);
+    const int skip = (u - (begin / a.tokens + lo)) * a.tokens;
+    if (skip < 0 || skip >= end - begin) return false;
+    row = begin + skip;
+    rows = min(a.tokens, end - row);
+    pos = max(a.c.lens[lo], 0) - (end - row);
+    return true;
+}
+
+// One tile and KV head to a wave.
+template <int HD>
+__global__ __launch_bounds__(64) void kv4_attention_kernel(Kv4AttnArgs a) {
+    typedef Kv4Layout<HD> L;
+    const int lane = threadIdx.x, i = lane & 15, g = lane >> 4, kvh = blockIdx.y;
+    int s, row0, rows, pos0;
+    if (!kv4_tile(a, blockIdx.x, s, row0, rows, pos0)) return;
+    // the lane's column: row t, head h of the group
+    const int t = i / a.group, h = i - t * a.group;
+    const bool mine = t < rows;
+    const long head = (long)kvh * a.group + h;
+    const int to = mine ? pos0 + t : -1;
+    const int from = a.window > 0 ? max(to - a.window + 1, 0) : 0;
+    Kv4Query<HD> q;
+    q.load(mine ? a.q + (row0 + t) * a.ld_q + head * HD : nullptr, a.scale * kLog2e, g);
+    Kv4State<HD> st;
+    st.clear();
+    const int last = min(pos0 + rows, a.c.cap);          // tokens [begin, last) are seen by some row
+    const int begin = a.window > 0 ? max(pos0 - a.window + 1, 0) : 0;
+    const int all_from = a.window > 0 ? max(pos0 + rows - a.window, 0) : 0;
+    const int plen = 1 << a.c.page_shift;
+    for (int first = begin & ~31; first < last; first += 32) {
+        const int page = a.c.table[(long)s * a.c.table_stride + (first >> a.c.page_shift)];
+        if (page < 0 || page >= a.c.n_pages) continue;
+        const uint8_t* base = a.c.cache + ((long)page * a.c.n_kv + kvh) * L::bytes(plen);
+        Kv4Chunk<HD> c;
+        c.load(base, first & (plen - 1), plen, lane);
+        const bool masked = first < all_from || first + 31 > pos0;
+        st.add(c, q, first, masked, from, to, last - first, lane);
+    }
+    float l = st.l;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (!mine) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;          // a row that has seen nothing is zero
+    float* o = a.out + (row0 + t) * a.ld_out + head * HD;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < Kv4State<HD>::J; j += 4)
+            *reinterpret_cast<f32x4*>(o + (4 * g + r) * (HD / 16) + j) =
+                f32x4{st.o[j][r] * inv, st.o[j + 1][r] * inv, st.o[j + 2][r] * inv, st.o[j + 3][r] * inv};
+}
+
+// ---- launches ---------------------------------------------------------------------
+
+static int kv4_check(const char* who, const atlas_kv4_cache& c) {
+    ATLAS_REQUIRE(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, "%s: head_dim %d (64, 128 or 256)", who,
+                  c.head_dim);
+    ATLAS_REQUIRE(c.page_len >= 32 && c.page_len <= 1 << 24 && (c.page_len & (c.page_len - 1)) == 0,
+                  "%s: page_len %d (a power of two from 32 to 2^24)", who, c.page_len);
+    ATLAS_REQUIRE(c.n_pages >= 0 && c.n_kv > 0 && c.n_kv <= 4096, "%s: %d pages, %d KV heads", who, c.n_pages, c.n_kv);
+    return ATLAS_OK;
+}
+
+int64_t kv4_cache_bytes(const atlas_kv4_cache& c) {
+    const int rc = kv4_check("kv4_cache_bytes", c);
+    if (rc) return rc;
+    return (int64_t)c.n_pages * c.n_kv * ((int64_t)c.page_len * (c.head_dim + c.head_dim / 16));
+}
+
+// fills the kernels' arguments; *n_rows 0: nothing to do
+static int kv4_args(const char* who, const atlas_kv4_cache& c, const atlas_kv4_batch& b, Kv4Args& a) {
+    const int rc = kv4_check(who, c);
+    if (rc) return rc;
+    ATLAS_REQUIRE(b.n_seqs >= 0 && b.n_rows >= 0 && b.table_stride >= 0 && b.max_len >= 0,
+                  "%s: %d sequences, %d rows, table stride %d, max_len %d", who, b.n_seqs, b.n_rows, b.table_stride,
+                  b.max_len);
+    ATLAS_REQUIRE(b.row_starts || b.n_rows == b.n_seqs, "%s: %d rows of %d sequences need row_starts", who, b.n_rows,
+                  b.n_seqs);
+    ATLAS_REQUIRE(b.n_seqs <= 1 << 22 && b.n_rows <= 1 << 22, "%s: %d rows of %d sequences", who, b.n_rows, b.n_seqs);
+    a = Kv4Args{};
+    a.n_rows = b.n_seqs == 0 ? 0 : b.n_rows;
+    if (a.n_rows == 0) return ATLAS_OK;
+    ATLAS_REQUIRE(b.kv_lens && (b.table_stride == 0 || b.block_table) && (c.n_pages == 0 || c.data), "%s: null argument", who);
+    ATLAS_REQUIRE(((uintptr_t)c.data & 15) == 0, "%s: the cache starts on 16 bytes", who);
+    ATLAS_REQUIRE((((uintptr_t)b.kv_lens | (uintptr_t)b.block_table | (uintptr_t)b.row_starts) & 3) == 0,
+                  "%s: misaligned batch", who);
+    a.cache = static_cast<uint8_t*>(c.data);
+    a.n_pages = c.n_pages;
+    a.n_kv = c.n_kv;
+    while ((1 << a.page_shift) < c.page_len) ++a.page_shift;
+    a.starts = b.row_starts;
+    a.lens = b.kv_lens;
+    a.table = b.block_table;
+    a.table_stride = b.table_stride;
+    a.n_seqs = b.n_seqs;
+    // (positions are 32-bit and a chunk reaches 31 past one)
+    a.cap = (int)std::min<int64_t>((int64_t)b.table_stride * c.page_len, 0x7FFFFFC0);
+    return ATLAS_OK;
+}
+
+static int kv4_rows_check(const char* who, const void* p, const void* q, long ld, long wide) {
+    ATLAS_REQUIRE(p && q, "%s: null argument", who);
+    ATLAS_REQUIRE((((uintptr_t)p | (uintptr_t)q) & 15) == 0 && ld % 4 == 0 && ld >= wide,
+                  "%s: rows start on 16 bytes, at least %ld elements apart (stride %ld)", who, wide, ld);
+    return ATLAS_OK;
+}
+
+int kv4_write_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, const float* k, const float* v, long ld,
+                     hipStream_t st) {
+    Kv4Args a;
+    int rc = kv4_args("kv4_write", c, b, a);
+    if (rc || a.n_rows == 0) return rc;
+    const long wide = (long)c.n_kv * c.head_dim;
+    if ((rc = kv4_rows_check("kv4_write", k, v, ld, wide))) return rc;
+    const dim3 grid(a.n_rows, (unsigned)((wide + 2047) / 2048), 2);
+    if (c.head_dim == 64) hipLaunchKernelGGL(kv4_write_kernel<64>, grid, dim3(256), 0, st, a, k, v, ld);
+    else if (c.head_dim == 128) hipLaunchKernelGGL(kv4_write_kernel<128>, grid, dim3(256), 0, st, a, k, v, ld);
+    else hipLaunchKernelGGL(kv4_write_kernel<256>, grid, dim3(256), 0, st, a, k, v, ld);
+    ATLAS_LAUNCH_CHECK("kv4_write");
+    return ATLAS_OK;
+}
+
+int kv4_read_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, float* k, float* v, long ld, hipStream_t st) {
+    Kv4Args a;
+    int rc = kv4_args("kv4_read", c, b, a);
+    if (rc || a.n_rows == 0) return rc;
+    const long wide = (long)c.n_kv * c.head_dim;
+    if ((rc = kv4_rows_check("kv4_read", k, v, ld, wide))) return rc;
+    const dim3 grid(a.n_rows, (unsigned)((wide + 2047) / 2048), 2);
+    if (c.head_dim == 64) hipLaunchKernelGGL(kv4_read_kernel<64>, grid, dim3(256), 0, st, a, k, v, ld);
+    else if (c.head_dim == 128) hipLaunchKernelGGL(kv4_read_kernel<128>, grid, dim3(256), 0, st, a, k, v, ld);
+    else hipLaunchKernelGGL(kv4_read_kernel<256>, grid, dim3(256), 0, st, a, k, v, ld);
+    ATLAS_LAUNCH_CHECK("kv4_read");
+    return ATLAS_OK;
+}
+
+int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, const float* q, long ld_q, int n_heads,
+                         float scale, int window, float* out, long ld_out, hipStream_t st) {
+    Kv4AttnArgs a{};
+    int rc = kv4_args("kv4_attention", c, b, a.c);
+    if (rc) return rc;
+    ATLAS_REQUIRE(n_heads > 0 && n_heads % c.n_kv == 0 && n_heads / c.n_kv <= 16,
+                  "kv4_attention: %d heads over %d KV heads (up to 16 to each)", n_heads, c.n_kv);
+    ATLAS_REQUIRE(window >= 0, "kv4_attention: window %d", window);
+    if (a.c.n_rows == 0) return ATLAS_OK;
+    const long wide = (long)n_heads * c.head_dim;
+    if ((rc = kv4_rows_check("kv4_attention", q, q, ld_q, wide))) return rc;
+    if ((rc = kv4_rows_check("kv4_attention", out, out, ld_out, wide))) return rc;
+    a.q = q;
+    a.ld_q = ld_q;
+    a.out = out;
+    a.ld_out = ld_out;
+    a.group = n_heads / c.n_kv;
+    a.tokens = 16 / a.group;
+    a.scale = scale;
+    a.window = window;
+    const long tiles = b.row_starts ? (long)a.c.n_rows / a.tokens + a.c.n_seqs : a.c.n_rows;
+    const dim3 grid((unsigned)tiles, c.n_kv);
+    if (c.head_dim == 64) hipLaunchKernelGGL(kv4_attention_kernel<64>, grid, dim3(64), 0, st, a);
+    else if (c.head_dim == 128) hipLaunchKernelGGL(kv4_attention_kernel<128>, grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL(kv4_attention_kernel<256>, grid, dim3(64), 0, st, a);
+    ATLAS_LAUNCH_CHECK("kv4_attention");
+    return ATLAS_OK;
+}
+
+}  // namespace atlas

@@ -8,6 +8,10 @@ two nibbles per byte with the even element in the high nibble; scales
 zero.  Quantisation runs in the library's host code
 (atlas_quantize_int8_host / atlas_quantize_int4_host); the same rules run on
 the device in atlas_quantize_int8_dev / atlas_quantize_int4_dev.
+
+``MxFp4Tensor`` (no reference counterpart) holds a matrix in MXFP4: E2M1 codes in
+blocks of 32 along a row, the first of a byte in its low nibble, and a power of
+two for each block (atlas_quantize_mxfp4_host / atlas_quantize_mxfp4_dev).
 """
 from __future__ import annotations
 
@@ -84,6 +88,44 @@ class Int4Tensor:
 
     def memory_bytes(self) -> int:
         return self.data.size + self.scales.size * 4
+
+    def compression_ratio(self) -> float:
+        return self.rows * self.cols * 4 / self.memory_bytes()
+
+
+MXFP4_BLOCK_SIZE = 32
+MXFP4_VALUES = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], np.float32)
+
+
+@dataclass
+class MxFp4Tensor:
+    data: np.ndarray      # uint8 [rows * ceil(cols / 32) * 16]
+    scales: np.ndarray    # uint8 [rows * ceil(cols / 32)]; b stands for 2^(b - 127), 255 for NaN
+    rows: int
+    cols: int
+
+    @staticmethod
+    def quantize(t: np.ndarray) -> "MxFp4Tensor":
+        t = np.ascontiguousarray(t, np.float32)
+        if t.ndim != 2:
+            raise ValueError("MxFp4Tensor.quantize requires a 2D tensor")
+        rows, cols = t.shape
+        blocks = rows * -(-cols // MXFP4_BLOCK_SIZE)
+        data = np.empty(blocks * 16, np.uint8)
+        scales = np.empty(blocks, np.uint8)
+        check(load().atlas_quantize_mxfp4_host(_p(t), rows, cols, _p(data), _p(scales)))
+        return MxFp4Tensor(data, scales, rows, cols)
+
+    def dequantize(self) -> np.ndarray:
+        codes = np.stack([self.data & 15, self.data >> 4], -1).reshape(-1, MXFP4_BLOCK_SIZE)
+        with np.errstate(over="ignore"):
+            scale = np.where(self.scales == 255, np.float32(np.nan),
+                             np.ldexp(np.float32(1), self.scales.astype(np.int32) - 127)).astype(np.float32)
+            v = MXFP4_VALUES[codes] * scale[:, None]
+        return v.reshape(self.rows, -1)[:, :self.cols].astype(np.float32)
+
+    def memory_bytes(self) -> int:
+        return self.data.size + self.scales.size
 
     def compression_ratio(self) -> float:
         return self.rows * self.cols * 4 / self.memory_bytes()

@@ -6,7 +6,8 @@ Same names and argument meaning as crates/atlas-tensor/src/lib.rs:
 ``GpuKvCache`` (701-785) and the free functions (97-142, 570-654), over the
 C ABI of include/atlas_kernels.h.  Extensions: ``GpuBufKind.INT8`` /
 ``GpuBufKind.INT4`` and ``GpuMatrix.upload_int8`` / ``upload_int4`` for the
-dequant-fused GEMVs.
+dequant-fused GEMVs, ``GpuBufKind.MXFP4`` / ``upload_mxfp4`` for products of
+4-bit matrices, and ``GpuKv4Cache``, a paged KV cache in 4 bits.
 
 Error behaviour follows the reference's Option/bool contract where it has
 one (allocation -> None, ``sgemm`` -> False when no device is present), but
@@ -21,7 +22,7 @@ from typing import Optional
 
 import numpy as np
 
-from ._lib import AtlasError, check, check_void, load
+from ._lib import AtlasError, Kv4BatchC, Kv4CacheC, check, check_void, load
 
 
 def _p(a: np.ndarray):
@@ -157,11 +158,12 @@ class _QuantBuf:
 
 
 class GpuBufKind(Enum):
-    """lib.rs:284-292 (F32, BF16) plus the INT8 / INT4 extensions."""
+    """lib.rs:284-292 (F32, BF16) plus the INT8 / INT4 / MXFP4 extensions."""
     F32 = 0
     BF16 = 1
     INT8 = 2
     INT4 = 3
+    MXFP4 = 4
 
     def is_bf16(self) -> bool:
         return self is GpuBufKind.BF16
@@ -200,6 +202,14 @@ class GpuMatrix:
                         t.block_size) if cuda_available() else None
         return GpuMatrix(GpuBufKind.INT4 if buf else None, buf, t.rows, t.cols)
 
+    @staticmethod
+    def upload_mxfp4(t) -> "GpuMatrix":
+        """From an ``atlas_amd.quant.MxFp4Tensor`` (extension).  Products encode
+        their activations as MXFP4 too: both operands have 4 bits."""
+        buf = _QuantBuf(np.ascontiguousarray(t.data, np.uint8), np.ascontiguousarray(t.scales, np.uint8), 0) \
+            if cuda_available() else None
+        return GpuMatrix(GpuBufKind.MXFP4 if buf else None, buf, t.rows, t.cols)
+
     def is_on_gpu(self) -> bool:
         return self.buf is not None
 
@@ -215,6 +225,8 @@ class GpuMatrix:
         elif self.kind is GpuBufKind.BF16:
             lib.atlas_sgemm_bf16_f32(self.buf.ptr, x_ptr, y_ptr, m, n, k)
             check_void()
+        elif self.kind is GpuBufKind.MXFP4 and n == 1:
+            self._launch_mxfp4(x_ptr, y_ptr, 1)
         else:
             fmt = 2 if self.kind is GpuBufKind.INT8 else 3
             if n == 1:
@@ -222,6 +234,14 @@ class GpuMatrix:
                                          x_ptr, y_ptr, m, k))
             else:
                 raise AtlasError(-4, "quantised GpuMatrix: use sgemm_rows for n > 1")
+
+    def _launch_mxfp4(self, x_ptr: int, y_ptr: int, n: int) -> None:
+        lib = load()
+        blocks = n * -(-self.cols // 32)
+        data, scales = _DevMem(max(16 * blocks, 16), sync_alloc=False), _DevMem(max(blocks, 4), sync_alloc=False)
+        check(lib.atlas_quantize_mxfp4_dev(x_ptr, 0, n, self.cols, self.cols, data.ptr, scales.ptr))
+        check(lib.atlas_gemm_mxfp4_f32(self.buf.ptr, self.buf.scales_ptr, data.ptr, scales.ptr, y_ptr,
+                                       self.rows, n, self.cols, self.rows))
 
     def sgemm(self, rhs, k: int, n: int, out: np.ndarray) -> bool:
         """out[m x n] = self[m x k] rhs[k x n]; H2D rhs, D2H out (lib.rs:371-400)."""
@@ -232,7 +252,10 @@ class GpuMatrix:
         c = GpuBuf.alloc(self.rows * n)
         if b is None or c is None:
             return False
-        self._launch(b.ptr, c.ptr, n)
+        try:
+            self._launch(b.ptr, c.ptr, n)
+        except MemoryError:                  # the encoded activations of an MXFP4 product
+            return False
         out[...] = c.download().reshape(out.shape)
         return True
 
@@ -243,7 +266,10 @@ class GpuMatrix:
         out = GpuBuf.alloc(self.rows * n)
         if out is None:
             return None
-        self._launch(x.buf.ptr, out.ptr, n)
+        try:
+            self._launch(x.buf.ptr, out.ptr, n)
+        except MemoryError:
+            return None
         return GpuVec(out, np.zeros(self.rows * n, np.float32), self.rows * n)
 
     def sgemm_rows(self, x: "GpuVec", n: int) -> "GpuVec":
@@ -252,6 +278,11 @@ class GpuMatrix:
         if self.buf is None or x.buf is None:
             raise AtlasError(-1, "sgemm_rows: operands are not on the GPU")
         out = GpuBuf.alloc(self.rows * n)
+        if self.kind is GpuBufKind.MXFP4:
+            if x.len < n * self.cols:
+                raise AtlasError(-1, f"sgemm_rows: {n} rows of {self.cols} elements expected")
+            self._launch_mxfp4(x.buf.ptr, out.ptr, n)
+            return GpuVec(out, np.zeros(self.rows * n, np.float32), self.rows * n)
         fmt = {GpuBufKind.BF16: 1, GpuBufKind.INT8: 2, GpuBufKind.INT4: 3}[self.kind]
         scales = getattr(self.buf, "scales_ptr", None)
         block = getattr(self.buf, "block", 0)
@@ -427,3 +458,69 @@ class GpuKvCache:
 
     def reset(self) -> None:
         """No-op by design (lib.rs:772-784): positions beyond pos are never read."""
+
+
+class Kv4Batch:
+    """The sequences of one step over a ``GpuKv4Cache`` (extension): lengths with
+    the new tokens included, a row of page ids for each sequence (-1: no page),
+    and how many of its last tokens are the step's rows (default one)."""
+
+    def __init__(self, kv_lens, block_table, row_lens=None):
+        lens = np.ascontiguousarray(kv_lens, np.int32).reshape(-1)
+        table = np.ascontiguousarray(block_table, np.int32).reshape(lens.size, -1)
+        rows = np.ones(lens.size, np.int64) if row_lens is None else np.asarray(row_lens, np.int64).reshape(-1)
+        if rows.size != lens.size or (rows < 0).any() or (lens < 0).any() or (rows > lens).any():
+            raise AtlasError(-1, "Kv4Batch: each sequence has 0 <= new rows <= length")
+        starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        self.kv_lens, self.block_table, self.row_starts = lens, table, starts
+        self.n_seqs, self.n_rows = lens.size, int(starts[-1])
+        # (each in its own piece of one allocation)
+        flat = np.concatenate([lens, starts, table.reshape(-1)])
+        self._mem = _DevMem(max(flat.nbytes, 4), sync_alloc=False)
+        check(load().atlas_memcpy_h2d(self._mem.ptr, _p(flat), flat.nbytes))
+        p = self._mem.ptr
+        self.c = Kv4BatchC(None if row_lens is None else p + 4 * lens.size, p,
+                           p + 4 * (lens.size + starts.size), table.shape[1], self.n_seqs, self.n_rows,
+                           int(lens.max(initial=0)))
+
+
+class GpuKv4Cache:
+    """One layer's K and V in MXFP4 pages (extension; ``GpuKvCache`` holds f32)."""
+
+    def __init__(self, mem: _DevMem, c: Kv4CacheC):
+        self._mem, self.c = mem, c
+
+    @staticmethod
+    def new(n_pages: int, page_len: int, n_kv_heads: int, head_dim: int) -> Optional["GpuKv4Cache"]:
+        c = Kv4CacheC(None, n_pages, page_len, n_kv_heads, head_dim)
+        nbytes = check(load().atlas_kv4_cache_bytes(C.byref(c)))
+        if not cuda_available():
+            return None
+        mem = _DevMem(max(nbytes, 16), sync_alloc=True)
+        check(load().atlas_memset_zero(mem.ptr, mem.nbytes))
+        c.data = mem.ptr
+        return GpuKv4Cache(mem, c)
+
+    def _need(self, batch: Kv4Batch, *rows) -> None:
+        for x, wide in rows:
+            if x.buf is None or x.len < batch.n_rows * wide:
+                raise AtlasError(-1, f"GpuKv4Cache: {batch.n_rows} rows of {wide} elements expected on the GPU")
+
+    def write(self, batch: Kv4Batch, k: GpuVec, v: GpuVec) -> None:
+        wide = self.c.n_kv * self.c.head_dim
+        self._need(batch, (k, wide), (v, wide))
+        check(load().atlas_kv4_write_f32(C.byref(self.c), C.byref(batch.c), k.buf.ptr, v.buf.ptr, wide))
+
+    def read(self, batch: Kv4Batch):
+        wide = self.c.n_kv * self.c.head_dim
+        k, v = GpuVec.zeros(batch.n_rows * wide), GpuVec.zeros(batch.n_rows * wide)
+        check(load().atlas_kv4_read_f32(C.byref(self.c), C.byref(batch.c), k.buf.ptr, v.buf.ptr, wide))
+        return k, v
+
+    def attention(self, batch: Kv4Batch, q: GpuVec, n_heads: int, scale: float, window_size: int = 0) -> GpuVec:
+        wide = n_heads * self.c.head_dim
+        self._need(batch, (q, wide))
+        out = GpuVec.zeros(batch.n_rows * wide)
+        check(load().atlas_kv4_attention_f32(C.byref(self.c), C.byref(batch.c), q.buf.ptr, wide, n_heads, scale,
+                                             window_size, out.buf.ptr, wide))
+        return out

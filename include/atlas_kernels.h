@@ -272,6 +272,88 @@ int atlas_quantize_int8_host(const float* w, int64_t rows, int64_t cols, int8_t*
 int atlas_quantize_int4_host(const float* w, int64_t rows, int64_t cols, int64_t block,
                              uint8_t* data, float* scales);
 
+/* ----- MXFP4 matrices (no reference counterpart) ---------------------------
+ * A row of k elements is ceil(k/32) blocks: 16 bytes of E2M1 codes each (0, .5,
+ * 1, 1.5, 2, 3, 4, 6 and a sign bit; the first element of a byte in its low
+ * nibble) and a scale byte b of value 2^(b - 127).  data: [rows][ceil(k/32)][16],
+ * scales: [rows][ceil(k/32)], both without gaps.
+ * Encoding: b = max(e - 2, 0) with e the f32 exponent field of the block's
+ * largest magnitude (127 for a block of zeros), codes the values times
+ * 2^(127 - b) rounded to nearest (ties to the even code), at most 6.  A block
+ * with an infinity or NaN gets b = 255 and reads as NaN throughout.  A last
+ * block that is not full is filled up with zeros.
+ * Source rows (f32 or bf16 bits) and decoded rows lie ld >= cols elements apart
+ * (ld = cols: no gaps).  data is 4-byte aligned.                             */
+int atlas_quantize_mxfp4_dev(const void* src, int src_is_bf16, int64_t rows, int64_t cols,
+                             int64_t ld, uint8_t* data, uint8_t* scales);
+int atlas_dequantize_mxfp4_dev(const uint8_t* data, const uint8_t* scales, int64_t rows,
+                               int64_t cols, float* out, int64_t ld);
+/* The same encoding on the host (rows without gaps), bit for bit.           */
+int atlas_quantize_mxfp4_host(const float* w, int64_t rows, int64_t cols, uint8_t* data,
+                              uint8_t* scales);
+/* Y[n, m] = sum_k X[n, k] W[m, k] of two MXFP4 matrices (W: m rows, X: n rows of
+ * k elements), f32 sums; rows of Y lie ld >= m elements apart.  Any m, n, k.
+ * w and x are 16-byte aligned.  Elements that fill up a last block have to be
+ * zero in one of the two, as the encoders leave them.                       */
+int atlas_gemm_mxfp4_f32(const uint8_t* w, const uint8_t* w_scales, const uint8_t* x,
+                         const uint8_t* x_scales, float* y, int m, int n, int k, int64_t ld);
+
+/* ----- 4-bit KV cache (no reference counterpart) ----------------------------
+ * K and V of one layer in MXFP4 along the head dimension, 17/32 of a byte an
+ * element, in pages of page_len tokens:
+ * [n_pages][n_kv] of
+ *   K codes [page_len][head_dim/2], K scales [page_len/8][head_dim/32][8],
+ *   V codes [page_len/8][16][8][head_dim/32], V scales as K's
+ * (V: 16 groups of head_dim/16 elements, for each of them eight tokens side by
+ * side).  head_dim 64, 128 or 256; page_len a power of two, 32 to 2^24 (one page
+ * of max_seq tokens for each sequence is a cache without paging).           */
+typedef struct {
+    void* data;                  /* device, 16-byte aligned, atlas_kv4_cache_bytes */
+    int n_pages, page_len, n_kv, head_dim;
+} atlas_kv4_cache;
+
+/* A batch of sequences and their newest rows; the arrays are on the device and
+ * read when the kernels run (a captured call follows their contents).
+ * Sequence s has kv_lens[s] tokens, token t in page block_table[s * table_stride
+ * + t / page_len].  Its last q = row_starts[s + 1] - row_starts[s] tokens are the
+ * batch's rows row_starts[s] ..; row_starts (n_seqs + 1 ascending entries from 0
+ * on) may be NULL for one row to a sequence.  Rows from row_starts[n_seqs] on
+ * belong to no sequence: nothing is read or written for them.
+ * A table entry outside [0, n_pages), and a token past the table, is a token
+ * that is not there: not written, read as zeros, not attended to.           */
+typedef struct {
+    const int* row_starts;       /* [n_seqs + 1] or NULL                       */
+    const int* kv_lens;          /* [n_seqs], the new rows included            */
+    const int* block_table;      /* [n_seqs][table_stride]                     */
+    int table_stride, n_seqs;
+    int n_rows;                  /* rows that k, v, q and out have             */
+    int max_len;                 /* no kv_lens entry is larger, as far as the
+                                    caller knows (0: what the table holds): only
+                                    how the work is split goes by it           */
+} atlas_kv4_batch;
+
+/* Bytes of a cache, or a negative ATLAS_E* code. */
+int64_t atlas_kv4_cache_bytes(const atlas_kv4_cache* cache);
+/* Encodes the batch's K and V rows ([n_rows][n_kv * head_dim] f32, ld elements
+ * apart, 16-byte aligned) into their tokens' places.  Two rows of one call must
+ * not share a place.                                                        */
+int atlas_kv4_write_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch, const float* k,
+                        const float* v, int64_t ld);
+/* Decodes the batch's tokens from the cache into K and V rows. */
+int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch, float* k, float* v,
+                       int64_t ld);
+/* Attention of the batch's query rows ([n_rows][n_heads * head_dim] f32, ld_q
+ * elements apart) over the cached tokens: the row of token p sees tokens
+ * max(0, p - window + 1) .. p (window 0: from the first on), scores times scale,
+ * in f32 (K and V exactly as encoded; 2^-16 relative in the softmax's weights).
+ * n_heads / n_kv in 1 .. 16.  One row to a sequence is decode, more are
+ * (chunks of) prompts, whose K and V have to be written before.  A row that
+ * sees no token gives zeros, one with an infinity or NaN in q NaN.  A token that
+ * reads as NaN is NaN to the rows that see it and nothing to the others.    */
+int atlas_kv4_attention_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch,
+                            const float* q, int64_t ld_q, int n_heads, float scale, int window,
+                            float* out, int64_t ld_out);
+
 /* Seeded synthetic fills on the device: SplitMix64 counter + Box-Muller.
  * kind 0: N(a, b) f32; 1: N(a, b) bf16 by truncation; 2: U(a, b) f32.        */
 int atlas_fill_random(int kind, void* out, int64_t n, uint64_t seed, float a, float b);

@@ -1,0 +1,164 @@
+"""MXFP4 and the 4-bit KV cache without a device: the host encoder, and the calls that are refused."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tests import mx_ref
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+
+    import atlas_amd
+    from atlas_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        from atlas_amd import build
+        build.build()
+    return atlas_amd.load()
+
+
+def special():
+    """Blocks with ties, the format's limits, zeros of both signs, tiny and huge values, infinities and NaN."""
+    ties = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 6, 7, 7.99, 4, 0, 0.2499, 0.2501, 4.99, 5.01], np.float32)
+    b = np.concatenate([ties, -ties])
+    tiny = np.float32(2.0) ** -149
+    rows = [b, b * np.float32(2.0) ** 100, b * np.float32(2.0) ** -100, np.zeros(32, np.float32), -np.zeros(32, np.float32),
+            b * np.float32(2.0) ** -128, np.full(32, tiny), b * np.float32(2.0) ** -146, np.full(32, 3.4e38, np.float32)]
+    for bad in (np.inf, -np.inf, np.nan):
+        x = b.copy()
+        x[17] = bad
+        rows.append(x)
+    one = np.zeros(32, np.float32)
+    one[31] = 1
+    rows.append(one)
+    return np.stack(rows).astype(np.float32)
+
+
+def test_host_encoder(lib):
+    from atlas_amd.quant import MxFp4Tensor
+    rng = np.random.default_rng(3)
+    cases = [special()]
+    for shape in [(1, 1), (3, 31), (5, 32), (7, 33), (4, 576), (2, 1000)]:
+        cases.append((rng.standard_normal(shape) * np.exp(3 * rng.standard_normal(shape))).astype(np.float32))
+    for x in cases:
+        t = MxFp4Tensor.quantize(x)
+        data, scales = mx_ref.matrix(x)
+        np.testing.assert_array_equal(t.data, data.reshape(-1))
+        np.testing.assert_array_equal(t.scales, scales.reshape(-1))
+        # every value of the format is an f32 (2^-128 the smallest), or reads as NaN
+        np.testing.assert_array_equal(t.dequantize(), mx_ref.rounded(x).astype(np.float32))
+        assert t.memory_bytes() == 17 * t.scales.size
+
+
+def test_encoding_is_nearest(lib):
+    """Against the definition by distance: no other magnitude of the block's scale lies nearer."""
+    from atlas_amd.quant import MxFp4Tensor
+    x = np.random.default_rng(5).standard_normal((64, 96)).astype(np.float32)
+    t = MxFp4Tensor.quantize(x)
+    got = t.dequantize().astype(np.float64).reshape(-1, 32)
+    scale = np.exp2(t.scales.astype(np.float64) - 127)[:, None, None]
+    all_of = scale * mx_ref.VALUES[None, None, :]
+    best = np.abs(all_of - x.astype(np.float64).reshape(-1, 32, 1)).min(-1)
+    np.testing.assert_array_equal(np.abs(got - x.reshape(-1, 32)), best)
+    # a step is at most 2 of a largest magnitude of 4 or more, and 8 becomes 6: 1/4 of it at most
+    top = np.abs(x.reshape(-1, 32)).max(-1, keepdims=True)
+    assert (np.abs(got - x.reshape(-1, 32)) <= top / 4).all()
+
+
+def _refused(lib, rc):
+    assert rc == -1
+    assert lib.atlas_last_error()
+    lib.atlas_clear_error()
+
+
+def test_matrix_refusals(lib):
+    a = 4096                      # an aligned address that no refused call looks at
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a, 0, -1, 32, 32, a, a))
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a, 0, 2, 32, 31, a, a))       # rows that overlap
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(None, 0, 2, 32, 32, a, a))
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a + 2, 0, 2, 32, 32, a, a))   # f32 off its alignment
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a + 1, 1, 2, 32, 32, a, a))
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a, 0, 2, 32, 32, a + 2, a))
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a, 0, 1 << 40, 1 << 20, 1 << 20, a, a))
+    _refused(lib, lib.atlas_quantize_mxfp4_dev(a, 0, 1, 1 << 40, 1 << 40, a, a))
+    _refused(lib, lib.atlas_dequantize_mxfp4_dev(a, a, 2, 32, None, 32))
+    _refused(lib, lib.atlas_dequantize_mxfp4_dev(a, a, 2, 33, a, 32))
+    _refused(lib, lib.atlas_dequantize_mxfp4_dev(a, a, 2, 32, a + 2, 32))
+    _refused(lib, lib.atlas_quantize_mxfp4_host(None, 2, 32, a, a))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, a, a, -1, 1, 32, 4))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, a, a, 5, 1, 32, 4))      # rows of y that overlap
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a + 8, a, a, a, a, 4, 1, 32, 4))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a + 4, a, a, 4, 1, 32, 4))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, a, a + 2, 4, 1, 32, 4))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, None, a, 4, 1, 32, 4))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, a, None, 4, 1, 32, 4))
+    # nothing to do is done without a device
+    assert lib.atlas_quantize_mxfp4_dev(None, 0, 0, 32, 32, None, None) == 0
+    assert lib.atlas_dequantize_mxfp4_dev(None, None, 3, 0, None, 0) == 0
+    assert lib.atlas_gemm_mxfp4_f32(None, None, None, None, None, 0, 3, 32, 0) == 0
+
+
+def test_cache_refusals(lib):
+    from atlas_amd._lib import Kv4BatchC, Kv4CacheC
+    a = 4096
+
+    def cache(**kw):
+        d = dict(data=a, n_pages=4, page_len=64, n_kv=2, head_dim=128)
+        d.update(kw)
+        return C.byref(Kv4CacheC(*[d[n] for n, _ in Kv4CacheC._fields_]))
+
+    def batch(**kw):
+        d = dict(row_starts=a, kv_lens=a, block_table=a, table_stride=2, n_seqs=2, n_rows=3, max_len=0)
+        d.update(kw)
+        return C.byref(Kv4BatchC(*[d[n] for n, _ in Kv4BatchC._fields_]))
+
+    assert lib.atlas_kv4_cache_bytes(cache()) == 4 * 2 * 64 * (128 + 8)
+    bad = [dict(head_dim=96), dict(head_dim=0), dict(page_len=16), dict(page_len=48), dict(page_len=1 << 25),
+           dict(n_pages=-1), dict(n_kv=0), dict(n_kv=5000)]
+    for kw in bad:
+        _refused(lib, lib.atlas_kv4_cache_bytes(cache(**kw)))
+        _refused(lib, lib.atlas_kv4_write_f32(cache(**kw), batch(), a, a, 256))
+        _refused(lib, lib.atlas_kv4_read_f32(cache(**kw), batch(), a, a, 256))
+        _refused(lib, lib.atlas_kv4_attention_f32(cache(**kw), batch(), a, 512, 4, 1.0, 0, a, 512))
+    _refused(lib, lib.atlas_kv4_cache_bytes(None))
+    wrong = [dict(n_seqs=-1), dict(n_rows=-1), dict(table_stride=-1), dict(max_len=-1), dict(kv_lens=None),
+             dict(block_table=None), dict(row_starts=None), dict(kv_lens=a + 2), dict(n_rows=1 << 23)]
+    for kw in wrong:
+        _refused(lib, lib.atlas_kv4_write_f32(cache(), batch(**kw), a, a, 256))
+        _refused(lib, lib.atlas_kv4_read_f32(cache(), batch(**kw), a, a, 256))
+        _refused(lib, lib.atlas_kv4_attention_f32(cache(), batch(**kw), a, 512, 4, 1.0, 0, a, 512))
+    for fn in (lib.atlas_kv4_write_f32, lib.atlas_kv4_read_f32):
+        _refused(lib, fn(cache(), batch(), None, a, 256))
+        _refused(lib, fn(cache(), batch(), a + 4, a, 256))
+        _refused(lib, fn(cache(), batch(), a, a, 255))
+        _refused(lib, fn(cache(), batch(), a, a, 258))
+        _refused(lib, fn(cache(data=None), batch(), a, a, 256))
+        _refused(lib, fn(cache(data=a + 8), batch(), a, a, 256))
+        _refused(lib, fn(cache(), None, a, a, 256))
+        assert fn(cache(), batch(n_rows=0), None, None, 0) == 0
+        assert fn(cache(), batch(n_seqs=0), None, None, 0) == 0
+    fn = lib.atlas_kv4_attention_f32
+    _refused(lib, fn(cache(), batch(), a, 512, 3, 1.0, 0, a, 512))             # heads that do not divide
+    _refused(lib, fn(cache(), batch(), a, 512 * 17, 34, 1.0, 0, a, 512 * 17))  # 17 to a KV head
+    _refused(lib, fn(cache(), batch(), a, 512, 4, 1.0, -1, a, 512))
+    _refused(lib, fn(cache(), batch(), a, 508, 4, 1.0, 0, a, 512))
+    _refused(lib, fn(cache(), batch(), a, 512, 4, 1.0, 0, a, 510))
+    _refused(lib, fn(cache(), batch(), a, 512, 4, 1.0, 0, None, 512))
+    _refused(lib, fn(cache(), batch(), a + 4, 512, 4, 1.0, 0, a, 512))
+    _refused(lib, fn(None, batch(), a, 512, 4, 1.0, 0, a, 512))
+    assert fn(cache(), batch(n_rows=0), None, 0, 4, 1.0, 0, None, 0) == 0
+
+
+def test_batches_that_are_refused(lib):
+    from atlas_amd import AtlasError
+    from atlas_amd.tensor import GpuKv4Cache, Kv4Batch, cuda_available
+    for lens, table, rows in [([3], [[0]], [4]), ([3, -1], [[0], [1]], None), ([3, 4], [[0], [1]], [1]),
+                              ([3], [[0]], [-1])]:
+        with pytest.raises(AtlasError):
+            Kv4Batch(lens, table, rows)
+    with pytest.raises(AtlasError):
+        GpuKv4Cache.new(4, 48, 2, 128)
+    if not cuda_available():
+        assert GpuKv4Cache.new(4, 64, 2, 128) is None
