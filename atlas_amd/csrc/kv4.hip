@@ -18,8 +18,6 @@
 
 namespace atlas {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 // what the kernels take of a cache and a batch
 struct Kv4Args {
     uint8_t* cache;
@@ -150,19 +148,22 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, float* __restr
 // chunk, with lane = 16 g + i and the token of a matrix row r of part t (0, 1)
 // being 2 r + t:
 //   S_t = K_t q       v_mfma_scale_f32_16x16x128_f8f6f4: K as it is stored (lane
-//                     (g, i): block g of token 2i + t), q as a sum of E4M3 parts
+//                     (g, i): block g of token 2i + t), q as a sum of E2M1 parts
 //                     with falling scales.  Lane (g, i) gets tokens 8g .. 8g+7
 //                     of column i.
 //   O  += V^T P       v_mfma_f32_16x16x32_bf16: lane (g, i) gives tokens 8g ..
 //                     8g+7 of elements of group i of V, made bf16 exactly, and of
-//                     column i of P = exp2(S - m), which it has already, in two
+//                     column i of P = exp2(S - m), which it has already, in three
 //                     bf16 parts.  It gets elements of groups 4g .. 4g+3 of
 //                     column i of O.
-// q in parts: the first is q / 2^e rounded to E4M3 (4 bits) with the row's
-// largest value in [128, 256) 2^e, each next one the remainder in units 16 times
-// smaller: after 5 parts 2^-20 of the row's largest value is left.
-// P in two parts: at most 2^-16 of each p is left (two roundings to 8 bits), beside
-// the 2^-2 to which the cache itself is rounded.
+// q in parts, for each block of 32: the first is q / 2^e rounded to E2M1 with the
+// block's largest value in [2, 4) 2^e, so at most 2^e / 2 off; each next one is the
+// remainder in units 8 times smaller.  7 parts leave 2^-20 of the block's largest
+// value.  Products of two E2M1 numbers and their sums of 128 are exact in this
+// instruction.  (With E4M3 parts, 5 for the same 20 bits, it drops the low bits of
+// products far below the largest one: 4e-6 of a sum for normal q, against none.)
+// P in three parts: its 24 bits.  (Two leave 2^-16 of each p, 2.6e-6 of an output
+// where f32 sums leave 1e-6, and take a third of the P V instructions less.)
 // The maximum is raised only when a score passes it by more than 2^8 (p then
 // stays below 2^8, far from any overflow); most chunks need no rescaling.
 
@@ -182,75 +183,69 @@ struct Kv4AttnArgs {
     int window;
 };
 
-// E4M3 parts of q: PARTS matrix instructions' operands and scale bytes.
+// E2M1 parts of q: the operands of N matrix instructions and their scale bytes.
 // HD 64: an instruction's 128 is two parts of the 64 (K's blocks given twice).
 // HD 256: part p's two halves are instructions 2p and 2p + 1.
 template <int HD>
 struct Kv4Query {
-    static constexpr int N = HD == 64 ? 3 : HD == 128 ? 5 : 10;
-    i32x8 q[N];
+    static constexpr int PARTS = HD == 64 ? 8 : 7;
+    static constexpr int N = HD == 64 ? 4 : HD == 128 ? 7 : 14;
+    u32x4 q[N];
     int byte[N];
 
-    // 8-bit operand: lane group g's first 16 bytes are elements 16g .. of the
-    // 128, the other 16 elements 64 + 16g ..; its scale is that of elements 32g ..
+    // the column's row of q times scale (null: zeros); lane group g has block g
+    // of an instruction's four
     __device__ __forceinline__ void load(const float* row, float scale, int g) {
-        constexpr int H = HD == 256 ? 2 : 1, W = HD == 64 ? 16 : 32;
-        float x[H][W];
-        float mx = 0.f;
+        constexpr int H = HD == 256 ? 2 : 1;
+        const int blk = HD == 64 ? g & 1 : g;
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+        for (int h = 0; h < H; ++h) {
+            float x[32], mx = 0.f;
 #pragma unroll
-            for (int j = 0; j < W / 4; ++j) {
+            for (int j = 0; j < 8; ++j) {
                 f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                if (row) v = *reinterpret_cast<const f32x4*>(row + h * 128 + (j >> 2) * 64 + g * 16 + (j & 3) * 4);
+                if (row) v = *reinterpret_cast<const f32x4*>(row + h * 128 + blk * 32 + j * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[h][4 * j + i] = v[i] * scale;
-                    mx = fmaxf(mx, mx_mag(x[h][4 * j + i]));
+                    x[4 * j + i] = v[i] * scale;
+                    mx = fmaxf(mx, mx_mag(x[4 * j + i]));
                 }
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const int top = max((int)(__float_as_uint(mx) >> 23) - 7, 0);
-        if constexpr (HD == 64) {
+            const int e = (int)(__float_as_uint(mx) >> 23), top = max(e - 1, 0);
 #pragma unroll
-            for (int f = 0; f < N; ++f) {
-                const int b0 = max(top - 8 * f, 0), b1 = max(top - 8 * f - 4, 0);
-                split16(x[0], 0, mx_scale(b0), q[f], 0);
-                split16(x[0], 0, mx_scale(b1), q[f], 4);
-                byte[f] = g < 2 ? b0 : b1;
-            }
-        } else {
-#pragma unroll
-            for (int p = 0; p < 5; ++p) {
-                const int b = max(top - 4 * p, 0);
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    split16(x[h], 0, mx_scale(b), q[p * H + h], 0);
-                    split16(x[h], 16, mx_scale(b), q[p * H + h], 4);
-                    byte[p * H + h] = b;
+            for (int p = 0; p < PARTS; ++p) {
+                const int b = max(top - 3 * p, 0);
+                const u32x4 w = part(x, mx_scale(b));
+                const int f = HD == 64 ? p / 2 : HD == 128 ? p : 2 * p + h;
+                if (HD != 64 || (p & 1) == 0) {
+                    q[f] = w;
+                    byte[f] = b;
+                } else if (g >= 2) {
+                    q[f] = w;
+                    byte[f] = b;
                 }
             }
+            if (e == 255) byte[HD == 256 ? h : 0] = kMxNan;    // an infinity or NaN: so is every score
         }
     }
 
-    // 16 elements from `at` rounded to E4M3 into dwords w .. w+3, x keeps the rest
-    template <int W>
-    __device__ __forceinline__ static void split16(float (&x)[W], int at, float scale, i32x8& to, int w) {
-        typedef short s16x2 __attribute__((ext_vector_type(2)));
-        typedef float f32x2 __attribute__((ext_vector_type(2)));
+    // x rounded to E2M1; x keeps the rest
+    __device__ __forceinline__ static u32x4 part(float (&x)[32], float scale) {
+        u32x4 to;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            float* e = x + at + 4 * d;
-            s16x2 c = {0, 0};
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, e[0], e[1], scale, false);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, e[2], e[3], scale, true);
-            const uint32_t u = __builtin_bit_cast(uint32_t, c);
-            const f32x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u, scale, false);
-            const f32x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(u, scale, true);
-            e[0] -= lo.x; e[1] -= lo.y; e[2] -= hi.x; e[3] -= hi.y;
-            to[w + d] = (int)u;
+            uint32_t w = 0;
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d], x[8 * d + 1], scale, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d + 2], x[8 * d + 3], scale, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d + 4], x[8 * d + 5], scale, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d + 6], x[8 * d + 7], scale, 3);
+            float y[8];
+            mx_decode8(w, scale, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[8 * d + i] -= y[i];
+            to[d] = w;
         }
+        return to;
     }
 };
 
@@ -340,20 +335,21 @@ struct Kv4State {
     }
 
     template <int E>
-    __device__ __forceinline__ void pv(const Kv4Chunk<HD>& c, const float (&s)[8], bf16x8 hi, bf16x8 lo) {
+    __device__ __forceinline__ void pv(const Kv4Chunk<HD>& c, const float (&s)[8], const bf16x8 (&p)[3]) {
         const uint32_t w[8] = {v_pair<0, E>(c, s[0]), v_pair<1, E>(c, s[1]), v_pair<2, E>(c, s[2]), v_pair<3, E>(c, s[3]),
                                v_pair<4, E>(c, s[4]), v_pair<5, E>(c, s[5]), v_pair<6, E>(c, s[6]), v_pair<7, E>(c, s[7])};
         u32x4 even, odd;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            even[p] = __builtin_amdgcn_perm(w[2 * p + 1], w[2 * p], 0x05040100u);
-            odd[p] = __builtin_amdgcn_perm(w[2 * p + 1], w[2 * p], 0x07060302u);
+        for (int j = 0; j < 4; ++j) {
+            even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+            odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
         }
         const bf16x8 a = __builtin_bit_cast(bf16x8, even), b = __builtin_bit_cast(bf16x8, odd);
-        o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, hi, o[2 * E], 0, 0, 0);
-        o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, hi, o[2 * E + 1], 0, 0, 0);
-        o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, lo, o[2 * E], 0, 0, 0);
-        o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, lo, o[2 * E + 1], 0, 0, 0);
+#pragma unroll
+        for (int j = 2; j >= 0; --j) {
+            o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[j], o[2 * E], 0, 0, 0);
+            o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p[j], o[2 * E + 1], 0, 0, 0);
+        }
     }
 
     // A chunk's tokens first .. first + 31.  masked: not every column sees all of
@@ -364,13 +360,13 @@ struct Kv4State {
         const int g = lane >> 4;
         f32x4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int f = 0; f < Kv4Query<HD>::N; ++f) {
+        for (int f = Kv4Query<HD>::N - 1; f >= 0; --f) {
             const int h = HD == 256 ? f & 1 : 0;
-            const i32x8 k0 = {(int)c.k[h][0].x, (int)c.k[h][0].y, (int)c.k[h][0].z, (int)c.k[h][0].w, 0, 0, 0, 0};
-            const i32x8 k1 = {(int)c.k[h][1].x, (int)c.k[h][1].y, (int)c.k[h][1].z, (int)c.k[h][1].w, 0, 0, 0, 0};
-            // operand formats: 4 = E2M1, 0 = E4M3; the third argument picks the scale's byte
-            d[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k0, q.q[f], d[0], 4, 0, 0, c.ks[h], 0, q.byte[f]);
-            d[1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k1, q.q[f], d[1], 4, 0, 1, c.ks[h], 0, q.byte[f]);
+            // (the argument before a scale picks its byte)
+            d[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(c.k[h][0]), mx_frag(q.q[f]), d[0], kFp4, kFp4, 0,
+                                                                    c.ks[h], 0, q.byte[f]);
+            d[1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(c.k[h][1]), mx_frag(q.q[f]), d[1], kFp4, kFp4, 1,
+                                                                    c.ks[h], 0, q.byte[f]);
         }
         float s[8];                                      // token first + 8 g + j
 #pragma unroll
@@ -394,13 +390,16 @@ struct Kv4State {
 #pragma unroll
             for (int j = 0; j < J; ++j) o[j] *= down;
         }
-        uint32_t hi[4], lo[4];
+        u32x4 part[3];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const float a = __builtin_amdgcn_exp2f(s[2 * p] - m), b = __builtin_amdgcn_exp2f(s[2 * p + 1] - m);
+        for (int j = 0; j < 4; ++j) {
+            float a = __builtin_amdgcn_exp2f(s[2 * j] - m), b = __builtin_amdgcn_exp2f(s[2 * j + 1] - m);
             l += a + b;
-            hi[p] = bf16_rne2(a, b);
-            lo[p] = bf16_rne2(a - bf16_lo(hi[p]), b - bf16_hi(hi[p]));
+            part[0][j] = bf16_rne2(a, b);
+            a -= bf16_lo(part[0][j]);
+            b -= bf16_hi(part[0][j]);
+            part[1][j] = bf16_rne2(a, b);
+            part[2][j] = bf16_rne2(a - bf16_lo(part[1][j]), b - bf16_hi(part[1][j]));
         }
         // tokens that are not there get the smallest scale: their p is zero, and
         // whatever their bytes are the product is too
@@ -424,19 +423,19 @@ struct Kv4State {
         float vsc[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) vsc[j] = mx_scale((sc[j >> 2] >> (8 * (j & 3))) & 255u);
-        const bf16x8 ph = __builtin_bit_cast(bf16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
-        const bf16x8 pl = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
-        pv<0>(c, vsc, ph, pl);
-        pv<1>(c, vsc, ph, pl);
+        const bf16x8 p[3] = {__builtin_bit_cast(bf16x8, part[0]), __builtin_bit_cast(bf16x8, part[1]),
+                             __builtin_bit_cast(bf16x8, part[2])};
+        pv<0>(c, vsc, p);
+        pv<1>(c, vsc, p);
         if constexpr (HD >= 128) {
-            pv<2>(c, vsc, ph, pl);
-            pv<3>(c, vsc, ph, pl);
+            pv<2>(c, vsc, p);
+            pv<3>(c, vsc, p);
         }
         if constexpr (HD >= 256) {
-            pv<4>(c, vsc, ph, pl);
-            pv<5>(c, vsc, ph, pl);
-            pv<6>(c, vsc, ph, pl);
-            pv<7>(c, vsc, ph, pl);
+            pv<4>(c, vsc, p);
+            pv<5>(c, vsc, p);
+            pv<6>(c, vsc, p);
+            pv<7>(c, vsc, p);
         }
     }
 };

@@ -1,4 +1,5 @@
 // mxfp4.hip -- MXFP4 matrices: encoding, decoding and their product.
+#include <type_traits>
 #include "mxfp4.hpp"
 
 namespace atlas {
@@ -10,7 +11,10 @@ namespace atlas {
 // loads, a dword of codes, the block's largest magnitude by two DPP steps.
 
 typedef u32x4 __attribute__((aligned(4))) u32x4_dw;    // a row of f32 starts on any dword,
-typedef u32x4 __attribute__((aligned(2))) u32x4_hw;    // one of bf16 on any halfword
+typedef u32x4 __attribute__((aligned(2))) u32x4_hw;    // one of bf16 on any halfword,
+typedef u32x4 __attribute__((aligned(1))) u32x4_b;     // and one of scale bytes on any byte
+typedef uint64_t __attribute__((aligned(1))) u64_b;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <bool BF>
 __device__ __forceinline__ void mx_load8(const void* src, long at, int left, float (&v)[8]) {
@@ -182,39 +186,232 @@ int mxfp4_dequant_launch(const uint8_t* data, const uint8_t* scales, long rows, 
 // 4g .. 4g+3 of column i of the product.  Codes and scales are exact, the sums
 // are f32.
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
+// 16 blocks (512 elements) of 16 rows: lane (g, i) has blocks 4s + g of row i for
+// s = 0 .. 3, and the row's scale bytes, four to a dword.
+struct MxUnit {
+    u32x4 d[4], s;
 
-__device__ __forceinline__ i32x8 mx_frag(u32x4 v) {
-    return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+    // row: its first block; blocks from kb on give zeros
+    __device__ __forceinline__ void load(const u32x4* data, const uint8_t* scales, long row, int u, int kb, int g) {
+        const int b0 = u * 16;
+        const u32x4* p = data + row + b0 + g;
+        const uint8_t* q = scales + row + b0;
+        if (b0 + 16 <= kb) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) d[t] = p[4 * t];
+            s = *reinterpret_cast<const u32x4_b*>(q);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const bool in = b0 + 4 * t + g < kb;
+                d[t] = in ? p[4 * t] : u32x4{0u, 0u, 0u, 0u};
+                s[t] = (in ? (uint32_t)q[4 * t + g] : 127u) << (8 * g);
+            }
+        }
+    }
+};
+
+// Few rows: the weights' stream.  A block has MT x 16 weight rows and NT x 16 rows
+// of x, its waves every WAVES-th unit of 512 elements, straight from global memory
+// into the matrix instructions' registers; their sums meet in LDS.
+template <int MT, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const u32x4* __restrict__ w, const uint8_t* __restrict__ ws,
+                                                                const u32x4* __restrict__ x, const uint8_t* __restrict__ xs,
+                                                                float* __restrict__ y, int m, int n, int kb, long ldy) {
+    __shared__ f32x4 part[WAVES][MT * NT * 64];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int m0 = blockIdx.x * (MT * 16), n0 = blockIdx.y * (NT * 16);
+    // rows past the last one repeat it; their results are not stored
+    long wr[MT], xr[NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) wr[t] = (long)min(m0 + 16 * t + i, m - 1) * kb;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) xr[t] = (long)min(n0 + 16 * t + i, n - 1) * kb;
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int units = (kb + 15) / 16;
+    for (int u = wave; u < units; u += WAVES) {
+        MxUnit wu[MT], xu[NT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) wu[t].load(w, ws, wr[t], u, kb, g);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) xu[t].load(x, xs, xr[t], u, kb, g);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int b = 0; b < NT; ++b)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        mx_frag(xu[b].d[s]), mx_frag(wu[a].d[s]), acc[a][b], kFp4, kFp4, 0, xu[b].s[s] >> (8 * g), 0,
+                        wu[a].s[s] >> (8 * g));
+    }
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) part[wave][(a * NT + b) * 64 + lane] = acc[a][b];
+    __syncthreads();
+    for (int e = threadIdx.x; e < MT * NT * 64; e += WAVES * 64) {
+        f32x4 sum = part[0][e];
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) sum += part[v][e];
+        const int tile = e >> 6, col = m0 + tile / NT * 16 + (e & 15), row = n0 + tile % NT * 16 + (e >> 4 & 3) * 4;
+        if (col < m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (row + r < n) y[(row + r) * ldy + col] = sum[r];
+    }
 }
 
-constexpr int kFp4 = 4;               // format code of both operands
+// Many rows: tiles of BM weight rows x BN rows of x through LDS, 256 elements (a
+// 128-byte line of each row) at a time, two such steps deep: one loads while the
+// other is multiplied.
+//  * Codes reach LDS by direct loads, 16-byte chunk c of row r into slot c ^ (r & 7),
+//    so that the fragment reads (32 rows, one chunk) hit every bank alike.  Scale
+//    bytes, whose rows start on any byte, go through registers, 8 to a thread.
+//  * v_mfma_scale_f32_32x32x64_f8f6f4, A = x, B = weights: lane (h, i) = 32 h + i gives
+//    block h of the 64 of row i, and has rows 8q + 4h + 0..3 (q = 0 .. 3) of column i,
+//    so that a store writes 128 bytes of a row of y.
+//  * Past the end of a row lies the next one: codes there are numbers whatever they
+//    are, and their scale bytes are set to 0, 2^-254 for a product, which is zero in
+//    an f32.  Rows past the last one are multiplied and not stored.
+constexpr int kMxStep = 8;            // blocks of a step
 
-// One 16 x 16 tile to a wave, straight from global memory.
-__global__ __launch_bounds__(256) void mxfp4_tile_kernel(const u32x4* __restrict__ w, const uint8_t* __restrict__ ws,
-                                                         const u32x4* __restrict__ x, const uint8_t* __restrict__ xs,
-                                                         float* __restrict__ y, int m, int n, int kb, long ldy) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int m0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, n0 = blockIdx.y * 16;
-    if (m0 >= m) return;
-    // rows past the last one repeat it; their results are not stored
-    const long wr = (long)min(m0 + i, m - 1) * kb, xr = (long)min(n0 + i, n - 1) * kb;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int b0 = 0; b0 < kb; b0 += 4) {
-        u32x4 a = {0u, 0u, 0u, 0u}, b = a;
-        int sa = 127, sb = 127;
-        if (b0 + g < kb) {
-            a = x[xr + b0 + g];
-            b = w[wr + b0 + g];
-            sa = xs[xr + b0 + g];
-            sb = ws[wr + b0 + g];
-        }
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(a), mx_frag(b), acc, kFp4, kFp4, 0, sa, 0, sb);
-    }
-    if (m0 + i >= m) return;
+// 16 bytes per lane from global memory to lds + 16 lane (lds wave-uniform); zeros
+// past the buffer's end.  All of the offset is in the register that is checked.
+__device__ __forceinline__ void mx_load_lds(__amdgpu_buffer_rsrc_t src, uint32_t at, void* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)lds, 16, at, 0, 0, 0);
+}
+
+// the wave's loads and LDS writes have landed; then the block meets
+__device__ __forceinline__ void mx_meet() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// rows of `pitch` bytes as a buffer
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const u32x4* p, int rows, uint32_t pitch) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<u32x4*>(p), 0, rows * pitch, 0x00020000);
+}
+
+template <int WM, int WN, int MT, int NT>
+struct MxTile {
+    static constexpr int WAVES = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, ROWS = BM + BN;
+    static constexpr int LOADS = ROWS / 8 / WAVES;       // of 8 rows each, for a wave and step
+    static constexpr int BYTES = 2 * ROWS * (128 + 8);
+    static_assert(ROWS % (8 * WAVES) == 0 && BM % 8 == 0 && ROWS <= WAVES * 64, "loads in whole waves");
+};
+
+template <int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* __restrict__ w, const uint8_t* __restrict__ ws,
+                                                                  const u32x4* __restrict__ x, const uint8_t* __restrict__ xs,
+                                                                  float* __restrict__ y, int m, int n, int kb, long ldy,
+                                                                  int tiles_m, int tiles_n) {
+    typedef MxTile<WM, WN, MT, NT> T;
+    // [2][ROWS * 8] chunks of codes, the weights' rows, then x's; [2][ROWS] eights of scale bytes
+    extern __shared__ __align__(1024) uint8_t lds[];
+    u32x4* const codes = reinterpret_cast<u32x4*>(lds);
+    uint64_t* const bytes = reinterpret_cast<uint64_t*>(lds + 2 * T::ROWS * 128);
+    // consecutive blocks run on different XCDs: each takes a run of the tiles, so
+    // that its L2 serves the weights of a tile to all but the first
+    const int per = (tiles_m * tiles_n + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (tile >= tiles_m * tiles_n) return;
+    const int m0 = tile / tiles_n * T::BM, n0 = tile % tiles_n * T::BN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 31, h = lane >> 5, wm = wave / WN, wn = wave % WN;
+    const uint32_t pitch = (uint32_t)kb * 16;
+    const auto wbuf = mx_rows(w + (long)m0 * kb, min(m - m0, T::BM), pitch), xbuf = mx_rows(x + (long)n0 * kb, min(n - n0, T::BN), pitch);
+    const uint32_t voff = (lane >> 3) * pitch + (((lane & 7) ^ (lane >> 3)) * 16);
+    const auto load_codes = [&](int step, int buf) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (n0 + 4 * g + r < n) y[(n0 + 4 * g + r) * ldy + m0 + i] = acc[r];
+        for (int l = 0; l < T::LOADS; ++l) {
+            const int r8 = (wave * T::LOADS + l) * 8;    // first of the load's rows
+            if (r8 < T::BM) mx_load_lds(wbuf, voff + r8 * pitch + step * 128, codes + (buf * T::ROWS + r8) * 8);
+            else mx_load_lds(xbuf, voff + (r8 - T::BM) * pitch + step * 128, codes + (buf * T::ROWS + r8) * 8);
+        }
+    };
+    const int sr = min((int)threadIdx.x, T::ROWS - 1);
+    const uint8_t* const sp = sr < T::BM ? ws + (long)min(m0 + sr, m - 1) * kb : xs + (long)min(n0 + sr - T::BM, n - 1) * kb;
+    // A row's last step is its last eight bytes, those of the step before shifted
+    // out: by trim, once the bytes have come.
+    const auto load_bytes = [&](int step) {
+        if (kb >= kMxStep) return *reinterpret_cast<const u64_b*>(sp + min(step * kMxStep, kb - kMxStep));
+        uint64_t v = 0;
+        for (int j = 0; j < kb; ++j) v |= (uint64_t)sp[j] << (8 * j);
+        return v;
+    };
+    const auto trim = [&](uint64_t v, int step) { return kb >= kMxStep ? v >> (8 * max(step * kMxStep - (kb - kMxStep), 0)) : v; };
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+
+    const int steps = (kb + kMxStep - 1) / kMxStep;
+    load_codes(0, 0);
+    bytes[sr] = trim(load_bytes(0), 0);
+    mx_meet();
+    for (int t = 0; t < steps; ++t) {
+        const int buf = t & 1;
+        uint64_t next = 0;
+        if (t + 1 < steps) {
+            load_codes(t + 1, buf ^ 1);
+            next = load_bytes(t + 1);
+        }
+        // h's byte of each pair in bytes 0 and 2
+        u32x2 sa[MT], sb[NT];
+#pragma unroll
+        for (int a = 0; a < MT; ++a) sa[a] = __builtin_bit_cast(u32x2, bytes[buf * T::ROWS + (wm * MT + a) * 32 + i]) >> (8 * h);
+#pragma unroll
+        for (int b = 0; b < NT; ++b) sb[b] = __builtin_bit_cast(u32x2, bytes[buf * T::ROWS + T::BM + (wn * NT + b) * 32 + i]) >> (8 * h);
+        // fragments one quarter of a step ahead
+        u32x4 fa[2][MT], fb[2][NT];
+        const auto read = [&](int s) {
+            const int slot = (2 * s + h) ^ (i & 7);
+#pragma unroll
+            for (int a = 0; a < MT; ++a) fa[s & 1][a] = codes[(buf * T::ROWS + (wm * MT + a) * 32 + i) * 8 + slot];
+#pragma unroll
+            for (int b = 0; b < NT; ++b) fb[s & 1][b] = codes[(buf * T::ROWS + T::BM + (wn * NT + b) * 32 + i) * 8 + slot];
+        };
+        const auto multiply = [&](auto sub) {
+            constexpr int s = decltype(sub)::value, pick = 2 * (s & 1);
+            if (s < 3) read(s + 1);
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int b = 0; b < NT; ++b)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        mx_frag(fb[s & 1][b]), mx_frag(fa[s & 1][a]), acc[a][b], kFp4, kFp4, pick, sb[b][s >> 1], pick, sa[a][s >> 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        read(0);
+        multiply(std::integral_constant<int, 0>{});
+        multiply(std::integral_constant<int, 1>{});
+        multiply(std::integral_constant<int, 2>{});
+        multiply(std::integral_constant<int, 3>{});
+        bytes[(buf ^ 1) * T::ROWS + sr] = trim(next, t + 1);
+        mx_meet();
+    }
+#pragma unroll
+    for (int a = 0; a < MT; ++a) {
+        const int col = m0 + (wm * MT + a) * 32 + i;
+        if (col >= m) continue;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            const int row = n0 + (wn * NT + b) * 32 + 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = row + 8 * (e >> 2) + (e & 3);
+                if (r < n) y[r * ldy + col] = acc[a][b][e];
+            }
+        }
+    }
 }
 
 int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, const uint8_t* xs, float* y,
@@ -225,10 +422,25 @@ int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, con
     ATLAS_REQUIRE(((uintptr_t)w & 15) == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)y & 3) == 0,
                   "gemm_mxfp4: w and x start on 16 bytes, y on 4");
     const int kb = (int)(((long)k + kMxBlock - 1) / kMxBlock);
-    const dim3 grid((m + 63L) / 64, (n + 15L) / 16);
-    ATLAS_REQUIRE(grid.y <= 65535, "gemm_mxfp4: %d rows", n);
-    hipLaunchKernelGGL(mxfp4_tile_kernel, grid, dim3(256), 0, st, reinterpret_cast<const u32x4*>(w), ws,
-                       reinterpret_cast<const u32x4*>(x), xs, y, m, n, kb, ldy);
+    ATLAS_REQUIRE(n <= 1 << 20, "gemm_mxfp4: %d rows", n);
+    const u32x4 *wv = reinterpret_cast<const u32x4*>(w), *xv = reinterpret_cast<const u32x4*>(x);
+#define MX_ROWS(MT, NT, WAVES)                                                                                        \
+    hipLaunchKernelGGL((mxfp4_rows_kernel<MT, NT, WAVES>), dim3((m + 16L * MT - 1) / (16 * MT), (n + 16L * NT - 1) / (16 * NT)), \
+                       dim3(WAVES * 64), 0, st, wv, ws, xv, xs, y, m, n, kb, ldy)
+#define MX_TILE(WM, WN, MT, NT)                                                                                       \
+    do {                                                                                                              \
+        typedef MxTile<WM, WN, MT, NT> T;                                                                             \
+        const int tm = (m + T::BM - 1) / T::BM, tn = (n + T::BN - 1) / T::BN;                                         \
+        hipLaunchKernelGGL((mxfp4_tile_kernel<WM, WN, MT, NT>), dim3((tm * tn + 7) / 8 * 8), dim3(T::WAVES * 64), T::BYTES, st, wv, \
+                           ws, xv, xs, y, m, n, kb, ldy, tm, tn);                                                     \
+    } while (0)
+    // (the tiles' buffers reach 4 GiB)
+    const bool wide = (long)m * n > 1L << 20 && kb < 1 << 20;
+    if (n <= 16) MX_ROWS(1, 1, 8);
+    else if (!wide) MX_ROWS(2, 2, 8);
+    else MX_TILE(2, 2, 2, 2);
+#undef MX_ROWS
+#undef MX_TILE
     ATLAS_LAUNCH_CHECK("gemm_mxfp4");
     return ATLAS_OK;
 }

@@ -69,6 +69,15 @@ __device__ __forceinline__ float quad_max(float v) {
     return v;
 }
 
+// the operand of a matrix instruction with scales: 32 codes of a lane, in the
+// lower half of the registers that its widest format takes
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+constexpr int kFp4 = 4;               // the instruction's format code of E2M1
+
+__device__ __forceinline__ i32x8 mx_frag(u32x4 v) {
+    return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+}
+
 int mxfp4_quant_launch(const void* src, int src_bf16, long rows, long cols, long ld, uint8_t* data,
                        uint8_t* scales, hipStream_t st);
 int mxfp4_dequant_launch(const uint8_t* data, const uint8_t* scales, long rows, long cols, float* out,

@@ -345,7 +345,7 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
 /* Attention of the batch's query rows ([n_rows][n_heads * head_dim] f32, ld_q
  * elements apart) over the cached tokens: the row of token p sees tokens
  * max(0, p - window + 1) .. p (window 0: from the first on), scores times scale,
- * in f32 (K and V exactly as encoded; 2^-16 relative in the softmax's weights).
+ * in f32 (K and V exactly as encoded, q to 2^-20 of its block's largest value).
  * n_heads / n_kv in 1 .. 16.  One row to a sequence is decode, more are
  * (chunks of) prompts, whose K and V have to be written before.  A row that
  * sees no token gives zeros, one with an infinity or NaN in q NaN.  A token that
