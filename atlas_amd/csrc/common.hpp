@@ -22,7 +22,7 @@ int device_cu_count();         // CUs of the current device (cached)
 
 // Device scratch owned by the calling thread on the current device, for entry
 // points that are not handed a workspace (split partials of the reference-ABI
-// attention, split-K partials of the skinny GEMMs, argmax partials).  Each
+// and 4-bit attention, split-K partials of the skinny GEMMs, argmax partials).  Each
 // slot has a buffer per stream that the thread calls on.  It grows
 // stream-ordered (the old one is freed after the work already queued on its
 // stream; one that a captured call used stays for its graph) and is kept until
@@ -36,6 +36,7 @@ enum ScratchSlot {
     SCR_FUSED_CNT,      // ... its merge counters (kept at zero by the kernel)
     SCR_ATTN_CNT,       // atlas_decode_attention merge counters (kept at zero)
     SCR_SAMPLE,         // atlas_sample_device: logits copy and settings
+    SCR_KV4,            // atlas_kv4_attention_f32 split partials
     SCR_N
 };
 // A slot that must grow while its stream is being captured is refused with

@@ -178,9 +178,14 @@ struct Kv4AttnArgs {
     float* out;
     long ld_out;
     int group;                          // heads of a KV head
-    int tokens;                         // rows of a tile: 16 / group
+    int tokens;                         // rows of a tile, at most 16 / group
+    int tiles;                          // of the batch, some of them empty
     float scale;
     int window;
+    // a split tile: most blocks, columns, and [tiles][n_kv][splits][cols] partial
+    // sums (each HD elements, and maximum and sum of the weights)
+    int splits, cols;
+    float *part_o, *part_ml;
 };
 
 // E2M1 parts of q: the operands of N matrix instructions and their scale bytes.
@@ -466,48 +471,199 @@ __device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int u, int& s, in
     return true;
 }
 
-// One tile and KV head to a wave.
+// A tile's work: its rows, the lane's column, the chunks that any column sees.
+template <int HD>
+struct Kv4Tile {
+    int s, row0, rows, pos0;
+    int first, last;                    // chunks [first, last)
+    int tokens_end;                     // tokens from here on are seen by no column
+    bool mine;                          // the lane's column is one
+    int t, from, to;                    // its row of the tile; it sees tokens [from, to]
+    long head;
+
+    __device__ __forceinline__ bool set(const Kv4AttnArgs& a, int u, int kvh, int lane) {
+        if (!kv4_tile(a, u, s, row0, rows, pos0)) return false;
+        const int i = lane & 15;
+        t = i / a.group;
+        head = (long)kvh * a.group + (i - t * a.group);
+        mine = t < rows;
+        to = mine ? pos0 + t : -1;
+        from = seen_from(a, to);
+        tokens_end = min(pos0 + rows, a.c.cap);
+        first = seen_from(a, pos0) >> 5;
+        last = tokens_end > 0 ? (tokens_end + 31) >> 5 : 0;
+        return true;
+    }
+
+    __device__ __forceinline__ static int seen_from(const Kv4AttnArgs& a, int pos) {
+        return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
+    }
+
+    // a chunk of which not every column sees every token
+    __device__ __forceinline__ bool masked(const Kv4AttnArgs& a, int chunk) const {
+        return chunk * 32 + 31 > pos0 || chunk * 32 < seen_from(a, pos0 + rows - 1);
+    }
+
+    // The bytes of a chunk's page and head, or null: no page.  (Uniform.)
+    __device__ __forceinline__ const uint8_t* base(const Kv4AttnArgs& a, int chunk, int kvh) const {
+        const int page = a.c.table[(long)s * a.c.table_stride + (chunk * 32 >> a.c.page_shift)];
+        if (page < 0 || page >= a.c.n_pages) return nullptr;
+        return a.c.cache + ((long)page * a.c.n_kv + kvh) * Kv4Layout<HD>::bytes(1 << a.c.page_shift);
+    }
+};
+
+// Chunks begin, begin + step, .. below end into st, each one's bytes loaded while
+// the one before is worked on.
+template <int HD>
+__device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile<HD>& tile, int kvh, int begin, int end, int step,
+                                         const float* row, Kv4State<HD>& st, int lane) {
+    const int plen = 1 << a.c.page_shift;
+    Kv4Chunk<HD> c[2];
+    bool there[2] = {false, false};
+    const auto fetch = [&](int chunk, int b) {
+        there[b] = false;
+        if (chunk >= end) return;
+        const uint8_t* base = tile.base(a, chunk, kvh);
+        there[b] = base != nullptr;
+        if (base) c[b].load(base, chunk * 32 & (plen - 1), plen, lane);
+    };
+    fetch(begin, 0);
+    Kv4Query<HD> q;
+    q.load(row, a.scale * kLog2e, lane >> 4);
+    st.clear();
+    for (int chunk = begin; chunk < end; chunk += 2 * step)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int at = chunk + b * step;
+            fetch(at + step, b ^ 1);
+            if (there[b])
+                st.add(c[b], q, at * 32, tile.masked(a, at), tile.from, tile.to, tile.tokens_end - at * 32, lane);
+        }
+    st.l += __shfl_xor(st.l, 16, 64);
+    st.l += __shfl_xor(st.l, 32, 64);
+}
+
+// block -> (tile, KV head): consecutive blocks run on different XCDs, so each takes
+// a run of the heads' tiles and its L2 the heads' tokens
+__device__ __forceinline__ bool kv4_place(int block, int tiles, int n_kv, int& u, int& kvh) {
+    const int per = (tiles * n_kv + 7) / 8, at = (block & 7) * per + (block >> 3);
+    if ((block >> 3) >= per || at >= tiles * n_kv) return false;
+    kvh = at / tiles;
+    u = at - kvh * tiles;
+    return true;
+}
+
+// Prompts: a tile and KV head to a wave, the last tiles (the longest) first.
 template <int HD>
 __global__ __launch_bounds__(64) void kv4_attention_kernel(Kv4AttnArgs a) {
-    typedef Kv4Layout<HD> L;
-    const int lane = threadIdx.x, i = lane & 15, g = lane >> 4, kvh = blockIdx.y;
-    int s, row0, rows, pos0;
-    if (!kv4_tile(a, blockIdx.x, s, row0, rows, pos0)) return;
-    // the lane's column: row t, head h of the group
-    const int t = i / a.group, h = i - t * a.group;
-    const bool mine = t < rows;
-    const long head = (long)kvh * a.group + h;
-    const int to = mine ? pos0 + t : -1;
-    const int from = a.window > 0 ? max(to - a.window + 1, 0) : 0;
-    Kv4Query<HD> q;
-    q.load(mine ? a.q + (row0 + t) * a.ld_q + head * HD : nullptr, a.scale * kLog2e, g);
+    const int lane = threadIdx.x, g = lane >> 4;
+    int u, kvh;
+    if (!kv4_place(blockIdx.x, a.tiles, a.c.n_kv, u, kvh)) return;
+    Kv4Tile<HD> tile;
+    if (!tile.set(a, a.tiles - 1 - u, kvh, lane)) return;
     Kv4State<HD> st;
-    st.clear();
-    const int last = min(pos0 + rows, a.c.cap);          // tokens [begin, last) are seen by some row
-    const int begin = a.window > 0 ? max(pos0 - a.window + 1, 0) : 0;
-    const int all_from = a.window > 0 ? max(pos0 + rows - a.window, 0) : 0;
-    const int plen = 1 << a.c.page_shift;
-    for (int first = begin & ~31; first < last; first += 32) {
-        const int page = a.c.table[(long)s * a.c.table_stride + (first >> a.c.page_shift)];
-        if (page < 0 || page >= a.c.n_pages) continue;
-        const uint8_t* base = a.c.cache + ((long)page * a.c.n_kv + kvh) * L::bytes(plen);
-        Kv4Chunk<HD> c;
-        c.load(base, first & (plen - 1), plen, lane);
-        const bool masked = first < all_from || first + 31 > pos0;
-        st.add(c, q, first, masked, from, to, last - first, lane);
-    }
-    float l = st.l;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (!mine) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;          // a row that has seen nothing is zero
-    float* o = a.out + (row0 + t) * a.ld_out + head * HD;
+    const float* row = tile.mine ? a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD : nullptr;
+    kv4_scan<HD>(a, tile, kvh, tile.first, tile.last, 1, row, st, lane);
+    if (!tile.mine) return;
+    const float inv = st.l == 0.f ? 0.f : 1.f / st.l;    // a row that has seen nothing is zero
+    float* o = a.out + (tile.row0 + tile.t) * a.ld_out + tile.head * HD;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < Kv4State<HD>::J; j += 4)
             *reinterpret_cast<f32x4*>(o + (4 * g + r) * (HD / 16) + j) =
                 f32x4{st.o[j][r] * inv, st.o[j + 1][r] * inv, st.o[j + 2][r] * inv, st.o[j + 3][r] * inv};
+}
+
+// Few tiles: a tile's chunks are split over up to a.splits blocks of WAVES waves.
+// A block's waves take every WAVES-th chunk of its run and join their sums in LDS;
+// the blocks' meet in kv4_join_kernel.
+constexpr int kKv4Waves = 4;
+constexpr int kKv4MinChunks = 2 * kKv4Waves;            // of a block, where a tile has more
+
+__device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int chunks) {
+    return max((chunks + a.splits - 1) / a.splits, kKv4MinChunks);
+}
+
+template <int HD>
+__global__ __launch_bounds__(kKv4Waves * 64) void kv4_attention_split_kernel(Kv4AttnArgs a) {
+    __shared__ float part_o[kKv4Waves][16][HD + 4];
+    __shared__ float part_m[kKv4Waves][16], part_l[kKv4Waves][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4, u = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
+    Kv4Tile<HD> tile;
+    if (!tile.set(a, u, kvh, lane)) return;
+    const int run = kv4_run(a, tile.last - tile.first), begin = tile.first + split * run;
+    if (split > 0 && begin >= tile.last) return;
+    const bool alone = tile.first + run >= tile.last;
+    Kv4State<HD> st;
+    const float* row = tile.mine ? a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD : nullptr;
+    kv4_scan<HD>(a, tile, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves, row, st, lane);
+    if (tile.mine) {
+        if (g == 0) {
+            part_m[wave][i] = st.m;
+            part_l[wave][i] = st.l;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < Kv4State<HD>::J; j += 4)
+                *reinterpret_cast<f32x4*>(&part_o[wave][i][(4 * g + r) * (HD / 16) + j]) =
+                    f32x4{st.o[j][r], st.o[j + 1][r], st.o[j + 2][r], st.o[j + 3][r]};
+    }
+    __syncthreads();
+    // four elements of a column to a thread
+    const int cols = tile.rows * a.group;
+    for (int e = threadIdx.x; e < cols * (HD / 4); e += kKv4Waves * 64) {
+        const int c = e / (HD / 4), d = e % (HD / 4) * 4;
+        float m = part_m[0][c];
+#pragma unroll
+        for (int w = 1; w < kKv4Waves; ++w) m = fmaxf(m, part_m[w][c]);
+        float l = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kKv4Waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(part_m[w][c] - m);
+            l += f * part_l[w][c];
+            o += f * *reinterpret_cast<const f32x4*>(&part_o[w][c][d]);
+        }
+        if (alone) {
+            const int t = c / a.group;
+            float* to = a.out + (tile.row0 + t) * a.ld_out + ((long)kvh * a.group + c - t * a.group) * HD + d;
+            *reinterpret_cast<f32x4*>(to) = o * (l == 0.f ? 0.f : 1.f / l);
+        } else {
+            const long at = (((long)u * a.c.n_kv + kvh) * a.splits + split) * a.cols + c;
+            *reinterpret_cast<f32x4*>(a.part_o + at * HD + d) = o;
+            if (d == 0) {
+                a.part_ml[2 * at] = m;
+                a.part_ml[2 * at + 1] = l;
+            }
+        }
+    }
+}
+
+// Joins a tile's runs: a column to a block, four of its elements to a thread.
+template <int HD>
+__global__ __launch_bounds__(HD / 4) void kv4_join_kernel(Kv4AttnArgs a) {
+    const int u = blockIdx.x / a.cols, c = blockIdx.x % a.cols, kvh = blockIdx.y, d = threadIdx.x * 4;
+    Kv4Tile<HD> tile;
+    if (!tile.set(a, u, kvh, 0)) return;
+    const int run = kv4_run(a, tile.last - tile.first), n = (tile.last - tile.first + run - 1) / run;
+    if (n <= 1 || c >= tile.rows * a.group) return;
+    const long at = (((long)u * a.c.n_kv + kvh) * a.splits) * a.cols + c;
+    float m = kKv4Floor;
+    for (int s = 0; s < n; ++s) m = fmaxf(m, a.part_ml[2 * (at + (long)s * a.cols)]);
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < n; ++s) {
+        const long p = at + (long)s * a.cols;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - m);
+        l += f * a.part_ml[2 * p + 1];
+        o += f * *reinterpret_cast<const f32x4*>(a.part_o + p * HD + d);
+    }
+    const int t = c / a.group;
+    float* to = a.out + (tile.row0 + t) * a.ld_out + ((long)kvh * a.group + c - t * a.group) * HD + d;
+    *reinterpret_cast<f32x4*>(to) = o * (l == 0.f ? 0.f : 1.f / l);
 }
 
 // ---- launches ---------------------------------------------------------------------
@@ -536,7 +692,7 @@ static int kv4_args(const char* who, const atlas_kv4_cache& c, const atlas_kv4_b
                   b.max_len);
     ATLAS_REQUIRE(b.row_starts || b.n_rows == b.n_seqs, "%s: %d rows of %d sequences need row_starts", who, b.n_rows,
                   b.n_seqs);
-    ATLAS_REQUIRE(b.n_seqs <= 1 << 22 && b.n_rows <= 1 << 22, "%s: %d rows of %d sequences", who, b.n_rows, b.n_seqs);
+    ATLAS_REQUIRE(b.n_seqs <= 1 << 20 && b.n_rows <= 1 << 20, "%s: %d rows of %d sequences", who, b.n_rows, b.n_seqs);
     a = Kv4Args{};
     a.n_rows = b.n_seqs == 0 ? 0 : b.n_rows;
     if (a.n_rows == 0) return ATLAS_OK;
@@ -611,14 +767,50 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     a.out = out;
     a.ld_out = ld_out;
     a.group = n_heads / c.n_kv;
-    a.tokens = 16 / a.group;
+    a.tokens = b.row_starts ? 16 / a.group : 1;
+    a.tiles = b.row_starts ? a.c.n_rows / a.tokens + a.c.n_seqs : a.c.n_rows;
     a.scale = scale;
     a.window = window;
-    const long tiles = b.row_starts ? (long)a.c.n_rows / a.tokens + a.c.n_seqs : a.c.n_rows;
-    const dim3 grid((unsigned)tiles, c.n_kv);
-    if (c.head_dim == 64) hipLaunchKernelGGL(kv4_attention_kernel<64>, grid, dim3(64), 0, st, a);
-    else if (c.head_dim == 128) hipLaunchKernelGGL(kv4_attention_kernel<128>, grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL(kv4_attention_kernel<256>, grid, dim3(64), 0, st, a);
+    a.cols = a.tokens * a.group;
+    // chunks of the longest row
+    int64_t chunks = b.max_len > 0 ? std::min(b.max_len, a.c.cap) : a.c.cap;
+    if (window > 0) chunks = std::min<int64_t>(chunks, (int64_t)window + a.tokens);
+    chunks = (chunks + 62) / 32;
+    const long units = (long)a.tiles * c.n_kv;
+    ATLAS_REQUIRE(units <= 1 << 25, "kv4_attention: %d tiles of rows and %d KV heads", a.tiles, c.n_kv);
+    const int cus = device_cu_count();
+    // Eight waves to a CU without splitting: only few rows to a sequence, whose
+    // lengths may differ, are split further, where one may be long.
+    if (units >= 8L * cus && (chunks <= 128 || b.n_rows >= 2 * b.n_seqs)) {
+        const dim3 grid((unsigned)((units + 7) / 8 * 8));
+        if (c.head_dim == 64) hipLaunchKernelGGL(kv4_attention_kernel<64>, grid, dim3(64), 0, st, a);
+        else if (c.head_dim == 128) hipLaunchKernelGGL(kv4_attention_kernel<128>, grid, dim3(64), 0, st, a);
+        else hipLaunchKernelGGL(kv4_attention_kernel<256>, grid, dim3(64), 0, st, a);
+        ATLAS_LAUNCH_CHECK("kv4_attention");
+        return ATLAS_OK;
+    }
+    // four blocks to a CU, at most 128 chunks to a block and 256 MB of partial sums
+    const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
+    const long want = std::max<long>((4L * cus + units - 1) / units, (chunks + 127) / 128);
+    const long most = std::min<long>({64L, (long)((chunks + kKv4MinChunks - 1) / kKv4MinChunks), (long)((256u << 20) / each)});
+    a.splits = (int)std::max(1L, std::min(want, most));
+    if (a.splits > 1) {
+        const size_t n = (size_t)units * a.splits * a.cols;
+        void* p = nullptr;
+        if ((rc = thread_scratch(SCR_KV4, each * a.splits, &p))) return rc;
+        a.part_o = static_cast<float*>(p);
+        a.part_ml = a.part_o + n * c.head_dim;
+    }
+    const dim3 grid(a.tiles, c.n_kv, a.splits), join((unsigned)((long)a.tiles * a.cols), c.n_kv);
+#define KV4_SPLIT(HD)                                                                                                 \
+    do {                                                                                                              \
+        hipLaunchKernelGGL(kv4_attention_split_kernel<HD>, grid, dim3(kKv4Waves * 64), 0, st, a);                     \
+        if (a.splits > 1) hipLaunchKernelGGL(kv4_join_kernel<HD>, join, dim3(HD / 4), 0, st, a);                      \
+    } while (0)
+    if (c.head_dim == 64) KV4_SPLIT(64);
+    else if (c.head_dim == 128) KV4_SPLIT(128);
+    else KV4_SPLIT(256);
+#undef KV4_SPLIT
     ATLAS_LAUNCH_CHECK("kv4_attention");
     return ATLAS_OK;
 }
