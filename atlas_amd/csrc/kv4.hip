@@ -184,7 +184,7 @@ struct Kv4AttnArgs {
     int window;
     // a split tile: most blocks, columns, and [tiles][n_kv][splits][cols] partial
     // sums (each HD elements, and maximum and sum of the weights)
-    int splits, cols;
+    int splits, cols, blocks;
     float *part_o, *part_ml;
 };
 
@@ -198,7 +198,7 @@ struct Kv4Query {
     u32x4 q[N];
     int byte[N];
 
-    // the column's row of q times scale (null: zeros); lane group g has block g
+    // the column's row of q times scale; lane group g has block g
     // of an instruction's four
     __device__ __forceinline__ void load(const float* row, float scale, int g) {
         constexpr int H = HD == 256 ? 2 : 1;
@@ -208,8 +208,7 @@ struct Kv4Query {
             float x[32], mx = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                if (row) v = *reinterpret_cast<const f32x4*>(row + h * 128 + blk * 32 + j * 4);
+                const f32x4 v = *reinterpret_cast<const f32x4*>(row + h * 128 + blk * 32 + j * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     x[4 * j + i] = v[i] * scale;
@@ -477,7 +476,7 @@ struct Kv4Tile {
     int s, row0, rows, pos0;
     int first, last;                    // chunks [first, last)
     int tokens_end;                     // tokens from here on are seen by no column
-    bool mine;                          // the lane's column is one
+    bool mine;                          // the lane's column is one (others repeat the last row)
     int t, from, to;                    // its row of the tile; it sees tokens [from, to]
     long head;
 
@@ -487,7 +486,8 @@ struct Kv4Tile {
         t = i / a.group;
         head = (long)kvh * a.group + (i - t * a.group);
         mine = t < rows;
-        to = mine ? pos0 + t : -1;
+        t = min(t, rows - 1);
+        to = pos0 + t;
         from = seen_from(a, to);
         tokens_end = min(pos0 + rows, a.c.cap);
         first = seen_from(a, pos0) >> 5;
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(64) void kv4_attention_kernel(Kv4AttnArgs a) {
     Kv4Tile<HD> tile;
     if (!tile.set(a, a.tiles - 1 - u, kvh, lane)) return;
     Kv4State<HD> st;
-    const float* row = tile.mine ? a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD : nullptr;
+    const float* row = a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD;
     kv4_scan<HD>(a, tile, kvh, tile.first, tile.last, 1, row, st, lane);
     if (!tile.mine) return;
     const float inv = st.l == 0.f ? 0.f : 1.f / st.l;    // a row that has seen nothing is zero
@@ -575,14 +575,37 @@ __global__ __launch_bounds__(64) void kv4_attention_kernel(Kv4AttnArgs a) {
                 f32x4{st.o[j][r] * inv, st.o[j + 1][r] * inv, st.o[j + 2][r] * inv, st.o[j + 3][r] * inv};
 }
 
-// Few tiles: a tile's chunks are split over up to a.splits blocks of WAVES waves.
-// A block's waves take every WAVES-th chunk of its run and join their sums in LDS;
-// the blocks' meet in kv4_join_kernel.
+// Few tiles: a tile's chunks are split over up to a.splits blocks of WAVES waves, in
+// runs of the same length for every tile.  A block's waves take every WAVES-th chunk
+// of its run and join their sums in LDS; the blocks' meet in kv4_join_kernel.
 constexpr int kKv4Waves = 4;
-constexpr int kKv4MinChunks = 2 * kKv4Waves;            // of a block, where a tile has more
+constexpr int kKv4MinRun = 2 * kKv4Waves;               // chunks of a block, where a tile has more
 
-__device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int chunks) {
-    return max((chunks + a.splits - 1) / a.splits, kKv4MinChunks);
+// The run's length: what the batch's chunks, as its lengths are now, come to over
+// a.blocks blocks; no tile has more than a.splits runs.  (Every lane of a wave
+// takes part.)
+__device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int lane) {
+    int all = 0, most = 0;
+    for (int s = lane; s < a.c.n_seqs; s += 64) {
+        const int n = min(max(a.c.lens[s], 0), a.c.cap);
+        int tiles = 1, tokens = n;
+        if (a.c.starts) {
+            const int rows = a.c.starts[s + 1] - a.c.starts[s];
+            tiles = rows <= 0 ? 0 : min((rows + a.tokens - 1) / a.tokens, a.tiles);
+        }
+        if (a.window > 0 && tokens - a.tokens > a.window) tokens = a.window + a.tokens;
+        const int chunks = tiles ? (tokens + 62) >> 5 : 0;
+        all += min(tiles * (long)chunks, 1L << 24);
+        most = max(most, chunks);
+    }
+    // (sums of up to 2^20 sequences stay below 2^31 as far as it matters: a longer run is still right)
+    for (int o = 32; o >= 1; o >>= 1) {
+        all = min(all, 1 << 29) + min(__shfl_xor(all, o, 64), 1 << 29);
+        most = max(most, __shfl_xor(most, o, 64));
+    }
+    const long run = ((long)all * a.c.n_kv + a.blocks - 1) / a.blocks;
+    const int n = max(max((int)min(run, 1L << 26), kKv4MinRun), (most + a.splits - 1) / a.splits);
+    return __builtin_amdgcn_readfirstlane(n);
 }
 
 template <int HD>
@@ -593,11 +616,11 @@ __global__ __launch_bounds__(kKv4Waves * 64) void kv4_attention_split_kernel(Kv4
     const int i = lane & 15, g = lane >> 4, u = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
     Kv4Tile<HD> tile;
     if (!tile.set(a, u, kvh, lane)) return;
-    const int run = kv4_run(a, tile.last - tile.first), begin = tile.first + split * run;
+    const int run = kv4_run(a, lane), begin = tile.first + split * run;
     if (split > 0 && begin >= tile.last) return;
     const bool alone = tile.first + run >= tile.last;
     Kv4State<HD> st;
-    const float* row = tile.mine ? a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD : nullptr;
+    const float* row = a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD;
     kv4_scan<HD>(a, tile, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves, row, st, lane);
     if (tile.mine) {
         if (g == 0) {
@@ -642,25 +665,36 @@ __global__ __launch_bounds__(kKv4Waves * 64) void kv4_attention_split_kernel(Kv4
     }
 }
 
-// Joins a tile's runs: a column to a block, four of its elements to a thread.
+// Joins a tile's runs: a wave to a column, four of its elements to a lane; the
+// lanes beyond take other runs (HD 64: every fourth, 128: every second).
 template <int HD>
-__global__ __launch_bounds__(HD / 4) void kv4_join_kernel(Kv4AttnArgs a) {
-    const int u = blockIdx.x / a.cols, c = blockIdx.x % a.cols, kvh = blockIdx.y, d = threadIdx.x * 4;
+__global__ __launch_bounds__(64) void kv4_join_kernel(Kv4AttnArgs a) {
+    constexpr int E = HD / 4, G = 64 / E;
+    const int lane = threadIdx.x, u = blockIdx.x / a.cols, c = blockIdx.x % a.cols, kvh = blockIdx.y, d = lane % E * 4;
     Kv4Tile<HD> tile;
     if (!tile.set(a, u, kvh, 0)) return;
-    const int run = kv4_run(a, tile.last - tile.first), n = (tile.last - tile.first + run - 1) / run;
+    const int run = kv4_run(a, lane), n = (tile.last - tile.first + run - 1) / run;
     if (n <= 1 || c >= tile.rows * a.group) return;
     const long at = (((long)u * a.c.n_kv + kvh) * a.splits) * a.cols + c;
-    float m = kKv4Floor;
-    for (int s = 0; s < n; ++s) m = fmaxf(m, a.part_ml[2 * (at + (long)s * a.cols)]);
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; ++s) {
-        const long p = at + (long)s * a.cols;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - m);
-        l += f * a.part_ml[2 * p + 1];
-        o += f * *reinterpret_cast<const f32x4*>(a.part_o + p * HD + d);
+    // lane s has run s (at most 64 of them)
+    float m = kKv4Floor, l = 0.f;
+    if (lane < n) {
+        m = a.part_ml[2 * (at + (long)lane * a.cols)];
+        l = a.part_ml[2 * (at + (long)lane * a.cols) + 1];
     }
+    const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
+    l = wave_sum(f * l);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < n; s += G) {
+        const int r = s + lane / E;
+        const float w = __shfl(f, r, 64);
+        if (r < n) o += w * *reinterpret_cast<const f32x4*>(a.part_o + (at + (long)r * a.cols) * HD + d);
+    }
+    for (int x = E; x < 64; x <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+    if (lane >= E) return;
     const int t = c / a.group;
     float* to = a.out + (tile.row0 + t) * a.ld_out + ((long)kvh * a.group + c - t * a.group) * HD + d;
     *reinterpret_cast<f32x4*>(to) = o * (l == 0.f ? 0.f : 1.f / l);
@@ -789,10 +823,13 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
         ATLAS_LAUNCH_CHECK("kv4_attention");
         return ATLAS_OK;
     }
-    // four blocks to a CU, at most 128 chunks to a block and 256 MB of partial sums
+    // As many blocks as run at once (their registers leave 3, 2 or 1 to a CU).  Of
+    // sequences of different lengths the longest get up to twice an even share of
+    // runs.  At most 128 chunks to a run, 64 runs to a tile, 256 MB of partial sums.
+    a.blocks = cus * (c.head_dim == 64 ? 3 : c.head_dim == 128 ? 2 : 1);
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
-    const long want = std::max<long>((4L * cus + units - 1) / units, (chunks + 127) / 128);
-    const long most = std::min<long>({64L, (long)((chunks + kKv4MinChunks - 1) / kKv4MinChunks), (long)((256u << 20) / each)});
+    const long want = std::max<long>(a.blocks * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
+    const long most = std::min<long>({64L, (long)((chunks + kKv4MinRun - 1) / kKv4MinRun), (long)((256u << 20) / each)});
     a.splits = (int)std::max(1L, std::min(want, most));
     if (a.splits > 1) {
         const size_t n = (size_t)units * a.splits * a.cols;
@@ -805,7 +842,7 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
 #define KV4_SPLIT(HD)                                                                                                 \
     do {                                                                                                              \
         hipLaunchKernelGGL(kv4_attention_split_kernel<HD>, grid, dim3(kKv4Waves * 64), 0, st, a);                     \
-        if (a.splits > 1) hipLaunchKernelGGL(kv4_join_kernel<HD>, join, dim3(HD / 4), 0, st, a);                      \
+        if (a.splits > 1) hipLaunchKernelGGL(kv4_join_kernel<HD>, join, dim3(64), 0, st, a);                          \
     } while (0)
     if (c.head_dim == 64) KV4_SPLIT(64);
     else if (c.head_dim == 128) KV4_SPLIT(128);
