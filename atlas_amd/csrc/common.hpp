@@ -37,6 +37,7 @@ enum ScratchSlot {
     SCR_ATTN_CNT,       // atlas_decode_attention merge counters (kept at zero)
     SCR_SAMPLE,         // atlas_sample_device: logits copy and settings
     SCR_KV4,            // atlas_kv4_attention_f32 split partials
+    SCR_KV4_CNT,        // ... its counters of finished blocks (kept at zero by the kernel)
     SCR_N
 };
 // A slot that must grow while its stream is being captured is refused with

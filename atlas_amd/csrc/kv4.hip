@@ -186,137 +186,153 @@ struct Kv4AttnArgs {
     // sums (each HD elements, and maximum and sum of the weights)
     int splits, cols, blocks;
     float *part_o, *part_ml;
+    int* counters;                      // [tiles][n_kv] blocks that are done, zero between calls
 };
 
 // E2M1 parts of q: the operands of N matrix instructions and their scale bytes.
 // HD 64: an instruction's 128 is two parts of the 64 (K's blocks given twice).
 // HD 256: part p's two halves are instructions 2p and 2p + 1.
-template <int HD>
+// A block's threads take the tile's columns apart together, eight elements to a
+// thread, and share the parts through LDS.
+template <int HD, int COLS>
 struct Kv4Query {
     static constexpr int PARTS = HD == 64 ? 8 : 7;
     static constexpr int N = HD == 64 ? 4 : HD == 128 ? 7 : 14;
+    static constexpr int EIGHTS = HD / 8, ITEMS = COLS * EIGHTS;
+    struct Shared {
+        uint32_t part[PARTS][COLS][EIGHTS];
+        int top[COLS][HD / 32];                            // scale byte of the first part, kMxNan: not finite
+    };
     u32x4 q[N];
     int byte[N];
 
-    // the column's row of q times scale; lane group g has block g
-    // of an instruction's four
-    __device__ __forceinline__ void load(const float* row, float scale, int g) {
-        constexpr int H = HD == 256 ? 2 : 1;
-        const int blk = HD == 64 ? g & 1 : g;
+    // what a thread of THREADS takes apart: items of eight elements of a column
+    template <int THREADS>
+    struct Mine {
+        static constexpr int PER = (ITEMS + THREADS - 1) / THREADS;
+        f32x4 x[PER][2];
+
+        __device__ __forceinline__ void fetch(const Kv4AttnArgs& a, int row0, int cols, int kvh) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            float x[32], mx = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(row + h * 128 + blk * 32 + j * 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[4 * j + i] = v[i] * scale;
-                    mx = fmaxf(mx, mx_mag(x[4 * j + i]));
-                }
+            for (int j = 0; j < PER; ++j) {
+                const int t = threadIdx.x + j * THREADS, c = t / EIGHTS, row = c / a.group;
+                if (c >= cols) continue;
+                const float* p = a.q + (row0 + row) * a.ld_q + ((long)kvh * a.group + c - row * a.group) * HD + t % EIGHTS * 8;
+                x[j][0] = reinterpret_cast<const f32x4*>(p)[0];
+                x[j][1] = reinterpret_cast<const f32x4*>(p)[1];
             }
-            const int e = (int)(__float_as_uint(mx) >> 23), top = max(e - 1, 0);
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                const int b = max(top - 3 * p, 0);
-                const u32x4 w = part(x, mx_scale(b));
-                const int f = HD == 64 ? p / 2 : HD == 128 ? p : 2 * p + h;
-                if (HD != 64 || (p & 1) == 0) {
-                    q[f] = w;
-                    byte[f] = b;
-                } else if (g >= 2) {
-                    q[f] = w;
-                    byte[f] = b;
-                }
-            }
-            if (e == 255) byte[HD == 256 ? h : 0] = kMxNan;    // an infinity or NaN: so is every score
         }
+
+        __device__ __forceinline__ void split(float scale, int cols, Shared& to) const {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int t = threadIdx.x + j * THREADS;
+                if (t < cols * EIGHTS) Kv4Query::split(x[j], scale, t, to);
+            }
+        }
+    };
+
+    __device__ __forceinline__ static void split(const f32x4 (&v)[2], float scale, int t, Shared& to) {
+        const int c = t / EIGHTS, e = t % EIGHTS;
+        float x[8], mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = v[i >> 2][i & 3] * scale;
+            mx = fmaxf(mx, mx_mag(x[i]));
+        }
+        mx = quad_max(mx);                               // of the block's four threads
+        const int field = (int)(__float_as_uint(mx) >> 23), top = max(field - 1, 0);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            const float s = mx_scale(max(top - 3 * p, 0));
+            const uint32_t w = mx_round8(x, s);
+            float y[8];
+            mx_decode8(w, s, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] -= y[i];
+            to.part[p][c][e] = w;
+        }
+        if ((e & 3) == 0) to.top[c][e >> 2] = field == 255 ? kMxNan : top;
     }
 
-    // x rounded to E2M1; x keeps the rest
-    __device__ __forceinline__ static u32x4 part(float (&x)[32], float scale) {
-        u32x4 to;
+    // the lane's column c, lane group g
+    __device__ __forceinline__ void load(const Shared& from, int c, int g) {
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            uint32_t w = 0;
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d], x[8 * d + 1], scale, 0);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d + 2], x[8 * d + 3], scale, 1);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d + 4], x[8 * d + 5], scale, 2);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[8 * d + 6], x[8 * d + 7], scale, 3);
-            float y[8];
-            mx_decode8(w, scale, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[8 * d + i] -= y[i];
-            to[d] = w;
+        for (int f = 0; f < N; ++f) {
+            const int part = HD == 64 ? 2 * f + (g >> 1) : HD == 128 ? f : f >> 1;
+            const int blk = HD == 64 ? g & 1 : HD == 128 ? g : 4 * (f & 1) + g;
+            q[f] = *reinterpret_cast<const u32x4*>(&from.part[part][c][4 * blk]);
+            const int top = from.top[c][blk];
+            byte[f] = top == kMxNan ? kMxNan : max(top - 3 * part, 0);
         }
-        return to;
     }
 };
 
-// a chunk's bytes in the registers of a wave
+// K of a chunk in the registers of a wave
 template <int HD>
-struct Kv4Chunk {
-    typedef Kv4Layout<HD> L;
-    static constexpr int H = HD == 256 ? 2 : 1;          // K steps of 128 elements
-    static constexpr int VW = HD / 64 * 4;               // dwords of V
+struct Kv4K {
+    static constexpr int KB = HD / 32, H = HD == 256 ? 2 : 1;   // steps of 128 elements
     u32x4 k[H][2];                                       // [step][part t]
-    uint16_t ks[H];                                      // scale bytes of parts 0 and 1
-    uint32_t v[VW];
-    u32x2 vs;
+    uint16_t s[H];                                       // scale bytes of parts 0 and 1
 
     // base: the (page, head)'s bytes; at: the chunk's first token in the page
     __device__ __forceinline__ void load(const uint8_t* base, int at, int plen, int lane) {
-        const int i = lane & 15, g = lane >> 4;
+        const int i = lane & 15, g = lane >> 4, blk = HD == 64 ? g & 1 : g;
         const uint8_t* kp = base + (long)at * (HD / 2);
-        const uint8_t* ksp = base + L::k_scales(plen) + at * L::KB;
-        const uint8_t* vp = base + L::v_codes(plen) + (long)at * (HD / 2);
-        const uint8_t* vsp = base + L::v_scales(plen) + at * L::KB;
-        const int blk = HD == 64 ? g & 1 : g;
+        const uint8_t* sp = base + Kv4Layout<HD>::k_scales(plen) + at * KB;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
                 k[h][t] = *reinterpret_cast<const u32x4*>(kp + (2 * i + t) * (HD / 2) + h * 64 + blk * 16);
-            ks[h] = *reinterpret_cast<const uint16_t*>(ksp + (i >> 2) * (8 * L::KB) + (4 * h + blk) * 8 + 2 * (i & 3));
+            s[h] = *reinterpret_cast<const uint16_t*>(sp + (i >> 2) * (8 * KB) + (4 * h + blk) * 8 + 2 * (i & 3));
+        }
+    }
+
+    // scores of tokens 8g + j of the chunk in the lane's column
+    template <typename Q>
+    __device__ __forceinline__ void scores(const Q& q, float (&to)[8]) const {
+        f32x4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int f = Q::N - 1; f >= 0; --f) {
+            const int h = HD == 256 ? f & 1 : 0;
+            // (the argument before a scale picks its byte)
+            d[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(k[h][0]), mx_frag(q.q[f]), d[0], kFp4, kFp4, 0, s[h],
+                                                                    0, q.byte[f]);
+            d[1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(k[h][1]), mx_frag(q.q[f]), d[1], kFp4, kFp4, 1, s[h],
+                                                                    0, q.byte[f]);
         }
 #pragma unroll
-        for (int w = 0; w < VW / 4; ++w) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(vp + (g * 16 + i) * (8 * L::KB) + 16 * w);
-            v[4 * w] = x.x; v[4 * w + 1] = x.y; v[4 * w + 2] = x.z; v[4 * w + 3] = x.w;
-        }
-        vs = *reinterpret_cast<const u32x2*>(vsp + (g * L::KB + i * (HD / 16) / 32) * 8);
+        for (int j = 0; j < 8; ++j) to[j] = d[j & 1][j >> 1];
     }
 };
 
-// Blocks of V that read as NaN (scale bytes past kMxMaxByte), found in sc, the
-// scale bytes of the lane's eight tokens: returns sc without those bytes, so that
-// the product leaves the columns that do not see their tokens as they were, and
-// in z the rows 4g + r of O^T (bit r) that have to be NaN in the lane's column,
-// which sees [from, to].  Rare, so its loops stay rolled.
+// V of a chunk
 template <int HD>
-__device__ __forceinline__ u32x4 kv4_nan_blocks(uint32_t s0, uint32_t s1, int first, int from, int to) {
-    constexpr int KB = HD / 32;
-    const int g = (threadIdx.x & 63) >> 4;
-    uint32_t rows = 0;
-#pragma unroll 1
-    for (int b = 0; b < KB; ++b)
-#pragma unroll 1
-        for (int j = 0; j < 32; ++j) {
-            // lane (j / 8, first group of block b) has token j's byte
-            const int lane = (j >> 3) * 16 + b * (16 / KB);
-            const uint32_t w0 = __shfl(s0, lane, 64), w1 = __shfl(s1, lane, 64);
-            const uint32_t byte = ((j & 4 ? w1 : w0) >> (8 * (j & 3))) & 255u;
-            const int key = first + j;
-            if ((int)byte <= kMxMaxByte || key < from || key > to) continue;
-            for (int r = 0; r < 4; ++r)
-                if ((4 * g + r) * (HD / 16) / 32 == b) rows |= 1u << r;
+struct Kv4V {
+    static constexpr int KB = HD / 32, W = HD / 16;      // dwords of a lane
+    uint32_t v[W];
+    u32x2 s;
+
+    __device__ __forceinline__ void load(const uint8_t* base, int at, int plen, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        const uint8_t* vp = base + Kv4Layout<HD>::v_codes(plen) + (long)at * (HD / 2);
+        const uint8_t* sp = base + Kv4Layout<HD>::v_scales(plen) + at * KB;
+#pragma unroll
+        for (int w = 0; w < W / 4; ++w) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(vp + (g * 16 + i) * (8 * KB) + 16 * w);
+            v[4 * w] = x.x; v[4 * w + 1] = x.y; v[4 * w + 2] = x.z; v[4 * w + 3] = x.w;
         }
-    for (int j = 0; j < 4; ++j) {
-        if ((int)((s0 >> (8 * j)) & 255u) > kMxMaxByte) s0 &= ~(255u << (8 * j));
-        if ((int)((s1 >> (8 * j)) & 255u) > kMxMaxByte) s1 &= ~(255u << (8 * j));
+        s = *reinterpret_cast<const u32x2*>(sp + (g * KB + i * (HD / 16) / 32) * 8);
     }
-    return u32x4{s0, s1, rows, 0u};
+};
+
+// scale bytes past kMxMaxByte, whose blocks read as NaN: their high bits
+__device__ __forceinline__ uint32_t kv4_nan_bytes(uint32_t w) {
+    return w & ((w & 0x7F7F7F7Fu) + 0x03030303u) & 0x80808080u;
 }
+
+typedef bf16x8 Kv4Weights[3];
 
 template <int HD>
 struct Kv4State {
@@ -331,57 +347,8 @@ struct Kv4State {
         l = 0.f;
     }
 
-    // V's code dword and byte of elements 2e, 2e+1 of token j
-    template <int J8, int E>
-    __device__ __forceinline__ static uint32_t v_pair(const Kv4Chunk<HD>& c, float s) {
-        constexpr int at = J8 * (HD / 32) + E;
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.v[at / 4], s, at % 4));
-    }
-
-    template <int E>
-    __device__ __forceinline__ void pv(const Kv4Chunk<HD>& c, const float (&s)[8], const bf16x8 (&p)[3]) {
-        const uint32_t w[8] = {v_pair<0, E>(c, s[0]), v_pair<1, E>(c, s[1]), v_pair<2, E>(c, s[2]), v_pair<3, E>(c, s[3]),
-                               v_pair<4, E>(c, s[4]), v_pair<5, E>(c, s[5]), v_pair<6, E>(c, s[6]), v_pair<7, E>(c, s[7])};
-        u32x4 even, odd;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
-            odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
-        }
-        const bf16x8 a = __builtin_bit_cast(bf16x8, even), b = __builtin_bit_cast(bf16x8, odd);
-#pragma unroll
-        for (int j = 2; j >= 0; --j) {
-            o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[j], o[2 * E], 0, 0, 0);
-            o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p[j], o[2 * E + 1], 0, 0, 0);
-        }
-    }
-
-    // A chunk's tokens first .. first + 31.  masked: not every column sees all of
-    // them; the lane's column sees [from, to].  live: tokens of the chunk that
-    // the sequence has (the bytes of others are not looked at).
-    __device__ __forceinline__ void add(Kv4Chunk<HD>& c, const Kv4Query<HD>& q, int first, bool masked, int from,
-                                        int to, int live, int lane) {
-        const int g = lane >> 4;
-        f32x4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int f = Kv4Query<HD>::N - 1; f >= 0; --f) {
-            const int h = HD == 256 ? f & 1 : 0;
-            // (the argument before a scale picks its byte)
-            d[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(c.k[h][0]), mx_frag(q.q[f]), d[0], kFp4, kFp4, 0,
-                                                                    c.ks[h], 0, q.byte[f]);
-            d[1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(c.k[h][1]), mx_frag(q.q[f]), d[1], kFp4, kFp4, 1,
-                                                                    c.ks[h], 0, q.byte[f]);
-        }
-        float s[8];                                      // token first + 8 g + j
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = d[j & 1][j >> 1];
-        if (masked) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = first + 8 * g + j;
-                if (key < from || key > to) s[j] = -__builtin_inff();
-            }
-        }
+    // the weights of 8 scores, in three bf16 parts; maximum and sum move on
+    __device__ __forceinline__ void weigh(const float (&s)[8], u32x4 (&part)[3]) {
         float top = s[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
@@ -394,7 +361,6 @@ struct Kv4State {
 #pragma unroll
             for (int j = 0; j < J; ++j) o[j] *= down;
         }
-        u32x4 part[3];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float a = __builtin_amdgcn_exp2f(s[2 * j] - m), b = __builtin_amdgcn_exp2f(s[2 * j + 1] - m);
@@ -405,41 +371,77 @@ struct Kv4State {
             part[1][j] = bf16_rne2(a, b);
             part[2][j] = bf16_rne2(a - bf16_lo(part[1][j]), b - bf16_hi(part[1][j]));
         }
-        // tokens that are not there get the smallest scale: their p is zero, and
-        // whatever their bytes are the product is too
-        uint32_t sc[2] = {c.vs.x, c.vs.y};
+    }
+};
+
+// V of a chunk as the matrix instructions take it
+template <int HD>
+struct Kv4Values {
+    const Kv4V<HD>& c;
+    float s[8];                                          // the tokens' scales
+    bool nans;                                           // there were blocks that read as NaN
+
+    // Tokens that are not there (the chunk has `live`) get the smallest scale:
+    // their p is zero, and so, whatever their bytes are, is the product.  Blocks
+    // that read as NaN are left out the same way, and seen to at the end.
+    __device__ __forceinline__ Kv4Values(const Kv4V<HD>& v, int live, int g) : c(v), nans(false) {
+        uint32_t sc[2] = {v.s.x, v.s.y};
         if (live < 32) {
             const int n = min(max(live - 8 * g, 0), 8);
             sc[0] &= n >= 4 ? ~0u : (1u << (8 * n)) - 1u;
             sc[1] &= n >= 8 ? ~0u : n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1u;
         }
-        const uint32_t bad = (((~sc[0] - 0x03030303u) & sc[0]) | ((~sc[1] - 0x03030303u) & sc[1])) & 0x80808080u;
-        if (__any(bad != 0)) {
-            const u32x4 x = kv4_nan_blocks<HD>(sc[0], sc[1], first, from, to);
-            sc[0] = x.x;
-            sc[1] = x.y;
+        const uint32_t bad[2] = {kv4_nan_bytes(sc[0]), kv4_nan_bytes(sc[1])};
+        if (__any((bad[0] | bad[1]) != 0)) {
+            nans = true;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (x.z >> r & 1u)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) o[j][r] = __builtin_nanf("");
+            for (int w = 0; w < 2; ++w) sc[w] &= ~((bad[w] >> 7) * 255u);
         }
-        float vsc[8];
+        // (the conversion takes the exponent field of its scale and nothing else)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vsc[j] = mx_scale((sc[j >> 2] >> (8 * (j & 3))) & 255u);
-        const bf16x8 p[3] = {__builtin_bit_cast(bf16x8, part[0]), __builtin_bit_cast(bf16x8, part[1]),
-                             __builtin_bit_cast(bf16x8, part[2])};
-        pv<0>(c, vsc, p);
-        pv<1>(c, vsc, p);
+        for (int j = 0; j < 8; ++j) s[j] = __uint_as_float((j & 3) == 3 ? sc[j >> 2] >> 1 : sc[j >> 2] << (23 - 8 * (j & 3)));
+    }
+
+    // elements 2e, 2e+1 of token j as bf16
+    template <int J8, int E>
+    __device__ __forceinline__ uint32_t at() const {
+        constexpr int byte = J8 * (HD / 32) + E;
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.v[byte / 4], s[J8], byte % 4));
+    }
+
+    // O += V^T P in elements 2e, 2e + 1 of the groups, for each column tile
+    template <int E, int CT>
+    __device__ __forceinline__ void pair(const Kv4Weights (&p)[CT], Kv4State<HD> (&st)[CT]) const {
+        const uint32_t w[8] = {at<0, E>(), at<1, E>(), at<2, E>(), at<3, E>(), at<4, E>(), at<5, E>(), at<6, E>(), at<7, E>()};
+        u32x4 even, odd;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+            odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+        }
+        const bf16x8 a = __builtin_bit_cast(bf16x8, even), b = __builtin_bit_cast(bf16x8, odd);
+#pragma unroll
+        for (int j = 2; j >= 0; --j)
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                st[t].o[2 * E] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, p[t][j], st[t].o[2 * E], 0, 0, 0);
+                st[t].o[2 * E + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, p[t][j], st[t].o[2 * E + 1], 0, 0, 0);
+            }
+    }
+
+    template <int CT>
+    __device__ __forceinline__ void add(const Kv4Weights (&p)[CT], Kv4State<HD> (&st)[CT]) const {
+        pair<0, CT>(p, st);
+        pair<1, CT>(p, st);
         if constexpr (HD >= 128) {
-            pv<2>(c, vsc, p);
-            pv<3>(c, vsc, p);
+            pair<2, CT>(p, st);
+            pair<3, CT>(p, st);
         }
         if constexpr (HD >= 256) {
-            pv<4>(c, vsc, p);
-            pv<5>(c, vsc, p);
-            pv<6>(c, vsc, p);
-            pv<7>(c, vsc, p);
+            pair<4, CT>(p, st);
+            pair<5, CT>(p, st);
+            pair<6, CT>(p, st);
+            pair<7, CT>(p, st);
         }
     }
 };
@@ -470,25 +472,21 @@ __device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int u, int& s, in
     return true;
 }
 
-// A tile's work: its rows, the lane's column, the chunks that any column sees.
-template <int HD>
+// A tile's work: its rows and columns (16 CT at most), the chunks that any column
+// sees, and the first pages of its sequence, one to a lane.
+// Where rows and heads are few, a tile's columns are given SLOTS times, each time
+// for other chunks: a wave then takes the scores of SLOTS chunks one after the
+// other, each into its columns, before it weighs them all at once.
 struct Kv4Tile {
-    int s, row0, rows, pos0;
+    int s, row0, rows, cols, pos0;
     int first, last;                    // chunks [first, last)
     int tokens_end;                     // tokens from here on are seen by no column
-    bool mine;                          // the lane's column is one (others repeat the last row)
-    int t, from, to;                    // its row of the tile; it sees tokens [from, to]
-    long head;
+    int pages;
 
-    __device__ __forceinline__ bool set(const Kv4AttnArgs& a, int u, int kvh, int lane) {
+    __device__ __forceinline__ bool set(const Kv4AttnArgs& a, int u, int lane) {
         if (!kv4_tile(a, u, s, row0, rows, pos0)) return false;
-        const int i = lane & 15;
-        t = i / a.group;
-        head = (long)kvh * a.group + (i - t * a.group);
-        mine = t < rows;
-        t = min(t, rows - 1);
-        to = pos0 + t;
-        from = seen_from(a, to);
+        pages = lane < a.c.table_stride ? a.c.table[(long)s * a.c.table_stride + lane] : -1;
+        cols = rows * a.group;
         tokens_end = min(pos0 + rows, a.c.cap);
         first = seen_from(a, pos0) >> 5;
         last = tokens_end > 0 ? (tokens_end + 31) >> 5 : 0;
@@ -503,44 +501,178 @@ struct Kv4Tile {
     __device__ __forceinline__ bool masked(const Kv4AttnArgs& a, int chunk) const {
         return chunk * 32 + 31 > pos0 || chunk * 32 < seen_from(a, pos0 + rows - 1);
     }
+};
 
-    // The bytes of a chunk's page and head, or null: no page.  (Uniform.)
-    __device__ __forceinline__ const uint8_t* base(const Kv4AttnArgs& a, int chunk, int kvh) const {
-        const int page = a.c.table[(long)s * a.c.table_stride + (chunk * 32 >> a.c.page_shift)];
-        if (page < 0 || page >= a.c.n_pages) return nullptr;
-        return a.c.cache + ((long)page * a.c.n_kv + kvh) * Kv4Layout<HD>::bytes(1 << a.c.page_shift);
+// a lane's column of column tile ct
+template <int SLOTS>
+struct Kv4Column {
+    bool mine;                          // it is one (others repeat one of them)
+    int slot, col;
+    int from, to;                       // it sees tokens [from, to]
+
+    __device__ __forceinline__ void set(const Kv4AttnArgs& a, const Kv4Tile& tile, int ct, int lane) {
+        const int i = 16 * ct + (lane & 15);
+        slot = SLOTS > 1 ? i / tile.cols : 0;
+        col = min(i - slot * tile.cols, tile.cols - 1);
+        mine = SLOTS > 1 ? slot < SLOTS : i < tile.cols;
+        to = tile.pos0 + col / a.group;
+        from = Kv4Tile::seen_from(a, to);
     }
 };
 
-// Chunks begin, begin + step, .. below end into st, each one's bytes loaded while
-// the one before is worked on.
-template <int HD>
-__device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile<HD>& tile, int kvh, int begin, int end, int step,
-                                         const float* row, Kv4State<HD>& st, int lane) {
-    const int plen = 1 << a.c.page_shift;
-    Kv4Chunk<HD> c[2];
-    bool there[2] = {false, false};
-    const auto fetch = [&](int chunk, int b) {
-        there[b] = false;
-        if (chunk >= end) return;
-        const uint8_t* base = tile.base(a, chunk, kvh);
-        there[b] = base != nullptr;
-        if (base) c[b].load(base, chunk * 32 & (plen - 1), plen, lane);
-    };
-    fetch(begin, 0);
-    Kv4Query<HD> q;
-    q.load(row, a.scale * kLog2e, lane >> 4);
-    st.clear();
-    for (int chunk = begin; chunk < end; chunk += 2 * step)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int at = chunk + b * step;
-            fetch(at + step, b ^ 1);
-            if (there[b])
-                st.add(c[b], q, at * 32, tile.masked(a, at), tile.from, tile.to, tile.tokens_end - at * 32, lane);
+// Chunks begin, begin + step, .. below end into st.  K and V of a chunk are loaded
+// BUF (1 or 2) chunks ahead, page numbers 64 at a time.
+// Every thread of a block of THREADS comes here, for the query.
+template <int HD, int SLOTS, int CT, int BUF, int THREADS>
+__device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& tile, const Kv4Column<SLOTS> (&col)[CT], int kvh,
+                                         int begin, int end, int step,
+                                         const typename Kv4Query<HD, 16 * CT>::template Mine<THREADS>& mine,
+                                         typename Kv4Query<HD, 16 * CT>::Shared& shared, Kv4State<HD> (&st)[CT], int lane) {
+    typedef Kv4Query<HD, 16 * CT> Q;
+    const int g = lane >> 4, plen = 1 << a.c.page_shift, n = end > begin ? (end - begin + step - 1) / step : 0;
+    const int* const table = a.c.table + (long)tile.s * a.c.table_stride;
+    const long head = (long)kvh * Kv4Layout<HD>::bytes(plen), page_bytes = a.c.n_kv * Kv4Layout<HD>::bytes(plen);
+    // pages window .. window + 63 of the sequence
+    int pages = tile.pages, window = 0;
+    const auto page = [&](int chunk) {
+        const int at = chunk * 32 >> a.c.page_shift;
+        if ((unsigned)(at - window) >= 64u) {
+            window = at;
+            pages = at + lane < a.c.table_stride ? table[at + lane] : -1;
         }
-    st.l += __shfl_xor(st.l, 16, 64);
-    st.l += __shfl_xor(st.l, 32, 64);
+        const int p = __builtin_amdgcn_readlane(pages, at - window);
+        return p < a.c.n_pages ? p : -1;
+    };
+    Kv4K<HD> k[BUF];
+    Kv4V<HD> v[BUF];
+    int k_page[BUF], v_page[BUF];
+    const auto fetch_k = [&](int t, int b) {
+        k_page[b] = t < n ? page(begin + t * step) : -1;
+        if (k_page[b] >= 0) k[b].load(a.c.cache + k_page[b] * page_bytes + head, (begin + t * step) * 32 & (plen - 1), plen, lane);
+    };
+    const auto fetch_v = [&](int t, int b) {
+        v_page[b] = t < n ? page(begin + t * step) : -1;
+        if (v_page[b] >= 0) v[b].load(a.c.cache + v_page[b] * page_bytes + head, (begin + t * step) * 32 & (plen - 1), plen, lane);
+    };
+#pragma unroll
+    for (int b = 0; b < BUF; ++b) {
+        fetch_k(b, b);
+        fetch_v(b, b);
+    }
+    mine.split(a.scale * kLog2e, tile.cols, shared);
+    __syncthreads();
+    Q q[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        q[c].load(shared, col[c].col, g);
+        st[c].clear();
+    }
+    bool nans = false;
+    // (loops stay rolled but for the two buffers: a wave may have few chunks, and
+    // then the instructions themselves have to come from memory)
+    constexpr int ROUNDS = SLOTS == 1 ? BUF : 1;
+    static_assert(SLOTS == 1 || BUF == 2, "slots go in twos");
+#pragma unroll 1
+    for (int t0 = 0; t0 < n; t0 += SLOTS * ROUNDS)
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            float s[CT][8];
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[c][j] = -__builtin_inff();
+            bool cut = false;
+            const auto take = [&](int j, int b) {
+                const int t = t0 + r + j;
+                if (t < n) cut = cut || tile.masked(a, begin + t * step);
+                if (k_page[b] >= 0)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) {
+                        float d[8];
+                        k[b].scores(q[c], d);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s[c][e] = SLOTS == 1 || col[c].slot == j ? d[e] : s[c][e];
+                    }
+                fetch_k(t + BUF, b);
+            };
+            const auto give = [&](const u32x4 (&part)[CT][3], int j, int b) {
+                const int t = t0 + r + j;
+                if (v_page[b] >= 0) {
+                    Kv4Weights p[CT];                    // other slots' weights are not of this chunk
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) {
+                            u32x4 x;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) x[w] = SLOTS == 1 || col[c].slot == j ? part[c][e][w] : 0u;
+                            p[c][e] = __builtin_bit_cast(bf16x8, x);
+                        }
+                    const Kv4Values<HD> values(v[b], tile.tokens_end - (begin + t * step) * 32, g);
+                    values.template add<CT>(p, st);
+                    nans = nans || values.nans;
+                }
+                fetch_v(t + BUF, b);
+            };
+            if constexpr (SLOTS == 1) take(0, r);
+            else
+#pragma unroll 1
+                for (int j = 0; j < SLOTS; j += 2) {
+                    take(j, 0);
+                    take(j + 1, 1);
+                }
+            if (cut)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const int first = (begin + (t0 + r + col[c].slot) * step) * 32 + 8 * g;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (first + j < col[c].from || first + j > col[c].to) s[c][j] = -__builtin_inff();
+                }
+            u32x4 part[CT][3];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) st[c].weigh(s[c], part[c]);
+            if constexpr (SLOTS == 1) give(part, 0, r);
+            else
+#pragma unroll 1
+                for (int j = 0; j < SLOTS; j += 2) {
+                    give(part, j, 0);
+                    give(part, j + 1, 1);
+                }
+        }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        st[c].l += __shfl_xor(st[c].l, 16, 64);
+        st[c].l += __shfl_xor(st[c].l, 32, 64);
+    }
+    // Blocks of V that read as NaN: the columns that see their token get NaN in the
+    // block's elements.  (Rare: the scale bytes are read again.)
+    if (nans) {
+        uint32_t rows[CT] = {};                          // rows 4g + r of O^T in the lane's column
+#pragma unroll 1
+        for (int t = 0; t < n; ++t) {
+            const int first = (begin + t * step) * 32, p = table[first >> a.c.page_shift];
+            if (p < 0 || p >= a.c.n_pages) continue;
+            const uint8_t* sp = a.c.cache + p * page_bytes + head + Kv4Layout<HD>::v_scales(plen) + (first & (plen - 1)) * (HD / 32);
+#pragma unroll 1
+            for (int e = 0; e < HD; ++e) {               // byte e: token e / (HD / 4) * 8 + e % 8, block e / 8 % (HD / 32)
+                const int key = first + e / (HD / 4) * 8 + e % 8, blk = e / 8 % (HD / 32);
+                if (key >= tile.tokens_end || sp[e] <= kMxMaxByte) continue;
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+                    if (key >= col[c].from && key <= col[c].to)
+                        for (int x = 0; x < 4; ++x)
+                            if ((4 * g + x) * (HD / 16) / 32 == blk) rows[c] |= 1u << x;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (rows[c] >> x & 1u)
+#pragma unroll
+                    for (int j = 0; j < Kv4State<HD>::J; ++j) st[c].o[j][x] = __builtin_nanf("");
+    }
 }
 
 // block -> (tile, KV head): consecutive blocks run on different XCDs, so each takes
@@ -553,151 +685,189 @@ __device__ __forceinline__ bool kv4_place(int block, int tiles, int n_kv, int& u
     return true;
 }
 
-// Prompts: a tile and KV head to a wave, the last tiles (the longest) first.
-template <int HD>
-__global__ __launch_bounds__(64) void kv4_attention_kernel(Kv4AttnArgs a) {
-    const int lane = threadIdx.x, g = lane >> 4;
-    int u, kvh;
-    if (!kv4_place(blockIdx.x, a.tiles, a.c.n_kv, u, kvh)) return;
-    Kv4Tile<HD> tile;
-    if (!tile.set(a, a.tiles - 1 - u, kvh, lane)) return;
-    Kv4State<HD> st;
-    const float* row = a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD;
-    kv4_scan<HD>(a, tile, kvh, tile.first, tile.last, 1, row, st, lane);
-    if (!tile.mine) return;
-    const float inv = st.l == 0.f ? 0.f : 1.f / st.l;    // a row that has seen nothing is zero
-    float* o = a.out + (tile.row0 + tile.t) * a.ld_out + tile.head * HD;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < Kv4State<HD>::J; j += 4)
-            *reinterpret_cast<f32x4*>(o + (4 * g + r) * (HD / 16) + j) =
-                f32x4{st.o[j][r] * inv, st.o[j + 1][r] * inv, st.o[j + 2][r] * inv, st.o[j + 3][r] * inv};
-}
-
-// Few tiles: a tile's chunks are split over up to a.splits blocks of WAVES waves, in
-// runs of the same length for every tile.  A block's waves take every WAVES-th chunk
-// of its run and join their sums in LDS; the blocks' meet in kv4_join_kernel.
+// A tile and KV head to up to a.splits blocks, in runs of the same length for every
+// tile.  A block's waves take every fourth chunk of its run and join their sums in
+// LDS; the blocks' are joined by the one that ends last.
 constexpr int kKv4Waves = 4;
 constexpr int kKv4MinRun = 2 * kKv4Waves;               // chunks of a block, where a tile has more
 
+// all lanes' sum or largest value, of integers
+template <bool MAX>
+__device__ __forceinline__ int wave_int(int v) {
+    const auto step = [&](int x) { v = MAX ? max(v, x) : v + x; };
+    step(__builtin_amdgcn_update_dpp(MAX ? v : 0, v, 0xB1, 0xF, 0xF, false));
+    step(__builtin_amdgcn_update_dpp(MAX ? v : 0, v, 0x4E, 0xF, 0xF, false));
+    step(__builtin_amdgcn_update_dpp(MAX ? v : 0, v, 0x141, 0xF, 0xF, false));
+    step(__builtin_amdgcn_update_dpp(MAX ? v : 0, v, 0x140, 0xF, 0xF, false));
+    step(__builtin_amdgcn_update_dpp(MAX ? v : 0, v, 0x142, 0xA, 0xF, false));
+    step(__builtin_amdgcn_update_dpp(MAX ? v : 0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 // The run's length: what the batch's chunks, as its lengths are now, come to over
-// a.blocks blocks; no tile has more than a.splits runs.  (Every lane of a wave
-// takes part.)
+// a.blocks blocks, a last run half full on average; no tile has more than a.splits
+// runs.  (Every lane of a wave takes part.)
 __device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int lane) {
-    int all = 0, most = 0;
+    if (a.splits == 1) return 1 << 26;
+    int all = 0, most = 0;              // (all: capped, so that 64 lanes' sum fits; longer runs are right as well)
     for (int s = lane; s < a.c.n_seqs; s += 64) {
-        const int n = min(max(a.c.lens[s], 0), a.c.cap);
-        int tiles = 1, tokens = n;
+        int tokens = min(max(a.c.lens[s], 0), a.c.cap), tiles = 1;
         if (a.c.starts) {
-            const int rows = a.c.starts[s + 1] - a.c.starts[s];
-            tiles = rows <= 0 ? 0 : min((rows + a.tokens - 1) / a.tokens, a.tiles);
+            const long rows = (long)a.c.starts[s + 1] - a.c.starts[s];
+            tiles = rows <= 0 ? 0 : (int)min((rows + a.tokens - 1) / a.tokens, (long)a.tiles);
         }
         if (a.window > 0 && tokens - a.tokens > a.window) tokens = a.window + a.tokens;
         const int chunks = tiles ? (tokens + 62) >> 5 : 0;
-        all += min(tiles * (long)chunks, 1L << 24);
+        all = (int)min(all + (long)tiles * chunks, 1L << 24);
         most = max(most, chunks);
     }
-    // (sums of up to 2^20 sequences stay below 2^31 as far as it matters: a longer run is still right)
-    for (int o = 32; o >= 1; o >>= 1) {
-        all = min(all, 1 << 29) + min(__shfl_xor(all, o, 64), 1 << 29);
-        most = max(most, __shfl_xor(most, o, 64));
-    }
-    const long run = ((long)all * a.c.n_kv + a.blocks - 1) / a.blocks;
-    const int n = max(max((int)min(run, 1L << 26), kKv4MinRun), (most + a.splits - 1) / a.splits);
-    return __builtin_amdgcn_readfirstlane(n);
+    const long run = ((long)wave_int<false>(all) * a.c.n_kv + a.blocks - 1) / a.blocks;
+    return max(max((int)min(run, 1L << 26), kKv4MinRun), (wave_int<true>(most) + a.splits - 1) / a.splits);
 }
 
-template <int HD>
-__global__ __launch_bounds__(kKv4Waves * 64) void kv4_attention_split_kernel(Kv4AttnArgs a) {
-    __shared__ float part_o[kKv4Waves][16][HD + 4];
-    __shared__ float part_m[kKv4Waves][16], part_l[kKv4Waves][16];
+// partial sums past this XCD's L2 and back (agent scope)
+__device__ __forceinline__ void kv4_put(float* p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void kv4_get(const float* p, float& a, float& b) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    a = __uint_as_float((uint32_t)v);
+    b = __uint_as_float((uint32_t)(v >> 32));
+}
+
+template <int HD, int COLS>
+struct Kv4Shared {
+    union {
+        typename Kv4Query<HD, COLS>::Shared q;
+        float o[kKv4Waves][COLS][HD + 4];                // the waves' sums
+        float f[64][COLS];                               // the runs' factors
+    };
+    f32x4 red[kKv4Waves * 64];
+    float m[kKv4Waves][COLS], l[kKv4Waves][COLS];
+    float sum[COLS];                                     // the columns' sums of weights
+    int last;
+};
+
+template <int HD, int SLOTS, int CT>
+__global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
+    __shared__ Kv4Shared<HD, 16 * CT> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i = lane & 15, g = lane >> 4, u = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-    Kv4Tile<HD> tile;
-    if (!tile.set(a, u, kvh, lane)) return;
+    const int i = lane & 15, g = lane >> 4, split = blockIdx.y;
+    int u, kvh;
+    if (!kv4_place(blockIdx.x, a.tiles, a.c.n_kv, u, kvh)) return;
+    u = a.tiles - 1 - u;                                 // a prompt's last tiles, the longest, first
+    Kv4Tile tile;
+    if (!tile.set(a, u, lane)) return;
+    typename Kv4Query<HD, 16 * CT>::template Mine<kKv4Waves * 64> mine;
+    mine.fetch(a, tile.row0, tile.cols, kvh);
     const int run = kv4_run(a, lane), begin = tile.first + split * run;
     if (split > 0 && begin >= tile.last) return;
-    const bool alone = tile.first + run >= tile.last;
-    Kv4State<HD> st;
-    const float* row = a.q + (tile.row0 + tile.t) * a.ld_q + tile.head * HD;
-    kv4_scan<HD>(a, tile, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves, row, st, lane);
-    if (tile.mine) {
+    const int runs = max((tile.last - tile.first + run - 1) / run, 1);
+    Kv4Column<SLOTS> col[CT];
+    Kv4State<HD> st[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) col[c].set(a, tile, c, lane);
+    // (two column tiles leave registers for one chunk ahead)
+    kv4_scan<HD, SLOTS, CT, CT == 1 ? 2 : 1, kKv4Waves * 64>(a, tile, col, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves,
+                                                             mine, sh.q, st, lane);
+    __syncthreads();                                     // the query has been read
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        if (!col[c].mine) continue;
         if (g == 0) {
-            part_m[wave][i] = st.m;
-            part_l[wave][i] = st.l;
+            sh.m[wave][16 * c + i] = st[c].m;
+            sh.l[wave][16 * c + i] = st[c].l;
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int j = 0; j < Kv4State<HD>::J; j += 4)
-                *reinterpret_cast<f32x4*>(&part_o[wave][i][(4 * g + r) * (HD / 16) + j]) =
-                    f32x4{st.o[j][r], st.o[j + 1][r], st.o[j + 2][r], st.o[j + 3][r]};
+                *reinterpret_cast<f32x4*>(&sh.o[wave][16 * c + i][(4 * g + r) * (HD / 16) + j]) =
+                    f32x4{st[c].o[j][r], st[c].o[j + 1][r], st[c].o[j + 2][r], st[c].o[j + 3][r]};
     }
     __syncthreads();
     // four elements of a column to a thread
-    const int cols = tile.rows * a.group;
+    const int cols = tile.cols;
+    const long part = (((long)u * a.c.n_kv + kvh) * a.splits) * a.cols;
+    const auto store = [&](int c, int d, f32x4 o, float l) {
+        const int t = c / a.group;
+        float* to = a.out + (tile.row0 + t) * a.ld_out + ((long)kvh * a.group + c - t * a.group) * HD + d;
+        *reinterpret_cast<f32x4*>(to) = o * (l == 0.f ? 0.f : 1.f / l);   // a row that has seen nothing is zero
+    };
     for (int e = threadIdx.x; e < cols * (HD / 4); e += kKv4Waves * 64) {
         const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-        float m = part_m[0][c];
+        // of each wave and slot
+        float m = kKv4Floor, l = 0.f;
 #pragma unroll
-        for (int w = 1; w < kKv4Waves; ++w) m = fmaxf(m, part_m[w][c]);
-        float l = 0.f;
+        for (int w = 0; w < kKv4Waves; ++w)
+#pragma unroll
+            for (int x = 0; x < SLOTS; ++x) m = fmaxf(m, sh.m[w][x * cols + c]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(part_m[w][c] - m);
-            l += f * part_l[w][c];
-            o += f * *reinterpret_cast<const f32x4*>(&part_o[w][c][d]);
-        }
-        if (alone) {
-            const int t = c / a.group;
-            float* to = a.out + (tile.row0 + t) * a.ld_out + ((long)kvh * a.group + c - t * a.group) * HD + d;
-            *reinterpret_cast<f32x4*>(to) = o * (l == 0.f ? 0.f : 1.f / l);
-        } else {
-            const long at = (((long)u * a.c.n_kv + kvh) * a.splits + split) * a.cols + c;
-            *reinterpret_cast<f32x4*>(a.part_o + at * HD + d) = o;
-            if (d == 0) {
-                a.part_ml[2 * at] = m;
-                a.part_ml[2 * at + 1] = l;
-            }
-        }
-    }
-}
-
-// Joins a tile's runs: a wave to a column, four of its elements to a lane; the
-// lanes beyond take other runs (HD 64: every fourth, 128: every second).
-template <int HD>
-__global__ __launch_bounds__(64) void kv4_join_kernel(Kv4AttnArgs a) {
-    constexpr int E = HD / 4, G = 64 / E;
-    const int lane = threadIdx.x, u = blockIdx.x / a.cols, c = blockIdx.x % a.cols, kvh = blockIdx.y, d = lane % E * 4;
-    Kv4Tile<HD> tile;
-    if (!tile.set(a, u, kvh, 0)) return;
-    const int run = kv4_run(a, lane), n = (tile.last - tile.first + run - 1) / run;
-    if (n <= 1 || c >= tile.rows * a.group) return;
-    const long at = (((long)u * a.c.n_kv + kvh) * a.splits) * a.cols + c;
-    // lane s has run s (at most 64 of them)
-    float m = kKv4Floor, l = 0.f;
-    if (lane < n) {
-        m = a.part_ml[2 * (at + (long)lane * a.cols)];
-        l = a.part_ml[2 * (at + (long)lane * a.cols) + 1];
-    }
-    const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
-    l = wave_sum(f * l);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < n; s += G) {
-        const int r = s + lane / E;
-        const float w = __shfl(f, r, 64);
-        if (r < n) o += w * *reinterpret_cast<const f32x4*>(a.part_o + (at + (long)r * a.cols) * HD + d);
-    }
-    for (int x = E; x < 64; x <<= 1)
+        for (int w = 0; w < kKv4Waves; ++w)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
-    if (lane >= E) return;
-    const int t = c / a.group;
-    float* to = a.out + (tile.row0 + t) * a.ld_out + ((long)kvh * a.group + c - t * a.group) * HD + d;
-    *reinterpret_cast<f32x4*>(to) = o * (l == 0.f ? 0.f : 1.f / l);
+            for (int x = 0; x < SLOTS; ++x) {
+                const float f = __builtin_amdgcn_exp2f(sh.m[w][x * cols + c] - m);
+                l += f * sh.l[w][x * cols + c];
+                o += f * *reinterpret_cast<const f32x4*>(&sh.o[w][x * cols + c][d]);
+            }
+        if (runs == 1) {
+            store(c, d, o, l);
+        } else {
+            const long at = part + (long)split * a.cols + c;
+            kv4_put(a.part_o + at * HD + d, o.x, o.y);
+            kv4_put(a.part_o + at * HD + d + 2, o.z, o.w);
+            if (d == 0) kv4_put(a.part_ml + 2 * at, m, l);
+        }
+    }
+    if (runs == 1) return;
+    // The block that ends last joins the runs.  Every thread's partial sums have
+    // arrived before its block is counted, so they are there for the last one.
+    __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0)
+    __syncthreads();
+    int* const counter = a.counters + (long)u * a.c.n_kv + kvh;
+    if (threadIdx.x == 0)
+        sh.last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == runs - 1;
+    __syncthreads();
+    if (!sh.last) return;
+    // a run to a lane (at most 64 of them), a column to a wave
+    for (int c = wave; c < cols; c += kKv4Waves) {
+        float m = kKv4Floor, l = 0.f;
+        if (lane < runs) kv4_get(a.part_ml + 2 * (part + (long)lane * a.cols + c), m, l);
+        const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
+        l = wave_sum(f * l);
+        if (lane < runs) sh.f[lane][c] = f;
+        if (lane == 0) sh.sum[c] = l;
+    }
+    __syncthreads();
+    // four elements to a thread; threads beyond the columns' take other runs
+    constexpr int T = kKv4Waves * 64;
+    const int items = cols * (HD / 4), groups = max(T / items, 1), group = groups > 1 ? threadIdx.x / items : 0;
+    for (int e = threadIdx.x - group * items; e < items && group < groups; e += T) {
+        const int c = e / (HD / 4), d = e % (HD / 4) * 4;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int r = group; r < runs; r += groups) {
+            const float* p = a.part_o + (part + (long)r * a.cols + c) * HD + d;
+            float x[4];
+            kv4_get(p, x[0], x[1]);
+            kv4_get(p + 2, x[2], x[3]);
+            o += sh.f[r][c] * f32x4{x[0], x[1], x[2], x[3]};
+        }
+        if (groups == 1) store(c, d, o, sh.sum[c]);
+        else sh.red[threadIdx.x] = o;
+    }
+    if (groups > 1) {
+        __syncthreads();
+        if (threadIdx.x < items) {
+            f32x4 o = sh.red[threadIdx.x];
+            for (int x = 1; x < groups; ++x) o += sh.red[x * items + threadIdx.x];
+            store(threadIdx.x / (HD / 4), threadIdx.x % (HD / 4) * 4, o, sh.sum[threadIdx.x / (HD / 4)]);
+        }
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- launches ---------------------------------------------------------------------
@@ -793,15 +963,18 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
                   "kv4_attention: %d heads over %d KV heads (up to 16 to each)", n_heads, c.n_kv);
     ATLAS_REQUIRE(window >= 0, "kv4_attention: window %d", window);
     if (a.c.n_rows == 0) return ATLAS_OK;
-    const long wide = (long)n_heads * c.head_dim;
-    if ((rc = kv4_rows_check("kv4_attention", q, q, ld_q, wide))) return rc;
-    if ((rc = kv4_rows_check("kv4_attention", out, out, ld_out, wide))) return rc;
+    const long row = (long)n_heads * c.head_dim;
+    if ((rc = kv4_rows_check("kv4_attention", q, q, ld_q, row))) return rc;
+    if ((rc = kv4_rows_check("kv4_attention", out, out, ld_out, row))) return rc;
     a.q = q;
     a.ld_q = ld_q;
     a.out = out;
     a.ld_out = ld_out;
     a.group = n_heads / c.n_kv;
-    a.tokens = b.row_starts ? 16 / a.group : 1;
+    // 32 columns where the rows of a sequence fill more than 16 (head dim 256 has no
+    // registers for them)
+    const bool wide = c.head_dim < 256 && (long)b.n_rows * a.group > 16L * b.n_seqs;
+    a.tokens = b.row_starts ? (wide ? 32 : 16) / a.group : 1;
     a.tiles = b.row_starts ? a.c.n_rows / a.tokens + a.c.n_seqs : a.c.n_rows;
     a.scale = scale;
     a.window = window;
@@ -811,43 +984,46 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     if (window > 0) chunks = std::min<int64_t>(chunks, (int64_t)window + a.tokens);
     chunks = (chunks + 62) / 32;
     const long units = (long)a.tiles * c.n_kv;
-    ATLAS_REQUIRE(units <= 1 << 25, "kv4_attention: %d tiles of rows and %d KV heads", a.tiles, c.n_kv);
-    const int cus = device_cu_count();
-    // Eight waves to a CU without splitting: only few rows to a sequence, whose
-    // lengths may differ, are split further, where one may be long.
-    if (units >= 8L * cus && (chunks <= 128 || b.n_rows >= 2 * b.n_seqs)) {
-        const dim3 grid((unsigned)((units + 7) / 8 * 8));
-        if (c.head_dim == 64) hipLaunchKernelGGL(kv4_attention_kernel<64>, grid, dim3(64), 0, st, a);
-        else if (c.head_dim == 128) hipLaunchKernelGGL(kv4_attention_kernel<128>, grid, dim3(64), 0, st, a);
-        else hipLaunchKernelGGL(kv4_attention_kernel<256>, grid, dim3(64), 0, st, a);
-        ATLAS_LAUNCH_CHECK("kv4_attention");
-        return ATLAS_OK;
-    }
+    ATLAS_REQUIRE(units <= 1 << 23, "kv4_attention: %d tiles of rows and %d KV heads", a.tiles, c.n_kv);
     // As many blocks as run at once (their registers leave 3, 2 or 1 to a CU).  Of
     // sequences of different lengths the longest get up to twice an even share of
-    // runs.  At most 128 chunks to a run, 64 runs to a tile, 256 MB of partial sums.
-    a.blocks = cus * (c.head_dim == 64 ? 3 : c.head_dim == 128 ? 2 : 1);
+    // runs.  At most 128 chunks to a run, 32 runs to a tile (64 of that length), 256
+    // MB of partial sums.
+    const int cus = device_cu_count(), at_once = cus * (c.head_dim == 256 ? 1 : c.head_dim == 64 && !wide ? 3 : 2);
+    a.blocks = b.n_seqs > 1 ? std::max<int>(at_once - (int)std::min<long>(units / 2, at_once), at_once / 4) : at_once;
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
-    const long want = std::max<long>(a.blocks * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
-    const long most = std::min<long>({64L, (long)((chunks + kKv4MinRun - 1) / kKv4MinRun), (long)((256u << 20) / each)});
+    const long want = std::max<long>(at_once * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
+    const long most = std::min<long>({std::max<long>(32L, (chunks + 127) / 128), 64L, (long)((chunks + kKv4MinRun - 1) / kKv4MinRun),
+                                      (long)((256u << 20) / each)});
     a.splits = (int)std::max(1L, std::min(want, most));
     if (a.splits > 1) {
         const size_t n = (size_t)units * a.splits * a.cols;
-        void* p = nullptr;
+        void *p = nullptr, *cnt = nullptr;
+        if ((rc = thread_scratch(SCR_KV4_CNT, (size_t)units * sizeof(int), &cnt, true))) return rc;
         if ((rc = thread_scratch(SCR_KV4, each * a.splits, &p))) return rc;
+        a.counters = static_cast<int*>(cnt);
         a.part_o = static_cast<float*>(p);
         a.part_ml = a.part_o + n * c.head_dim;
     }
-    const dim3 grid(a.tiles, c.n_kv, a.splits), join((unsigned)((long)a.tiles * a.cols), c.n_kv);
-#define KV4_SPLIT(HD)                                                                                                 \
+    const dim3 grid((unsigned)((units + 7) / 8 * 8), a.splits);
+    // chunks that fit side by side into the 16 columns
+    const int slots = a.cols <= 2 ? 8 : a.cols <= 4 ? 4 : a.cols <= 8 ? 2 : 1;
+#define KV4_RUN(HD, SLOTS, CT)                                                                                        \
+    hipLaunchKernelGGL((kv4_attention_kernel<HD, SLOTS, CT>), grid, dim3(kKv4Waves * 64), 0, st, a)
+#define KV4_SLOTS(HD)                                                                                                 \
     do {                                                                                                              \
-        hipLaunchKernelGGL(kv4_attention_split_kernel<HD>, grid, dim3(kKv4Waves * 64), 0, st, a);                     \
-        if (a.splits > 1) hipLaunchKernelGGL(kv4_join_kernel<HD>, join, dim3(64), 0, st, a);                          \
+        if (slots == 8) KV4_RUN(HD, 8, 1);                                                                            \
+        else if (slots == 4) KV4_RUN(HD, 4, 1);                                                                       \
+        else if (slots == 2) KV4_RUN(HD, 2, 1);                                                                       \
+        else KV4_RUN(HD, 1, 1);                                                                                       \
     } while (0)
-    if (c.head_dim == 64) KV4_SPLIT(64);
-    else if (c.head_dim == 128) KV4_SPLIT(128);
-    else KV4_SPLIT(256);
-#undef KV4_SPLIT
+    if (c.head_dim == 64 && wide) KV4_RUN(64, 1, 2);
+    else if (c.head_dim == 64) KV4_SLOTS(64);
+    else if (c.head_dim == 128 && wide) KV4_RUN(128, 1, 2);
+    else if (c.head_dim == 128) KV4_SLOTS(128);
+    else KV4_SLOTS(256);
+#undef KV4_SLOTS
+#undef KV4_RUN
     ATLAS_LAUNCH_CHECK("kv4_attention");
     return ATLAS_OK;
 }

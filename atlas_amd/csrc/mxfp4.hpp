@@ -39,14 +39,19 @@ __device__ __forceinline__ float mx_mag(float v) {
     return a < __builtin_inff() ? a : __builtin_inff();
 }
 
-// codes of 8 values of a block with this scale byte (the first in the low nibble)
-__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], int byte) {
-    const float scale = mx_scale(byte);
+// codes of 8 values at this scale (the first in the low nibble)
+__device__ __forceinline__ uint32_t mx_round8(const float (&v)[8], float scale) {
     uint32_t w = 0;
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
+    return w;
+}
+
+// ... of a block with this scale byte
+__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], int byte) {
+    const uint32_t w = mx_round8(v, mx_scale(byte));
     return byte == kMxNan ? 0u : w;
 }
 
