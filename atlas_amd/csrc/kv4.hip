@@ -275,35 +275,43 @@ struct Kv4K {
     u32x4 k[H][2];                                       // [step][part t]
     uint16_t s[H];                                       // scale bytes of parts 0 and 1
 
-    // base: the (page, head)'s bytes; at: the chunk's first token in the page
-    __device__ __forceinline__ void load(const uint8_t* base, int at, int plen, int lane) {
+    // at: the chunk's first token in the page
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t page, int at, int plen, int lane) {
         const int i = lane & 15, g = lane >> 4, blk = HD == 64 ? g & 1 : g;
-        const uint8_t* kp = base + (long)at * (HD / 2);
-        const uint8_t* sp = base + Kv4Layout<HD>::k_scales(plen) + at * KB;
+        const uint32_t codes = at * (HD / 2), bytes = (uint32_t)Kv4Layout<HD>::k_scales(plen) + at * KB;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                k[h][t] = *reinterpret_cast<const u32x4*>(kp + (2 * i + t) * (HD / 2) + h * 64 + blk * 16);
-            s[h] = *reinterpret_cast<const uint16_t*>(sp + (i >> 2) * (8 * KB) + (4 * h + blk) * 8 + 2 * (i & 3));
+                k[h][t] = __builtin_amdgcn_raw_buffer_load_b128(page, (2 * i + t) * (HD / 2) + h * 64 + blk * 16, codes, 0);
+            s[h] = __builtin_amdgcn_raw_buffer_load_b16(page, (i >> 2) * (8 * KB) + (4 * h + blk) * 8 + 2 * (i & 3), bytes, 0);
         }
     }
 
-    // scores of tokens 8g + j of the chunk in the lane's column
-    template <typename Q>
-    __device__ __forceinline__ void scores(const Q& q, float (&to)[8]) const {
-        f32x4 d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    // scores of tokens 8g + j of the chunk in the lane's column of each tile; the
+    // 2 CT sums take turns, so that no instruction waits for the one before
+    template <typename Q, int CT>
+    __device__ __forceinline__ void scores(const Q (&q)[CT], float (&to)[CT][8]) const {
+        f32x4 d[CT][2];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) d[c][0] = d[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int f = Q::N - 1; f >= 0; --f) {
             const int h = HD == 256 ? f & 1 : 0;
-            // (the argument before a scale picks its byte)
-            d[0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(k[h][0]), mx_frag(q.q[f]), d[0], kFp4, kFp4, 0, s[h],
-                                                                    0, q.byte[f]);
-            d[1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(k[h][1]), mx_frag(q.q[f]), d[1], kFp4, kFp4, 1, s[h],
-                                                                    0, q.byte[f]);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                // (the argument before a scale picks its byte)
+                d[c][0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(k[h][0]), mx_frag(q[c].q[f]), d[c][0], kFp4, kFp4,
+                                                                           0, s[h], 0, q[c].byte[f]);
+                d[c][1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_frag(k[h][1]), mx_frag(q[c].q[f]), d[c][1], kFp4, kFp4,
+                                                                           1, s[h], 0, q[c].byte[f]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) to[j] = d[j & 1][j >> 1];
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[c][j] = d[c][j & 1][j >> 1];
     }
 };
 
@@ -314,18 +322,26 @@ struct Kv4V {
     uint32_t v[W];
     u32x2 s;
 
-    __device__ __forceinline__ void load(const uint8_t* base, int at, int plen, int lane) {
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t page, int at, int plen, int lane) {
         const int i = lane & 15, g = lane >> 4;
-        const uint8_t* vp = base + Kv4Layout<HD>::v_codes(plen) + (long)at * (HD / 2);
-        const uint8_t* sp = base + Kv4Layout<HD>::v_scales(plen) + at * KB;
+        const uint32_t codes = (uint32_t)Kv4Layout<HD>::v_codes(plen) + at * (HD / 2);
+        const uint32_t bytes = (uint32_t)Kv4Layout<HD>::v_scales(plen) + at * KB;
 #pragma unroll
         for (int w = 0; w < W / 4; ++w) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(vp + (g * 16 + i) * (8 * KB) + 16 * w);
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(page, (g * 16 + i) * (8 * KB) + 16 * w, codes, 0);
             v[4 * w] = x.x; v[4 * w + 1] = x.y; v[4 * w + 2] = x.z; v[4 * w + 3] = x.w;
         }
-        s = *reinterpret_cast<const u32x2*>(sp + (g * KB + i * (HD / 16) / 32) * 8);
+        s = __builtin_amdgcn_raw_buffer_load_b64(page, (g * KB + i * (HD / 16) / 32) * 8, bytes, 0);
     }
 };
+
+// The bytes of a (page, head) as a buffer.  No page: an empty one (at the cache's
+// start), whose loads come back at once with zeros.  Every load of the scan is made
+// whether its chunk is there or not: a load under a condition would have the
+// compiler wait for all of them wherever it needs one.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv4_buffer(const uint8_t* p, bool there) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, there ? 0xFFFFFFFFu : 0u, 0x00020000);
+}
 
 // scale bytes past kMxMaxByte, whose blocks read as NaN: their high bits
 __device__ __forceinline__ uint32_t kv4_nan_bytes(uint32_t w) {
@@ -365,11 +381,14 @@ struct Kv4State {
         for (int j = 0; j < 4; ++j) {
             float a = __builtin_amdgcn_exp2f(s[2 * j] - m), b = __builtin_amdgcn_exp2f(s[2 * j + 1] - m);
             l += a + b;
-            part[0][j] = bf16_rne2(a, b);
-            a -= bf16_lo(part[0][j]);
-            b -= bf16_hi(part[0][j]);
-            part[1][j] = bf16_rne2(a, b);
-            part[2][j] = bf16_rne2(a - bf16_lo(part[1][j]), b - bf16_hi(part[1][j]));
+            // two truncations and the rest: 8 + 8 + 8 bits, each p exactly
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                part[e][j] = bf16_hi2(a, b);
+                a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+                b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+            }
+            part[2][j] = bf16_hi2(a, b);
         }
     }
 };
@@ -484,7 +503,13 @@ struct Kv4Tile {
     int pages;
 
     __device__ __forceinline__ bool set(const Kv4AttnArgs& a, int u, int lane) {
-        if (!kv4_tile(a, u, s, row0, rows, pos0)) return false;
+        const bool any = kv4_tile(a, u, s, row0, rows, pos0);
+        // (all of it is the same in every lane; said here, the loops stay in scalar registers)
+        s = __builtin_amdgcn_readfirstlane(s);
+        row0 = __builtin_amdgcn_readfirstlane(row0);
+        rows = __builtin_amdgcn_readfirstlane(rows);
+        pos0 = __builtin_amdgcn_readfirstlane(pos0);
+        if (!any) return false;
         pages = lane < a.c.table_stride ? a.c.table[(long)s * a.c.table_stride + lane] : -1;
         cols = rows * a.group;
         tokens_end = min(pos0 + rows, a.c.cap);
@@ -521,7 +546,9 @@ struct Kv4Column {
 };
 
 // Chunks begin, begin + step, .. below end into st.  K and V of a chunk are loaded
-// BUF (1 or 2) chunks ahead, page numbers 64 at a time.
+// BUF chunks ahead, page numbers 64 at a time.  (The scores of SLOTS chunks follow
+// each other closely, and so do their products with V: with fewer than SLOTS
+// buffers the loads of each would be waited for.)
 // Every thread of a block of THREADS comes here, for the query.
 template <int HD, int SLOTS, int CT, int BUF, int THREADS>
 __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& tile, const Kv4Column<SLOTS> (&col)[CT], int kvh,
@@ -529,7 +556,7 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
                                          const typename Kv4Query<HD, 16 * CT>::template Mine<THREADS>& mine,
                                          typename Kv4Query<HD, 16 * CT>::Shared& shared, Kv4State<HD> (&st)[CT], int lane) {
     typedef Kv4Query<HD, 16 * CT> Q;
-    const int g = lane >> 4, plen = 1 << a.c.page_shift, n = end > begin ? (end - begin + step - 1) / step : 0;
+    const int g = lane >> 4, plen = 1 << a.c.page_shift, n = end > begin && a.c.n_pages > 0 ? (end - begin + step - 1) / step : 0;
     const int* const table = a.c.table + (long)tile.s * a.c.table_stride;
     const long head = (long)kvh * Kv4Layout<HD>::bytes(plen), page_bytes = a.c.n_kv * Kv4Layout<HD>::bytes(plen);
     // pages window .. window + 63 of the sequence
@@ -546,18 +573,25 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
     Kv4K<HD> k[BUF];
     Kv4V<HD> v[BUF];
     int k_page[BUF], v_page[BUF];
+    const auto place = [&](int t, int& there, int& at) {
+        there = t < n ? page(begin + t * step) : -1;
+        at = there >= 0 ? (begin + t * step) * 32 & (plen - 1) : 0;
+        return kv4_buffer(a.c.cache + (there >= 0 ? there * page_bytes + head : 0), there >= 0);
+    };
+    int at;
     const auto fetch_k = [&](int t, int b) {
-        k_page[b] = t < n ? page(begin + t * step) : -1;
-        if (k_page[b] >= 0) k[b].load(a.c.cache + k_page[b] * page_bytes + head, (begin + t * step) * 32 & (plen - 1), plen, lane);
+        const auto buf = place(t, k_page[b], at);
+        k[b].load(buf, at, plen, lane);
     };
     const auto fetch_v = [&](int t, int b) {
-        v_page[b] = t < n ? page(begin + t * step) : -1;
-        if (v_page[b] >= 0) v[b].load(a.c.cache + v_page[b] * page_bytes + head, (begin + t * step) * 32 & (plen - 1), plen, lane);
+        const auto buf = place(t, v_page[b], at);
+        v[b].load(buf, at, plen, lane);
     };
+    if (n > 0) {
 #pragma unroll
-    for (int b = 0; b < BUF; ++b) {
-        fetch_k(b, b);
-        fetch_v(b, b);
+        for (int b = 0; b < BUF; ++b) fetch_k(b, b);
+#pragma unroll
+        for (int b = 0; b < BUF; ++b) fetch_v(b, b);
     }
     mine.split(a.scale * kLog2e, tile.cols, shared);
     __syncthreads();
@@ -568,10 +602,8 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
         st[c].clear();
     }
     bool nans = false;
-    // (loops stay rolled but for the two buffers: a wave may have few chunks, and
-    // then the instructions themselves have to come from memory)
     constexpr int ROUNDS = SLOTS == 1 ? BUF : 1;
-    static_assert(SLOTS == 1 || BUF == 2, "slots go in twos");
+    static_assert(SLOTS == 1 || BUF == SLOTS, "a buffer to a slot");
 #pragma unroll 1
     for (int t0 = 0; t0 < n; t0 += SLOTS * ROUNDS)
 #pragma unroll
@@ -585,14 +617,14 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
             const auto take = [&](int j, int b) {
                 const int t = t0 + r + j;
                 if (t < n) cut = cut || tile.masked(a, begin + t * step);
-                if (k_page[b] >= 0)
+                if (k_page[b] >= 0) {
+                    float d[CT][8];
+                    k[b].scores(q, d);
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        float d[8];
-                        k[b].scores(q[c], d);
+                    for (int c = 0; c < CT; ++c)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) s[c][e] = SLOTS == 1 || col[c].slot == j ? d[e] : s[c][e];
-                    }
+                        for (int e = 0; e < 8; ++e) s[c][e] = SLOTS == 1 || col[c].slot == j ? d[c][e] : s[c][e];
+                }
                 fetch_k(t + BUF, b);
             };
             const auto give = [&](const u32x4 (&part)[CT][3], int j, int b) {
@@ -614,13 +646,8 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
                 }
                 fetch_v(t + BUF, b);
             };
-            if constexpr (SLOTS == 1) take(0, r);
-            else
-#pragma unroll 1
-                for (int j = 0; j < SLOTS; j += 2) {
-                    take(j, 0);
-                    take(j + 1, 1);
-                }
+#pragma unroll
+            for (int j = 0; j < SLOTS; ++j) take(j, r + j);
             if (cut)
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
@@ -632,13 +659,8 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
             u32x4 part[CT][3];
 #pragma unroll
             for (int c = 0; c < CT; ++c) st[c].weigh(s[c], part[c]);
-            if constexpr (SLOTS == 1) give(part, 0, r);
-            else
-#pragma unroll 1
-                for (int j = 0; j < SLOTS; j += 2) {
-                    give(part, j, 0);
-                    give(part, j + 1, 1);
-                }
+#pragma unroll
+            for (int j = 0; j < SLOTS; ++j) give(part, j, r + j);
         }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -704,25 +726,46 @@ __device__ __forceinline__ int wave_int(int v) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
-// The run's length: what the batch's chunks, as its lengths are now, come to over
-// a.blocks blocks, a last run half full on average; no tile has more than a.splits
-// runs.  (Every lane of a wave takes part.)
+// The run's length: the batch's chunks, as its lengths are now, over a.blocks blocks,
+// raised until the runs are no more than that (a last run is part of one, and a
+// block too many would double the time); no tile has more than a.splits runs.
+// (Every lane of a wave takes part.)
 __device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int lane) {
     if (a.splits == 1) return 1 << 26;
-    int all = 0, most = 0;              // (all: capped, so that 64 lanes' sum fits; longer runs are right as well)
-    for (int s = lane; s < a.c.n_seqs; s += 64) {
-        int tokens = min(max(a.c.lens[s], 0), a.c.cap), tiles = 1;
+    // tiles and chunks of sequence s
+    const auto size = [&](int s, int& tiles, int& chunks) {
+        int tokens = min(max(a.c.lens[s], 0), a.c.cap);
+        tiles = 1;
         if (a.c.starts) {
             const long rows = (long)a.c.starts[s + 1] - a.c.starts[s];
             tiles = rows <= 0 ? 0 : (int)min((rows + a.tokens - 1) / a.tokens, (long)a.tiles);
         }
         if (a.window > 0 && tokens - a.tokens > a.window) tokens = a.window + a.tokens;
-        const int chunks = tiles ? (tokens + 62) >> 5 : 0;
+        chunks = tiles ? (tokens + 31) >> 5 : 0;
+    };
+    // (sums capped, so that 64 lanes' fit: longer runs are right as well)
+    int all = 0, most = 0, count = 0, tiles, chunks;
+    for (int s = lane; s < a.c.n_seqs; s += 64) {
+        size(s, tiles, chunks);
         all = (int)min(all + (long)tiles * chunks, 1L << 24);
+        count = min(count + tiles, 1 << 24);
         most = max(most, chunks);
     }
-    const long run = ((long)wave_int<false>(all) * a.c.n_kv + a.blocks - 1) / a.blocks;
-    return max(max((int)min(run, 1L << 26), kKv4MinRun), (wave_int<true>(most) + a.splits - 1) / a.splits);
+    const int units = wave_int<false>(count), long_run = wave_int<true>(most);
+    const float per = (float)a.c.n_kv / a.blocks;
+    const int least = max(kKv4MinRun, (long_run + a.splits - 1) / a.splits);
+    int run = max(least, (int)ceilf(wave_int<false>(all) * per));
+    for (int turn = 0; turn < 3 && units * per <= 1.f; ++turn) {
+        count = 0;
+        for (int s = lane; s < a.c.n_seqs; s += 64) {
+            size(s, tiles, chunks);
+            count = min(count + tiles * ((chunks + run - 1) / run), 1 << 24);
+        }
+        const float over = wave_int<false>(count) * per;
+        if (over <= 1.f) break;
+        run = (int)ceilf(run * over);
+    }
+    return __builtin_amdgcn_readfirstlane(run);
 }
 
 // partial sums past this XCD's L2 and back (agent scope)
@@ -770,7 +813,8 @@ __global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attenti
 #pragma unroll
     for (int c = 0; c < CT; ++c) col[c].set(a, tile, c, lane);
     // (two column tiles leave registers for one chunk ahead)
-    kv4_scan<HD, SLOTS, CT, CT == 1 ? 2 : 1, kKv4Waves * 64>(a, tile, col, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves,
+    constexpr int BUF = CT > 1 ? 1 : SLOTS > 1 ? SLOTS : 2;
+    kv4_scan<HD, SLOTS, CT, BUF, kKv4Waves * 64>(a, tile, col, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves,
                                                              mine, sh.q, st, lane);
     __syncthreads();                                     // the query has been read
 #pragma unroll
@@ -875,8 +919,8 @@ __global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attenti
 static int kv4_check(const char* who, const atlas_kv4_cache& c) {
     ATLAS_REQUIRE(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, "%s: head_dim %d (64, 128 or 256)", who,
                   c.head_dim);
-    ATLAS_REQUIRE(c.page_len >= 32 && c.page_len <= 1 << 24 && (c.page_len & (c.page_len - 1)) == 0,
-                  "%s: page_len %d (a power of two from 32 to 2^24)", who, c.page_len);
+    ATLAS_REQUIRE(c.page_len >= 32 && c.page_len <= 1 << 22 && (c.page_len & (c.page_len - 1)) == 0,
+                  "%s: page_len %d (a power of two from 32 to 2^22)", who, c.page_len);
     ATLAS_REQUIRE(c.n_pages >= 0 && c.n_kv > 0 && c.n_kv <= 4096, "%s: %d pages, %d KV heads", who, c.n_pages, c.n_kv);
     return ATLAS_OK;
 }
@@ -990,7 +1034,7 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     // runs.  At most 128 chunks to a run, 32 runs to a tile (64 of that length), 256
     // MB of partial sums.
     const int cus = device_cu_count(), at_once = cus * (c.head_dim == 256 ? 1 : c.head_dim == 64 && !wide ? 3 : 2);
-    a.blocks = b.n_seqs > 1 ? std::max<int>(at_once - (int)std::min<long>(units / 2, at_once), at_once / 4) : at_once;
+    a.blocks = at_once;
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
     const long want = std::max<long>(at_once * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
     const long most = std::min<long>({std::max<long>(32L, (chunks + 127) / 128), 64L, (long)((chunks + kKv4MinRun - 1) / kKv4MinRun),
@@ -1007,13 +1051,12 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     }
     const dim3 grid((unsigned)((units + 7) / 8 * 8), a.splits);
     // chunks that fit side by side into the 16 columns
-    const int slots = a.cols <= 2 ? 8 : a.cols <= 4 ? 4 : a.cols <= 8 ? 2 : 1;
+    const int slots = a.cols <= 4 ? 4 : a.cols <= 8 ? 2 : 1;
 #define KV4_RUN(HD, SLOTS, CT)                                                                                        \
     hipLaunchKernelGGL((kv4_attention_kernel<HD, SLOTS, CT>), grid, dim3(kKv4Waves * 64), 0, st, a)
 #define KV4_SLOTS(HD)                                                                                                 \
     do {                                                                                                              \
-        if (slots == 8) KV4_RUN(HD, 8, 1);                                                                            \
-        else if (slots == 4) KV4_RUN(HD, 4, 1);                                                                       \
+        if (slots == 4) KV4_RUN(HD, 4, 1);                                                                            \
         else if (slots == 2) KV4_RUN(HD, 2, 1);                                                                       \
         else KV4_RUN(HD, 1, 1);                                                                                       \
     } while (0)

@@ -305,7 +305,7 @@ int atlas_gemm_mxfp4_f32(const uint8_t* w, const uint8_t* w_scales, const uint8_
  *   K codes [page_len][head_dim/2], K scales [page_len/8][head_dim/32][8],
  *   V codes [page_len/8][16][8][head_dim/32], V scales as K's
  * (V: 16 groups of head_dim/16 elements, for each of them eight tokens side by
- * side).  head_dim 64, 128 or 256; page_len a power of two, 32 to 2^24 (one page
+ * side).  head_dim 64, 128 or 256; page_len a power of two, 32 to 2^22 (one page
  * of max_seq tokens for each sequence is a cache without paging).           */
 typedef struct {
     void* data;                  /* device, 16-byte aligned, atlas_kv4_cache_bytes */

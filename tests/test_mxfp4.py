@@ -115,7 +115,7 @@ def test_cache_refusals(lib):
         return C.byref(Kv4BatchC(*[d[n] for n, _ in Kv4BatchC._fields_]))
 
     assert lib.atlas_kv4_cache_bytes(cache()) == 4 * 2 * 64 * (128 + 8)
-    bad = [dict(head_dim=96), dict(head_dim=0), dict(page_len=16), dict(page_len=48), dict(page_len=1 << 25),
+    bad = [dict(head_dim=96), dict(head_dim=0), dict(page_len=16), dict(page_len=48), dict(page_len=1 << 23),
            dict(n_pages=-1), dict(n_kv=0), dict(n_kv=5000)]
     for kw in bad:
         _refused(lib, lib.atlas_kv4_cache_bytes(cache(**kw)))
