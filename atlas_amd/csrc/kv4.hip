@@ -1031,10 +1031,13 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     ATLAS_REQUIRE(units <= 1 << 23, "kv4_attention: %d tiles of rows and %d KV heads", a.tiles, c.n_kv);
     // As many blocks as run at once (their registers leave 3, 2 or 1 to a CU).  Of
     // sequences of different lengths the longest get up to twice an even share of
-    // runs.  At most 128 chunks to a run, 32 runs to a tile (64 of that length), 256
-    // MB of partial sums.
+    // runs; the blocks beyond the others' runs come and go between the working ones,
+    // and these then fill about 3/4 of the places before some of them have to wait
+    // (24 sequences of up to 4000 tokens, heads 32/8 of 128: 26 us with that many
+    // runs, 37 with a third more of shorter ones).  At most 128 chunks to a run, 32
+    // runs to a tile (64 of that length), 256 MB of partial sums.
     const int cus = device_cu_count(), at_once = cus * (c.head_dim == 256 ? 1 : c.head_dim == 64 && !wide ? 3 : 2);
-    a.blocks = at_once;
+    a.blocks = b.n_seqs > 1 ? at_once * 3 / 4 : at_once;
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
     const long want = std::max<long>(at_once * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
     const long most = std::min<long>({std::max<long>(32L, (chunks + 127) / 128), 64L, (long)((chunks + kKv4MinRun - 1) / kKv4MinRun),
