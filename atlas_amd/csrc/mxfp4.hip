@@ -1,4 +1,5 @@
 // mxfp4.hip -- MXFP4 matrices: encoding, decoding and their product.
+#include <algorithm>
 #include <type_traits>
 #include "mxfp4.hpp"
 
@@ -408,7 +409,8 @@ __global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* _
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int r = row + 8 * (e >> 2) + (e & 3);
-                if (r < n) y[r * ldy + col] = acc[a][b][e];
+                // (past the L2, which the operands are to have)
+                if (r < n) __builtin_nontemporal_store(acc[a][b][e], &y[r * ldy + col]);
             }
         }
     }
@@ -434,11 +436,33 @@ int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, con
         hipLaunchKernelGGL((mxfp4_tile_kernel<WM, WN, MT, NT>), dim3((tm * tn + 7) / 8 * 8), dim3(T::WAVES * 64), T::BYTES, st, wv, \
                            ws, xv, xs, y, m, n, kb, ldy, tm, tn);                                                     \
     } while (0)
-    // (the tiles' buffers reach 4 GiB)
-    const bool wide = (long)m * n > 1L << 20 && kb < 1 << 20;
-    if (n <= 16) MX_ROWS(1, 1, 8);
-    else if (!wide) MX_ROWS(2, 2, 8);
-    else MX_TILE(2, 2, 2, 2);
+    // Times in us, m x n x k.  While the blocks are no more than the CUs, the one with
+    // fewer rows: it has the shorter way through k (4096 x 32 x 4096: 5.7 with 32 x 16,
+    // 6.8 with 32 x 32).  For up to 16 rows of x 16 of the weights as long as they
+    // are no more than four blocks to a CU (4096 x 13 x 4096: 4.4, 5.5 with 32; 8192:
+    // alike), then 32 (22016: 14.5 and 11.8).  32 x 32 gives way to the tiles, which read
+    // the weights for 64 rows of x or more, at 1.5 blocks to a CU (4096 x 64 x 4096: 7.1,
+    // 11.3 in tiles; 4096 x 129 x 4096: 15.5 and 11.6).
+    const long cus = device_cu_count(), m16 = (m + 15L) / 16, n16 = (n + 15L) / 16, m32 = (m + 31L) / 32, n32 = (n + 31L) / 32;
+    const bool long_rows = kb >= 1 << 20;                // more than a tile's buffers address
+    if (m16 * n16 <= cus || (n16 == 1 && m16 <= 4 * cus)) MX_ROWS(1, 1, 8);
+    else if (n16 == 1 || m32 * n16 <= cus) MX_ROWS(2, 1, 4);
+    else if (long_rows || 2 * m32 * n32 <= 3 * cus) MX_ROWS(2, 2, 8);
+    else {
+        // The tile that takes least by the time of its rounds, in us for 4096 elements: a
+        // CU does its 64 x 64 tiles at one per 6 us, and the first in 11; 128 x 128 at 14 and
+        // 16; it has one at a time of 192 x 256, 35 us, and of 256 x 256, 43.
+        // Measured in this order: 2048 x 511 x 2048 6.4 10.3 16.5 20.2; 4096 x 2047 x 4096
+        // 47 28.8 29.8 34.3; 11008 x 2047 x 4096 176 78 69 79; 8192 x 4096 x 8192 (565)
+        // 304 245 166.
+        const auto rounds = [&](long bm, long bn) { return ((m + bm - 1) / bm * ((n + bn - 1) / bn) + cus - 1) / cus; };
+        const long t64 = std::max(6 * rounds(64, 64), 11L), t128 = std::max(14 * rounds(128, 128), 16L);
+        const long t192 = 35 * rounds(192, 256), t256 = 43 * rounds(256, 256);
+        if (t64 <= std::min({t128, t192, t256})) MX_TILE(2, 2, 1, 1);
+        else if (t128 <= std::min(t192, t256)) MX_TILE(2, 2, 2, 2);
+        else if (t192 <= t256) MX_TILE(2, 4, 3, 2);
+        else MX_TILE(4, 2, 2, 4);
+    }
 #undef MX_ROWS
 #undef MX_TILE
     ATLAS_LAUNCH_CHECK("gemm_mxfp4");

@@ -121,6 +121,13 @@ def test_gemm_shapes(m, n, k, ld):
     _gemm(m, n, k, ld)
 
 
+@pytest.mark.parametrize("k", [32, 100, 288, 1056])
+@pytest.mark.parametrize("m,n", [(20001, 16), (2050, 63), (2050, 129), (1500, 600), (4100, 1030), (22001, 501), (11000, 1030)])
+def test_gemm_tiles(m, n, k):
+    """Products of every size of tile, with ragged ends of each."""
+    _gemm(m, n, k, ld=m + 3)
+
+
 def test_gemm_scales_apart():
     """Scales that leave nothing of some blocks beside others, up to the ends of f32."""
     for spread in (4.0, 12.0):
