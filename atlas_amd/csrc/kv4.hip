@@ -631,26 +631,26 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
     };
     Kv4K<HD> k[BUF];
     Kv4V<HD> v[BUF];
-    int k_page[BUF], v_page[BUF];
-    const auto place = [&](int t, int& there, int& at) {
-        there = t < n ? page(begin + t * step) : -1;
-        at = there >= 0 ? (begin + t * step) * 32 & (plen - 1) : 0;
-        return kv4_buffer(a.c.cache + (there >= 0 ? there * page_bytes + head : 0), there >= 0);
-    };
-    int at;
+    // where a buffer's chunk is: K's, and V's from when K's next one is on its way
+    bool k_there[BUF], v_there[BUF];
+    __amdgpu_buffer_rsrc_t from[BUF];
+    int at[BUF];
     const auto fetch_k = [&](int t, int b) {
-        const auto buf = place(t, k_page[b], at);
-        k[b].load(buf, at, plen, lane);
+        const int p = t < n ? page(begin + t * step) : -1;
+        k_there[b] = p >= 0;
+        at[b] = p >= 0 ? (begin + t * step) * 32 & (plen - 1) : 0;
+        from[b] = kv4_buffer(a.c.cache + (p >= 0 ? p * page_bytes + head : 0), p >= 0);
+        k[b].load(from[b], at[b], plen, lane);
     };
-    const auto fetch_v = [&](int t, int b) {
-        const auto buf = place(t, v_page[b], at);
-        v[b].load(buf, at, plen, lane);
+    const auto fetch_v = [&](int b) {                    // of the chunk that K's buffer has
+        v_there[b] = k_there[b];
+        v[b].load(from[b], at[b], plen, lane);
     };
     if (n > 0) {
 #pragma unroll
         for (int b = 0; b < BUF; ++b) fetch_k(b, b);
 #pragma unroll
-        for (int b = 0; b < BUF; ++b) fetch_v(b, b);
+        for (int b = 0; b < BUF; ++b) fetch_v(b);
     }
     mine.split(a.scale * kLog2e, tile.cols, shared);
     __syncthreads();
@@ -676,7 +676,7 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
             const auto take = [&](int j, int b) {
                 const int t = t0 + r + j;
                 if (t < n) cut = cut || tile.masked(a, begin + t * step);
-                if (k_page[b] >= 0) {
+                if (k_there[b]) {
                     float d[CT][8];
                     k[b].scores(q, d);
 #pragma unroll
@@ -688,7 +688,7 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
             };
             const auto give = [&](const u32x4 (&part)[CT][3], int j, int b) {
                 const int t = t0 + r + j;
-                if (v_page[b] >= 0) {
+                if (v_there[b]) {
                     Kv4Weights p[CT];                    // other slots' weights are not of this chunk
 #pragma unroll
                     for (int c = 0; c < CT; ++c)
@@ -703,7 +703,7 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
                     values.template add<CT>(p, st);
                     nans = nans || values.nans;
                 }
-                fetch_v(t + BUF, b);
+                fetch_v(b);
             };
 #pragma unroll
             for (int j = 0; j < SLOTS; ++j) take(j, r + j);
