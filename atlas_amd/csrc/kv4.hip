@@ -757,12 +757,20 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
 }
 
 // block -> (tile, KV head): consecutive blocks run on different XCDs, so each takes
-// a run of the heads' tiles and its L2 the heads' tokens
+// a run of the heads and its L2 their tokens; of its heads, a tile's one after the
+// other, so that the tiles come in the order of their lengths.
 __device__ __forceinline__ bool kv4_place(int block, int tiles, int n_kv, int& u, int& kvh) {
-    const int per = (tiles * n_kv + 7) / 8, at = (block & 7) * per + (block >> 3);
-    if ((block >> 3) >= per || at >= tiles * n_kv) return false;
-    kvh = at / tiles;
-    u = at - kvh * tiles;
+    const int xcd = block & 7, at = block >> 3;
+    if (n_kv % 8 == 0) {
+        const int heads = n_kv / 8;
+        u = at / heads;
+        kvh = xcd * heads + at - u * heads;
+        return u < tiles;
+    }
+    const int per = (tiles * n_kv + 7) / 8, all = xcd * per + at;
+    if (at >= per || all >= tiles * n_kv) return false;
+    kvh = all / tiles;
+    u = all - kvh * tiles;
     return true;
 }
 
