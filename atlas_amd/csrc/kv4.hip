@@ -524,30 +524,16 @@ struct Kv4Values {
     }
 };
 
-// The tile u of a batch: its sequence, first row and rows; false: none.  Tiles
-// of sequence s begin at starts[s] / tokens + s, which leaves each sequence as
-// many as it needs, whatever the lengths.
-__device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int u, int& s, int& row, int& rows, int& pos) {
-    if (!a.c.starts) {
-        s = row = u;
-        rows = 1;
-        pos = max(a.c.lens[u], 0) - 1;
-        return true;
-    }
+// The sequence of a batch's tile u.  Tiles of sequence s begin at starts[s] / tokens
+// + s, which leaves each sequence as many as it needs, whatever the lengths.
+__device__ __forceinline__ int kv4_sequence(const Kv4AttnArgs& a, int u) {
     int lo = 0, hi = a.c.n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (a.c.starts[mid] / a.tokens + mid <= u) lo = mid;
         else hi = mid;
     }
-    s = lo;
-    const int begin = max(a.c.starts[lo], 0), end = min(a.c.starts[lo + 1], a.c.n_rows);
-    const int skip = (u - (begin / a.tokens + lo)) * a.tokens;
-    if (skip < 0 || skip >= end - begin) return false;
-    row = begin + skip;
-    rows = min(a.tokens, end - row);
-    pos = max(a.c.lens[lo], 0) - (end - row);
-    return true;
+    return lo;
 }
 
 // A tile's work: its rows and columns (16 CT at most), the chunks that any column
@@ -562,14 +548,22 @@ struct Kv4Tile {
     int pages;
 
     __device__ __forceinline__ bool set(const Kv4AttnArgs& a, int u, int lane) {
-        const bool any = kv4_tile(a, u, s, row0, rows, pos0);
-        // (all of it is the same in every lane; said here, the loops stay in scalar registers)
-        s = __builtin_amdgcn_readfirstlane(s);
-        row0 = __builtin_amdgcn_readfirstlane(row0);
-        rows = __builtin_amdgcn_readfirstlane(rows);
-        pos0 = __builtin_amdgcn_readfirstlane(pos0);
-        if (!any) return false;
+        s = a.c.starts ? __builtin_amdgcn_readfirstlane(kv4_sequence(a, u)) : u;
+        // (the table's entries on their way before the lengths are here)
         pages = lane < a.c.table_stride ? a.c.table[(long)s * a.c.table_stride + lane] : -1;
+        const int len = max(a.c.lens[s], 0);
+        int end = u + 1;
+        row0 = u;
+        if (a.c.starts) {
+            const int begin = max(a.c.starts[s], 0), skip = (u - (begin / a.tokens + s)) * a.tokens;
+            end = min(a.c.starts[s + 1], a.c.n_rows);
+            if (skip < 0 || skip >= end - begin) return false;
+            row0 = begin + skip;
+        }
+        // (all of it is the same in every lane; said here, the loops stay in scalar registers)
+        row0 = __builtin_amdgcn_readfirstlane(row0);
+        rows = __builtin_amdgcn_readfirstlane(min(a.tokens, end - row0));
+        pos0 = __builtin_amdgcn_readfirstlane(len - (end - row0));
         cols = rows * a.group;
         tokens_end = min(pos0 + rows, a.c.cap);
         first = seen_from(a, pos0) >> 5;
@@ -797,20 +791,31 @@ __device__ __forceinline__ int wave_int(int v) {
 // raised until the runs are no more than that (a last run is part of one, and a
 // block too many would double the time); no tile has more than a.splits runs.
 // (Every lane of a wave takes part.)
-__device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int lane) {
+// tokens and rows of sequence s, as the caller wrote them
+struct Kv4Seq {
+    int tokens, begin, end;
+
+    __device__ __forceinline__ void load(const Kv4AttnArgs& a, int s) {
+        tokens = a.c.lens[s];
+        begin = a.c.starts ? a.c.starts[s] : s;
+        end = a.c.starts ? a.c.starts[s + 1] : s + 1;
+    }
+};
+
+// first: sequence `lane`
+__device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, const Kv4Seq& first, int lane) {
     if (a.splits == 1) return 1 << 26;
-    // tiles and chunks of sequence s
+    // tiles and chunks of a sequence
+    const float per_tile = 1.f / a.tokens;
     const auto size = [&](int s, int& tiles, int& chunks) {
-        int tokens = min(max(a.c.lens[s], 0), a.c.cap);
-        tiles = 1;
-        if (a.c.starts) {
-            const long rows = (long)a.c.starts[s + 1] - a.c.starts[s];
-            tiles = rows <= 0 ? 0 : (int)min((rows + a.tokens - 1) / a.tokens, (long)a.tiles);
-        }
+        Kv4Seq seq = first;
+        if (s >= 64) seq.load(a, s);
+        int tokens = min(max(seq.tokens, 0), a.c.cap);
+        tiles = min((int)ceilf(max((float)seq.end - (float)seq.begin, 0.f) * per_tile), a.tiles);
         if (a.window > 0 && tokens - a.tokens > a.window) tokens = a.window + a.tokens;
         chunks = tiles ? (tokens + 31) >> 5 : 0;
     };
-    // (sums capped, so that 64 lanes' fit: longer runs are right as well)
+    // (sums capped, so that 64 lanes' fit, and roughly rounded: any run is right)
     int all = 0, most = 0, count = 0, tiles, chunks;
     for (int s = lane; s < a.c.n_seqs; s += 64) {
         size(s, tiles, chunks);
@@ -824,9 +829,10 @@ __device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, int lane) {
     int run = max(least, (int)ceilf(wave_int<false>(all) * per));
     for (int turn = 0; turn < 3 && units * per <= 1.f; ++turn) {
         count = 0;
+        const float in_run = __builtin_amdgcn_rcpf((float)run);
         for (int s = lane; s < a.c.n_seqs; s += 64) {
             size(s, tiles, chunks);
-            count = min(count + tiles * ((chunks + run - 1) / run), 1 << 24);
+            count = min(count + tiles * (int)ceilf(chunks * in_run), 1 << 24);
         }
         const float over = wave_int<false>(count) * per;
         if (over <= 1.f) break;
@@ -868,11 +874,13 @@ __global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attenti
     int u, kvh;
     if (!kv4_place(blockIdx.x, a.tiles, a.c.n_kv, u, kvh)) return;
     u = a.tiles - 1 - u;                                 // a prompt's last tiles, the longest, first
+    Kv4Seq first = {0, 0, 0};                            // (on its way before the tile's own loads are waited for)
+    if (lane < a.c.n_seqs) first.load(a, lane);
     Kv4Tile tile;
     if (!tile.set(a, u, lane)) return;
     typename Kv4Query<HD, 16 * CT>::template Mine<kKv4Waves * 64> mine;
     mine.fetch(a, tile.row0, tile.cols, kvh);
-    const int run = kv4_run(a, lane), begin = tile.first + split * run;
+    const int run = kv4_run(a, first, lane), begin = tile.first + split * run;
     if (split > 0 && begin >= tile.last) return;
     const int runs = max((tile.last - tile.first + run - 1) / run, 1);
     Kv4Column<SLOTS> col[CT];
