@@ -812,7 +812,8 @@ __device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, const Kv4Seq& first
         if (s >= 64) seq.load(a, s);
         int tokens = min(max(seq.tokens, 0), a.c.cap);
         tiles = min((int)ceilf(max((float)seq.end - (float)seq.begin, 0.f) * per_tile), a.tiles);
-        if (a.window > 0 && tokens - a.tokens > a.window) tokens = a.window + a.tokens;
+        // (a window's first and last chunk are parts)
+        if (a.window > 0 && tokens - a.tokens - 31 > a.window) tokens = a.window + a.tokens + 31;
         chunks = tiles ? (tokens + 31) >> 5 : 0;
     };
     // (sums capped, so that 64 lanes' fit, and roughly rounded: any run is right)
@@ -880,7 +881,9 @@ __global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attenti
     if (!tile.set(a, u, lane)) return;
     typename Kv4Query<HD, 16 * CT>::template Mine<kKv4Waves * 64> mine;
     mine.fetch(a, tile.row0, tile.cols, kvh);
-    const int run = kv4_run(a, first, lane), begin = tile.first + split * run;
+    // (never more runs than the grid has blocks for, whatever the starts hold)
+    const int run = max(kv4_run(a, first, lane), (tile.last - tile.first + a.splits - 1) / a.splits);
+    const int begin = tile.first + split * run;
     if (split > 0 && begin >= tile.last) return;
     const int runs = max((tile.last - tile.first + run - 1) / run, 1);
     Kv4Column<SLOTS> col[CT];

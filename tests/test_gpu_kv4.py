@@ -243,6 +243,15 @@ def test_window(window, hd):
     _check_attention(c, 4, window=window)
 
 
+@pytest.mark.parametrize("window", [2046, 2047, 2048, 2049])
+@pytest.mark.parametrize("n_kv,hd,length,rows", [(96, 64, 2500, 1), (64, 128, 2500, 1), (96, 64, 2511, 3), (32, 128, 2060, 1)])
+def test_window_in_runs(n_kv, hd, length, rows, window):
+    """As many runs as the window's chunks have room for; its first and last chunks are parts."""
+    c = Case(window + length, [length], None if rows == 1 else [rows], n_kv, hd, 64)
+    for _ in range(2):                                 # the second call finds what the first left
+        _check_attention(c, n_kv, window=window)
+
+
 @pytest.mark.parametrize("hd,group,n_kv", [(64, 4, 2), (64, 3, 3), (128, 1, 4), (128, 8, 1), (128, 5, 2), (256, 2, 2), (256, 16, 1)])
 @pytest.mark.parametrize("lens,rows", [([1], [1]), ([33], [33]), ([100, 65, 200], [100, 1, 37]), ([5, 0, 64, 70], [5, 0, 0, 70]),
                                        ([300], [17]), ([130, 129], [128, 129])])
