@@ -132,7 +132,8 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Args a, const float* 
                                                         const float* __restrict__ v, long ld) {
     Kv4Place<HD> to;
     f32x4 in[2][2] = {};
-    if (to.inside(a)) {
+    // (on their way before the row's place is known; rows behind the last sequence may not be there)
+    if (to.inside(a) && (!a.starts || to.row < a.starts[a.n_seqs])) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             in[0][i] = reinterpret_cast<const f32x4*>(k + to.row * ld + to.e)[i];
@@ -1000,6 +1001,8 @@ static int kv4_check(const char* who, const atlas_kv4_cache& c) {
     ATLAS_REQUIRE(c.page_len >= 32 && c.page_len <= 1 << 22 && (c.page_len & (c.page_len - 1)) == 0,
                   "%s: page_len %d (a power of two from 32 to 2^22)", who, c.page_len);
     ATLAS_REQUIRE(c.n_pages >= 0 && c.n_kv > 0 && c.n_kv <= 4096, "%s: %d pages, %d KV heads", who, c.n_pages, c.n_kv);
+    const int64_t page = (int64_t)c.n_kv * c.page_len * (c.head_dim + c.head_dim / 16);
+    ATLAS_REQUIRE(c.n_pages <= INT64_MAX / page, "%s: %d pages of %lld bytes", who, c.n_pages, (long long)page);
     return ATLAS_OK;
 }
 

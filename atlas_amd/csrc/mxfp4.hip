@@ -424,7 +424,8 @@ int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, con
     ATLAS_REQUIRE(((uintptr_t)w & 15) == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)y & 3) == 0,
                   "gemm_mxfp4: w and x start on 16 bytes, y on 4");
     const int kb = (int)(((long)k + kMxBlock - 1) / kMxBlock);
-    ATLAS_REQUIRE(n <= 1 << 20, "gemm_mxfp4: %d rows", n);
+    // (a launch has fewer than 2^32 threads)
+    ATLAS_REQUIRE(m <= 1 << 28 && n <= 1 << 20, "gemm_mxfp4: %d rows of weights, %d of x", m, n);
     const u32x4 *wv = reinterpret_cast<const u32x4*>(w), *xv = reinterpret_cast<const u32x4*>(x);
 #define MX_ROWS(MT, NT, WAVES)                                                                                        \
     hipLaunchKernelGGL((mxfp4_rows_kernel<MT, NT, WAVES>), dim3((m + 16L * MT - 1) / (16 * MT), (n + 16L * NT - 1) / (16 * NT)), \

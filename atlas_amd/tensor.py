@@ -466,11 +466,14 @@ class Kv4Batch:
     and how many of its last tokens are the step's rows (default one)."""
 
     def __init__(self, kv_lens, block_table, row_lens=None):
-        lens = np.ascontiguousarray(kv_lens, np.int32).reshape(-1)
-        table = np.ascontiguousarray(block_table, np.int32).reshape(lens.size, -1)
+        lens = np.asarray(kv_lens, np.int64).reshape(-1)
         rows = np.ones(lens.size, np.int64) if row_lens is None else np.asarray(row_lens, np.int64).reshape(-1)
-        if rows.size != lens.size or (rows < 0).any() or (lens < 0).any() or (rows > lens).any():
-            raise AtlasError(-1, "Kv4Batch: each sequence has 0 <= new rows <= length")
+        if rows.size != lens.size or (rows < 0).any() or (rows > lens).any() or (lens >= 1 << 31).any():
+            raise AtlasError(-1, "Kv4Batch: each sequence has 0 <= new rows <= length < 2^31")
+        lens = lens.astype(np.int32)
+        table = np.asarray(block_table, np.int64)
+        table = np.where((table < 0) | (table >= 1 << 31), -1, table).astype(np.int32)
+        table = table.reshape(lens.size, table.size // max(lens.size, 1))
         starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
         self.kv_lens, self.block_table, self.row_starts = lens, table, starts
         self.n_seqs, self.n_rows = lens.size, int(starts[-1])
@@ -496,7 +499,10 @@ class GpuKv4Cache:
         nbytes = check(load().atlas_kv4_cache_bytes(C.byref(c)))
         if not cuda_available():
             return None
-        mem = _DevMem(max(nbytes, 16), sync_alloc=True)
+        try:
+            mem = _DevMem(max(nbytes, 16), sync_alloc=True)
+        except MemoryError:
+            return None
         check(load().atlas_memset_zero(mem.ptr, mem.nbytes))
         c.data = mem.ptr
         return GpuKv4Cache(mem, c)

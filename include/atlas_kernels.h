@@ -28,7 +28,8 @@
  *
  * Library scratch: entry points that need device scratch and are not handed
  * a workspace (atlas_decode_attention, atlas_gpu_argmax,
- * atlas_gemm_skinny_f32, atlas_attention_fused_f32) keep it per calling
+ * atlas_gemm_skinny_f32, atlas_attention_fused_f32,
+ * atlas_kv4_attention_f32 for long caches) keep it per calling
  * thread, grow it on first use of a larger shape and free it when the
  * thread exits.  A call that would grow it while its stream is being
  * captured into a graph returns / records ATLAS_EUNSUPPORTED instead: warm
@@ -292,7 +293,7 @@ int atlas_dequantize_mxfp4_dev(const uint8_t* data, const uint8_t* scales, int64
 int atlas_quantize_mxfp4_host(const float* w, int64_t rows, int64_t cols, uint8_t* data,
                               uint8_t* scales);
 /* Y[n, m] = sum_k X[n, k] W[m, k] of two MXFP4 matrices (W: m rows, X: n rows of
- * k elements), f32 sums; rows of Y lie ld >= m elements apart.  Any m, n, k.
+ * k elements), f32 sums; rows of Y lie ld >= m elements apart.  Any k, m up to 2^28, n up to 2^20.
  * w and x are 16-byte aligned.  Elements that fill up a last block have to be
  * zero in one of the two, as the encoders leave them.                       */
 int atlas_gemm_mxfp4_f32(const uint8_t* w, const uint8_t* w_scales, const uint8_t* x,
@@ -306,7 +307,7 @@ int atlas_gemm_mxfp4_f32(const uint8_t* w, const uint8_t* w_scales, const uint8_
  *   V codes [page_len/8][16][8][head_dim/32], V scales as K's
  * (V: 16 groups of head_dim/16 elements, for each of them eight tokens side by
  * side).  head_dim 64, 128 or 256; page_len a power of two, 32 to 2^22 (one page
- * of max_seq tokens for each sequence is a cache without paging).           */
+ * of max_seq tokens for each sequence is a cache without paging).  n_kv up to 4096. */
 typedef struct {
     void* data;                  /* device, 16-byte aligned, atlas_kv4_cache_bytes */
     int n_pages, page_len, n_kv, head_dim;

@@ -531,3 +531,112 @@ def test_two_graphs_and_two_streams():
                 assert (np.abs(want[i][row].reshape(heads, 128) - mx_ref.attend(*w)) <= _bound(*w)).all()
 
     on_thread(work)
+
+
+def test_capture_that_has_to_grow():
+    """A captured call that needs more scratch than the thread has is refused; after an eager one it is recorded."""
+    def work(hip):
+        heads, hd = 4, 64
+        c = Case(40, [3000], None, 2, hd, 64)
+        args = c.upload()
+        q = c.rng.standard_normal((1, heads * hd)).astype(np.float32)
+        qd, out = Dev(q), Dev(np.full(q.shape, 7, np.float32))
+
+        def call():
+            return lib().atlas_kv4_attention_f32(*args, qd.ptr, heads * hd, heads, 0.1, 0, out.ptr, heads * hd)
+
+        with Stream(hip) as st:
+            def refused():
+                rc = call()
+                # (a kernel for the graph to hold)
+                assert lib().atlas_kv4_write_f32(*args, out.ptr, out.ptr, 2 * hd) == 0
+                return rc
+
+            _, rc = st.capture(refused)
+            assert rc == -4 and b"scratch" in lib().atlas_last_error()
+            lib().atlas_clear_error()
+            st.sync()
+            assert (out.get() == 7).all()
+            assert call() == 0
+            st.sync()
+            want = out.get()
+            exe, rc = st.capture(call)
+            assert rc == 0
+            for _ in range(3):
+                check(lib().atlas_memset_zero(out.ptr, out.a.nbytes))
+                st.launch(exe)
+                st.sync()
+                np.testing.assert_array_equal(out.get(), want)
+
+    on_thread(work)
+
+
+def test_two_threads():
+    """Calls of two threads on streams of their own at once: each thread has its own scratch."""
+    import threading
+    heads, hd = 8, 128
+    cs = [Case(50 + i, [1500 + 700 * i, 40], None, 2, hd, 64) for i in range(2)]
+    args = [c.upload() for c in cs]
+    q = [Dev(c.rng.standard_normal((2, heads * hd)).astype(np.float32)) for c in cs]
+    outs = [[Dev(np.zeros((2, heads * hd), np.float32)) for _ in range(12)] for _ in cs]
+
+    def call(i, out):
+        assert lib().atlas_kv4_attention_f32(*args[i], q[i].ptr, heads * hd, heads, 0.1, 0, out.ptr, heads * hd) == 0
+
+    for i in range(2):
+        call(i, outs[i][0])
+    sync()
+    want, gate = [outs[i][0].get() for i in range(2)], threading.Barrier(2)
+
+    def work(i):
+        def run(hip):
+            with Stream(hip) as st:
+                gate.wait(60)
+                for out in outs[i][1:]:
+                    call(i, out)
+                st.sync()
+        return run
+
+    threads = [threading.Thread(target=on_thread, args=(work(i),)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        for out in outs[i][1:]:
+            np.testing.assert_array_equal(out.get(), want[i])
+
+
+def test_nothing_and_no_memory():
+    """Batches without sequences or rows; allocations that fail."""
+    from atlas_amd.quant import MxFp4Tensor
+    from atlas_amd.tensor import GpuKv4Cache, GpuMatrix, GpuVec, Kv4Batch
+    cache = GpuKv4Cache.new(2, 32, 1, 64)
+    for batch in (Kv4Batch([], []), Kv4Batch([5, 0], [[0], [1]], [0, 0])):
+        none = GpuVec.zeros(0)
+        cache.write(batch, none, none)
+        assert cache.read(batch)[0].len == 0
+        assert cache.attention(batch, none, 2, 1.0).len == 0
+    g = GpuMatrix.upload_mxfp4(MxFp4Tensor.quantize(np.ones((64, 64), np.float32)))
+    x, out = np.ones((64, 1), np.float32), np.zeros((64, 1), np.float32)
+
+    def work(hip):
+        c = Case(60, [3000], None, 2, 64, 64)
+        args = c.upload()
+        q = Dev(np.ones((1, 256), np.float32))
+        try:
+            for skip in (0, 1):                            # the counters, the partial sums
+                lib().atlas_debug_fail_allocations(skip, 1)
+                assert lib().atlas_kv4_attention_f32(*args, q.ptr, 256, 4, 0.1, 0, q.ptr, 256) == -3
+                lib().atlas_clear_error()
+            lib().atlas_debug_fail_allocations(0, 1)
+            assert GpuKv4Cache.new(2, 32, 1, 64) is None
+            lib().atlas_debug_fail_allocations(2, 1)       # the activations' codes, after x and out
+            assert not g.sgemm(x, 64, 1, out)
+        finally:
+            lib().atlas_debug_fail_allocations(0, 0)
+            lib().atlas_clear_error()
+        _check_attention(c, 4, args=args)
+        assert g.sgemm(x, 64, 1, out) and (out == 64).all()
+
+    on_thread(work)

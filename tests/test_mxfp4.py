@@ -162,3 +162,21 @@ def test_batches_that_are_refused(lib):
         GpuKv4Cache.new(4, 48, 2, 128)
     if not cuda_available():
         assert GpuKv4Cache.new(4, 64, 2, 128) is None
+
+
+def test_sizes_past_the_limits(lib):
+    """More bytes than an address has, more blocks than a launch has, lengths that an int32 does not hold."""
+    from atlas_amd import AtlasError
+    from atlas_amd._lib import Kv4BatchC, Kv4CacheC
+    from atlas_amd.tensor import Kv4Batch
+    a = 4096
+    huge = Kv4CacheC(a, (1 << 31) - 1, 1 << 22, 4096, 256)
+    one = Kv4BatchC(None, a, a, 1, 1, 1, 0)
+    _refused(lib, lib.atlas_kv4_cache_bytes(C.byref(huge)))
+    _refused(lib, lib.atlas_kv4_write_f32(C.byref(huge), C.byref(one), a, a, 4096 * 256))
+    assert lib.atlas_kv4_cache_bytes(C.byref(Kv4CacheC(a, 1 << 20, 1 << 22, 1, 256))) == (272 << 42)
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, a, a, (1 << 28) + 1, 1, 32, 1 << 29))
+    _refused(lib, lib.atlas_gemm_mxfp4_f32(a, a, a, a, a, 4, (1 << 20) + 1, 32, 4))
+    for lens, table, rows in [([1 << 31], [[0]], [1]), ([1 << 32], [[0]], [0])]:
+        with pytest.raises(AtlasError):
+            Kv4Batch(lens, table, rows)
