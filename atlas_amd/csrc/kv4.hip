@@ -12,6 +12,7 @@
 // instruction has eight tokens of the same elements, and so finds them in one
 // piece.  A token still fills whole bytes, so that writing one touches no other.
 #include <algorithm>
+#include <type_traits>
 
 #include "mfma.hpp"
 #include "mxfp4.hpp"
@@ -658,8 +659,8 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
     bool nans = false;
     constexpr int ROUNDS = SLOTS == 1 ? BUF : 1;
     static_assert(SLOTS == 1 || BUF == SLOTS, "a buffer to a slot");
-#pragma unroll 1
-    for (int t0 = 0; t0 < n; t0 += SLOTS * ROUNDS)
+    // (without loads ahead in the last round)
+    const auto round = [&](int t0, auto more) {
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             float s[CT][8];
@@ -679,7 +680,7 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
 #pragma unroll
                         for (int e = 0; e < 8; ++e) s[c][e] = SLOTS == 1 || col[c].slot == j ? d[c][e] : s[c][e];
                 }
-                fetch_k(t + BUF, b);
+                if constexpr (decltype(more)::value) fetch_k(t + BUF, b);
             };
             const auto give = [&](const u32x4 (&part)[CT][3], int j, int b) {
                 const int t = t0 + r + j;
@@ -698,7 +699,7 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
                     values.template add<CT>(p, st);
                     nans = nans || values.nans;
                 }
-                fetch_v(b);
+                if constexpr (decltype(more)::value) fetch_v(b);
             };
 #pragma unroll
             for (int j = 0; j < SLOTS; ++j) take(j, r + j);
@@ -716,6 +717,11 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
 #pragma unroll
             for (int j = 0; j < SLOTS; ++j) give(part, j, r + j);
         }
+    };
+    int t0 = 0;
+#pragma unroll 1
+    for (; t0 + SLOTS * ROUNDS < n; t0 += SLOTS * ROUNDS) round(t0, std::true_type{});
+    if (t0 < n) round(t0, std::false_type{});
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         st[c].l += __shfl_xor(st[c].l, 16, 64);
