@@ -246,6 +246,7 @@ struct Kv4AttnArgs {
     // a split tile: most blocks, columns, and [tiles][n_kv][splits][cols] partial
     // sums (each HD elements, and maximum and sum of the weights)
     int splits, cols, blocks;
+    int min_run;                        // chunks of a run, where there are several; up to twice as many are one
     float *part_o, *part_ml;
     int* counters;                      // [tiles][n_kv] blocks that are done, zero between calls
 };
@@ -779,7 +780,6 @@ __device__ __forceinline__ bool kv4_place(int block, int tiles, int n_kv, int& u
 // tile.  A block's waves take every fourth chunk of its run and join their sums in
 // LDS; the blocks' are joined by the one that ends last.
 constexpr int kKv4Waves = 4;
-constexpr int kKv4MinRun = 2 * kKv4Waves;               // chunks of a block, where a tile has more
 
 // all lanes' sum or largest value, of integers
 template <bool MAX>
@@ -833,7 +833,8 @@ __device__ __forceinline__ int kv4_run(const Kv4AttnArgs& a, const Kv4Seq& first
     }
     const int units = wave_int<false>(count), long_run = wave_int<true>(most);
     const float per = (float)a.c.n_kv / a.blocks;
-    const int least = max(kKv4MinRun, (long_run + a.splits - 1) / a.splits);
+    if (long_run <= 2 * a.min_run) return 2 * a.min_run;
+    const int least = max(a.min_run, (long_run + a.splits - 1) / a.splits);
     int run = max(least, (int)ceilf(wave_int<false>(all) * per));
     for (int turn = 0; turn < 3 && units * per <= 1.f; ++turn) {
         count = 0;
@@ -1111,9 +1112,10 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     a.window = window;
     a.cols = a.tokens * a.group;
     // chunks of the longest row
+    // (of a window, the first and the last are parts)
     int64_t chunks = b.max_len > 0 ? std::min(b.max_len, a.c.cap) : a.c.cap;
-    if (window > 0) chunks = std::min<int64_t>(chunks, (int64_t)window + a.tokens);
-    chunks = (chunks + 62) / 32;
+    if (window > 0) chunks = std::min<int64_t>(chunks, (int64_t)window + a.tokens + 31);
+    chunks = (chunks + 31) / 32;
     const long units = (long)a.tiles * c.n_kv;
     ATLAS_REQUIRE(units <= 1 << 23, "kv4_attention: %d tiles of rows and %d KV heads", a.tiles, c.n_kv);
     // As many blocks as run at once (their registers leave 3, 2 or 1 to a CU).  Of
@@ -1123,13 +1125,21 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     // (24 sequences of up to 4000 tokens, heads 32/8 of 128: 26 us with that many
     // runs, 37 with a third more of shorter ones).  At most 128 chunks to a run, 32
     // runs to a tile (64 of that length), 256 MB of partial sums.
+    // Runs are joined in 3 to 8 us, by the columns: up to 32 chunks are one run and
+    // longer ones have 16 at least (900 tokens, 9 heads of 64 over 3: 9.3 us, 10.3 in runs
+    // of 16; 8 rows of 32 over 8 of 128: 16.7 and 20.4; 2000 tokens of the former: 12.4 in
+    // runs of 32, 10.1 of 16, 9.7 of 8; 300 tokens: 6.8 and, in runs of 8, 9.4); half of
+    // both at head dim 256, where a chunk takes twice as long.
     const int cus = device_cu_count(), at_once = cus * (c.head_dim == 256 ? 1 : c.head_dim == 64 && !wide ? 3 : 2);
     a.blocks = b.n_seqs > 1 ? at_once * 3 / 4 : at_once;
+    // chunks that fit side by side into the 16 columns
+    const int slots = a.cols <= 4 ? 4 : a.cols <= 8 ? 2 : 1;
+    a.min_run = c.head_dim == 256 ? 8 : 16;
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
     const long want = std::max<long>(at_once * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
-    const long most = std::min<long>({std::max<long>(32L, (chunks + 127) / 128), 64L, (long)((chunks + kKv4MinRun - 1) / kKv4MinRun),
+    const long most = std::min<long>({std::max<long>(32L, (chunks + 127) / 128), 64L, (long)((chunks + a.min_run - 1) / a.min_run),
                                       (long)((256u << 20) / each)});
-    a.splits = (int)std::max(1L, std::min(want, most));
+    a.splits = chunks <= 2 * a.min_run ? 1 : (int)std::max(1L, std::min(want, most));
     if (a.splits > 1) {
         const size_t n = (size_t)units * a.splits * a.cols;
         void *p = nullptr, *cnt = nullptr;
@@ -1140,8 +1150,6 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
         a.part_ml = a.part_o + n * c.head_dim;
     }
     const dim3 grid((unsigned)((units + 7) / 8 * 8), a.splits);
-    // chunks that fit side by side into the 16 columns
-    const int slots = a.cols <= 4 ? 4 : a.cols <= 8 ? 2 : 1;
 #define KV4_RUN(HD, SLOTS, CT)                                                                                        \
     hipLaunchKernelGGL((kv4_attention_kernel<HD, SLOTS, CT>), grid, dim3(kKv4Waves * 64), 0, st, a)
 #define KV4_SLOTS(HD)                                                                                                 \
