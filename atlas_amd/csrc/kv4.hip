@@ -426,7 +426,8 @@ struct Kv4State {
     }
 
     // the weights of 8 scores, in three bf16 parts; maximum and sum move on
-    __device__ __forceinline__ void weigh(const float (&s)[8], u32x4 (&part)[3]) {
+    __device__ __forceinline__ void weigh(const float (&s)[8], Kv4Weights& p) {
+        u32x4 part[3];
         float top = s[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
@@ -452,6 +453,8 @@ struct Kv4State {
             }
             part[2][j] = bf16_hi2(a, b);
         }
+#pragma unroll
+        for (int e = 0; e < 3; ++e) p[e] = __builtin_bit_cast(bf16x8, part[e]);
     }
 };
 
@@ -541,9 +544,6 @@ __device__ __forceinline__ int kv4_sequence(const Kv4AttnArgs& a, int u) {
 
 // A tile's work: its rows and columns (16 CT at most), the chunks that any column
 // sees, and the first pages of its sequence, one to a lane.
-// Where rows and heads are few, a tile's columns are given SLOTS times, each time
-// for other chunks: a wave then takes the scores of SLOTS chunks one after the
-// other, each into its columns, before it weighs them all at once.
 struct Kv4Tile {
     int s, row0, rows, cols, pos0;
     int first, last;                    // chunks [first, last)
@@ -585,29 +585,25 @@ struct Kv4Tile {
 };
 
 // a lane's column of column tile ct
-template <int SLOTS>
 struct Kv4Column {
-    bool mine;                          // it is one (others repeat one of them)
-    int slot, col;
+    bool mine;                          // it is one (others repeat the last)
+    int col;
     int from, to;                       // it sees tokens [from, to]
 
     __device__ __forceinline__ void set(const Kv4AttnArgs& a, const Kv4Tile& tile, int ct, int lane) {
         const int i = 16 * ct + (lane & 15);
-        slot = SLOTS > 1 ? i / tile.cols : 0;
-        col = min(i - slot * tile.cols, tile.cols - 1);
-        mine = SLOTS > 1 ? slot < SLOTS : i < tile.cols;
+        col = min(i, tile.cols - 1);
+        mine = i < tile.cols;
         to = tile.pos0 + col / a.group;
         from = Kv4Tile::seen_from(a, to);
     }
 };
 
 // Chunks begin, begin + step, .. below end into st.  K and V of a chunk are loaded
-// BUF chunks ahead, page numbers 64 at a time.  (The scores of SLOTS chunks follow
-// each other closely, and so do their products with V: with fewer than SLOTS
-// buffers the loads of each would be waited for.)
+// BUF chunks ahead, page numbers 64 at a time.
 // Every thread of a block of THREADS comes here, for the query.
-template <int HD, int SLOTS, int CT, int BUF, int THREADS>
-__device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& tile, const Kv4Column<SLOTS> (&col)[CT], int kvh,
+template <int HD, int CT, int BUF, int THREADS>
+__device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& tile, const Kv4Column (&col)[CT], int kvh,
                                          int begin, int end, int step,
                                          const typename Kv4Query<HD, 16 * CT>::template Mine<THREADS>& mine,
                                          typename Kv4Query<HD, 16 * CT>::Shared& shared, Kv4State<HD> (&st)[CT], int lane) {
@@ -658,70 +654,43 @@ __device__ __forceinline__ void kv4_scan(const Kv4AttnArgs& a, const Kv4Tile& ti
         st[c].clear();
     }
     bool nans = false;
-    constexpr int ROUNDS = SLOTS == 1 ? BUF : 1;
-    static_assert(SLOTS == 1 || BUF == SLOTS, "a buffer to a slot");
     // (without loads ahead in the last round)
     const auto round = [&](int t0, auto more) {
 #pragma unroll
-        for (int r = 0; r < ROUNDS; ++r) {
+        for (int b = 0; b < BUF; ++b) {
+            const int chunk = begin + (t0 + b) * step;
             float s[CT][8];
+            if (k_there[b]) {
+                k[b].scores(q, s);
+            } else {
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+                for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s[c][j] = -__builtin_inff();
-            bool cut = false;
-            const auto take = [&](int j, int b) {
-                const int t = t0 + r + j;
-                if (t < n) cut = cut || tile.masked(a, begin + t * step);
-                if (k_there[b]) {
-                    float d[CT][8];
-                    k[b].scores(q, d);
+                    for (int j = 0; j < 8; ++j) s[c][j] = -__builtin_inff();
+            }
+            if constexpr (decltype(more)::value) fetch_k(t0 + b + BUF, b);
+            if (t0 + b < n && tile.masked(a, chunk))
 #pragma unroll
-                    for (int c = 0; c < CT; ++c)
+                for (int c = 0; c < CT; ++c)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) s[c][e] = SLOTS == 1 || col[c].slot == j ? d[c][e] : s[c][e];
-                }
-                if constexpr (decltype(more)::value) fetch_k(t + BUF, b);
-            };
-            const auto give = [&](const u32x4 (&part)[CT][3], int j, int b) {
-                const int t = t0 + r + j;
-                if (v_there[b]) {
-                    Kv4Weights p[CT];                    // other slots' weights are not of this chunk
+                    for (int j = 0; j < 8; ++j) {
+                        const int key = chunk * 32 + 8 * g + j;
+                        if (key < col[c].from || key > col[c].to) s[c][j] = -__builtin_inff();
+                    }
+            Kv4Weights p[CT];
 #pragma unroll
-                    for (int c = 0; c < CT; ++c)
-#pragma unroll
-                        for (int e = 0; e < 3; ++e) {
-                            u32x4 x;
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) x[w] = SLOTS == 1 || col[c].slot == j ? part[c][e][w] : 0u;
-                            p[c][e] = __builtin_bit_cast(bf16x8, x);
-                        }
-                    const Kv4Values<HD> values(v[b], tile.tokens_end - (begin + t * step) * 32, g);
-                    values.template add<CT>(p, st);
-                    nans = nans || values.nans;
-                }
-                if constexpr (decltype(more)::value) fetch_v(b);
-            };
-#pragma unroll
-            for (int j = 0; j < SLOTS; ++j) take(j, r + j);
-            if (cut)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const int first = (begin + (t0 + r + col[c].slot) * step) * 32 + 8 * g;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (first + j < col[c].from || first + j > col[c].to) s[c][j] = -__builtin_inff();
-                }
-            u32x4 part[CT][3];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) st[c].weigh(s[c], part[c]);
-#pragma unroll
-            for (int j = 0; j < SLOTS; ++j) give(part, j, r + j);
+            for (int c = 0; c < CT; ++c) st[c].weigh(s[c], p[c]);
+            if (v_there[b]) {
+                const Kv4Values<HD> values(v[b], tile.tokens_end - chunk * 32, g);
+                values.template add<CT>(p, st);
+                nans = nans || values.nans;
+            }
+            if constexpr (decltype(more)::value) fetch_v(b);
         }
     };
     int t0 = 0;
 #pragma unroll 1
-    for (; t0 + SLOTS * ROUNDS < n; t0 += SLOTS * ROUNDS) round(t0, std::true_type{});
+    for (; t0 + BUF < n; t0 += BUF) round(t0, std::true_type{});
     if (t0 < n) round(t0, std::false_type{});
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -875,8 +844,11 @@ struct Kv4Shared {
     int last;
 };
 
-template <int HD, int SLOTS, int CT>
-__global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attention_kernel(Kv4AttnArgs a) {
+// waves of a SIMD for the registers of HD and CT, and so blocks of a CU
+constexpr int kv4_at_once(int hd, int ct) { return ct > 1 || hd == 256 ? 2 : hd == 128 ? 3 : 4; }
+
+template <int HD, int CT>
+__global__ __launch_bounds__(kKv4Waves * 64, kv4_at_once(HD, CT)) void kv4_attention_kernel(Kv4AttnArgs a) {
     __shared__ Kv4Shared<HD, 16 * CT> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4, split = blockIdx.y;
@@ -894,13 +866,13 @@ __global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attenti
     const int begin = tile.first + split * run;
     if (split > 0 && begin >= tile.last) return;
     const int runs = max((tile.last - tile.first + run - 1) / run, 1);
-    Kv4Column<SLOTS> col[CT];
+    Kv4Column col[CT];
     Kv4State<HD> st[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) col[c].set(a, tile, c, lane);
-    // (two column tiles leave registers for one chunk ahead)
-    constexpr int BUF = CT > 1 ? 1 : SLOTS > 1 ? SLOTS : 2;
-    kv4_scan<HD, SLOTS, CT, BUF, kKv4Waves * 64>(a, tile, col, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves,
+    // (two column tiles, or 256 elements, leave registers for one chunk ahead)
+    constexpr int BUF = CT > 1 || HD == 256 ? 1 : 2;
+    kv4_scan<HD, CT, BUF, kKv4Waves * 64>(a, tile, col, kvh, begin + wave, min(begin + run, tile.last), kKv4Waves,
                                                              mine, sh.q, st, lane);
     __syncthreads();                                     // the query has been read
 #pragma unroll
@@ -928,21 +900,16 @@ __global__ __launch_bounds__(kKv4Waves * 64, HD == 256 ? 1 : 2) void kv4_attenti
     };
     for (int e = threadIdx.x; e < cols * (HD / 4); e += kKv4Waves * 64) {
         const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-        // of each wave and slot
         float m = kKv4Floor, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; ++w)
-#pragma unroll
-            for (int x = 0; x < SLOTS; ++x) m = fmaxf(m, sh.m[w][x * cols + c]);
+        for (int w = 0; w < kKv4Waves; ++w) m = fmaxf(m, sh.m[w][c]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; ++w)
-#pragma unroll
-            for (int x = 0; x < SLOTS; ++x) {
-                const float f = __builtin_amdgcn_exp2f(sh.m[w][x * cols + c] - m);
-                l += f * sh.l[w][x * cols + c];
-                o += f * *reinterpret_cast<const f32x4*>(&sh.o[w][x * cols + c][d]);
-            }
+        for (int w = 0; w < kKv4Waves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sh.m[w][c] - m);
+            l += f * sh.l[w][c];
+            o += f * *reinterpret_cast<const f32x4*>(&sh.o[w][c][d]);
+        }
         if (runs == 1) {
             store(c, d, o, l);
         } else {
@@ -1118,25 +1085,24 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     chunks = (chunks + 31) / 32;
     const long units = (long)a.tiles * c.n_kv;
     ATLAS_REQUIRE(units <= 1 << 23, "kv4_attention: %d tiles of rows and %d KV heads", a.tiles, c.n_kv);
-    // As many blocks as run at once (their registers leave 3, 2 or 1 to a CU).  Of
-    // sequences of different lengths the longest get up to twice an even share of
-    // runs; the blocks beyond the others' runs come and go between the working ones,
-    // and these then fill about 3/4 of the places before some of them have to wait
-    // (24 sequences of up to 4000 tokens, heads 32/8 of 128: 26 us with that many
-    // runs, 37 with a third more of shorter ones).  At most 128 chunks to a run, 32
-    // runs to a tile (64 of that length), 256 MB of partial sums.
+    // Working blocks: two to a CU for a single sequence.  Of sequences of different
+    // lengths the longest get up to twice an even share of runs; the blocks beyond the
+    // others' runs come and go between the working ones, and these then fill about 5/8
+    // of the places before some of them have to wait.  (24 sequences of up to 8191 tokens,
+    // heads 32/8 of 64: 23.8 us with 9/4 to a CU, 25.9 with 2, 28.9 with 11/4; of 128: 36 with
+    // 15/8, 41 with 3/2, 36.5 with 21/8; up to 4000 tokens, heads 16/8 of 256: 33 with 3/2, 38 with
+    // 1, 40 with 2.)  At most 128 chunks to a run, 32 runs to a tile (64 of that
+    // length), 256 MB of partial sums.
     // Runs are joined in 3 to 8 us, by the columns: up to 32 chunks are one run and
     // longer ones have 16 at least (900 tokens, 9 heads of 64 over 3: 9.3 us, 10.3 in runs
     // of 16; 8 rows of 32 over 8 of 128: 16.7 and 20.4; 2000 tokens of the former: 12.4 in
     // runs of 32, 10.1 of 16, 9.7 of 8; 300 tokens: 6.8 and, in runs of 8, 9.4); half of
     // both at head dim 256, where a chunk takes twice as long.
-    const int cus = device_cu_count(), at_once = cus * (c.head_dim == 256 ? 1 : c.head_dim == 64 && !wide ? 3 : 2);
-    a.blocks = b.n_seqs > 1 ? at_once * 3 / 4 : at_once;
-    // chunks that fit side by side into the 16 columns
-    const int slots = a.cols <= 4 ? 4 : a.cols <= 8 ? 2 : 1;
+    const int eighths = b.n_seqs == 1 ? 16 : wide || c.head_dim == 256 ? 12 : c.head_dim == 128 ? 15 : 18;
+    a.blocks = device_cu_count() * eighths / 8;
     a.min_run = c.head_dim == 256 ? 8 : 16;
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
-    const long want = std::max<long>(at_once * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
+    const long want = std::max<long>(a.blocks * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
     const long most = std::min<long>({std::max<long>(32L, (chunks + 127) / 128), 64L, (long)((chunks + a.min_run - 1) / a.min_run),
                                       (long)((256u << 20) / each)});
     a.splits = chunks <= 2 * a.min_run ? 1 : (int)std::max(1L, std::min(want, most));
@@ -1150,20 +1116,12 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
         a.part_ml = a.part_o + n * c.head_dim;
     }
     const dim3 grid((unsigned)((units + 7) / 8 * 8), a.splits);
-#define KV4_RUN(HD, SLOTS, CT)                                                                                        \
-    hipLaunchKernelGGL((kv4_attention_kernel<HD, SLOTS, CT>), grid, dim3(kKv4Waves * 64), 0, st, a)
-#define KV4_SLOTS(HD)                                                                                                 \
-    do {                                                                                                              \
-        if (slots == 4) KV4_RUN(HD, 4, 1);                                                                            \
-        else if (slots == 2) KV4_RUN(HD, 2, 1);                                                                       \
-        else KV4_RUN(HD, 1, 1);                                                                                       \
-    } while (0)
-    if (c.head_dim == 64 && wide) KV4_RUN(64, 1, 2);
-    else if (c.head_dim == 64) KV4_SLOTS(64);
-    else if (c.head_dim == 128 && wide) KV4_RUN(128, 1, 2);
-    else if (c.head_dim == 128) KV4_SLOTS(128);
-    else KV4_SLOTS(256);
-#undef KV4_SLOTS
+#define KV4_RUN(HD, CT) hipLaunchKernelGGL((kv4_attention_kernel<HD, CT>), grid, dim3(kKv4Waves * 64), 0, st, a)
+    if (c.head_dim == 64 && wide) KV4_RUN(64, 2);
+    else if (c.head_dim == 64) KV4_RUN(64, 1);
+    else if (c.head_dim == 128 && wide) KV4_RUN(128, 2);
+    else if (c.head_dim == 128) KV4_RUN(128, 1);
+    else KV4_RUN(256, 1);
 #undef KV4_RUN
     ATLAS_LAUNCH_CHECK("kv4_attention");
     return ATLAS_OK;
