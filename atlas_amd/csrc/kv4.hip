@@ -227,6 +227,23 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, float* __restr
 // where f32 sums leave 1e-6, and take a third of the P V instructions less.)
 // The maximum is raised only when a score passes it by more than 2^8 (p then
 // stays below 2^8, far from any overflow); most chunks need no rescaling.
+//
+// What bounds it.  Decode reads 17/16 bytes an element pair: 16001 tokens of 32 heads
+// of 128 (70 MB) in 19.9 us, 3.5 TB/s; 10.7 of them pass between the first load and
+// the last, the others are the start, the last chunk's products and the join.  24
+// sequences of up to 8191 tokens, heads 32/8 of 64 (57 MB): 22.9 us.  A short context is
+// latency, a chain of kernel arguments, lengths and table, K and V, LDS, the store:
+// 4.9 us at 19 tokens.  Prompts are bound by the matrix instructions (of a chunk and 32
+// columns at head dim 128, 28 of 16 cycles for the scores and 48 of 16 for P V, the
+// latter's three parts) and the VALU beside them: 2048 rows of 32 heads of 128 in 86 us,
+// 400 TFLOP/s of the products asked for.
+// Why this shape.  16 columns, the least that the instructions have, and as few
+// registers as that leaves, so that three or four blocks of a CU have their loads on
+// their way (three or four chunks side by side in the 16 columns, where heads are
+// few, take fewer instructions a chunk but registers for as many buffers: 24
+// sequences of 32 heads of 128 took 70 us with them, 53 without).  32 columns for
+// prompts: a chunk's V is made bf16 once for both (three prompts of 36 to 1023 rows of 32
+// heads of 128: 67 us, 72 with 16).
 
 constexpr float kKv4Floor = -3.0e38f;  // running maximum of a row that has seen nothing
 constexpr float kKv4Lazy = 8.0f;
@@ -1070,9 +1087,10 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     a.out = out;
     a.ld_out = ld_out;
     a.group = n_heads / c.n_kv;
-    // 32 columns where the rows of a sequence fill more than 16 (head dim 256 has no
-    // registers for them)
-    const bool wide = c.head_dim < 256 && (long)b.n_rows * a.group > 16L * b.n_seqs;
+    // 32 columns where a sequence fills several such tiles (2048 rows of 32 heads of 128:
+    // 87 us, 92 with 16; 8 rows of 32 over 8 heads, 2000 tokens: 24 and 20); head dim 256
+    // has no registers for them
+    const bool wide = c.head_dim < 256 && (long)b.n_rows * a.group > 128L * b.n_seqs;
     a.tokens = b.row_starts ? (wide ? 32 : 16) / a.group : 1;
     a.tiles = b.row_starts ? a.c.n_rows / a.tokens + a.c.n_seqs : a.c.n_rows;
     a.scale = scale;
@@ -1091,15 +1109,17 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     // of the places before some of them have to wait.  (24 sequences of up to 8191 tokens,
     // heads 32/8 of 64: 23.8 us with 9/4 to a CU, 25.9 with 2, 28.9 with 11/4; of 128: 36 with
     // 15/8, 41 with 3/2, 36.5 with 21/8; up to 4000 tokens, heads 16/8 of 256: 33 with 3/2, 38 with
-    // 1, 40 with 2.)  At most 128 chunks to a run, 32 runs to a tile (64 of that
+    // 1, 40 with 2.  Of 64 for 64 sequences of up to 8000 tokens 50 with 3 and 67 with
+    // 9/4, which cut only the longest ones.)  At most 128 chunks to a run, 32 runs to a tile (64 of that
     // length), 256 MB of partial sums.
     // Runs are joined in 3 to 8 us, by the columns: up to 32 chunks are one run and
     // longer ones have 16 at least (900 tokens, 9 heads of 64 over 3: 9.3 us, 10.3 in runs
     // of 16; 8 rows of 32 over 8 of 128: 16.7 and 20.4; 2000 tokens of the former: 12.4 in
     // runs of 32, 10.1 of 16, 9.7 of 8; 300 tokens: 6.8 and, in runs of 8, 9.4); half of
     // both at head dim 256, where a chunk takes twice as long.
-    const int eighths = b.n_seqs == 1 ? 16 : wide || c.head_dim == 256 ? 12 : c.head_dim == 128 ? 15 : 18;
-    a.blocks = device_cu_count() * eighths / 8;
+    const int cus = device_cu_count();
+    const int eighths = b.n_seqs == 1 ? 16 : wide || c.head_dim == 256 ? 12 : c.head_dim == 128 ? 15 : units > cus ? 24 : 18;
+    a.blocks = cus * eighths / 8;
     a.min_run = c.head_dim == 256 ? 8 : 16;
     const size_t each = (size_t)units * a.cols * (c.head_dim + 2) * sizeof(float);
     const long want = std::max<long>(a.blocks * (b.n_seqs > 1 ? 2L : 1L) / units, (chunks + 127) / 128);
