@@ -260,6 +260,15 @@ def test_prompts(hd, group, n_kv, lens, rows):
     _check_attention(c, group * n_kv, pad_q=8, pad_o=4)
 
 
+@pytest.mark.parametrize("hd,group,n_kv", [(64, 4, 1), (128, 1, 2), (128, 7, 1), (256, 2, 1)])
+@pytest.mark.parametrize("rows", [[140, 70], [9, 40]])
+def test_prompts_in_runs(hd, group, n_kv, rows):
+    """Tiles of 16 and of 32 columns over caches that several blocks share."""
+    c = Case(rows[0] + group, [2500, 1300], rows, n_kv, hd, 64, tail_rows=2)
+    for _ in range(2):
+        _check_attention(c, group * n_kv)
+
+
 def test_many_sequences():
     """More sequences than lanes, empty ones among them, in one packed batch."""
     rng = np.random.default_rng(1)
