@@ -326,13 +326,15 @@ __global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* _
     const int i = lane & 31, h = lane >> 5, wm = wave / WN, wn = wave % WN;
     const uint32_t pitch = (uint32_t)kb * 16;
     const auto wbuf = mx_rows(w + (long)m0 * kb, min(m - m0, T::BM), pitch), xbuf = mx_rows(x + (long)n0 * kb, min(n - n0, T::BN), pitch);
-    const uint32_t voff = (lane >> 3) * pitch + (((lane & 7) ^ (lane >> 3)) * 16);
+    // of a load's eight rows, for those whose number has bit 3 clear and set
+    const uint32_t voff[2] = {(lane >> 3) * pitch + ((lane & 7) ^ (lane >> 4)) * 16, (lane >> 3) * pitch + ((lane & 7) ^ (lane >> 4) ^ 4) * 16};
     const auto load_codes = [&](int step, int buf) {
 #pragma unroll
         for (int l = 0; l < T::LOADS; ++l) {
             const int r8 = (wave * T::LOADS + l) * 8;    // first of the load's rows
-            if (r8 < T::BM) mx_load_lds(wbuf, voff + r8 * pitch + step * 128, codes + (buf * T::ROWS + r8) * 8);
-            else mx_load_lds(xbuf, voff + (r8 - T::BM) * pitch + step * 128, codes + (buf * T::ROWS + r8) * 8);
+            const uint32_t off = r8 & 8 ? voff[1] : voff[0];
+            if (r8 < T::BM) mx_load_lds(wbuf, off + r8 * pitch + step * 128, codes + (buf * T::ROWS + r8) * 8);
+            else mx_load_lds(xbuf, off + (r8 - T::BM) * pitch + step * 128, codes + (buf * T::ROWS + r8) * 8);
         }
     };
     const int sr = min((int)threadIdx.x, T::ROWS - 1);
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* _
         // fragments one quarter of a step ahead
         u32x4 fa[2][MT], fb[2][NT];
         const auto read = [&](int s) {
-            const int slot = (2 * s + h) ^ (i & 7);
+            const int slot = (2 * s + h) ^ (i >> 1 & 7);
 #pragma unroll
             for (int a = 0; a < MT; ++a) fa[s & 1][a] = codes[(buf * T::ROWS + (wm * MT + a) * 32 + i) * 8 + slot];
 #pragma unroll
