@@ -10,6 +10,7 @@ namespace atlas {
 // Both move bytes: 4 (f32) or 2 (bf16) in and 17/32 out for each element, or the
 // reverse.  A thread has 8 elements, so four lanes a block: one or two 16-byte
 // loads, a dword of codes, the block's largest magnitude by two DPP steps.
+// 11008 x 4096 from bf16 and back to f32 (318 MB): 57 us, 5.6 TB/s, a large copy's rate.
 
 typedef u32x4 __attribute__((aligned(4))) u32x4_dw;    // a row of f32 starts on any dword,
 typedef u32x4 __attribute__((aligned(2))) u32x4_hw;    // one of bf16 on any halfword,
@@ -214,7 +215,10 @@ struct MxUnit {
 
 // Few rows: the weights' stream.  A block has MT x 16 weight rows and NT x 16 rows
 // of x, its waves every WAVES-th unit of 512 elements, straight from global memory
-// into the matrix instructions' registers; their sums meet in LDS.
+// into the matrix instructions' registers; their sums meet in LDS.  Bound by the
+// weights' bytes: 22016 x 1 x 4096 (48 MB) in 10.4 us, 4.6 TB/s, 128000 x 1 x 2048 in 23.6,
+// 5.9; small ones by a launch's latency, 4 us.  (A unit on its way while the one before
+// is multiplied changes nothing: there are several waves to a SIMD.)
 template <int MT, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const u32x4* __restrict__ w, const uint8_t* __restrict__ ws,
                                                                 const u32x4* __restrict__ x, const uint8_t* __restrict__ xs,
@@ -270,8 +274,9 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const u32x4* __r
 // Many rows: tiles of BM weight rows x BN rows of x through LDS, 256 elements (a
 // 128-byte line of each row) at a time, two such steps deep: one loads while the
 // other is multiplied.
-//  * Codes reach LDS by direct loads, 16-byte chunk c of row r into slot c ^ (r & 7),
-//    so that the fragment reads (32 rows, one chunk) hit every bank alike.  Scale
+//  * Codes reach LDS by direct loads, 16-byte chunk c of row r into slot
+//    c ^ (r >> 1 & 7), so that the fragment reads (32 rows, one chunk) hit the 64 banks
+//    alike (no conflicts; with r & 7 there are 3.3 cycles to a read).  Scale
 //    bytes, whose rows start on any byte, go through registers, 8 to a thread.
 //  * v_mfma_scale_f32_32x32x64_f8f6f4, A = x, B = weights: lane (h, i) = 32 h + i gives
 //    block h of the 64 of row i, and has rows 8q + 4h + 0..3 (q = 0 .. 3) of column i,
@@ -279,6 +284,14 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const u32x4* __r
 //  * Past the end of a row lies the next one: codes there are numbers whatever they
 //    are, and their scale bytes are set to 0, 2^-254 for a product, which is zero in
 //    an f32.  Rows past the last one are multiplied and not stored.
+//  * What it reaches: 8192 x 4096 x 8192 in 166 us, 3.3 PFLOP/s, 11008 x 2047 x 4096 in 69,
+//    2.7, where a bare loop of these instructions makes 6.3 on such data (and the library's
+//    bf16 product of that size 1.3).  Of the 69 us the products are 29, y's 90 MB to
+//    memory 17, which a CU's one tile does not overlap, and a step's loads and barrier
+//    the rest.  No faster: steps of 128 elements in a ring of four (89 us: half a
+//    line to a request), 256 x 128 with three steps in LDS (78), the block's meeting
+//    before a step's last quarter (69; 5 % less with the small tiles, and 256 x 256 out of
+//    registers).
 constexpr int kMxStep = 8;            // blocks of a step
 
 // 16 bytes per lane from global memory to lds + 16 lane (lds wave-uniform); zeros
@@ -455,9 +468,8 @@ int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, con
         // The tile that takes least by the time of its rounds, in us for 4096 elements: a
         // CU does its 64 x 64 tiles at one per 6 us, and the first in 11; 128 x 128 at 14 and
         // 16; it has one at a time of 192 x 256, 35 us, and of 256 x 256, 43.
-        // Measured in this order: 2048 x 511 x 2048 6.4 10.3 16.5 20.2; 4096 x 2047 x 4096
-        // 47 28.8 29.8 34.3; 11008 x 2047 x 4096 176 78 69 79; 8192 x 4096 x 8192 (565)
-        // 304 245 166.
+        // Measured in this order: 4096 x 256 x 4096 12.5 18.0 29.6 34.8; 11008 x 2047 x 4096
+        // 119 77 69 78; 4096 x 4096 x 4096 100 56 64 46; 8192 x 4096 x 8192 366 203 182 166.
         const auto rounds = [&](long bm, long bn) { return ((m + bm - 1) / bm * ((n + bn - 1) / bn) + cus - 1) / cus; };
         const long t64 = std::max(6 * rounds(64, 64), 11L), t128 = std::max(14 * rounds(128, 128), 16L);
         const long t192 = 35 * rounds(192, 256), t256 = 43 * rounds(256, 256);
