@@ -289,6 +289,22 @@ def test_large_scores():
         _check_attention(c, 2, scale=-0.7)
 
 
+def test_scores_at_the_documented_limit():
+    """A score whose products sum to 0.98 2^127: a row that has seen only such has seen its tokens."""
+    c = Case(11, [1, 40], None, 1, 64, 32)
+    c.k[:] = 1.0
+    c.bytes = mx_ref.pages(c.k, c.v, 32)
+    scale = 0.98 * 2.0 ** 127 / 64
+    for sign in (-1, 1):
+        q, out = Dev(np.full((2, 64), sign, np.float32)), Dev(np.zeros((2, 64), np.float32))
+        check(lib().atlas_kv4_attention_f32(*c.upload(), q.ptr, 64, 1, scale, 0, out.ptr, 64))
+        sync()
+        vd = mx_ref.rounded(c.v)
+        want = np.stack([vd[[c.slot(s, t) for t in range(n)], 0].mean(0) for s, n in enumerate(c.lens)])
+        # equal scores: weights of exactly 1, sums of up to 40 of them
+        assert (np.abs(out.get() - want) <= 64 * 2.0 ** -23 * np.abs(vd).max()).all()
+
+
 def test_scale_zero_and_equal_scores():
     """Every weight the same: the mean of V."""
     c = Case(10, [333], None, 2, 64, 32)
