@@ -214,3 +214,39 @@ def test_chain_on_a_stream_and_in_a_graph():
                 assert (np.abs(y.get() - r @ wv.T) <= bound).all()
 
     on_thread(work)
+
+
+@pytest.mark.parametrize("m,n,kb", [(300, 1, (1 << 20) + 3), (520, 400, 1 << 20), (1024, 416, (1 << 20) - 1)])
+def test_gemm_rows_of_16_megabytes(m, n, kb):
+    """Operands past 4 GB, zero but for the first, a middle and the last block of some rows."""
+    from atlas_amd.tensor import _DevMem
+    rng = np.random.default_rng(kb + m)
+    blocks = [0, kb // 2 + 1, kb - 1]
+    rows, values, held = [], [], []
+    for count in (m, n):
+        data, scales = _DevMem(count * kb * 16, sync_alloc=True), _DevMem((count * kb + 3) // 4 * 4, sync_alloc=True)
+        held += [data, scales]
+        check(lib().atlas_memset_zero(data.ptr, data.nbytes))
+        check(lib().atlas_memset_zero(scales.ptr, scales.nbytes))
+        pick = sorted({0, count // 2, count - 1})
+        x = rng.standard_normal((len(pick), 3 * 32)).astype(np.float32)
+        codes, sc = mx_ref.matrix(x)
+        codes, sc = codes.reshape(len(pick), 3, 16), sc.reshape(len(pick), 3)
+        for r, row in enumerate(pick):
+            for b, at in enumerate(blocks):
+                for mem, src, width in ((data, codes[r, b], 16), (scales, sc[r, b:b + 1], 1)):
+                    src = np.ascontiguousarray(src)
+                    check(lib().atlas_memcpy_h2d(mem.ptr + (row * kb + at) * width, src.ctypes.data, src.nbytes))
+        rows.append(pick)
+        values.append(mx_ref.rounded(x))
+    y = Dev(np.full((n, m), 7, np.float32))
+    check(lib().atlas_gemm_mxfp4_f32(held[0].ptr, held[1].ptr, held[2].ptr, held[3].ptr, y.ptr, m, n, kb * 32, m))
+    sync()
+    want = np.zeros((n, m))
+    want[np.ix_(rows[1], rows[0])] = values[1] @ values[0].T
+    size = np.zeros((n, m))
+    size[np.ix_(rows[1], rows[0])] = np.abs(values[1]) @ np.abs(values[0]).T
+    # 96 products in three instructions, and at most 8 partial sums of which the others are zero
+    assert (np.abs(y.get() - want) <= 110 * 2.0 ** -23 * size).all()
+    for mem in held:
+        mem.free()
