@@ -206,6 +206,9 @@ class GpuMatrix:
     def upload_mxfp4(t) -> "GpuMatrix":
         """From an ``atlas_amd.quant.MxFp4Tensor`` (extension).  Products encode
         their activations as MXFP4 too: both operands have 4 bits."""
+        blocks = t.rows * -(-t.cols // 32)
+        if np.size(t.data) != 16 * blocks or np.size(t.scales) != blocks:
+            raise AtlasError(-1, f"upload_mxfp4: {t.rows} x {t.cols} has {blocks} blocks of 16 bytes and a scale")
         buf = _QuantBuf(np.ascontiguousarray(t.data, np.uint8), np.ascontiguousarray(t.scales, np.uint8), 0) \
             if cuda_available() else None
         return GpuMatrix(GpuBufKind.MXFP4 if buf else None, buf, t.rows, t.cols)
@@ -248,6 +251,8 @@ class GpuMatrix:
         if self.buf is None:
             return False
         assert self.cols == k
+        if self.kind is GpuBufKind.MXFP4 and np.size(rhs) != k * n:
+            raise AtlasError(-1, f"sgemm: a right operand of {k} x {n} expected")
         b = GpuBuf.upload(np.ascontiguousarray(rhs, np.float32).reshape(-1))
         c = GpuBuf.alloc(self.rows * n)
         if b is None or c is None:
@@ -263,6 +268,8 @@ class GpuMatrix:
         """Device-to-device GEMV; returns a new GpuVec (lib.rs:409-435)."""
         if self.buf is None or x.buf is None:
             return None
+        if self.kind is GpuBufKind.MXFP4 and x.len < self.cols * n:
+            raise AtlasError(-1, f"sgemm_vec: {n} x {self.cols} elements expected")
         out = GpuBuf.alloc(self.rows * n)
         if out is None:
             return None

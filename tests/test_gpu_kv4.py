@@ -215,6 +215,14 @@ def test_tokens_without_a_page():
     np.testing.assert_array_equal(c.d["cache"].get()[pages], before[pages])
 
 
+def test_sequences_that_share_pages():
+    """A page in the tables of several sequences, and twice in one's: read by all of them."""
+    c = Case(7, [100, 77, 128], None, 2, 128, 32, junk=False)
+    c.table[1, :2] = c.table[0, :2]
+    c.table[2] = c.table[0, 0]
+    _check_attention(c, 4)
+
+
 # ---- attention ----------------------------------------------------------------------
 
 

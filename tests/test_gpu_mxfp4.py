@@ -250,3 +250,15 @@ def test_gemm_rows_of_16_megabytes(m, n, kb):
     assert (np.abs(y.get() - want) <= 110 * 2.0 ** -23 * size).all()
     for mem in held:
         mem.free()
+
+
+def test_activations_that_are_too_few():
+    from atlas_amd._lib import AtlasError
+    from atlas_amd.quant import MxFp4Tensor
+    from atlas_amd.tensor import GpuMatrix, GpuVec
+    g = GpuMatrix.upload_mxfp4(MxFp4Tensor.quantize(np.ones((4, 96), np.float32)))
+    with pytest.raises(AtlasError):
+        g.sgemm_vec(GpuVec.from_slice(np.ones(95, np.float32)))
+    with pytest.raises(AtlasError):
+        g.sgemm(np.ones(95, np.float32), 96, 1, np.zeros(4, np.float32))
+    assert (g.sgemm_vec(GpuVec.from_slice(np.ones(96, np.float32))).download() == 96).all()

@@ -180,3 +180,14 @@ def test_sizes_past_the_limits(lib):
     for lens, table, rows in [([1 << 31], [[0]], [1]), ([1 << 32], [[0]], [0])]:
         with pytest.raises(AtlasError):
             Kv4Batch(lens, table, rows)
+
+
+def test_matrix_of_another_size_is_refused(lib):
+    """Codes and scales that are not those of rows x cols."""
+    from atlas_amd import AtlasError
+    from atlas_amd.quant import MxFp4Tensor
+    from atlas_amd.tensor import GpuMatrix
+    t = MxFp4Tensor.quantize(np.ones((3, 40), np.float32))
+    for kw in (dict(rows=4), dict(cols=65), dict(data=t.data[:-1]), dict(scales=t.scales[:-1])):
+        with pytest.raises(AtlasError):
+            GpuMatrix.upload_mxfp4(MxFp4Tensor(**{**t.__dict__, **kw}))
