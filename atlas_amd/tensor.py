@@ -478,9 +478,15 @@ class Kv4Batch:
         if rows.size != lens.size or (rows < 0).any() or (rows > lens).any() or (lens >= 1 << 31).any():
             raise AtlasError(-1, "Kv4Batch: each sequence has 0 <= new rows <= length < 2^31")
         lens = lens.astype(np.int32)
-        table = np.asarray(block_table, np.int64)
+        try:
+            table = np.asarray(block_table, np.int64)
+        except ValueError:
+            raise AtlasError(-1, "Kv4Batch: the block table's rows have one length") from None
+        if lens.size == 0 and table.size == 0:
+            table = table.reshape(0, 0)
+        if table.ndim != 2 or table.shape[0] != lens.size:
+            raise AtlasError(-1, f"Kv4Batch: a block table of shape {table.shape} for {lens.size} sequences")
         table = np.where((table < 0) | (table >= 1 << 31), -1, table).astype(np.int32)
-        table = table.reshape(lens.size, table.size // max(lens.size, 1))
         starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
         self.kv_lens, self.block_table, self.row_starts = lens, table, starts
         self.n_seqs, self.n_rows = lens.size, int(starts[-1])

@@ -191,3 +191,14 @@ def test_matrix_of_another_size_is_refused(lib):
     for kw in (dict(rows=4), dict(cols=65), dict(data=t.data[:-1]), dict(scales=t.scales[:-1])):
         with pytest.raises(AtlasError):
             GpuMatrix.upload_mxfp4(MxFp4Tensor(**{**t.__dict__, **kw}))
+
+
+def test_tables_of_another_number_of_sequences_are_refused(lib):
+    """A table is a row of pages for each sequence; its entries are never dealt out anew."""
+    from atlas_amd import AtlasError
+    from atlas_amd.tensor import Kv4Batch
+    four = np.arange(12).reshape(4, 3)
+    for lens, table in [([3, 4], four), ([3, 4], four.T), ([3], four[:2]), ([3, 4], four[:1]), ([3, 4], [1, 2]), ([3], [0, 1]),
+                        ([3, 4], 7), ([], four), ([3, 4], [[0, 1], [2]]), ([3, 4], four.reshape(2, 2, 3))]:
+        with pytest.raises(AtlasError):
+            Kv4Batch(lens, table)
