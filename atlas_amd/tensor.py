@@ -477,6 +477,8 @@ class Kv4Batch:
         rows = np.ones(lens.size, np.int64) if row_lens is None else np.asarray(row_lens, np.int64).reshape(-1)
         if rows.size != lens.size or (rows < 0).any() or (rows > lens).any() or (lens >= 1 << 31).any():
             raise AtlasError(-1, "Kv4Batch: each sequence has 0 <= new rows <= length < 2^31")
+        if rows.sum() >= 1 << 31:            # (row_starts are int32)
+            raise AtlasError(-1, f"Kv4Batch: {rows.sum()} rows")
         lens = lens.astype(np.int32)
         try:
             table = np.asarray(block_table, np.int64)

@@ -202,3 +202,12 @@ def test_tables_of_another_number_of_sequences_are_refused(lib):
                         ([3, 4], 7), ([], four), ([3, 4], [[0, 1], [2]]), ([3, 4], four.reshape(2, 2, 3))]:
         with pytest.raises(AtlasError):
             Kv4Batch(lens, table)
+
+
+def test_more_rows_than_row_starts_can_count(lib):
+    """Rows whose number an int32 does not hold, or holds as another one (2^32: 0), are refused."""
+    from atlas_amd import AtlasError
+    from atlas_amd.tensor import Kv4Batch
+    for n in (2, 3, 4, 5):
+        with pytest.raises(AtlasError):
+            Kv4Batch([1 << 30] * n, [[0]] * n, [1 << 30] * n)
