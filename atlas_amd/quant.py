@@ -122,7 +122,7 @@ class MxFp4Tensor:
             scale = np.where(self.scales == 255, np.float32(np.nan),
                              np.ldexp(np.float32(1), self.scales.astype(np.int32) - 127)).astype(np.float32)
             v = MXFP4_VALUES[codes] * scale[:, None]
-        return v.reshape(self.rows, -1)[:, :self.cols].astype(np.float32)
+        return v.reshape(self.rows, MXFP4_BLOCK_SIZE * -(-self.cols // MXFP4_BLOCK_SIZE))[:, :self.cols].astype(np.float32)
 
     def memory_bytes(self) -> int:
         return self.data.size + self.scales.size

@@ -211,3 +211,11 @@ def test_more_rows_than_row_starts_can_count(lib):
     for n in (2, 3, 4, 5):
         with pytest.raises(AtlasError):
             Kv4Batch([1 << 30] * n, [[0]] * n, [1 << 30] * n)
+
+
+def test_empty_matrices(lib):
+    """No rows, or rows of no columns: decoded to their shape."""
+    from atlas_amd.quant import MxFp4Tensor
+    for shape in [(0, 64), (0, 33), (3, 0), (0, 0)]:
+        t = MxFp4Tensor.quantize(np.zeros(shape, np.float32))
+        assert t.dequantize().shape == shape and t.memory_bytes() == 0
