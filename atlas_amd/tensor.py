@@ -284,11 +284,16 @@ class GpuMatrix:
         [n x rows] (extension, skinny MFMA GEMM)."""
         if self.buf is None or x.buf is None:
             raise AtlasError(-1, "sgemm_rows: operands are not on the GPU")
+        if self.kind is GpuBufKind.MXFP4 and x.len < n * self.cols:
+            raise AtlasError(-1, f"sgemm_rows: {n} rows of {self.cols} elements expected")
         out = GpuBuf.alloc(self.rows * n)
+        if out is None:
+            raise AtlasError(-3, f"sgemm_rows: no device memory for {n} rows of {self.rows} results")
         if self.kind is GpuBufKind.MXFP4:
-            if x.len < n * self.cols:
-                raise AtlasError(-1, f"sgemm_rows: {n} rows of {self.cols} elements expected")
-            self._launch_mxfp4(x.buf.ptr, out.ptr, n)
+            try:
+                self._launch_mxfp4(x.buf.ptr, out.ptr, n)
+            except MemoryError as e:         # the encoded activations
+                raise AtlasError(-3, f"sgemm_rows: {e}") from None
             return GpuVec(out, np.zeros(self.rows * n, np.float32), self.rows * n)
         fmt = {GpuBufKind.BF16: 1, GpuBufKind.INT8: 2, GpuBufKind.INT4: 3}[self.kind]
         scales = getattr(self.buf, "scales_ptr", None)

@@ -262,3 +262,21 @@ def test_activations_that_are_too_few():
     with pytest.raises(AtlasError):
         g.sgemm(np.ones(95, np.float32), 96, 1, np.zeros(4, np.float32))
     assert (g.sgemm_vec(GpuVec.from_slice(np.ones(96, np.float32))).download() == 96).all()
+
+
+def test_rows_without_memory():
+    """sgemm_rows says so when the results, or the encoded activations, find no memory, and works again after."""
+    from atlas_amd._lib import AtlasError
+    from atlas_amd.quant import MxFp4Tensor
+    from atlas_amd.tensor import GpuMatrix, GpuVec
+    g = GpuMatrix.upload_mxfp4(MxFp4Tensor.quantize(np.ones((4, 96), np.float32)))
+    x = GpuVec.from_slice(np.ones((3, 96), np.float32))
+    try:
+        for skip in range(3):                              # the results, the codes, the scales
+            lib().atlas_debug_fail_allocations(skip, 1)
+            with pytest.raises(AtlasError) as bad:
+                g.sgemm_rows(x, 3)
+            assert bad.value.code == -3
+    finally:
+        lib().atlas_debug_fail_allocations(0, 0)
+    assert (g.sgemm_rows(x, 3).download() == 96).all()

@@ -219,3 +219,31 @@ def test_empty_matrices(lib):
     for shape in [(0, 64), (0, 33), (3, 0), (0, 0)]:
         t = MxFp4Tensor.quantize(np.zeros(shape, np.float32))
         assert t.dequantize().shape == shape and t.memory_bytes() == 0
+
+
+class _Gone:
+    """Device memory that there is none of (a stand-in for it that holds nothing, and one that fails)."""
+    def __init__(self, nbytes, sync_alloc):
+        raise MemoryError(f"{nbytes} bytes")
+
+
+class _Held:
+    def __init__(self, ptr=4096):
+        self.ptr = self.scales_ptr = ptr
+
+
+def test_rows_without_memory(lib, monkeypatch):
+    """sgemm_rows reports a failed allocation as every caller of it expects: AtlasError with ATLAS_ENOMEM."""
+    import atlas_amd.tensor as tensor
+    from atlas_amd import AtlasError
+    x = tensor.GpuVec(_Held(), np.ones(96, np.float32), 96)
+    monkeypatch.setattr(tensor, "_DevMem", _Gone)
+    for kind in (tensor.GpuBufKind.MXFP4, tensor.GpuBufKind.BF16):
+        g = tensor.GpuMatrix(kind, _Held(), 4, 32)
+        with pytest.raises(AtlasError) as bad:
+            g.sgemm_rows(x, 3)
+        assert bad.value.code == -3
+    monkeypatch.setattr(tensor.GpuBuf, "alloc", staticmethod(lambda n: _Held()))
+    with pytest.raises(AtlasError) as bad:                 # the encoded activations
+        tensor.GpuMatrix(tensor.GpuBufKind.MXFP4, _Held(), 4, 32).sgemm_rows(x, 3)
+    assert bad.value.code == -3
