@@ -532,6 +532,14 @@ class GpuKv4Cache:
             if x.buf is None or x.len < batch.n_rows * wide:
                 raise AtlasError(-1, f"GpuKv4Cache: {batch.n_rows} rows of {wide} elements expected on the GPU")
 
+    @staticmethod
+    def _rows(batch: Kv4Batch, wide: int) -> GpuVec:
+        """The result's rows, cleared."""
+        out = GpuVec.zeros(batch.n_rows * wide)
+        if out.buf is None:
+            raise AtlasError(-3, f"GpuKv4Cache: no device memory for {batch.n_rows} rows of {wide} elements")
+        return out
+
     def write(self, batch: Kv4Batch, k: GpuVec, v: GpuVec) -> None:
         wide = self.c.n_kv * self.c.head_dim
         self._need(batch, (k, wide), (v, wide))
@@ -539,14 +547,14 @@ class GpuKv4Cache:
 
     def read(self, batch: Kv4Batch):
         wide = self.c.n_kv * self.c.head_dim
-        k, v = GpuVec.zeros(batch.n_rows * wide), GpuVec.zeros(batch.n_rows * wide)
+        k, v = self._rows(batch, wide), self._rows(batch, wide)
         check(load().atlas_kv4_read_f32(C.byref(self.c), C.byref(batch.c), k.buf.ptr, v.buf.ptr, wide))
         return k, v
 
     def attention(self, batch: Kv4Batch, q: GpuVec, n_heads: int, scale: float, window_size: int = 0) -> GpuVec:
         wide = n_heads * self.c.head_dim
         self._need(batch, (q, wide))
-        out = GpuVec.zeros(batch.n_rows * wide)
+        out = self._rows(batch, wide)
         check(load().atlas_kv4_attention_f32(C.byref(self.c), C.byref(batch.c), q.buf.ptr, wide, n_heads, scale,
                                              window_size, out.buf.ptr, wide))
         return out

@@ -673,3 +673,22 @@ def test_nothing_and_no_memory():
         assert g.sgemm(x, 64, 1, out) and (out == 64).all()
 
     on_thread(work)
+
+
+def test_rows_without_memory():
+    """Results of the cache's class that find no memory are reported; the cache is as it was."""
+    from atlas_amd.tensor import AtlasError, GpuKv4Cache, GpuVec, Kv4Batch
+    cache, batch = GpuKv4Cache.new(2, 32, 1, 64), Kv4Batch([3], [[1]], [3])
+    x = np.random.default_rng(8).standard_normal((3, 64)).astype(np.float32)
+    k = GpuVec.from_slice(x)
+    cache.write(batch, k, k)
+    try:
+        for skip, call in [(0, lambda: cache.read(batch)), (1, lambda: cache.read(batch)),
+                           (0, lambda: cache.attention(batch, k, 1, 0.1))]:
+            lib().atlas_debug_fail_allocations(skip, 1)
+            with pytest.raises(AtlasError) as bad:
+                call()
+            assert bad.value.code == -3
+    finally:
+        lib().atlas_debug_fail_allocations(0, 0)
+    np.testing.assert_array_equal(cache.read(batch)[1].download().reshape(3, 64), mx_ref.rounded(x).astype(np.float32))

@@ -247,3 +247,20 @@ def test_rows_without_memory(lib, monkeypatch):
     with pytest.raises(AtlasError) as bad:                 # the encoded activations
         tensor.GpuMatrix(tensor.GpuBufKind.MXFP4, _Held(), 4, 32).sgemm_rows(x, 3)
     assert bad.value.code == -3
+
+
+def test_cache_rows_without_memory(lib, monkeypatch):
+    """The same of a 4-bit cache's read and attention, which allocate their results."""
+    import atlas_amd.tensor as tensor
+    from atlas_amd import AtlasError
+    from atlas_amd._lib import Kv4BatchC, Kv4CacheC
+    cache = tensor.GpuKv4Cache(_Held(), Kv4CacheC(4096, 4, 64, 2, 64))
+    batch = object.__new__(tensor.Kv4Batch)
+    batch.n_rows, batch.c = 1, Kv4BatchC(None, 4096, 4096, 1, 1, 1, 3)
+    q = tensor.GpuVec(_Held(), np.ones(256, np.float32), 256)
+    monkeypatch.setattr(tensor, "cuda_available", lambda: True)
+    monkeypatch.setattr(tensor, "_DevMem", _Gone)
+    for call in (lambda: cache.read(batch), lambda: cache.attention(batch, q, 4, 1.0)):
+        with pytest.raises(AtlasError) as bad:
+            call()
+        assert bad.value.code == -3
