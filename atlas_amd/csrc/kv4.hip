@@ -573,17 +573,18 @@ struct Kv4Tile {
         // (the table's entries on their way before the lengths are here)
         pages = lane < a.c.table_stride ? a.c.table[(long)s * a.c.table_stride + lane] : -1;
         const int len = max(a.c.lens[s], 0);
-        int end = u + 1;
+        int end = u + 1, there = end;                    // of the sequence's rows, and of those that q and out have
         row0 = u;
         if (a.c.starts) {
             const int begin = max(a.c.starts[s], 0), skip = (u - (begin / a.tokens + s)) * a.tokens;
-            end = min(a.c.starts[s + 1], a.c.n_rows);
-            if (skip < 0 || skip >= end - begin) return false;
+            end = a.c.starts[s + 1];
+            there = min(end, a.c.n_rows);
+            if (skip < 0 || skip >= there - begin) return false;
             row0 = begin + skip;
         }
         // (all of it is the same in every lane; said here, the loops stay in scalar registers)
         row0 = __builtin_amdgcn_readfirstlane(row0);
-        rows = __builtin_amdgcn_readfirstlane(min(a.tokens, end - row0));
+        rows = __builtin_amdgcn_readfirstlane(min(a.tokens, there - row0));
         pos0 = __builtin_amdgcn_readfirstlane(len - (end - row0));
         cols = rows * a.group;
         tokens_end = min(pos0 + rows, a.c.cap);

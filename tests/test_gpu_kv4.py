@@ -692,3 +692,31 @@ def test_rows_without_memory():
     finally:
         lib().atlas_debug_fail_allocations(0, 0)
     np.testing.assert_array_equal(cache.read(batch)[1].download().reshape(3, 64), mx_ref.rounded(x).astype(np.float32))
+
+
+@pytest.mark.parametrize("have", [45, 50, 61, 64])
+@pytest.mark.parametrize("heads", [2, 16])
+def test_fewer_rows_than_the_starts_count(have, heads):
+    """Buffers that end inside a sequence's rows: each row that is there is the token that row_starts make it."""
+    c = Case(70 + have, [70, 40], [40, 25], 2, 64, 32)
+    wide = 2 * 64
+    k, v = (c.rng.standard_normal((have, 2, 64)).astype(np.float32) for _ in range(2))
+    q = c.rng.standard_normal((have, heads, 64)).astype(np.float32)
+    args = c.upload()
+    c.b.n_rows = have
+    kd, vd, qd = Dev(k), Dev(v), Dev(q)
+    ko, vo, out = Dev(np.zeros_like(k)), Dev(np.zeros_like(v)), Dev(np.zeros_like(q))
+    check(lib().atlas_kv4_write_f32(*args, kd.ptr, vd.ptr, wide))
+    check(lib().atlas_kv4_read_f32(*args, ko.ptr, vo.ptr, wide))
+    check(lib().atlas_kv4_attention_f32(*args, qd.ptr, heads * 64, heads, 0.125, 0, out.ptr, heads * 64))
+    sync()
+    np.testing.assert_array_equal(ko.get(), mx_ref.rounded(k).astype(np.float32))
+    rows = [(row, s, pos) for row, s, pos in c.each_row() if row < have]
+    for row, s, pos in rows:
+        c.k[c.slot(s, pos)], c.v[c.slot(s, pos)] = k[row], v[row]
+    kr, vr, got = mx_ref.rounded(c.k), mx_ref.rounded(c.v), out.get()
+    for row, s, pos in rows:
+        keys = np.arange(pos + 1)
+        at = np.array([c.slot(s, t) for t in keys])
+        x = q[row], keys, kr[at], vr[at], pos, 0.125, 0
+        assert (np.abs(got[row] - mx_ref.attend(*x)) <= _bound(*x)).all(), (row, s, pos)
