@@ -312,6 +312,31 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rows(const u32x4* p, int ro
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<u32x4*>(p), 0, rows * pitch, 0x00020000);
 }
 
+// Scale bytes of step `step` of a row of kb >= kMxStep blocks, from the eight that are loaded at
+// mx_bytes_at: a row's last step is its last eight bytes, those of the step before shifted out.
+constexpr int mx_bytes_at(int step, int kb) { return step * kMxStep < kb - kMxStep ? step * kMxStep : kb - kMxStep; }
+constexpr uint64_t mx_bytes(uint64_t v, int step, int kb) { return v >> (8 * (step * kMxStep - mx_bytes_at(step, kb))); }
+// The step whose bytes are loaded during step t: after the last one there is none to come,
+// and its own come again.  (With the load under a condition, as the codes' are, the kernels
+// take 16 to 55 registers more and the largest spills: 8192 x 4096 x 8192 207 us, 165 so.)
+constexpr int mx_ahead(int t, int steps) { return t + 1 < steps ? t + 1 : steps - 1; }
+
+// every byte of a row in its place, whatever the row's length
+constexpr bool mx_bytes_hold() {
+    for (int kb = kMxStep; kb <= 4 * kMxStep; ++kb) {
+        const int steps = (kb + kMxStep - 1) / kMxStep;
+        for (int t = -1; t < steps; ++t) {
+            const int step = mx_ahead(t, steps);
+            uint64_t v = 0, want = 0;
+            for (int j = 0; j < kMxStep; ++j) v |= (uint64_t)(mx_bytes_at(step, kb) + j + 1) << (8 * j);
+            for (int j = 0; j < kMxStep; ++j) want |= (uint64_t)(step * kMxStep + j < kb ? step * kMxStep + j + 1 : 0) << (8 * j);
+            if (mx_bytes(v, step, kb) != want) return false;
+        }
+    }
+    return true;
+}
+static_assert(mx_bytes_hold(), "scale bytes of a row's steps");
+
 template <int WM, int WN, int MT, int NT>
 struct MxTile {
     static constexpr int WAVES = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, ROWS = BM + BN;
@@ -352,15 +377,14 @@ __global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* _
     };
     const int sr = min((int)threadIdx.x, T::ROWS - 1);
     const uint8_t* const sp = sr < T::BM ? ws + (long)min(m0 + sr, m - 1) * kb : xs + (long)min(n0 + sr - T::BM, n - 1) * kb;
-    // A row's last step is its last eight bytes, those of the step before shifted
-    // out: by trim, once the bytes have come.
+    // (shifted out by trim, once the bytes have come)
     const auto load_bytes = [&](int step) {
-        if (kb >= kMxStep) return *reinterpret_cast<const u64_b*>(sp + min(step * kMxStep, kb - kMxStep));
+        if (kb >= kMxStep) return *reinterpret_cast<const u64_b*>(sp + mx_bytes_at(step, kb));
         uint64_t v = 0;
         for (int j = 0; j < kb; ++j) v |= (uint64_t)sp[j] << (8 * j);
         return v;
     };
-    const auto trim = [&](uint64_t v, int step) { return kb >= kMxStep ? v >> (8 * max(step * kMxStep - (kb - kMxStep), 0)) : v; };
+    const auto trim = [&](uint64_t v, int step) { return kb >= kMxStep ? mx_bytes(v, step, kb) : v; };
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int a = 0; a < MT; ++a)
@@ -375,11 +399,9 @@ __global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* _
     mx_meet();
     for (int t = 0; t < steps; ++t) {
         const int buf = t & 1;
-        uint64_t next = 0;
-        if (t + 1 < steps) {
-            load_codes(t + 1, buf ^ 1);
-            next = load_bytes(t + 1);
-        }
+        const int ahead = mx_ahead(t, steps);
+        if (t + 1 < steps) load_codes(ahead, buf ^ 1);
+        const uint64_t next = load_bytes(ahead);
         // h's byte of each pair in bytes 0 and 2
         u32x2 sa[MT], sb[NT];
 #pragma unroll
@@ -411,7 +433,7 @@ __global__ __launch_bounds__(WM * WN * 64) void mxfp4_tile_kernel(const u32x4* _
         multiply(std::integral_constant<int, 1>{});
         multiply(std::integral_constant<int, 2>{});
         multiply(std::integral_constant<int, 3>{});
-        bytes[(buf ^ 1) * T::ROWS + sr] = trim(next, t + 1);
+        bytes[(buf ^ 1) * T::ROWS + sr] = trim(next, ahead);
         mx_meet();
     }
 #pragma unroll
