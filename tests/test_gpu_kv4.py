@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from atlas_amd._lib import Kv4BatchC, Kv4CacheC, check
-from tests import mx_ref
+from tests import kv4_parts, mx_ref
 from tests.gpu_util import Dev, lib, sync
 from tests.stream_util import Stream, on_thread
 
@@ -720,3 +720,19 @@ def test_fewer_rows_than_the_starts_count(have, heads):
         at = np.array([c.slot(s, t) for t in keys])
         x = q[row], keys, kr[at], vr[at], pos, 0.125, 0
         assert (np.abs(got[row] - mx_ref.attend(*x)) <= _bound(*x)).all(), (row, s, pos)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form", kv4_parts.FORMS)
+def test_parts_of_q_and_of_the_weights(hd, form):
+    """As exact as the documented parts are: within a bound that two parts of q less, or one of the weights', pass
+    (tests/test_kv4_parts.py)."""
+    c, heads, q = kv4_parts.case(Case, hd, form)
+    scale = hd ** -0.5
+    at, want, size, parts = kv4_parts.outputs(c, heads, q, scale, kv4_parts.q_parts(hd), 3)
+    qd, out = Dev(q), Dev.empty(q.shape)
+    check(lib().atlas_kv4_attention_f32(*c.upload(), qd.ptr, heads * hd, heads, scale, 0, out.ptr, heads * hd))
+    sync()
+    left, limit = kv4_parts.error(out.get()[at], want, size), kv4_parts.limit(parts, want, size)
+    print(f"hd {hd} {form}: {left:.2e}, the parts {kv4_parts.error(parts, want, size):.2e}, limit {limit:.2e}", flush=True)
+    assert left <= limit
