@@ -350,7 +350,8 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
  * (A score's products, times scale, have to sum to less than 2^127 in magnitude.)
  * n_heads / n_kv in 1 .. 16.  One row to a sequence is decode, more are
  * (chunks of) prompts, whose K and V have to be written before.  A row that
- * sees no token gives zeros, one with an infinity or NaN in q NaN.  A token that
+ * sees no token gives zeros, whatever its q; of the others one with an infinity or
+ * NaN in q gives NaN.  A token that
  * reads as NaN is NaN to the rows that see it and nothing to the others.    */
 int atlas_kv4_attention_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch,
                             const float* q, int64_t ld_q, int n_heads, float scale, int window,

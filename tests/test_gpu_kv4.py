@@ -736,3 +736,70 @@ def test_parts_of_q_and_of_the_weights(hd, form):
     left, limit = kv4_parts.error(out.get()[at], want, size), kv4_parts.limit(parts, want, size)
     print(f"hd {hd} {form}: {left:.2e}, the parts {kv4_parts.error(parts, want, size):.2e}, limit {limit:.2e}", flush=True)
     assert left <= limit
+
+
+def _check_bad_tokens(c, heads, bad, window, q=None, blind=()):
+    """NaN where a row sees one of the tokens `bad` ((sequence, token, head, block of V or None for K)) or its q is not
+    finite (unless it sees nothing: rows `blind`), values elsewhere; twice, for what the first call leaves."""
+    hd, n_kv = c.hd, c.n_kv
+    k, v = c.k.copy(), c.v.copy()
+    for s, t, head, blk in bad:
+        at = c.slot(s, t)
+        if blk is None:
+            c.k[at, head, 5], k[at, head, :32] = np.nan, 0
+        else:
+            c.v[at, head, 32 * blk + 3], v[at, head, 32 * blk:32 * blk + 32] = np.nan, 0
+    c.bytes = mx_ref.pages(c.k, c.v, c.page)
+    k, v = mx_ref.rounded(k), mx_ref.rounded(v)
+    if q is None:
+        q = c.rng.standard_normal((c.n_rows, heads, hd)).astype(np.float32)
+    want, per = np.zeros(q.shape, bool), heads // n_kv
+    for row, s, pos in c.each_row():
+        for seq, t, head, blk in bad:
+            if seq == s and t <= pos and (not window or t > pos - window):
+                want[row, head * per:(head + 1) * per, slice(None) if blk is None else slice(32 * blk, 32 * blk + 32)] = True
+        if row not in blind:
+            want[row, ~np.isfinite(q[row]).all(-1)] = True
+    args, qd = c.upload(), Dev(q)
+    for _ in range(2):
+        out = Dev(np.full(q.shape, 7, np.float32))
+        check(lib().atlas_kv4_attention_f32(*args, qd.ptr, heads * hd, heads, hd ** -0.5, window, out.ptr, heads * hd))
+        sync()
+        got = out.get()
+        np.testing.assert_array_equal(np.isnan(got), want)
+    clean = np.where(np.isfinite(q).all(-1, keepdims=True), q, 0)
+    for row, s, pos in list(c.each_row())[::1 if c.n_rows < 16 else 9]:
+        keys = np.array([t for t in range(pos + 1) if c.slot(s, t) is not None], np.int64)
+        at = np.array([c.slot(s, t) for t in keys], np.int64)
+        x = clean[row], keys, k[at], v[at], pos, hd ** -0.5, window
+        ok = ~want[row]
+        assert (np.abs(got[row] - mx_ref.attend(*x))[ok] <= _bound(*x)[ok]).all(), (row, s, pos)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("part", ["k", "v"])
+@pytest.mark.parametrize("rows,group", [(1, 2), (5, 1), (70, 4)])
+def test_nan_tokens_in_runs(hd, part, rows, group):
+    """Several blocks to a sequence, 16 and 32 columns: NaN in a first, a middle and the last run, in each block of V."""
+    for bad, window in [([1200], 0), ([2499], 0), ([2455], 0), ([1100, 2410], 1400), ([10, 900], 1400)]:
+        c = Case(hd + rows + len(bad), [2500, 1500], None if rows == 1 else [rows, 1], 2, hd, 64, junk=False)
+        tokens = [(0, t, i % 2, None if part == "k" else t % (hd // 32)) for i, t in enumerate(bad)]
+        _check_bad_tokens(c, 2 * group, tokens, window)
+
+
+@pytest.mark.parametrize("hd,group", [(64, 2), (128, 1), (128, 2), (256, 2)])
+def test_query_not_finite_in_runs(hd, group):
+    c = Case(90 + hd, [2500], [90], 2, hd, 64)
+    q = c.rng.standard_normal((90, 2 * group, hd)).astype(np.float32)
+    q[3, 0, 1], q[40, 1, hd - 1], q[89, 0, 40] = np.nan, np.inf, -np.inf
+    _check_bad_tokens(c, 2 * group, [], 0, q)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_query_not_finite_and_nothing_to_see(hd):
+    """A row that sees no token is zero, whatever its q: before the sequence's start, or without a page."""
+    c = Case(95 + hd, [2, 40, 2000], [5, 1, 3], 2, hd, 32, junk=False)
+    c.table[1:] = -1
+    q = c.rng.standard_normal((9, 4, hd)).astype(np.float32)
+    q[1, 0, 1], q[4, 1, 2], q[5, 2, 3], q[7] = np.nan, np.inf, np.nan, np.inf
+    _check_bad_tokens(c, 4, [], 0, q, blind=(0, 1, 2, 5, 6, 7, 8))
