@@ -352,7 +352,9 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
  * (chunks of) prompts, whose K and V have to be written before.  A row that
  * sees no token gives zeros, whatever its q; of the others one with an infinity or
  * NaN in q gives NaN.  A token that
- * reads as NaN is NaN to the rows that see it and nothing to the others.    */
+ * reads as NaN is NaN to the rows that see it and nothing to the others.  (Scale
+ * bytes 253 and 254, which no encoder writes and whose larger codes are past f32's
+ * range, count as NaN in V.)                                                */
 int atlas_kv4_attention_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch,
                             const float* q, int64_t ld_q, int n_heads, float scale, int window,
                             float* out, int64_t ld_out);

@@ -803,3 +803,27 @@ def test_query_not_finite_and_nothing_to_see(hd):
     q = c.rng.standard_normal((9, 4, hd)).astype(np.float32)
     q[1, 0, 1], q[4, 1, 2], q[5, 2, 3], q[7] = np.nan, np.inf, np.nan, np.inf
     _check_bad_tokens(c, 4, [], 0, q, blind=(0, 1, 2, 5, 6, 7, 8))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_scale_bytes_past_the_encoders(hd):
+    """V's scale bytes 253 and 254, from elsewhere: NaN to the rows that see their token, nothing to the others;
+    252, the largest that is encoded, is a scale as any."""
+    c = Case(97 + hd, [90], [60], 1, hd, 32, junk=False)
+    d, kb = 16 * hd, hd // 32
+    seen = {253: 45, 254: 62, 255: 80}
+    c.v[c.slot(0, 33), 0, hd - 32:] = 0                    # codes of 0, whose scale changes nothing
+    c.bytes = mx_ref.pages(c.k, c.v, 32)
+    for byte, t in [(252, 33)] + list(seen.items()):
+        at = c.slot(0, t)
+        c.bytes[at // 32, 0, 2 * d + kb * 32:].reshape(4, kb, 8)[at % 32 // 8, kb - 1, at % 8] = byte
+    q = c.rng.standard_normal((60, 1, hd)).astype(np.float32)
+    for window in (0, 10):
+        args, qd, out = c.upload(), Dev(q), Dev.empty(q.shape)
+        check(lib().atlas_kv4_attention_f32(*args, qd.ptr, hd, 1, hd ** -0.5, window, out.ptr, hd))
+        sync()
+        want = np.zeros((60, 1, hd), bool)
+        for row, s, pos in c.each_row():
+            want[row, 0, hd - 32:] = any(t <= pos and (not window or t > pos - window) for t in seen.values())
+        np.testing.assert_array_equal(np.isnan(out.get()), want)
+        assert np.isfinite(out.get()[~want]).all()
