@@ -827,3 +827,22 @@ def test_scale_bytes_past_the_encoders(hd):
             want[row, 0, hd - 32:] = any(t <= pos and (not window or t > pos - window) for t in seen.values())
         np.testing.assert_array_equal(np.isnan(out.get()), want)
         assert np.isfinite(out.get()[~want]).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_values_at_the_documented_limit(hd):
+    """Elements of V that sum to 0.94 2^119 over 160 tokens, under weights that grow to 2^7.9 without a new maximum
+    (chunks of 32 tokens; the fifth follows the first in its wave)."""
+    c = Case(98 + hd, [160], None, 1, hd, 32)
+    at = np.array([c.slot(0, t) for t in range(160)])
+    c.k[:] = 0
+    c.k[at[128:], 0, 0] = 1
+    c.v[:] = 1.5 * 2.0 ** 111 * np.where(c.rng.random(c.v.shape) < 0.02, -1, 1)
+    c.bytes = mx_ref.pages(c.k, c.v, 32)
+    q = np.zeros((1, 1, hd), np.float32)
+    q[0, 0, 0] = 7.9 * np.log(2)
+    args, qd, out = c.upload(), Dev(q), Dev.empty(q.shape)
+    check(lib().atlas_kv4_attention_f32(*args, qd.ptr, hd, 1, 1.0, 0, out.ptr, hd))
+    sync()
+    x = q[0], np.arange(160), mx_ref.rounded(c.k)[at], mx_ref.rounded(c.v)[at], 159, 1.0, 0
+    assert (np.abs(out.get()[0] - mx_ref.attend(*x)) <= _bound(*x)).all()
