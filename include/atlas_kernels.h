@@ -321,7 +321,8 @@ typedef struct {
  * on) may be NULL for one row to a sequence.  Rows from row_starts[n_seqs] on
  * belong to no sequence: nothing is read or written for them.
  * A table entry outside [0, n_pages), and a token past the table, is a token
- * that is not there: not written, read as zeros, not attended to.           */
+ * that is not there: not written, read as zeros, not attended to.
+ * Up to 2^20 sequences and 2^20 rows (the attention: also limited as said there). */
 typedef struct {
     const int* row_starts;       /* [n_seqs + 1] or NULL                       */
     const int* kv_lens;          /* [n_seqs], the new rows included            */
@@ -350,7 +351,10 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
  * (A score's products, times scale, have to sum to less than 2^127 in magnitude,
  * and 2^8 times an element of V, summed over the tokens that a row sees, likewise:
  * weights are kept up to 2^8 before they are divided by their sum.)
- * n_heads / n_kv in 1 .. 16.  One row to a sequence is decode, more are
+ * n_heads / n_kv in 1 .. 16.  n_kv times the sequences, and with row_starts times
+ * (n_seqs + n_rows / r) for tiles of r rows (the whole part of 16 n_kv / n_heads; of
+ * 32 n_kv / n_heads, if head_dim is below 256, for more than 128 n_kv / n_heads rows to a
+ * sequence on average), is at most 2^23.  One row to a sequence is decode, more are
  * (chunks of) prompts, whose K and V have to be written before.  A row that
  * sees no token gives zeros, whatever its q; of the others one with an infinity or
  * NaN in q gives NaN.  A token that

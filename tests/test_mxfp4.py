@@ -264,3 +264,23 @@ def test_cache_rows_without_memory(lib, monkeypatch):
         with pytest.raises(AtlasError) as bad:
             call()
         assert bad.value.code == -3
+
+
+def test_batches_at_the_documented_limits(lib):
+    """One past each limit of the header is refused (what is within it would be launched)."""
+    from atlas_amd._lib import Kv4BatchC, Kv4CacheC
+    a, top = 4096, 1 << 20
+    one = C.byref(Kv4CacheC(a, 4, 64, 1, 64))
+    for n_seqs, n_rows in [(top + 1, 5), (5, top + 1)]:
+        b = C.byref(Kv4BatchC(a, a, a, 1, n_seqs, n_rows, 0))
+        for fn in (lib.atlas_kv4_write_f32, lib.atlas_kv4_read_f32):
+            _refused(lib, fn(one, b, a, a, 64))
+        _refused(lib, lib.atlas_kv4_attention_f32(one, b, a, 64, 1, 1.0, 0, a, 64))
+    # n_kv, n_heads, head_dim, sequences, rows (None: no row_starts): n_kv times the tiles is 2^23 + 1 at least
+    for n_kv, heads, hd, seqs, rows in [(9, 9, 64, 932068, None), (1025, 1025, 64, 8185, None), (8, 128, 256, 1, top),
+                                        (128, 128, 256, 1, top), (256, 256, 128, 1, top), (4096, 4096, 64, 2047, 32)]:
+        cache = C.byref(Kv4CacheC(a, 4, 64, n_kv, hd))
+        b = C.byref(Kv4BatchC(a if rows else None, a, a, 1, seqs, rows or seqs, 0))
+        per = 1 if rows is None else (32 if hd < 256 and rows * heads // n_kv > 128 * seqs else 16) * n_kv // heads
+        assert n_kv * (seqs if rows is None else seqs + rows // per) > 1 << 23
+        _refused(lib, lib.atlas_kv4_attention_f32(cache, b, a, heads * hd, heads, 1.0, 0, a, heads * hd))
