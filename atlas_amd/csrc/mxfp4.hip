@@ -482,7 +482,8 @@ int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, con
     // the weights for 64 rows of x or more, at 1.5 blocks to a CU (4096 x 64 x 4096: 7.1,
     // 11.3 in tiles; 4096 x 129 x 4096: 15.5 and 11.6).
     const long cus = device_cu_count(), m16 = (m + 15L) / 16, n16 = (n + 15L) / 16, m32 = (m + 31L) / 32, n32 = (n + 31L) / 32;
-    const bool long_rows = kb >= 1 << 20;                // more than a tile's buffers address
+    // more than a tile's buffers address, or none, where operands need not be there (a tile loads its first step whatever k is)
+    const bool long_rows = kb >= 1 << 20 || kb == 0;
     if (m16 * n16 <= cus || (n16 == 1 && m16 <= 4 * cus)) MX_ROWS(1, 1, 8);
     else if (n16 == 1 || m32 * n16 <= cus) MX_ROWS(2, 1, 4);
     else if (long_rows || 2 * m32 * n32 <= 3 * cus) MX_ROWS(2, 2, 8);

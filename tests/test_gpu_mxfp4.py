@@ -280,3 +280,29 @@ def test_rows_without_memory():
     finally:
         lib().atlas_debug_fail_allocations(0, 0)
     assert (g.sgemm_rows(x, 3).download() == 96).all()
+
+
+@pytest.mark.parametrize("m,n", [(40, 3), (3000, 16), (2050, 63), (4100, 129), (1500, 600), (4100, 1030), (11000, 1030)])
+def test_gemm_without_inner_elements(m, n):
+    """k = 0: zeros, and operands that are not there, in every kernel."""
+    y = Dev(np.full((n, m + 1), 7, np.float32))
+    check(lib().atlas_gemm_mxfp4_f32(None, None, None, None, y.ptr, m, n, 0, m + 1))
+    sync()
+    got = y.get()
+    assert (got[:, :m] == 0).all() and (got[:, m] == 7).all()
+
+
+@pytest.mark.parametrize("shift", [1, 3, 15])
+@pytest.mark.parametrize("m,n,k", [(300, 5, 1000), (2050, 129, 1056), (1500, 600, 100)])
+def test_gemm_scales_on_any_byte(m, n, k, shift):
+    rng = np.random.default_rng(m + shift)
+    held = [_operand(rng, rows, k, 0.5) for rows in (m, n)]
+    moved = []
+    for _, scales, _ in held:
+        s = scales.get().reshape(-1)
+        moved.append(Dev(np.concatenate([np.full(shift, 255, np.uint8), s, np.full(16, 255, np.uint8)])))
+    ys = [Dev.empty((n, m)) for _ in range(2)]
+    for y, ptrs in zip(ys, ([h[1].ptr for h in held], [d.ptr + shift for d in moved])):
+        check(lib().atlas_gemm_mxfp4_f32(held[0][0].ptr, ptrs[0], held[1][0].ptr, ptrs[1], y.ptr, m, n, k, m))
+    sync()
+    np.testing.assert_array_equal(ys[1].get(), ys[0].get())
