@@ -360,7 +360,7 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
  * NaN in q gives NaN.  A token that
  * reads as NaN is NaN to the rows that see it and nothing to the others.  (Scale
  * bytes 253 and 254, which no encoder writes and whose larger codes are past f32's
- * range, count as NaN in V.)                                                */
+ * range, count as NaN in V.)  out may be q, with ld_out = ld_q.              */
 int atlas_kv4_attention_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch,
                             const float* q, int64_t ld_q, int n_heads, float scale, int window,
                             float* out, int64_t ld_out);

@@ -846,3 +846,57 @@ def test_values_at_the_documented_limit(hd):
     sync()
     x = q[0], np.arange(160), mx_ref.rounded(c.k)[at], mx_ref.rounded(c.v)[at], 159, 1.0, 0
     assert (np.abs(out.get()[0] - mx_ref.attend(*x)) <= _bound(*x)).all()
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_caches_and_tables_without_pages(hd):
+    """A cache of no pages, a table of no columns, lengths below zero: nothing is there, and nothing is touched."""
+    rows = Dev(np.ones((4, 2 * hd), np.float32))
+    lens, starts, table = Dev(np.array([70, -3], np.int32)), Dev(np.array([0, 3, 4], np.int32)), Dev(np.zeros((2, 3), np.int32))
+    page = Dev(np.full((2, 32 * hd * 17 // 16), 0xA5, np.uint8))
+    past = Dev(np.ones((2, 3), np.int32))
+    for cache, table_ptr, stride in [(Kv4CacheC(None, 0, 32, 2, hd), table.ptr, 3), (Kv4CacheC(page.ptr, 1, 32, 2, hd), None, 0),
+                                     (Kv4CacheC(page.ptr, 1, 32, 2, hd), past.ptr, 3)]:
+        for starts_ptr, n_rows in ((starts.ptr, 4), (None, 2)):
+            batch = Kv4BatchC(starts_ptr, lens.ptr, table_ptr, stride, 2, n_rows, 0)
+            args = C.byref(cache), C.byref(batch)
+            ko, vo, out = (Dev(np.full((4, 2 * hd), 7, np.float32)) for _ in range(3))
+            check(lib().atlas_kv4_write_f32(*args, rows.ptr, rows.ptr, 2 * hd))
+            check(lib().atlas_kv4_read_f32(*args, ko.ptr, vo.ptr, 2 * hd))
+            check(lib().atlas_kv4_attention_f32(*args, rows.ptr, 2 * hd, 2, 1.0, 0, out.ptr, 2 * hd))
+            sync()
+            want = np.zeros((4, 2 * hd), np.float32)
+            want[n_rows:] = 7
+            for x in (ko, vo, out):
+                np.testing.assert_array_equal(x.get(), want)
+    assert (page.get() == 0xA5).all()
+
+
+def test_lengths_below_zero_beside_others():
+    """A sequence of length -1 or the least int32 sees nothing; its neighbour is not touched."""
+    c = Case(99, [40, 64, 33], None, 2, 64, 32)
+    args = c.upload()
+    _put(c.d["lens"], np.array([-1, 64, -(1 << 31)], np.int32))
+    q = c.rng.standard_normal((3, 4, 64)).astype(np.float32)
+    qd, out = Dev(q), Dev.empty(q.shape)
+    check(lib().atlas_kv4_attention_f32(*args, qd.ptr, 256, 4, 0.125, 0, out.ptr, 256))
+    sync()
+    got, keys = out.get(), np.arange(64)
+    assert (got[[0, 2]] == 0).all()
+    at = np.array([c.slot(1, t) for t in keys])
+    x = q[1], keys, mx_ref.rounded(c.k)[at], mx_ref.rounded(c.v)[at], 63, 0.125, 0
+    assert (np.abs(got[1] - mx_ref.attend(*x)) <= _bound(*x)).all()
+
+
+@pytest.mark.parametrize("lens,rows,heads", [([300, 40], None, 4), ([3000], None, 4), ([150, 40], [150, 9], 8), ([2500], [90], 4)])
+def test_attention_into_its_query(lens, rows, heads):
+    """out may be q: a tile's rows and heads are read by its own blocks, all of them before the results are stored."""
+    for hd in (64, 128, 256):
+        c = Case(sum(lens) + hd, lens, rows, 2, hd, 32)
+        args = c.upload()
+        q = c.rng.standard_normal((c.n_rows, heads, hd)).astype(np.float32)
+        qd, both, out = Dev(q), Dev(q), Dev.empty(q.shape)
+        for to, src in ((out, qd), (both, both)):
+            check(lib().atlas_kv4_attention_f32(*args, src.ptr, heads * hd, heads, hd ** -0.5, 0, to.ptr, heads * hd))
+        sync()
+        np.testing.assert_array_equal(both.get(), out.get())
