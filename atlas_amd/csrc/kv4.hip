@@ -219,10 +219,12 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, float* __restr
 //                     column i of O.
 // q in parts, for each block of 32: the first is q / 2^e rounded to E2M1 with the
 // block's largest value in [2, 4) 2^e, so at most 2^e / 2 off; each next one is the
-// remainder in units 8 times smaller.  7 parts leave 2^-20 of the block's largest
+// remainder in units 8 times smaller.  8 parts leave 2^-23 of the block's largest
 // value.  Products of two E2M1 numbers and their sums of 128 are exact in this
-// instruction.  (With E4M3 parts, 5 for the same 20 bits, it drops the low bits of
-// products far below the largest one: 4e-6 of a sum for normal q, against none.)
+// instruction.  (With E4M3 parts, 5 for 20 bits, it drops the low bits of
+// products far below the largest one: 4e-6 of a sum for normal q, against none.  7 parts
+// take 1 to 3 % less time and leave 2.3e-7 of an output at 20 to 60 tokens, where f32
+// sums, and these 8, leave 5e-8.)
 // P in three parts: its 24 bits.  (Two, rounded to nearest, leave 2^-18 of each p, 2.4e-6
 // of an output where f32 sums leave 1e-6, and take a third of the P V instructions less:
 // three prompts in 61 us, 67 with three parts.)
@@ -276,8 +278,7 @@ struct Kv4AttnArgs {
 // thread, and share the parts through LDS.
 template <int HD, int COLS>
 struct Kv4Query {
-    static constexpr int PARTS = HD == 64 ? 8 : 7;
-    static constexpr int N = HD == 64 ? 4 : HD == 128 ? 7 : 14;
+    static constexpr int PARTS = 8, N = PARTS * HD / 128;
     static constexpr int EIGHTS = HD / 8, ITEMS = COLS * EIGHTS;
     struct Shared {
         uint32_t part[PARTS][COLS][EIGHTS];

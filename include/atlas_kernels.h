@@ -347,7 +347,7 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
 /* Attention of the batch's query rows ([n_rows][n_heads * head_dim] f32, ld_q
  * elements apart) over the cached tokens: the row of token p sees tokens
  * max(0, p - window + 1) .. p (window 0: from the first on), scores times scale,
- * in f32 (K and V exactly as encoded, q to 2^-20 of its block's largest value).
+ * in f32 (K and V exactly as encoded, q to 2^-23 of its block's largest value).
  * (A score's products, times scale, have to sum to less than 2^127 in magnitude,
  * and 2^8 times an element of V, summed over the tokens that a row sees, likewise:
  * weights are kept up to 2^8 before they are divided by their sum.)

@@ -1,8 +1,7 @@
 """The roundings of the 4-bit attention, made again in NumPy: what its parts of q and of the weights leave of
 an output, and what would be missing without some of them.
 
-q times scale log2 e is a sum of E2M1 parts, each an eighth of the one before (8 at head dim 64, 7 at 128 and
-256); its products with K are exact and summed in f32.  A weight is exp2 of an f32 difference, to one last place,
+q times scale log2 e is a sum of eight E2M1 parts, each an eighth of the one before; its products with K are exact and summed in f32.  A weight is exp2 of an f32 difference, to one last place,
 and a sum of three bf16 parts, each cut off; their products with V are summed in f32, as are the weights.
 """
 import numpy as np
@@ -10,8 +9,7 @@ import numpy as np
 from tests import mx_ref
 
 
-def q_parts(hd):
-    return 8 if hd == 64 else 7
+Q_PARTS = 8
 
 
 def split(x, parts):
@@ -54,16 +52,15 @@ def attend(rng, q, k, v, scale, n_q, n_p=3):
 
 
 def error(got, want, size):
-    """Root mean square of the difference in units of the sums of magnitudes, where these are not zero."""
-    at = size > 0
-    return float(np.sqrt(np.mean(((got - want)[at] / size[at]) ** 2)))
+    """Root mean square of the difference, in units of the mean sum of magnitudes of each row and head."""
+    return float(np.sqrt(np.mean(((got - want) / size.mean(-1, keepdims=True)) ** 2)))
 
 
-def limit(parts, want, size):
+def limit(parts, want, size, steps=20, times=4):
     """What an output may be off by, in the units of `error`: four times what the parts' roundings leave by themselves,
     and the sums in the matrix units, which cut off what is below their last place, half a place (2^-24) a step: a
     row here has up to 4 chunks of 32 tokens with three parts each, and 4 waves' and 4 blocks' sums joined."""
-    return 4 * error(parts, want, size) + 20 * 2.0 ** -24 * error(want, 0 * want, size)
+    return times * error(parts, want, size) + steps * 2.0 ** -24 * error(want, 0 * want, size)
 
 
 FORMS = ["decode", "prompt16", "prompt32", "runs", "runs32"]
@@ -105,3 +102,15 @@ def outputs(c, heads, q, scale, n_q, n_p, every=1):
             size.append(p @ np.abs(v))
             got.append(attend(rng, q[row, h], k, v, scale, n_q, n_p))
     return tuple(np.array(places).T), np.array(want), np.array(size), np.array(got)
+
+
+SHORT_FORMS = ["prompt16", "prompt32"]                     # (single tokens run the kernel of the former)
+SHORT_STEPS = 5                                            # three parts of one chunk, its wave's sum, the division
+SHORT_SCALE = 12                                           # over sqrt(hd): scores far apart
+
+
+def short_case(make, hd, form):
+    """The same for rows that see 20 tokens at most, one chunk, so that q is what they are off by."""
+    group = 2 if form == "prompt16" else 8
+    c = make(3 * hd + len(form), [20], [20], 2, hd, 32)
+    return c, 2 * group, c.rng.standard_normal((20, 2 * group, hd)).astype(np.float32)

@@ -722,19 +722,33 @@ def test_fewer_rows_than_the_starts_count(have, heads):
         assert (np.abs(got[row] - mx_ref.attend(*x)) <= _bound(*x)).all(), (row, s, pos)
 
 
+def _left(case, scale, *terms):
+    """Error and limit of the outputs of a case of tests/kv4_parts.py."""
+    c, heads, q = case
+    at, want, size, parts = kv4_parts.outputs(c, heads, q, scale, kv4_parts.Q_PARTS, 3)
+    qd, out, wide = Dev(q), Dev.empty(q.shape), heads * c.hd
+    check(lib().atlas_kv4_attention_f32(*c.upload(), qd.ptr, wide, heads, scale, 0, out.ptr, wide))
+    sync()
+    left, limit = kv4_parts.error(out.get()[at], want, size), kv4_parts.limit(parts, want, size, *terms)
+    print(f"{left:.2e}, the parts {kv4_parts.error(parts, want, size):.2e}, limit {limit:.2e}", flush=True)
+    return left, limit
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("form", kv4_parts.FORMS)
 def test_parts_of_q_and_of_the_weights(hd, form):
     """As exact as the documented parts are: within a bound that two parts of q less, or one of the weights', pass
     (tests/test_kv4_parts.py)."""
-    c, heads, q = kv4_parts.case(Case, hd, form)
-    scale = hd ** -0.5
-    at, want, size, parts = kv4_parts.outputs(c, heads, q, scale, kv4_parts.q_parts(hd), 3)
-    qd, out = Dev(q), Dev.empty(q.shape)
-    check(lib().atlas_kv4_attention_f32(*c.upload(), qd.ptr, heads * hd, heads, scale, 0, out.ptr, heads * hd))
-    sync()
-    left, limit = kv4_parts.error(out.get()[at], want, size), kv4_parts.limit(parts, want, size)
-    print(f"hd {hd} {form}: {left:.2e}, the parts {kv4_parts.error(parts, want, size):.2e}, limit {limit:.2e}", flush=True)
+    left, limit = _left(kv4_parts.case(Case, hd, form), hd ** -0.5)
+    assert left <= limit
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form", kv4_parts.SHORT_FORMS)
+def test_every_part_of_q(hd, form):
+    """Few tokens and scores far apart, and a bound that one part of q less passes."""
+    case = kv4_parts.short_case(Case, hd, form)
+    left, limit = _left(case, kv4_parts.SHORT_SCALE * hd ** -0.5, kv4_parts.SHORT_STEPS, 2)
     assert left <= limit
 
 
