@@ -227,19 +227,20 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a, float* __restr
 // sums, and these 8, leave 5e-8.)
 // P in three parts: its 24 bits.  (Two, rounded to nearest, leave 2^-18 of each p, 2.4e-6
 // of an output where f32 sums leave 1e-6, and take a third of the P V instructions less:
-// three prompts in 61 us, 67 with three parts.)
+// three prompts in 61 us, 67 with three parts.  These figures, and the comparisons of shapes below, are with
+// seven parts of q on both sides.)
 // The maximum is raised only when a score passes it by more than 2^8 (p then
 // stays below 2^8, far from any overflow); most chunks need no rescaling.
 //
 // What bounds it.  Decode reads 17/16 bytes an element pair: 16001 tokens of 32 heads
-// of 128 (70 MB) in 19.9 us, 3.5 TB/s; 10.7 of them pass between the first load and
+// of 128 (70 MB) in 20.2 us, 3.5 TB/s; 10.7 of them pass between the first load and
 // the last, the others are the start, the last chunk's products and the join.  24
-// sequences of up to 8191 tokens, heads 32/8 of 64 (57 MB): 22.9 us.  A short context is
+// sequences of up to 8191 tokens, heads 32/8 of 64 (57 MB): 23.0 us.  A short context is
 // latency, a chain of kernel arguments, lengths and table, K and V, LDS, the store:
 // 4.9 us at 19 tokens.  Prompts are bound by the matrix instructions (of a chunk and 32
-// columns at head dim 128, 28 of 16 cycles for the scores and 48 of 16 for P V, the
-// latter's three parts) and the VALU beside them: 2048 rows of 32 heads of 128 in 86 us,
-// 400 TFLOP/s of the products asked for.
+// columns at head dim 128, 32 of 16 cycles for the scores and 48 of 16 for P V, the
+// latter's three parts) and the VALU beside them: 2048 rows of 32 heads of 128 in 87 us,
+// 390 TFLOP/s of the products asked for.
 // Why this shape.  16 columns, the least that the instructions have, and as few
 // registers as that leaves, so that three or four blocks of a CU have their loads on
 // their way (three or four chunks side by side in the 16 columns, where heads are
@@ -1113,8 +1114,10 @@ int kv4_attention_launch(const atlas_kv4_cache& c, const atlas_kv4_batch& b, con
     // heads 32/8 of 64: 23.8 us with 9/4 to a CU, 25.9 with 2, 28.9 with 11/4; of 128: 36 with
     // 15/8, 41 with 3/2, 36.5 with 21/8; up to 4000 tokens, heads 16/8 of 256: 33 with 3/2, 38 with
     // 1, 40 with 2.  Of 64 for 64 sequences of up to 8000 tokens 50 with 3 and 67 with
-    // 9/4, which cut only the longest ones.)  At most 128 chunks to a run, 32 runs to a tile (64 of that
-    // length), 256 MB of partial sums.
+    // 9/4, which cut only the longest ones.)  A tile has up to 32 runs, or as
+    // many as keep a run to 128 chunks, 64 at most (262144 tokens, and from there longer runs);
+    // 256 MB of partial sums.  So one sequence of 1, 2 or 4 KV heads works with 32, 64 or 128 blocks
+    // whatever its length: 32768 tokens of 128 take 18.5, 18.6 and 17.3 us, and of 32 heads 30.
     // Runs are joined in 3 to 8 us, by the columns: up to 32 chunks are one run and
     // longer ones have 16 at least (900 tokens, 9 heads of 64 over 3: 9.3 us, 10.3 in runs
     // of 16; 8 rows of 32 over 8 of 128: 16.7 and 20.4; 2000 tokens of the former: 12.4 in

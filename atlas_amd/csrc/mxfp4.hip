@@ -288,8 +288,10 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const u32x4* __r
 //    2.7, where a bare loop of these instructions makes 6.3 on such data (and the library's
 //    bf16 product of that size 1.3).  Of the 69 us the products are 29, y's 90 MB to
 //    memory 17, which a CU's one tile does not overlap, and a step's loads and barrier
-//    the rest.  No faster: steps of 128 elements in a ring of four (89 us: half a
-//    line to a request), 256 x 128 with three steps in LDS (78), the block's meeting
+//    the rest.  Rows of y that are not whole 128-byte lines cost much more, since these stores
+//    put no line together: 9001 x 3000 x 1024 takes 100 us and writes 138 MB for 108, where
+//    9024 takes 36 and writes 108.  No faster: steps of 128 elements in a ring of four (89 us: half
+//    a line to a request), 256 x 128 with three steps in LDS (78), the block's meeting
 //    before a step's last quarter (69; 5 % less with the small tiles, and 256 x 256 out of
 //    registers).
 constexpr int kMxStep = 8;            // blocks of a step
@@ -493,6 +495,9 @@ int mxfp4_gemm_launch(const uint8_t* w, const uint8_t* ws, const uint8_t* x, con
         // 16; it has one at a time of 192 x 256, 35 us, and of 256 x 256, 43.
         // Measured in this order: 4096 x 256 x 4096 12.5 18.0 29.6 34.8; 11008 x 2047 x 4096
         // 119 77 69 78; 4096 x 4096 x 4096 100 56 64 46; 8192 x 4096 x 8192 366 203 182 166.
+        // (Both sides are known at these k alone, and for rows of y that are whole lines; the
+        // rule has no k, and a short k's epilogue weighs more than it says: 11008 x 2047 x 512 takes
+        // 26 us, 18 of bytes.)
         const auto rounds = [&](long bm, long bn) { return ((m + bm - 1) / bm * ((n + bn - 1) / bn) + cus - 1) / cus; };
         const long t64 = std::max(6 * rounds(64, 64), 11L), t128 = std::max(14 * rounds(128, 128), 16L);
         const long t192 = 35 * rounds(192, 256), t256 = 43 * rounds(256, 256);
