@@ -294,7 +294,7 @@ int atlas_quantize_mxfp4_host(const float* w, int64_t rows, int64_t cols, uint8_
                               uint8_t* scales);
 /* Y[n, m] = sum_k X[n, k] W[m, k] of two MXFP4 matrices (W: m rows, X: n rows of
  * k elements), f32 sums; rows of Y lie ld >= m elements apart.  Any k, m up to 2^28, n up to 2^20.
- * w and x are 16-byte aligned (k = 0: not looked at).  Elements that fill up a last block have to be
+ * w and x are 16-byte aligned (k = 0: not read).  Elements that fill up a last block have to be
  * zero in one of the two, as the encoders leave them.                       */
 int atlas_gemm_mxfp4_f32(const uint8_t* w, const uint8_t* w_scales, const uint8_t* x,
                          const uint8_t* x_scales, float* y, int m, int n, int k, int64_t ld);
@@ -328,7 +328,8 @@ typedef struct {
     const int* kv_lens;          /* [n_seqs], the new rows included            */
     const int* block_table;      /* [n_seqs][table_stride]                     */
     int table_stride, n_seqs;
-    int n_rows;                  /* rows that k, v, q and out have             */
+    int n_rows;                  /* rows that k, v, q and out have; those past
+                                    them that row_starts count are left out    */
     int max_len;                 /* no kv_lens entry is larger, as far as the
                                     caller knows (0: what the table holds): only
                                     how the work is split goes by it           */

@@ -1,8 +1,9 @@
 """The roundings of the 4-bit attention, made again in NumPy: what its parts of q and of the weights leave of
 an output, and what would be missing without some of them.
 
-q times scale log2 e is a sum of eight E2M1 parts, each an eighth of the one before; its products with K are exact and summed in f32.  A weight is exp2 of an f32 difference, to one last place,
-and a sum of three bf16 parts, each cut off; their products with V are summed in f32, as are the weights.
+q times scale log2 e is a sum of eight E2M1 parts, each an eighth of the one before; its products with K are exact
+and summed in f32.  A weight is exp2 of an f32 difference, to one last place, and a sum of three bf16 parts, each cut
+off; their products with V are summed in f32, as are the weights.
 """
 import numpy as np
 
