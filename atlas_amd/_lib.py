@@ -55,6 +55,25 @@ class Kv4BatchC(C.Structure):
                 ("table_stride", C.c_int), ("n_seqs", C.c_int), ("n_rows", C.c_int), ("max_len", C.c_int)]
 
 
+class SlotCacheC(C.Structure):
+    """atlas_slot_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_slots", C.c_int), ("max_seq", C.c_int), ("n_kv", C.c_int),
+                ("head_dim", C.c_int)]
+
+
+class PrefixBatchC(C.Structure):
+    """atlas_prefix_batch"""
+    _fields_ = [("group_starts", C.c_void_p), ("prefix_slots", C.c_void_p), ("prefix_lens", C.c_void_p),
+                ("kv_lens", C.c_void_p), ("slots", C.c_void_p), ("slot_stride", C.c_int), ("n_groups", C.c_int),
+                ("n_rows", C.c_int), ("max_prefix", C.c_int), ("max_own", C.c_int)]
+
+
+class LoraC(C.Structure):
+    """atlas_lora"""
+    _fields_ = [("fmt", C.c_int), ("a", C.c_void_p), ("b", C.c_void_p), ("scales", C.c_void_p),
+                ("n_adapters", C.c_int), ("rank", C.c_int), ("m", C.c_int), ("k", C.c_int)]
+
+
 HOOK_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c_int,
                       C.POINTER(C.c_float))
 TOKEN_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint32)
@@ -134,6 +153,10 @@ SIGNATURES = {
     "atlas_kv4_write_f32": (I, [C.POINTER(Kv4CacheC), C.POINTER(Kv4BatchC), P, P, I64]),
     "atlas_kv4_read_f32": (I, [C.POINTER(Kv4CacheC), C.POINTER(Kv4BatchC), P, P, I64]),
     "atlas_kv4_attention_f32": (I, [C.POINTER(Kv4CacheC), C.POINTER(Kv4BatchC), P, I64, I, F, I, P, I64]),
+    "atlas_prefix_attention_f32": (I, [C.POINTER(SlotCacheC), C.POINTER(PrefixBatchC), P, I64, I, F, I, P, I64]),
+    "atlas_beam_select_f32": (I, [P, I64, I, P, I, I, I, P, P, P]),
+    "atlas_beam_reorder": (I, [C.POINTER(P), C.POINTER(P), I, I64, I64, P, I, I]),
+    "atlas_lora_add_f32": (I, [C.POINTER(LoraC), P, P, I64, P, I64, P, I64, I]),
     "atlas_fill_random": (I, [I, P, I64, U64, F, F]),
     # engine (include/atlas_engine.h)
     "atlas_model_create": (P, [C.POINTER(ModelConfigC)]),

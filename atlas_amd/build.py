@@ -25,6 +25,7 @@ OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libatlas_kernels.so")
 
 SOURCES = ["gemv.hip", "skinny.hip", "prompt_gemm.hip", "attention.hip", "fused.hip", "mxfp4.hip", "kv4.hip",
+           "prefix.hip", "beam.hip", "lora.hip",
            "errors.cpp", "runtime.cpp",
            "capi.cpp", "engine.cpp", "st_format.cpp", "loader.cpp", "blas.cpp"]
 

@@ -7,6 +7,7 @@
 #include "common.hpp"
 #include "fused.hpp"
 #include "gemv.hpp"
+#include "many.hpp"
 #include "mxfp4.hpp"
 
 using namespace atlas;
@@ -329,6 +330,30 @@ ATLAS_API int atlas_kv4_attention_f32(const atlas_kv4_cache* c, const atlas_kv4_
                                       int64_t ld_out) {
     ATLAS_REQUIRE(c && b, "kv4_attention: null argument");
     return kv4_attention_launch(*c, *b, q, (long)ld_q, n_heads, scale, window, out, (long)ld_out, stream());
+}
+
+ATLAS_API int atlas_prefix_attention_f32(const atlas_slot_cache* c, const atlas_prefix_batch* b, const float* q,
+                                         int64_t ld_q, int n_heads, float scale, int window, float* out,
+                                         int64_t ld_out) {
+    ATLAS_REQUIRE(c && b, "prefix_attention: null argument");
+    return prefix_attention_launch(*c, *b, q, (long)ld_q, n_heads, scale, window, out, (long)ld_out, Workspace{}, stream());
+}
+
+ATLAS_API int atlas_beam_select_f32(const float* logits, int64_t ld, int vocab, const double* scores, int n_groups,
+                                    int width, int n_out, uint32_t* tokens, int* parents, double* out_scores) {
+    return beam_select_launch(logits, (long)ld, vocab, scores, n_groups, width, n_out, tokens, parents, out_scores,
+                              Workspace{}, stream());
+}
+
+ATLAS_API int atlas_beam_reorder(void* const* dst, const void* const* src, int n_states, int64_t row_bytes,
+                                 int64_t row_stride, const int* parents, int n_groups, int width) {
+    return beam_reorder_launch(dst, src, n_states, (long)row_bytes, (long)row_stride, parents, n_groups, width, stream());
+}
+
+ATLAS_API int atlas_lora_add_f32(const atlas_lora* l, const int* adapters, const float* x, int64_t ld_x, const float* base,
+                                 int64_t ld_base, float* y, int64_t ld_y, int n) {
+    ATLAS_REQUIRE(l, "lora_add: null argument");
+    return lora_add_launch(*l, adapters, x, (long)ld_x, base, (long)ld_base, y, (long)ld_y, n, stream());
 }
 
 ATLAS_API int atlas_fill_random(int kind, void* out, int64_t n, uint64_t seed, float a, float b) {

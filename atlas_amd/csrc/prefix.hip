@@ -1,0 +1,535 @@
+// prefix.hip -- decode attention of rows that share their first tokens, over an f32
+// cache of slots.
+//
+// The rows of a group (a prompt's beams, requests over one system prompt) see the
+// same first tokens, which lie in one slot; their own follow, each in a slot that a
+// table names.  A tile is up to 16 CT columns of (row, head of the KV head's group):
+// the shared tokens are read once for all of them, and their products are matrix
+// instructions.  A row's own tokens go through the same instructions, seen by its
+// columns only.
+#include <algorithm>
+
+#include "many.hpp"
+
+namespace atlas {
+
+constexpr float kPfFloor = -3.0e38f;   // running maximum of a column that has seen nothing
+constexpr float kPfLazy = 8.0f;
+constexpr float kPfLog2e = 1.4426950408889634f;
+constexpr int kPfWaves = 4;
+constexpr int kPfChunk = 16;           // tokens that a wave takes at a time
+constexpr int kPfMaxSplits = 64;
+
+struct PfArgs {
+    const float *k, *v;
+    int n_slots, max_seq, n_kv;
+    const int *starts, *prefix_slots, *prefix_lens, *lens, *slots;
+    int slot_stride, n_groups, n_rows;
+    const float* q;
+    long ld_q;
+    float* out;
+    long ld_out;
+    int group;                         // heads of a KV head
+    int rows;                          // of a tile, at most
+    int tiles;                         // of the batch, some of them empty
+    float scale;
+    int window;
+    int splits, cols;                  // blocks of a tile and KV head at most; [tiles][n_kv][splits][cols] partial sums
+    float *part_o, *part_ml;
+    int* counters;                     // [tiles][n_kv] blocks that are done, zero between calls
+};
+
+// The group of the batch's tile u.  Tiles of group g begin at starts[g] / rows + g,
+// which leaves each group as many as it needs, whatever the sizes.
+__device__ __forceinline__ int pf_group(const PfArgs& a, int u) {
+    int lo = 0, hi = a.n_groups;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.starts[mid] / a.rows + mid <= u) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// partial sums past this XCD's L2 and back (agent scope)
+__device__ __forceinline__ void pf_put(float* p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void pf_get(const float* p, float& a, float& b) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    a = __uint_as_float((uint32_t)v);
+    b = __uint_as_float((uint32_t)(v >> 32));
+}
+
+// What a tile's rows see: the shared tokens [first, last), and `own` tokens of their
+// own in the rows' order, row r's from own_at[r] on.
+template <int CT>
+struct PfRows {
+    int from[16 * CT], to[16 * CT];    // a row sees tokens [from, to)
+    int own_from[16 * CT];             // its first own one that is seen
+    int own_at[16 * CT + 1];
+};
+
+template <int HD, int CT>
+struct PfShared {
+    union {
+        f32x4 q[CT][HD / 16][64];      // [column tile][step of 16 elements][lane]
+        float o[kPfWaves][16][HD + 4]; // the waves' sums of a column tile
+        float f[kPfMaxSplits][16 * CT];    // the runs' factors
+    };
+    float m[kPfWaves][16 * CT], l[kPfWaves][16 * CT];
+    float sum[16 * CT];                // the columns' sums of weights
+    PfRows<CT> rows;
+    int last;
+};
+
+__device__ __forceinline__ bool pf_infinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+
+template <int HD, int CT>
+__global__ __launch_bounds__(kPfWaves * 64) void pf_attention_kernel(PfArgs a) {
+    constexpr int S = HD / 16, H = HD / 64, R = 16 * CT;
+    __shared__ PfShared<HD, CT> sh;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    // block -> (tile, KV head, split): consecutive blocks run on different XCDs; the
+    // tiles of a KV head and split, which read the same tokens if their group is the
+    // same, come one after the other on one
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, pair = at / a.tiles * 8 + xcd, u = at % a.tiles;
+    if (pair >= a.n_kv * a.splits) return;
+    const int split = pair / a.n_kv, kvh = pair - split * a.n_kv;
+
+    // ---- the tile's rows
+    int grp = 0, row0 = u * a.rows, end = a.n_rows;
+    if (a.starts) {
+        grp = __builtin_amdgcn_readfirstlane(pf_group(a, u));
+        const int begin = min(max(a.starts[grp], 0), a.n_rows), skip = (u - (a.starts[grp] / a.rows + grp)) * a.rows;
+        end = min(a.starts[grp + 1], a.n_rows);
+        if (skip < 0 || skip >= end - begin) return;
+        row0 = begin + skip;
+    }
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    const int n_rows = __builtin_amdgcn_readfirstlane(min(a.rows, end - row0)), cols = n_rows * a.group;
+    const int shared_len = max(a.prefix_lens[grp], 0), shared_slot = a.prefix_slots[grp];
+    const bool cells = a.n_slots > 0 && a.max_seq > 0;
+    const int own_cap = cells ? min(a.slot_stride ? a.slot_stride : a.max_seq, max(a.max_seq - shared_len, 0)) : 0;
+    if (wave == 0) {
+        // rows beyond the last see nothing
+        const bool mine = lane < n_rows;
+        const int len = mine ? max(a.lens[row0 + lane], 0) : 0;
+        const int from = a.window > 0 && len > a.window ? len - a.window : 0;
+        const int own_from = max(from - shared_len, 0), own = max(min(len - shared_len, own_cap) - own_from, 0);
+        int sum = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += x;
+        }
+        if (lane < R) {
+            sh.rows.from[lane] = from;
+            sh.rows.to[lane] = len;
+            sh.rows.own_from[lane] = own_from;
+            sh.rows.own_at[lane + 1] = sum;
+        }
+        if (lane == 0) sh.rows.own_at[0] = 0;
+    }
+    // the query, scaled for exp2; columns past the last repeat it
+    for (int e = threadIdx.x; e < CT * S * 64; e += kPfWaves * 64) {
+        const int l = e & 63, s = e / 64 % S, c = min(e / (64 * S) * 16 + (l & 15), cols - 1), row = c / a.group;
+        const float* p = a.q + (row0 + row) * a.ld_q + ((long)kvh * a.group + c - row * a.group) * HD + s * 16 + (l >> 4) * 4;
+        sh.q[0][0][e] = *reinterpret_cast<const f32x4*>(p) * (a.scale * kPfLog2e);
+    }
+    __syncthreads();
+    // what every row sees, and what any does
+    int lo = 0x7FFFFFFF, hi = 0, lo_all = 0, hi_all = 0x7FFFFFFF;
+    for (int r = 0; r < n_rows; ++r) {
+        const int f = sh.rows.from[r], t = sh.rows.to[r];
+        if (t > f) lo = min(lo, f);
+        hi = max(hi, t);
+        lo_all = max(lo_all, f);
+        hi_all = min(hi_all, t);
+    }
+    const bool there = cells && shared_slot >= 0 && shared_slot < a.n_slots;
+    const int last = there ? min(min(shared_len, a.max_seq), hi) : 0, first = min(lo, last);
+    const int own = sh.rows.own_at[n_rows];
+    const int shared_chunks = (last - first + kPfChunk - 1) / kPfChunk;
+    const int chunks = __builtin_amdgcn_readfirstlane(shared_chunks + (own + kPfChunk - 1) / kPfChunk);
+    // the block's run
+    const int run = (max((chunks + a.splits - 1) / a.splits, 2 * kPfWaves) + kPfWaves - 1) / kPfWaves * kPfWaves;
+    const int begin = split * run, stop = min(begin + run, chunks);
+    if (split > 0 && begin >= chunks) return;
+    const int runs = max((chunks + run - 1) / run, 1);
+
+    int col_row[CT], from[CT], to[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const int col = 16 * c + i;
+        col_row[c] = col < cols ? col / a.group : -1;
+        from[c] = col < cols ? sh.rows.from[col / a.group] : 0;
+        to[c] = col < cols ? sh.rows.to[col / a.group] : 0;
+    }
+    f32x4 o[CT][H][4];
+    float m[CT], l[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        m[c] = kPfFloor;
+        l[c] = 0.f;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][h][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const long pitch = (long)a.n_kv * HD;
+    const float *const kb = a.k + (long)kvh * HD, *const vb = a.v + (long)kvh * HD;
+#pragma unroll 1
+    for (int chunk = begin + wave; chunk < stop; chunk += kPfWaves) {
+        // Token i of the chunk: its cell (one that is not there: some cell that is, and
+        // `live` says so), and the row that it belongs to (-1: shared).
+        long cell;
+        int row, t;
+        bool live, plain;
+        if (chunk < shared_chunks) {
+            t = first + chunk * kPfChunk + i;
+            live = t < last;
+            cell = (long)shared_slot * a.max_seq + min(t, last - 1);
+            row = -1;
+            const int c0 = first + chunk * kPfChunk;
+            plain = c0 >= lo_all && c0 + kPfChunk <= min(hi_all, last);
+        } else {
+            const int e = (chunk - shared_chunks) * kPfChunk + i;
+            int r = 0, r_end = n_rows;
+            while (r_end - r > 1) {
+                const int mid = (r + r_end) >> 1;
+                if (sh.rows.own_at[mid] <= e) r = mid;
+                else r_end = mid;
+            }
+            row = r;
+            const int x = e - sh.rows.own_at[r] + sh.rows.own_from[r];
+            live = e < own;
+            const int slot = live ? a.slots[(long)(row0 + r) * max(a.slot_stride, 1) + (a.slot_stride ? x : 0)] : -1;
+            live = slot >= 0 && slot < a.n_slots;
+            t = shared_len + x;
+            cell = live ? (long)slot * a.max_seq + t : 0;
+            plain = false;
+        }
+        f32x4 kf[S], vf[4][H];
+        {
+            const float* p = kb + cell * pitch + 4 * g;
+#pragma unroll
+            for (int s = 0; s < S; ++s) kf[s] = *reinterpret_cast<const f32x4*>(p + 16 * s);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const long vc = __shfl(cell, 4 * g + r, 64);
+                const float* pv = vb + vc * pitch + 4 * i;
+#pragma unroll
+                for (int h = 0; h < H; ++h) vf[r][h] = *reinterpret_cast<const f32x4*>(pv + 64 * h);
+            }
+        }
+        // S: tokens 4g + r of column i
+        float sc[CT][4];
+        {
+            f32x4 d[CT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) d[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const f32x4 qf = sh.q[c][s][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[s][e], qf[e], d[c], 0, 0, 0);
+                }
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[c][r] = d[c][r];
+        }
+        uint32_t seen[CT];
+        if (!plain) {
+            // (without short circuits, which would be branches)
+            int tok_row[4], tok[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                tok_row[r] = __shfl(row, 4 * g + r, 64);
+                tok[r] = __shfl(live ? t : -1, 4 * g + r, 64);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                seen[c] = 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t ok = (uint32_t)(tok[r] >= from[c]) & (uint32_t)(tok[r] < to[c]) &
+                                        ((uint32_t)(tok_row[r] < 0) | (uint32_t)(tok_row[r] == col_row[c]));
+                    seen[c] |= ok << r;
+                    sc[c][r] = ok ? sc[c][r] : -__builtin_inff();
+                }
+            }
+        }
+        // weights; the maximum is raised only when a score passes it by more than 2^8
+        f32x4 p[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            float top = fmaxf(fmaxf(sc[c][0], sc[c][1]), fmaxf(sc[c][2], sc[c][3]));
+            if (__any(top > m[c] + kPfLazy)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float up = fmaxf(m[c], top), down = __builtin_amdgcn_exp2f(m[c] - up);
+                m[c] = up;
+                l[c] *= down;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[c][h][e] *= down;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[c][r] = __builtin_amdgcn_exp2f(sc[c][r] - m[c]);
+                l[c] += p[c][r];
+            }
+        }
+        if (!plain) {
+            // Infinities and NaN of V are nothing to the columns that do not see their
+            // token: they leave the matrix product and are added where they are seen.
+            bool bad = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bad = bad || pf_infinite(vf[r][h][e]);
+            if (__any(bad)) {
+#pragma unroll 1
+                for (int gt = 0; gt < 4; ++gt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) {
+                            const float w = __shfl(p[c][r], 16 * gt + i, 64);
+                            const bool ok = __shfl((int)(seen[c] >> r & 1u), 16 * gt + i, 64) != 0;
+#pragma unroll
+                            for (int h = 0; h < H; ++h)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                    for (int x = 0; x < 4; ++x) {
+                                        const float y = __shfl(vf[r][h][e], 16 * gt + 4 * g + x, 64);
+                                        if (ok && pf_infinite(y)) o[c][h][e][x] += w * y;
+                                    }
+                        }
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (pf_infinite(vf[r][h][e])) vf[r][h][e] = 0.f;
+            }
+        }
+        // O^T += V^T P: elements 64 h + 4 (4g + r) + e of column i
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+                        o[c][h][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][h][e], p[c][r], o[c][h][e], 0, 0, 0);
+    }
+
+    // ---- the waves' sums, a column tile at a time
+    const auto store = [&](int c, int d, f32x4 x, float sum) {
+        const int r = c / a.group;
+        float* p = a.out + (row0 + r) * a.ld_out + ((long)kvh * a.group + c - r * a.group) * HD + d;
+        *reinterpret_cast<f32x4*>(p) = x * (sum == 0.f ? 0.f : 1.f / sum);   // a row that has seen nothing is zero
+    };
+    const long part = (((long)u * a.n_kv + kvh) * a.splits) * a.cols;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        l[c] += __shfl_xor(l[c], 16, 64);
+        l[c] += __shfl_xor(l[c], 32, 64);
+        if (g == 0) {
+            sh.m[wave][16 * c + i] = m[c];
+            sh.l[wave][16 * c + i] = l[c];
+        }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4*>(&sh.o[wave][i][64 * h + 16 * g + 4 * x]) =
+                    f32x4{o[ct][h][0][x], o[ct][h][1][x], o[ct][h][2][x], o[ct][h][3][x]};
+        __syncthreads();
+        const int here = min(max(cols - 16 * ct, 0), 16);
+        for (int e = threadIdx.x; e < here * (HD / 4); e += kPfWaves * 64) {
+            const int c = e / (HD / 4), d = e % (HD / 4) * 4, col = 16 * ct + c;
+            float top = kPfFloor, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kPfWaves; ++w) top = fmaxf(top, sh.m[w][col]);
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kPfWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sh.m[w][col] - top);
+                sum += f * sh.l[w][col];
+                x += f * *reinterpret_cast<const f32x4*>(&sh.o[w][c][d]);
+            }
+            if (runs == 1) {
+                store(col, d, x, sum);
+            } else {
+                const long at = part + (long)split * a.cols + col;
+                pf_put(a.part_o + at * HD + d, x.x, x.y);
+                pf_put(a.part_o + at * HD + d + 2, x.z, x.w);
+                if (d == 0) pf_put(a.part_ml + 2 * at, top, sum);
+            }
+        }
+    }
+    if (runs == 1) return;
+    // The block that ends last joins the runs.  Every thread's partial sums have
+    // arrived before its block is counted, so they are there for the last one.
+    __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0)
+    __syncthreads();
+    int* const counter = a.counters + (long)u * a.n_kv + kvh;
+    if (threadIdx.x == 0)
+        sh.last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == runs - 1;
+    __syncthreads();
+    if (!sh.last) return;
+    // a run to a lane, a column to a wave
+    for (int c = wave; c < cols; c += kPfWaves) {
+        float top = kPfFloor, sum = 0.f;
+        if (lane < runs) pf_get(a.part_ml + 2 * (part + (long)lane * a.cols + c), top, sum);
+        const float f = __builtin_amdgcn_exp2f(top - wave_max(top));
+        sum = wave_sum(lane < runs ? f * sum : 0.f);
+        if (lane < runs) sh.f[lane][c] = f;
+        if (lane == 0) sh.sum[c] = sum;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < cols * (HD / 4); e += kPfWaves * 64) {
+        const int c = e / (HD / 4), d = e % (HD / 4) * 4;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int r = 0; r < runs; ++r) {
+            const float* p = a.part_o + (part + (long)r * a.cols + c) * HD + d;
+            float y[4];
+            pf_get(p, y[0], y[1]);
+            pf_get(p + 2, y[2], y[3]);
+            x += sh.f[r][c] * f32x4{y[0], y[1], y[2], y[3]};
+        }
+        store(c, d, x, sh.sum[c]);
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- launches ---------------------------------------------------------------------
+
+// The shape of a launch: tile, splits, scratch.
+struct PfShape {
+    int ct, rows, tiles, splits, cols;
+    size_t parts() const { return (size_t)tiles * splits * cols; }
+};
+
+static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window) {
+    PfShape s{};
+    const int group = n_heads / c.n_kv;
+    // columns of an average group
+    const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
+    s.ct = wide <= 16 ? 1 : wide <= 32 ? 2 : 4;
+    if (c.head_dim == 256) s.ct = std::min(s.ct, 2);
+    s.rows = 16 * s.ct / group;
+    s.cols = s.rows * group;
+    s.tiles = b.group_starts ? b.n_rows / s.rows + b.n_groups : (b.n_rows + s.rows - 1) / s.rows;
+    if (b.n_groups == 1) s.tiles = (b.n_rows + s.rows - 1) / s.rows;
+    // chunks of a tile, by the caller's hints
+    const int64_t prefix = std::min(b.max_prefix > 0 ? b.max_prefix : c.max_seq, c.max_seq);
+    int64_t own = std::min(b.max_own > 0 ? b.max_own : c.max_seq, c.max_seq);
+    if (b.slot_stride > 0) own = std::min<int64_t>(own, b.slot_stride);
+    if (window > 0) own = std::min<int64_t>(own, window);
+    const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
+    const long units = std::max(1L, (long)s.tiles * c.n_kv);
+    const long want = device_cu_count() * 3L / units, most = (chunks + 2 * kPfWaves - 1) / (2 * kPfWaves);
+    const long fit = (long)((256u << 20) / ((size_t)units * s.cols * (c.head_dim + 2) * sizeof(float)));
+    s.splits = (int)std::max(1L, std::min({want, most, fit, (long)kPfMaxSplits}));
+    return s;
+}
+
+void prefix_attention_workspace(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window, size_t* bytes,
+                                size_t* counters) {
+    const PfShape s = pf_shape(c, b, n_heads, window);
+    *bytes = s.splits > 1 ? s.parts() * c.n_kv * (c.head_dim + 2) * sizeof(float) : 0;
+    *counters = s.splits > 1 ? (size_t)s.tiles * c.n_kv : 0;
+}
+
+int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch& b, const float* q, long ld_q, int n_heads,
+                            float scale, int window, float* out, long ld_out, const Workspace& ws, hipStream_t st) {
+    const char* who = "prefix_attention";
+    ATLAS_REQUIRE(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 256, "%s: head_dim %d (64, 128 or 256)", who,
+                  c.head_dim);
+    ATLAS_REQUIRE(c.n_slots >= 0 && c.max_seq >= 0 && c.max_seq <= 1 << 24 && c.n_kv > 0 && c.n_kv <= 4096, "%s: %d slots of %d tokens, %d KV heads",
+                  who, c.n_slots, c.max_seq, c.n_kv);
+    ATLAS_REQUIRE((long)c.n_slots * c.max_seq <= INT64_MAX / 4 / ((long)c.n_kv * c.head_dim), "%s: %d slots of %d tokens", who,
+                  c.n_slots, c.max_seq);
+    ATLAS_REQUIRE(b.n_groups >= 0 && b.n_rows >= 0 && b.slot_stride >= 0 && b.max_prefix >= 0 && b.max_own >= 0,
+                  "%s: %d groups, %d rows, slot stride %d, max_prefix %d, max_own %d", who, b.n_groups, b.n_rows,
+                  b.slot_stride, b.max_prefix, b.max_own);
+    ATLAS_REQUIRE(b.group_starts || b.n_groups <= 1, "%s: %d groups need group_starts", who, b.n_groups);
+    ATLAS_REQUIRE(b.n_groups <= 1 << 20 && b.n_rows <= 1 << 20, "%s: %d rows of %d groups", who, b.n_rows, b.n_groups);
+    ATLAS_REQUIRE(n_heads > 0 && n_heads % c.n_kv == 0 && n_heads / c.n_kv <= 16, "%s: %d heads over %d KV heads (up to 16 to each)",
+                  who, n_heads, c.n_kv);
+    ATLAS_REQUIRE(window >= 0, "%s: window %d", who, window);
+    if (b.n_rows == 0 || b.n_groups == 0) return ATLAS_OK;
+    ATLAS_REQUIRE(b.prefix_slots && b.prefix_lens && b.kv_lens && b.slots && ((long)c.n_slots * c.max_seq == 0 || (c.k && c.v)) && q && out,
+                  "%s: null argument", who);
+    ATLAS_REQUIRE((((uintptr_t)b.group_starts | (uintptr_t)b.prefix_slots | (uintptr_t)b.prefix_lens | (uintptr_t)b.kv_lens |
+                    (uintptr_t)b.slots) & 3) == 0, "%s: misaligned batch", who);
+    const long wide = (long)n_heads * c.head_dim;
+    ATLAS_REQUIRE((((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)q | (uintptr_t)out) & 15) == 0 && ld_q % 4 == 0 &&
+                      ld_out % 4 == 0 && ld_q >= wide && ld_out >= wide,
+                  "%s: the cache and rows start on 16 bytes, rows at least %ld elements apart (strides %ld and %ld)", who, wide,
+                  ld_q, ld_out);
+    const PfShape s = pf_shape(c, b, n_heads, window);
+    const long units = (long)s.tiles * c.n_kv;
+    ATLAS_REQUIRE(units <= 1 << 23, "%s: %d tiles of rows and %d KV heads", who, s.tiles, c.n_kv);
+    PfArgs a{};
+    a.k = c.k; a.v = c.v;
+    a.n_slots = c.n_slots; a.max_seq = c.max_seq; a.n_kv = c.n_kv;
+    a.starts = b.group_starts;
+    a.prefix_slots = b.prefix_slots; a.prefix_lens = b.prefix_lens; a.lens = b.kv_lens; a.slots = b.slots;
+    a.slot_stride = b.slot_stride; a.n_groups = b.n_groups; a.n_rows = b.n_rows;
+    a.q = q; a.ld_q = ld_q; a.out = out; a.ld_out = ld_out;
+    a.group = n_heads / c.n_kv;
+    a.rows = s.rows; a.tiles = s.tiles; a.cols = s.cols; a.splits = s.splits;
+    a.scale = scale; a.window = window;
+    if (s.splits > 1) {
+        const size_t parts = s.parts() * c.n_kv, bytes = parts * (c.head_dim + 2) * sizeof(float);
+        void *p = ws.p, *cnt = ws.counters;
+        if (p) {
+            ATLAS_REQUIRE(ws.bytes >= bytes && cnt && ws.n_counters >= (size_t)units, "%s: workspace of %zu bytes, %zu needed",
+                          who, ws.bytes, bytes);
+        } else {
+            int rc;
+            if ((rc = thread_scratch(SCR_PREFIX_CNT, (size_t)units * sizeof(int), &cnt, true))) return rc;
+            if ((rc = thread_scratch(SCR_PREFIX, bytes, &p))) return rc;
+        }
+        a.counters = static_cast<int*>(cnt);
+        a.part_o = static_cast<float*>(p);
+        a.part_ml = a.part_o + parts * c.head_dim;
+    }
+    const dim3 grid((unsigned)(((long)c.n_kv * s.splits + 7) / 8 * 8 * s.tiles));
+#define PF_RUN(HD, CT) hipLaunchKernelGGL((pf_attention_kernel<HD, CT>), grid, dim3(kPfWaves * 64), 0, st, a)
+    if (c.head_dim == 64) {
+        if (s.ct == 1) PF_RUN(64, 1); else if (s.ct == 2) PF_RUN(64, 2); else PF_RUN(64, 4);
+    } else if (c.head_dim == 128) {
+        if (s.ct == 1) PF_RUN(128, 1); else if (s.ct == 2) PF_RUN(128, 2); else PF_RUN(128, 4);
+    } else {
+        if (s.ct == 1) PF_RUN(256, 1); else PF_RUN(256, 2);
+    }
+#undef PF_RUN
+    ATLAS_LAUNCH_CHECK("prefix_attention");
+    return ATLAS_OK;
+}
+
+}  // namespace atlas

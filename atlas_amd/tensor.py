@@ -7,7 +7,9 @@ Same names and argument meaning as crates/atlas-tensor/src/lib.rs:
 C ABI of include/atlas_kernels.h.  Extensions: ``GpuBufKind.INT8`` /
 ``GpuBufKind.INT4`` and ``GpuMatrix.upload_int8`` / ``upload_int4`` for the
 dequant-fused GEMVs, ``GpuBufKind.MXFP4`` / ``upload_mxfp4`` for products of
-4-bit matrices, and ``GpuKv4Cache``, a paged KV cache in 4 bits.
+4-bit matrices, ``GpuKv4Cache``, a paged KV cache in 4 bits, and what decodes many
+continuations together: ``GpuSlotCache`` with attention over shared prefixes,
+``beam_select_gpu`` and ``beam_reorder_gpu``, ``GpuLora``.
 
 Error behaviour follows the reference's Option/bool contract where it has
 one (allocation -> None, ``sgemm`` -> False when no device is present), but
@@ -22,7 +24,8 @@ from typing import Optional
 
 import numpy as np
 
-from ._lib import AtlasError, Kv4BatchC, Kv4CacheC, check, check_void, load
+from ._lib import (AtlasError, Kv4BatchC, Kv4CacheC, LoraC, PrefixBatchC, SlotCacheC, check, check_void,
+                   load)
 
 
 def _p(a: np.ndarray):
@@ -279,9 +282,20 @@ class GpuMatrix:
             return None
         return GpuVec(out, np.zeros(self.rows * n, np.float32), self.rows * n)
 
-    def sgemm_rows(self, x: "GpuVec", n: int) -> "GpuVec":
+    def sgemm_rows(self, x: "GpuVec", n: int, lora: Optional["GpuLora"] = None, adapters=None) -> "GpuVec":
         """Ragged micro-batch: x holds n activation rows [n x cols]; returns
-        [n x rows] (extension, skinny MFMA GEMM)."""
+        [n x rows] (extension, skinny MFMA GEMM).  With ``lora`` each row r gets the product
+        of its adapter ``adapters[r]`` (-1: none) on top."""
+        if lora is not None and (lora.rows, lora.cols) != (self.rows, self.cols):
+            raise AtlasError(-1, f"sgemm_rows: adapters of {lora.rows}x{lora.cols} beside {self.rows}x{self.cols}")
+        if lora is not None and np.size(adapters) != n:
+            raise AtlasError(-1, f"sgemm_rows: {np.size(adapters)} adapters for {n} rows")
+        out = self._sgemm_rows(x, n)
+        if lora is not None:
+            lora.add(out, x, adapters)
+        return out
+
+    def _sgemm_rows(self, x: "GpuVec", n: int) -> "GpuVec":
         if self.buf is None or x.buf is None:
             raise AtlasError(-1, "sgemm_rows: operands are not on the GPU")
         if self.kind is GpuBufKind.MXFP4 and x.len < n * self.cols:
@@ -558,3 +572,185 @@ class GpuKv4Cache:
         check(load().atlas_kv4_attention_f32(C.byref(self.c), C.byref(batch.c), q.buf.ptr, wide, n_heads, scale,
                                              window_size, out.buf.ptr, wide))
         return out
+
+
+def _scratch(nbytes: int) -> _DevMem:
+    try:
+        return _DevMem(max(nbytes, 4), sync_alloc=False)
+    except MemoryError as e:
+        raise AtlasError(-3, str(e)) from None
+
+
+def _upload(a: np.ndarray) -> _DevMem:
+    """A device copy of a host array."""
+    a = np.ascontiguousarray(a)
+    mem = _scratch(a.nbytes)
+    check(load().atlas_memcpy_h2d(mem.ptr, _p(a), a.nbytes))
+    return mem
+
+
+def _ints(who: str, x, lo: int = -(1 << 31)) -> np.ndarray:
+    a = np.asarray(x, np.int64)
+    if (a < lo).any() or (a >= 1 << 31).any():
+        raise AtlasError(-1, f"{who}: values from {lo} to 2^31 - 1 expected")
+    return a.astype(np.int32)
+
+
+class PrefixBatch:
+    """The rows of one step over a ``GpuSlotCache`` (extension).  Groups of
+    ``group_sizes`` rows (default: all rows are one) share their first ``prefix_lens[g]``
+    tokens, in slot ``prefix_slots[g]``; row r has ``kv_lens[r]`` tokens, its newest
+    included, of which those of its own lie in slot ``slots[r]``, or token i of
+    them in slot ``slots[r][i]`` where ``slots`` is a table."""
+
+    def __init__(self, kv_lens, prefix_slots, prefix_lens, slots, group_sizes=None):
+        who = "PrefixBatch"
+        lens, at, pre = (_ints(who, x, 0 if i != 1 else -(1 << 31)).reshape(-1)
+                         for i, x in enumerate((kv_lens, prefix_slots, prefix_lens)))
+        try:
+            slots = _ints(who, slots)
+        except ValueError:
+            raise AtlasError(-1, f"{who}: the table's rows have one length") from None
+        sizes = _ints(who, [lens.size] if group_sizes is None else group_sizes, 0).reshape(-1)
+        if sizes.size != at.size or sizes.size != pre.size or int(sizes.astype(np.int64).sum()) != lens.size:
+            raise AtlasError(-1, f"{who}: {sizes.size} groups of {sizes.sum()} rows, {at.size} slots and {pre.size} lengths of "
+                                 f"prefixes, {lens.size} rows")
+        if slots.ndim not in (1, 2) or slots.shape[0] != lens.size:
+            raise AtlasError(-1, f"{who}: slots of shape {slots.shape} for {lens.size} rows")
+        if slots.ndim == 2 and slots.shape[1] == 0:
+            slots = np.full((lens.size, 1), -1, np.int32)
+        self.n_rows, self.n_groups = lens.size, sizes.size
+        starts = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+        own = lens - np.repeat(pre, sizes)
+        parts = [starts, at, pre, lens, slots.reshape(-1)]
+        self._mem = _upload(np.concatenate(parts))
+        p = self._mem.ptr + 4 * np.concatenate([[0], np.cumsum([x.size for x in parts])])
+        self.c = PrefixBatchC(int(p[0]), int(p[1]), int(p[2]), int(p[3]), int(p[4]),
+                              slots.shape[1] if slots.ndim == 2 else 0, self.n_groups, self.n_rows,
+                              max(int(pre.max(initial=0)), 1), max(int(own.max(initial=0)), 1))
+
+
+class GpuSlotCache:
+    """f32 KV caches of several sequences side by side (extension): keys and values
+    [n_slots x max_seq x n_kv_heads x head_dim], ``GpuKvCache``'s layout slot after slot."""
+
+    def __init__(self, keys: GpuVec, values: GpuVec, n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int):
+        self.keys, self.values = keys, values
+        self.n_slots, self.max_seq, self.n_kv_heads, self.head_dim = n_slots, max_seq, n_kv_heads, head_dim
+        self.c = SlotCacheC(keys.gpu_ptr(), values.gpu_ptr(), n_slots, max_seq, n_kv_heads, head_dim)
+
+    @staticmethod
+    def new(n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int) -> Optional["GpuSlotCache"]:
+        if min(n_slots, max_seq, n_kv_heads, head_dim) < 0:
+            raise AtlasError(-1, f"GpuSlotCache: {n_slots} slots of {max_seq} tokens, {n_kv_heads} heads of {head_dim}")
+        if not cuda_available():
+            return None
+        total = n_slots * max_seq * n_kv_heads * head_dim
+        keys, values = GpuVec.zeros(total), GpuVec.zeros(total)
+        if keys.buf is None or values.buf is None:
+            return None
+        return GpuSlotCache(keys, values, n_slots, max_seq, n_kv_heads, head_dim)
+
+    def write(self, slot: int, pos: int, new_k: GpuVec, new_v: GpuVec) -> None:
+        """K and V rows of one or more tokens from position ``pos`` on."""
+        wide = self.n_kv_heads * self.head_dim
+        n = new_k.len // max(wide, 1)
+        if new_k.len != n * wide or new_v.len != new_k.len or not 0 <= slot < self.n_slots or not 0 <= pos <= self.max_seq - n:
+            raise AtlasError(-1, f"GpuSlotCache.write: {new_k.len} and {new_v.len} elements at slot {slot}, position {pos}")
+        self.keys._need(self.values, new_k, new_v)
+        for cache, new in ((self.keys, new_k), (self.values, new_v)):
+            check(load().atlas_memcpy_d2d(cache.buf.ptr + 4 * wide * (slot * self.max_seq + pos), new.buf.ptr, 4 * new.len))
+
+    def attention(self, batch: PrefixBatch, q: GpuVec, n_heads: int, scale: float, window_size: int = 0) -> GpuVec:
+        """Attention of the batch's query rows [n_rows x n_heads x head_dim]."""
+        wide = n_heads * self.head_dim
+        if q.buf is None or q.len < batch.n_rows * wide:
+            raise AtlasError(-1, f"GpuSlotCache: {batch.n_rows} rows of {wide} elements expected on the GPU")
+        out = GpuBuf.alloc(batch.n_rows * wide)
+        if out is None:
+            raise AtlasError(-3, f"GpuSlotCache: no device memory for {batch.n_rows} rows of {wide} elements")
+        check(load().atlas_prefix_attention_f32(C.byref(self.c), C.byref(batch.c), q.buf.ptr, wide, n_heads, scale,
+                                                window_size, out.ptr, wide))
+        return GpuVec(out, np.zeros(out.len, np.float32), out.len)
+
+    def reorder(self, parents, begin: int = 0, end: Optional[int] = None) -> None:
+        """Slot g * width + b takes over positions [begin, end) of slot g * width + parents[g][b],
+        for the first slots ([n_groups x width] parents, or [width] of one group)."""
+        end = self.max_seq if end is None else end
+        p = np.atleast_2d(_ints("GpuSlotCache.reorder", parents))
+        wide = 4 * self.n_kv_heads * self.head_dim
+        if p.ndim != 2 or p.size > self.n_slots or not 0 <= begin <= end <= self.max_seq:
+            raise AtlasError(-1, f"GpuSlotCache.reorder: parents of shape {p.shape}, positions {begin} to {end}")
+        self.keys._need(self.values)
+        _reorder([self.keys.buf.ptr + wide * begin, self.values.buf.ptr + wide * begin], wide * (end - begin),
+                 wide * self.max_seq, p)
+
+
+def _reorder(ptrs, row_bytes: int, stride: int, parents: np.ndarray) -> None:
+    mem = _upload(parents)
+    states = (C.c_void_p * max(len(ptrs), 1))(*ptrs)
+    check(load().atlas_beam_reorder(states, states, len(ptrs), row_bytes, stride, mem.ptr, parents.shape[0], parents.shape[1]))
+
+
+def beam_reorder_gpu(states, parents) -> None:
+    """Beams take over the states of the beams that they continue, in place (extension):
+    row g * width + b of each ``GpuVec`` becomes row g * width + parents[g][b]
+    ([n_groups x width], or [width] of one group; another number: the row stays)."""
+    p = np.atleast_2d(_ints("beam_reorder_gpu", parents))
+    if p.ndim != 2 or p.size == 0:
+        raise AtlasError(-1, f"beam_reorder_gpu: parents of shape {p.shape}")
+    for x in states:
+        x._need()
+        if x.len % p.size:
+            raise AtlasError(-1, f"beam_reorder_gpu: {x.len} elements in {p.size} rows")
+    for wide in sorted({x.len // p.size for x in states}):
+        _reorder([x.buf.ptr for x in states if x.len // p.size == wide], 4 * wide, 4 * wide, p)
+
+
+def beam_select_gpu(logits: GpuVec, scores, n_out: int):
+    """Beam search's choice (extension): the ``n_out`` best continuations of each group, from
+    logits [n_groups x width x vocab] and the beams' sums of log probabilities
+    [n_groups x width] (or [width]; not finite: no such beam).  Returns tokens, parents and scores,
+    each [n_groups x n_out] in descending order; parent -1: there are no more."""
+    s = np.atleast_2d(np.asarray(scores, np.float64))
+    if s.ndim != 2 or s.size == 0 or logits.buf is None or logits.len == 0 or logits.len % s.size:
+        raise AtlasError(-1, f"beam_select_gpu: {logits.len} logits on the GPU for scores of shape {s.shape}")
+    vocab = logits.len // s.size
+    if not 1 <= n_out <= 64:
+        raise AtlasError(-1, f"beam_select_gpu: {n_out} continuations (1 to 64)")
+    n = s.shape[0] * n_out
+    mem, out = _upload(s), _scratch(16 * n)      # scores, tokens, parents
+    check(load().atlas_beam_select_f32(logits.buf.ptr, vocab, vocab, mem.ptr, s.shape[0], s.shape[1], n_out, out.ptr + 8 * n,
+                                       out.ptr + 12 * n, out.ptr))
+    got = np.empty(16 * n, np.uint8)
+    check(load().atlas_memcpy_d2h(_p(got), out.ptr, got.nbytes))
+    shape = (s.shape[0], n_out)
+    return (got[8 * n:12 * n].view(np.uint32).reshape(shape), got[12 * n:].view(np.int32).reshape(shape),
+            got[:8 * n].view(np.float64).reshape(shape))
+
+
+class GpuLora:
+    """Low-rank adapters of one rows x cols projection (extension): ``a`` [n x rank x cols] and
+    ``b`` [n x rows x rank], f32, or uint16 bf16 bits, and a scale for each (default 1)."""
+
+    def __init__(self, a, b, scales=None):
+        a, b = np.asarray(a), np.asarray(b)
+        fmt = {np.dtype(np.uint16): 1, np.dtype(np.float32): 0}.get(a.dtype)
+        if fmt is None or a.dtype != b.dtype or a.ndim != 3 or b.ndim != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise AtlasError(-1, f"GpuLora: a {a.shape} {a.dtype}, b {b.shape} {b.dtype}")
+        self.n, self.rank, self.cols, self.rows = a.shape[0], a.shape[1], a.shape[2], b.shape[1]
+        if scales is not None and np.size(scales) != self.n:
+            raise AtlasError(-1, f"GpuLora: {np.size(scales)} scales for {self.n} adapters")
+        self._a, self._b = _upload(a), _upload(b)
+        self._s = None if scales is None else _upload(np.asarray(scales, np.float32))
+        self.c = LoraC(fmt, self._a.ptr, self._b.ptr, self._s.ptr if self._s else None, self.n, self.rank, self.rows, self.cols)
+
+    def add(self, y: GpuVec, x: GpuVec, adapters) -> None:
+        """y [n x rows] += the product of each row's adapter with x [n x cols]; -1: none."""
+        pick = _ints("GpuLora.add", adapters).reshape(-1)
+        y._need(x)
+        if x.len < pick.size * self.cols or y.len < pick.size * self.rows:
+            raise AtlasError(-1, f"GpuLora.add: {pick.size} rows of {self.cols} and {self.rows} elements expected")
+        mem = _upload(pick)
+        check(load().atlas_lora_add_f32(C.byref(self.c), mem.ptr, x.buf.ptr, self.cols, y.buf.ptr, self.rows, y.buf.ptr, self.rows,
+                                        pick.size))

@@ -29,7 +29,8 @@
  * Library scratch: entry points that need device scratch and are not handed
  * a workspace (atlas_decode_attention, atlas_gpu_argmax,
  * atlas_gemm_skinny_f32, atlas_attention_fused_f32,
- * atlas_kv4_attention_f32 for long caches) keep it per calling
+ * atlas_kv4_attention_f32 and atlas_prefix_attention_f32 for long caches,
+ * atlas_beam_select_f32, atlas_lora_add_f32) keep it per calling
  * thread, grow it on first use of a larger shape and free it when the
  * thread exits.  A call that would grow it while its stream is being
  * captured into a graph returns / records ATLAS_EUNSUPPORTED instead: warm
@@ -365,6 +366,88 @@ int atlas_kv4_read_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batc
 int atlas_kv4_attention_f32(const atlas_kv4_cache* cache, const atlas_kv4_batch* batch,
                             const float* q, int64_t ld_q, int n_heads, float scale, int window,
                             float* out, int64_t ld_out);
+
+/* ----- Many continuations decoded together (no reference counterpart) ------
+ * A f32 cache of slots: K and V [n_slots][max_seq][n_kv][head_dim], GpuKvCache's
+ * layout slot after slot.  head_dim 64, 128 or 256; max_seq up to 2^24.       */
+typedef struct {
+    const float* k;              /* device, 16-byte aligned                    */
+    const float* v;
+    int n_slots, max_seq, n_kv, head_dim;
+} atlas_slot_cache;
+
+/* Rows of which groups share their first tokens; the arrays are on the device and
+ * read when the kernels run (a captured call follows their contents).
+ * Group g's rows are group_starts[g] .. group_starts[g + 1] - 1 (n_groups + 1
+ * ascending entries from 0 on; NULL: one group of all rows); rows past the last
+ * group's are not read or written.  Row r attends to the last of its kv_lens[r]
+ * tokens (its newest included; the window says how many).  Tokens t below
+ * prefix_lens[g] are at position t of slot prefix_slots[g], for all of the group's
+ * rows; a row's others at position t of slot slots[r * slot_stride + t -
+ * prefix_lens[g]], with slot_stride 0 of slot slots[r].  A token whose slot is not
+ * one, whose position is past max_seq or that is past the table is not there.
+ * Up to 2^20 rows and groups.                                                */
+typedef struct {
+    const int* group_starts;     /* [n_groups + 1] or NULL                     */
+    const int* prefix_slots;     /* [n_groups]                                 */
+    const int* prefix_lens;      /* [n_groups]                                 */
+    const int* kv_lens;          /* [n_rows]                                   */
+    const int* slots;            /* [n_rows][slot_stride] or [n_rows]          */
+    int slot_stride, n_groups, n_rows;
+    int max_prefix, max_own;     /* no prefix, and no row's rest, is longer, as far as
+                                    the caller knows (0: max_seq): only how the work is
+                                    split goes by it                           */
+} atlas_prefix_batch;
+
+/* Attention of one query row ([n_rows][n_heads * head_dim] f32, ld_q elements
+ * apart) over its tokens, the last `window` of them (0: all), scores times scale, in
+ * f32.  A group's shared tokens are read once for up to 64 of its rows' heads.
+ * n_heads / n_kv in 1 .. 16.  A row without tokens gives zeros, whatever its q.  A
+ * token of infinities or NaN is nothing to the rows that do not see it.
+ * out may be q, with ld_out = ld_q.                                          */
+int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix_batch* batch,
+                               const float* q, int64_t ld_q, int n_heads, float scale, int window,
+                               float* out, int64_t ld_out);
+
+/* Beam search's choice for n_groups prompts of `width` beams: of the candidates
+ * (beam r, token t) of score scores[r] + logits[r][t] - log sum exp(logits[r]), in
+ * 64 bits, the n_out largest of each group in descending order (equal scores: the lower beam,
+ * then the larger logit, then the lower token).  logits [n_groups * width] rows of
+ * vocab, ld apart; scores [n_groups * width]; tokens, parents (the beam within its
+ * group) and out_scores [n_groups][n_out].  A beam whose score is not finite, a row
+ * of logits with NaN or +inf or of -inf only, and a logit of -inf give no candidates;
+ * where a group has too few, the rest is token 0 of parent -1 and score -inf.
+ * width and n_out 1 to 64, n_groups * width up to 65535.                     */
+int atlas_beam_select_f32(const float* logits, int64_t ld, int vocab, const double* scores,
+                          int n_groups, int width, int n_out, uint32_t* tokens, int* parents,
+                          double* out_scores);
+/* Beams take over the states of the beams they continue: row g * width + b of each
+ * of n_states states (dst[i], src[i]: arrays on the host of device pointers, read during the call)
+ * becomes row g * width + parents[g * width + b]; rows of row_bytes, row_stride bytes
+ * apart.  dst[i] may be src[i] (rows that stay are then left alone) and must not
+ * overlap it otherwise.  A parent that is no beam leaves its row of dst as it is.
+ * width up to 64, n_groups up to 65535.                                      */
+int atlas_beam_reorder(void* const* dst, const void* const* src, int n_states, int64_t row_bytes,
+                       int64_t row_stride, const int* parents, int n_groups, int width);
+
+/* Low-rank adapters of one projection of m x k: a [n_adapters][rank][k] and
+ * b [n_adapters][m][rank] without gaps, ATLAS_W_F32 or ATLAS_W_BF16 (an adapter of
+ * lower rank is filled up with zeros); scales [n_adapters] or NULL (1), all on the
+ * device.  rank 1 to 256.                                                    */
+typedef struct {
+    int fmt;
+    const void* a;
+    const void* b;
+    const float* scales;
+    int n_adapters, rank, m, k;
+} atlas_lora;
+
+/* y_r = base_r + scales[p] b_p (a_p x_r), p = adapters[r], for n rows (up to 2^20) of x (k
+ * elements, ld_x apart), base and y (m elements); a row whose p is no adapter is its
+ * base.  base is the shared projection's product and may be y (with ld_y = ld_base), but must not
+ * overlap it otherwise.  f32 sums of exact products.                          */
+int atlas_lora_add_f32(const atlas_lora* lora, const int* adapters, const float* x, int64_t ld_x,
+                       const float* base, int64_t ld_base, float* y, int64_t ld_y, int n);
 
 /* Seeded synthetic fills on the device: SplitMix64 counter + Box-Muller.
  * kind 0: N(a, b) f32; 1: N(a, b) bf16 by truncation; 2: U(a, b) f32.        */

@@ -1,0 +1,128 @@
+"""Refusals of attention over shared prefixes, beam selection, reordering of states and low-rank adapters:
+made on the host, before any device is needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from atlas_amd import tensor as T
+from atlas_amd._lib import AtlasError, LoraC, PrefixBatchC, SlotCacheC, check, load
+
+X = 1 << 12                            # a pointer that no refused call follows
+
+
+def _refused(rc):
+    with pytest.raises(AtlasError) as e:
+        check(rc)
+    assert e.value.code == -1
+    return str(e.value)
+
+
+CACHE = dict(k=X, v=X, n_slots=4, max_seq=64, n_kv=2, head_dim=64)
+BATCH = dict(group_starts=X, prefix_slots=X, prefix_lens=X, kv_lens=X, slots=X, slot_stride=8, n_groups=2, n_rows=4,
+             max_prefix=0, max_own=0)
+
+
+def _attention(cache=(), batch=(), q=X, ld_q=256, heads=4, window=0, out=X, ld_out=256):
+    c, b = SlotCacheC(**{**CACHE, **dict(cache)}), PrefixBatchC(**{**BATCH, **dict(batch)})
+    return load().atlas_prefix_attention_f32(C.byref(c), C.byref(b), q, ld_q, heads, 1.0, window, out, ld_out)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(cache=dict(head_dim=96)), dict(cache=dict(n_kv=0)), dict(cache=dict(n_slots=-1)), dict(cache=dict(max_seq=-1)),
+    dict(cache=dict(max_seq=(1 << 24) + 1)), dict(cache=dict(k=0)), dict(cache=dict(v=X + 4)), dict(batch=dict(n_rows=-1)),
+    dict(batch=dict(n_groups=-1)), dict(batch=dict(slot_stride=-1)), dict(batch=dict(max_own=-1)), dict(batch=dict(max_prefix=-1)),
+    dict(batch=dict(group_starts=0)), dict(batch=dict(prefix_slots=0)), dict(batch=dict(prefix_lens=0)), dict(batch=dict(kv_lens=0)),
+    dict(batch=dict(slots=0)), dict(batch=dict(slots=X + 2)), dict(batch=dict(n_rows=(1 << 20) + 1)),
+    dict(batch=dict(n_groups=(1 << 20) + 1)), dict(heads=3), dict(heads=0), dict(heads=34, ld_q=4096, ld_out=4096), dict(window=-1),
+    dict(q=0), dict(out=0), dict(q=X + 4), dict(out=X + 8), dict(ld_q=252), dict(ld_out=255), dict(ld_q=258),
+    dict(cache=dict(n_kv=4096, n_slots=1), heads=4096, ld_q=1 << 20, ld_out=1 << 20, batch=dict(n_rows=1 << 20)),
+], ids=str)
+def test_prefix_attention_refusals(kw):
+    assert "prefix_attention" in _refused(_attention(**kw))
+
+
+def test_prefix_attention_null_and_nothing_to_do():
+    lib = load()
+    c, b = SlotCacheC(**CACHE), PrefixBatchC(**BATCH)
+    _refused(lib.atlas_prefix_attention_f32(None, C.byref(b), X, 256, 4, 1.0, 0, X, 256))
+    _refused(lib.atlas_prefix_attention_f32(C.byref(c), None, X, 256, 4, 1.0, 0, X, 256))
+    check(_attention(batch=dict(n_rows=0), q=0, out=0))
+    check(_attention(batch=dict(n_groups=0, group_starts=0)))
+
+
+def _select(logits=X, ld=100, vocab=100, scores=X, groups=2, width=4, n_out=8, tokens=X, parents=X, out=X):
+    return load().atlas_beam_select_f32(logits, ld, vocab, scores, groups, width, n_out, tokens, parents, out)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(logits=0), dict(scores=0), dict(tokens=0), dict(parents=0), dict(out=0), dict(vocab=0), dict(ld=99), dict(groups=-1),
+    dict(width=0), dict(width=65), dict(n_out=0), dict(n_out=65), dict(groups=65536, width=1), dict(groups=20000, width=4),
+    dict(scores=X + 4), dict(out=X + 4), dict(logits=X + 2), dict(tokens=X + 1), dict(parents=X + 1)], ids=str)
+def test_beam_select_refusals(kw):
+    assert "beam_select" in _refused(_select(**kw))
+
+
+def test_beam_select_nothing_to_do():
+    check(_select(groups=0))
+
+
+def _reorder(dst=(X, 2 * X), src=(X, 2 * X), n=2, row=64, stride=128, parents=X, groups=1, width=4):
+    d, s = ((C.c_void_p * 2)(*x) if x is not None else None for x in (dst, src))
+    return load().atlas_beam_reorder(d, s, n, row, stride, parents, groups, width)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dst=None), dict(src=None), dict(dst=(X, 0)), dict(src=(0, X)), dict(n=-1), dict(row=-1), dict(row=129), dict(parents=0),
+    dict(parents=X + 1), dict(groups=-1), dict(groups=65536), dict(width=0), dict(width=65),
+    dict(dst=(X + 64, 2 * X)), dict(dst=(X, 2 * X - 3 * 128 - 63))], ids=str)
+def test_beam_reorder_refusals(kw):
+    assert "beam_reorder" in _refused(_reorder(**kw))
+
+
+def test_beam_reorder_nothing_to_do():
+    for kw in (dict(n=0), dict(row=0), dict(groups=0)):
+        check(_reorder(**kw))
+
+
+LORA = dict(fmt=1, a=X, b=X, scales=X, n_adapters=3, rank=8, m=64, k=32)
+
+
+def _lora(lora=(), adapters=X, x=X, ld_x=32, base=X, ld_base=64, y=X, ld_y=64, n=4):
+    return load().atlas_lora_add_f32(C.byref(LoraC(**{**LORA, **dict(lora)})), adapters, x, ld_x, base, ld_base, y, ld_y, n)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(lora=dict(fmt=2)), dict(lora=dict(a=0)), dict(lora=dict(b=0)), dict(lora=dict(n_adapters=-1)), dict(lora=dict(rank=0)),
+    dict(lora=dict(rank=257)), dict(lora=dict(m=0)), dict(lora=dict(k=0)), dict(lora=dict(m=(1 << 24) + 1), ld_base=1 << 25, ld_y=1 << 25),
+    dict(lora=dict(a=X + 1)), dict(lora=dict(fmt=0, b=X + 2)), dict(lora=dict(scales=X + 2)), dict(adapters=0), dict(x=0), dict(base=0),
+    dict(y=0), dict(ld_x=31), dict(ld_base=63), dict(ld_y=63), dict(n=-1), dict(n=(1 << 20) + 1), dict(x=X + 2), dict(y=X + 1)], ids=str)
+def test_lora_refusals(kw):
+    assert "lora_add" in _refused(_lora(**kw))
+
+
+def test_lora_null_and_nothing_to_do():
+    _refused(load().atlas_lora_add_f32(None, X, X, 32, X, 64, X, 64, 4))
+    check(_lora(n=0))
+
+
+@pytest.mark.parametrize("args", [
+    ([5, 5], [0], [3], [0, 1], [1]), ([5, 5], [0, 1], [3], [0, 1]), ([5, 5], [0], [3, 3], [0, 1]), ([5, 5], [0], [3], [0, 1, 2]),
+    ([5, -1], [0], [3], [0, 1]), ([5, 5], [0], [-3], [0, 1]), ([5, 5], [0], [3], [[0, 1], [1]]), ([5, 5], [0], [3], [[[0]], [[1]]]),
+    ([5, 1 << 31], [0], [3], [0, 1]), ([5, 5], [0, 0], [3, 3], [0, 1], [3, -1])], ids=str)
+def test_prefix_batch_refusals(args):
+    with pytest.raises(AtlasError) as e:
+        T.PrefixBatch(*args)
+    assert e.value.code == -1
+
+
+def test_host_side_refusals():
+    v = T.GpuVec(None, np.zeros(8, np.float32), 8)
+    for call in (lambda: T.beam_select_gpu(v, [0.0, 0.0], 2), lambda: T.beam_reorder_gpu([v], [0, 1]),
+                 lambda: T.beam_reorder_gpu([], []), lambda: T.GpuSlotCache.new(-1, 4, 2, 64),
+                 lambda: T.GpuLora(np.zeros((2, 4, 8), np.float32), np.zeros((2, 8, 3), np.float32)),
+                 lambda: T.GpuLora(np.zeros((2, 4, 8)), np.zeros((2, 8, 4))),
+                 lambda: T.GpuLora(np.zeros((2, 4, 8), np.float32), np.zeros((2, 8, 4), np.float32), [1.0])):
+        with pytest.raises(AtlasError) as e:
+            call()
+        assert e.value.code == -1
