@@ -177,6 +177,7 @@ SIGNATURES = {
     "atlas_model_generate_streaming": (I, [P, P, I, I, C.POINTER(SamplingC), TOKEN_FN, P,
                                            C.POINTER(C.c_int)]),
     "atlas_model_generate_batch": (I, [P, P, P, I, I, C.POINTER(SamplingC), P, P]),
+    "atlas_model_generate_beam": (I, [P, P, I, I, I, F, C.POINTER(SamplingC), P, P, P]),
     "atlas_model_decode_greedy": (I, [P, U32, I, P]),
     "atlas_model_decode_greedy_timed": (I, [P, U32, I, P, P]),
     "atlas_model_set_long_context": (I, [P, I]),

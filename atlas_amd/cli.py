@@ -47,6 +47,8 @@ def parse_args(argv: Sequence[str]) -> argparse.Namespace:
     ap.add_argument("--prompt", default="The capital of France is")
     ap.add_argument("--max-tokens", type=int, default=50)
     ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--beams", type=int, default=1, choices=range(1, 17), metavar="1..16",
+                    help="beam search of this width, whatever the temperature (1: none)")
     ap.add_argument("--model", default="smollm2-1.7b",
                     help=f"one of {', '.join(PRESETS)}, or auto (shapes from config.json)")
     ap.add_argument("--format", default="bf16", choices=sorted(FORMATS))
@@ -131,7 +133,7 @@ def run_infer(args: argparse.Namespace,
     sharded = os.path.exists(os.path.join(wdir, "model.safetensors.index.json"))
     out(f"\n  Loading weights from {wdir} (sharded={sharded}) ...")
     t0 = time.perf_counter()
-    m = loader.load_model_from_dir(wdir, cfg, weight_format=FORMATS[args.format])
+    m = loader.load_model_from_dir(wdir, cfg, weight_format=FORMATS[args.format], max_batch=args.beams)
     load_ms = (time.perf_counter() - t0) * 1e3
     out(f"  Weights loaded in {load_ms:.0f} ms ({m.weight_bytes() / 1e9:.2f} GB resident)")
 
@@ -168,7 +170,11 @@ def run_infer(args: argparse.Namespace,
 
     out(f"\n  Generating {args.max_tokens} tokens (temperature={args.temperature}) ...")
     t0 = time.perf_counter()
-    new = m.generate(prompt, args.max_tokens, args.temperature)
+    if args.beams > 1:
+        hyps = m.generate_beam(prompt, args.max_tokens, args.beams)
+        new = hyps[0][0] if hyps else []
+    else:
+        new = m.generate(prompt, args.max_tokens, args.temperature)
     gen_s = time.perf_counter() - t0
     tps = len(new) / max(gen_s, 1e-3)
     text = decode(tok, new)
@@ -181,6 +187,8 @@ def run_infer(args: argparse.Namespace,
     out(f"  Generation time  : {gen_s * 1e3:.0f} ms")
     out(f"  Throughput       : {tps:.1f} tok/s")
     out(f"  Token IDs        : {new[:20]}")
+    for toks, score in hyps if args.beams > 1 else ():
+        out(f"  Beam             : {score:10.4f}  {decode(tok, toks)!r}")
     out("\n  atlas infer complete")
     report.update(tokens=new, gen_ms=gen_s * 1e3, tok_s=tps, text=text)
     m.close()
@@ -191,7 +199,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     argv = list(sys.argv[1:] if argv is None else argv)
     if not argv or argv[0] != "infer":
         print("usage: python -m atlas_amd.cli infer --weights DIR [--model NAME|auto] "
-              "[--prompt TEXT] [--max-tokens N] [--temperature T] [--format bf16|int8|int4]",
+              "[--prompt TEXT] [--max-tokens N] [--temperature T] [--beams N] [--format bf16|int8|int4]",
               file=sys.stderr)
         return 1
     run_infer(parse_args(argv[1:]))

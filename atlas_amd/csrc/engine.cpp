@@ -33,6 +33,7 @@
 #include "common.hpp"
 #include "fused.hpp"
 #include "gemv.hpp"
+#include "many.hpp"
 
 using namespace atlas;
 
@@ -92,6 +93,19 @@ struct LayerW {
     float *attn_norm = nullptr, *ffn_norm = nullptr, *q_norm = nullptr, *k_norm = nullptr;
     float *kc = nullptr, *vc = nullptr;
     int window = 0;
+};
+
+// What a beam search's step reads (uploaded before each step) and what it chooses;
+// one block on the device, one pinned on the host.
+constexpr int kBeamOut = 64;             // candidates of a step, at most
+struct BeamBlock {
+    double scores[kMaxRows];
+    uint32_t tok[kMaxRows];
+    int pos[kMaxRows], slot[kMaxRows], lens[kMaxRows], parents[kMaxRows];
+    int prefix_slot, prefix_len;
+    double out_scores[kBeamOut];
+    uint32_t out_tok[kBeamOut];
+    int out_parents[kBeamOut];
 };
 
 // XorShift64 of the reference's sampling Rng (lib.rs:1190-1220)
@@ -166,6 +180,13 @@ struct atlas_model {
     int* ring = nullptr;             // [kRing][3][kMaxRows]
     hipEvent_t ring_ev[kRing] = {};
     bool ring_used[kRing] = {};
+    // beam search: the step's block, each beam's slots of its tokens ([kMaxRows][max_seq]),
+    // scratch of the prefix attention and the selection, steps by width and candidates
+    BeamBlock *beam_dev = nullptr, *beam_host = nullptr;
+    int* beam_slots = nullptr;
+    Workspace beam_attn, beam_pick;
+    hipGraphExec_t beam_exec[kMaxRows + 1] = {};
+    int beam_out[kMaxRows + 1] = {};
     // [n_layers][d_model] of the hooked step's per-layer hidden states: on the
     // device (mode 3 copies them there) and pinned on the host
     float* hook_dev = nullptr;
@@ -551,7 +572,7 @@ void drop_graphs(atlas_model* m) {
             (void)hipGraphExecDestroy(g);
             g = nullptr;
         }
-    for (auto* arr : {m->pgexec, m->pgexec_long})
+    for (auto* arr : {m->pgexec, m->pgexec_long, m->beam_exec})
         for (int k = 0; k <= kMaxRows; ++k)
             if (arr[k]) {
                 (void)hipGraphExecDestroy(arr[k]);
@@ -1145,13 +1166,24 @@ int blas_gemm(atlas_model* m, const DevMat& w, int n) {
     return blas_rows_gemm(m->blas, a, n, m->st);
 }
 
+// the beams' rows for the prefix attention: slot 0 has the prompt, row b's own
+// tokens are in the slots that its row of the table names
+atlas_prefix_batch beam_batch(const atlas_model* m, int n) {
+    const BeamBlock* b = m->beam_dev;
+    return {nullptr, &b->prefix_slot, &b->prefix_len, b->lens, m->beam_slots, m->cfg.max_seq, 1, n,
+            m->cfg.max_seq, m->cfg.max_seq};
+}
+
 // prompt_chunk = true: the n rows are ONE sequence's prompt tokens at
 // consecutive positions pos_dev[0] .. + n - 1, all in slot slots[0] (only
 // prefill_rows sets it); the step then skips the final norm, lm_head and
 // choice, and its attention may take the query-tiled prompt kernel, which
 // relies on exactly that layout.  Ragged rows (any other caller) pass false.
+// beam_out > 0: the n rows are the beams of one prompt, which m->beam_dev
+// describes (with long_ctx); their attention reads the prompt's keys and values
+// once for all of them, and the step ends with the beam_out best candidates.
 int batch_step(atlas_model* m, int n, const std::vector<int>& slots, bool long_ctx,
-               bool prompt_chunk = false) {
+               bool prompt_chunk = false, int beam_out = 0) {
     const atlas_model_config& c = m->cfg;
     const bool with_head = !prompt_chunk;
     // a pre-norm model's prompt keeps the 24-bit activations of its decode step
@@ -1163,7 +1195,8 @@ int batch_step(atlas_model* m, int n, const std::vector<int>& slots, bool long_c
     int8_t* xd = (int8_t*)xs;                                 // (int8: digit rows)
     float* xsc = bc ? blas_rows_xscale(m->blas) : nullptr;    // (int8: their row scales)
     float* dd = bc ? blas_rows_d(m->blas) : nullptr;          // product rows
-    TRY(embed_launch(m->embed, c.vocab, d, m->tok_dev, 0, m->x, d, n, m->st));
+    BeamBlock* const beam = beam_out > 0 ? m->beam_dev : nullptr;
+    TRY(embed_launch(m->embed, c.vocab, d, beam ? beam->tok : m->tok_dev, 0, m->x, d, n, m->st));
     if (bc && b8) TRY(digits_rows_launch(m->x, d, n, d, xd, xsc, m->st));
     else if (bc) TRY(split_rows_launch(m->x, d, n, d, xs, m->st));
     for (int li = 0; li < c.n_layers; ++li) {
@@ -1201,9 +1234,14 @@ int batch_step(atlas_model* m, int n, const std::vector<int>& slots, bool long_c
         q.q_norm = L.q_norm; q.k_norm = L.k_norm; q.qk_eps = 1e-6f;
         q.cos_tab = m->cos_tab; q.sin_tab = m->sin_tab;
         q.k_cache = L.kc; q.v_cache = L.vc; q.slot_stride = m->slot_stride;
-        q.slot_dev = m->slot_dev; q.pos_dev = m->pos_dev;
+        q.slot_dev = beam ? beam->slot : m->slot_dev; q.pos_dev = beam ? beam->pos : m->pos_dev;
         q.n_heads = c.n_heads; q.n_kv = c.n_kv_heads; q.head_dim = m->hd;
-        if (m->fused && long_ctx) {
+        if (beam) {
+            TRY(qkv_post_launch(q, n, m->st));
+            const atlas_slot_cache cache{L.kc, L.vc, m->B, c.max_seq, c.n_kv_heads, m->hd};
+            TRY(prefix_attention_launch(cache, beam_batch(m, n), m->qkv, m->qkv_rows, c.n_heads, m->scale, L.window,
+                                        m->att, d, m->beam_attn, m->st));
+        } else if (m->fused && long_ctx) {
             // long contexts: QK-norm/RoPE/KV write, then the split kernel over
             // (KV head, split, sequence) and the split merge as a second
             // kernel (no per-block device-scope fence)
@@ -1309,6 +1347,9 @@ int batch_step(atlas_model* m, int n, const std::vector<int>& slots, bool long_c
     if (!with_head) return ATLAS_OK;
     TRY(rmsnorm_launch(m->x, m->final_norm, m->xn, d, n, d, c.rms_eps, m->st));
     TRY(bmm(m, m->lm_head, m->xn, m->logits, n, EPI_STORE));
+    if (beam)
+        return beam_select_launch(m->logits, c.vocab, c.vocab, beam->scores, 1, n, beam_out, beam->out_tok,
+                                  beam->out_parents, beam->out_scores, m->beam_pick, m->st);
     // greedy choice of every row into choice_dev (last maximum wins): one
     // launch pair for all rows while their partial keys fit, else per row
     const int parts = std::min(512, (c.vocab + 255) / 256);
@@ -1355,6 +1396,87 @@ int run_batch_step(atlas_model* m, int n, const std::vector<int>& slots, bool lo
         }
     }
     ATLAS_HIP(hipGraphLaunch(ge, m->st));
+    return ATLAS_OK;
+}
+
+// What a beam search needs beside the model's own buffers, on its first call.
+int beam_setup(atlas_model* m) {
+    const atlas_model_config& c = m->cfg;
+    if (!m->beam_host) {
+        if (host_malloc_pinned(&m->beam_host, sizeof(BeamBlock)) != hipSuccess) {
+            (void)hipGetLastError();
+            m->beam_host = nullptr;
+            set_error(ATLAS_ENOMEM, "generate_beam: pinned staging block");
+            return ATLAS_ENOMEM;
+        }
+    }
+    if (!m->beam_dev) TRY(dalloc(m, (void**)&m->beam_dev, sizeof(BeamBlock)));
+    if (!m->beam_slots) TRY(dalloc(m, (void**)&m->beam_slots, (size_t)kMaxRows * c.max_seq * 4));
+    if (!m->beam_pick.p) {
+        const size_t bytes = beam_select_workspace(c.vocab, 1, kMaxRows, kBeamOut);
+        TRY(dalloc(m, &m->beam_pick.p, bytes));
+        m->beam_pick.bytes = bytes;
+    }
+    if (!m->beam_attn.counters) {
+        size_t bytes = 256, counters = 1;
+        const atlas_slot_cache cache{m->L[0].kc, m->L[0].vc, m->B, c.max_seq, c.n_kv_heads, m->hd};
+        for (int n = 1; n <= kMaxRows; ++n)
+            for (const LayerW& L : m->L) {
+                size_t b = 0, k = 0;
+                prefix_attention_workspace(cache, beam_batch(m, n), c.n_heads, L.window, &b, &k);
+                bytes = std::max(bytes, b);
+                counters = std::max(counters, k);
+            }
+        if (!m->beam_attn.p) TRY(dalloc(m, &m->beam_attn.p, bytes));
+        m->beam_attn.bytes = bytes;
+        m->beam_attn.n_counters = counters;
+        int* p = nullptr;
+        TRY(dalloc(m, (void**)&p, counters * sizeof(int)));
+        if (hipMemset(p, 0, counters * sizeof(int)) != hipSuccess) {
+            set_error(ATLAS_EHIP, "generate_beam: counter init failed");
+            return ATLAS_EHIP;
+        }
+        m->beam_attn.counters = p;
+    }
+    return ATLAS_OK;
+}
+
+// A beam step of n rows and n_out candidates, replayed from a graph.
+int run_beam_step(atlas_model* m, int n, int n_out) {
+    const std::vector<int> slots;
+    if (!m->use_graph) {
+        TRY(batch_step(m, n, slots, true, false, n_out));
+    } else {
+        hipGraphExec_t& ge = m->beam_exec[n];
+        if (ge && m->beam_out[n] != n_out) {
+            ATLAS_HIP(hipStreamSynchronize(m->st));
+            (void)hipGraphExecDestroy(ge);
+            ge = nullptr;
+        }
+        if (!ge) {
+            hipGraph_t g = nullptr;
+            ATLAS_HIP(hipStreamBeginCapture(m->st, hipStreamCaptureModeThreadLocal));
+            const int rc = batch_step(m, n, slots, true, false, n_out);
+            hipError_t e = hipStreamEndCapture(m->st, &g);
+            if (rc) {
+                if (g) (void)hipGraphDestroy(g);
+                return rc;
+            }
+            if (e != hipSuccess) {
+                set_error(ATLAS_EHIP, "graph capture: %s", hipGetErrorString(e));
+                return ATLAS_EHIP;
+            }
+            e = hipGraphInstantiate(&ge, g, nullptr, nullptr, 0);
+            (void)hipGraphDestroy(g);
+            if (e != hipSuccess) {
+                ge = nullptr;
+                set_error(ATLAS_EHIP, "graph instantiate: %s", hipGetErrorString(e));
+                return ATLAS_EHIP;
+            }
+            m->beam_out[n] = n_out;
+        }
+        ATLAS_HIP(hipGraphLaunch(ge, m->st));
+    }
     return ATLAS_OK;
 }
 
@@ -1628,6 +1750,7 @@ ATLAS_API void atlas_model_destroy(atlas_model* m) {
         if (e) (void)hipEventDestroy(e);
     if (m->ring) (void)hipHostFree(m->ring);
     if (m->hook_stage) (void)hipHostFree(m->hook_stage);
+    if (m->beam_host) (void)hipHostFree(m->beam_host);
     if (m->st) (void)hipStreamDestroy(m->st);
     delete m;
 }
@@ -2465,4 +2588,131 @@ ATLAS_API int atlas_model_generate_batch(atlas_model* m, const uint32_t* prompts
     TRY(sync_pos(m));
     ATLAS_HIP(hipStreamSynchronize(m->st));
     return ATLAS_OK;
+}
+
+namespace {
+
+// a hypothesis of a beam search
+struct BeamHyp {
+    std::vector<uint32_t> tok;
+    double score, rank;                  // its sum of log probabilities, and that over its length's power
+};
+
+int generate_beam(atlas_model* m, const uint32_t* prompt, int n_prompt, int max_new, int width, float length_penalty,
+                  const atlas_sampling* s, uint32_t* out, int* n_out, double* scores) {
+    const double minus_inf = -HUGE_VAL;
+    const int n_stop = s ? (s->eos_token_id >= 0) + std::max(s->n_extra_stop, 0) : 0;
+    // every beam may end with each of the stop tokens: as many candidates leave `width` that go on
+    const int n_cand = (int)std::min<long>(kBeamOut, (long)width * (1 + n_stop));
+    const auto rank = [&](double score, int len) { return score / std::pow((double)len, (double)length_penalty); };
+    std::vector<BeamHyp> done;
+    const auto finish = [&](BeamHyp h) {                 // the best `width`, of equal ones the earlier
+        const auto at = std::upper_bound(done.begin(), done.end(), h, [](const BeamHyp& a, const BeamHyp& b) { return a.rank > b.rank; });
+        done.insert(at, std::move(h));
+        if ((int)done.size() > width) done.pop_back();
+    };
+    TRY(reset_state(m));
+    TRY(prefill(m, prompt, n_prompt - 1));
+    TRY(sync_pos(m));
+    TRY(set_token(m, prompt[n_prompt - 1]));
+    TRY(run_step(m, 0));
+    BeamBlock& b = *m->beam_host;
+    std::memset(&b, 0, sizeof b);
+    // Beam r writes its tokens into slot r, so that the table of slots begins with
+    // r everywhere; reordering moves the part that is written.
+    {
+        std::vector<int> ids((size_t)width * max_new);
+        for (int r = 0; r < width; ++r) std::fill_n(ids.begin() + (size_t)r * max_new, max_new, r);
+        ATLAS_HIP(hipMemcpy2DAsync(m->beam_slots, (size_t)m->cfg.max_seq * 4, ids.data(), (size_t)max_new * 4,
+                                   (size_t)max_new * 4, width, hipMemcpyHostToDevice, m->st));
+        ATLAS_HIP(hipStreamSynchronize(m->st));
+    }
+    ATLAS_HIP(hipMemcpyAsync(m->beam_dev, &b, sizeof b, hipMemcpyHostToDevice, m->st));
+    TRY(beam_select_launch(m->logits, m->cfg.vocab, m->cfg.vocab, m->beam_dev->scores, 1, 1, n_cand, m->beam_dev->out_tok,
+                           m->beam_dev->out_parents, m->beam_dev->out_scores, m->beam_pick, m->st));
+    std::vector<std::vector<uint32_t>> live(width);
+    for (int len = 1; len <= max_new; ++len) {           // the candidates make sequences of len tokens
+        ATLAS_HIP(hipMemcpyAsync(&b, m->beam_dev, sizeof b, hipMemcpyDeviceToHost, m->st));
+        ATLAS_HIP(hipStreamSynchronize(m->st));
+        std::vector<std::vector<uint32_t>> next;
+        for (int r = 0; r < kMaxRows; ++r) {             // beams that are none: any token, no score
+            b.tok[r] = 0;
+            b.scores[r] = minus_inf;
+            b.parents[r] = r;
+            b.slot[r] = r;
+            b.pos[r] = n_prompt + len - 1;
+            b.lens[r] = n_prompt + len;
+        }
+        b.prefix_slot = 0;
+        b.prefix_len = n_prompt;
+        for (int i = 0; i < n_cand && (int)next.size() < width && b.out_parents[i] >= 0; ++i) {
+            const std::vector<uint32_t>& parent = live[b.out_parents[i]];
+            if (is_stop(s, b.out_tok[i])) {
+                if (i < width) finish({parent, b.out_scores[i], rank(b.out_scores[i], len)});
+                continue;
+            }
+            const int r = (int)next.size();
+            next.push_back(parent);
+            next.back().push_back(b.out_tok[i]);
+            b.tok[r] = b.out_tok[i];
+            b.scores[r] = b.out_scores[i];
+            b.parents[r] = b.out_parents[i];
+        }
+        if (next.empty()) break;
+        if (len == max_new) {
+            for (size_t r = 0; r < next.size(); ++r) finish({next[r], b.scores[r], rank(b.scores[r], len)});
+            break;
+        }
+        // nothing that is live can pass the worst of `width` that are done
+        if ((int)done.size() == width && std::max(rank(b.scores[0], len + 1), rank(b.scores[0], max_new)) <= done.back().rank) break;
+        live = std::move(next);
+        live.resize(width);
+        ATLAS_HIP(hipMemcpyAsync(m->beam_dev, &b, sizeof b, hipMemcpyHostToDevice, m->st));
+        void* const table = m->beam_slots;
+        const void* const from = table;
+        TRY(beam_reorder_launch(&table, &from, 1, (long)(len - 1) * 4, (long)m->cfg.max_seq * 4, m->beam_dev->parents, 1,
+                                width, m->st));
+        TRY(run_beam_step(m, width, n_cand));
+    }
+    for (int r = 0; r < width; ++r) {
+        const bool some = r < (int)done.size();
+        n_out[r] = some ? (int)done[r].tok.size() : 0;
+        scores[r] = some ? done[r].score : minus_inf;
+        if (some) std::copy(done[r].tok.begin(), done[r].tok.end(), out + (size_t)r * max_new);
+    }
+    return ATLAS_OK;
+}
+
+}  // namespace
+
+ATLAS_API int atlas_model_generate_beam(atlas_model* m, const uint32_t* prompt, int n_prompt, int max_new, int width,
+                                        float length_penalty, const atlas_sampling* s, uint32_t* out, int* n_out,
+                                        double* scores) {
+    ATLAS_REQUIRE(m && prompt && out && n_out && scores, "generate_beam: null argument");
+    ATLAS_REQUIRE(width >= 1 && width <= std::min(m->B, kMaxRows), "generate_beam: width %d outside 1..min(max_batch %d, %d)",
+                  width, m->B, kMaxRows);
+    ATLAS_REQUIRE(n_prompt >= 1 && max_new >= 1 && n_prompt <= m->cfg.max_seq - max_new, "generate_beam: %d prompt and %d new tokens, max_seq %d",
+                  n_prompt, max_new, m->cfg.max_seq);
+    ATLAS_REQUIRE(std::isfinite(length_penalty), "generate_beam: length_penalty %g", length_penalty);
+    ATLAS_REQUIRE(!s || s->n_extra_stop <= 0 || s->extra_stop_tokens, "generate_beam: null extra_stop_tokens");
+    if (!m->fused) {
+        set_error(ATLAS_EUNSUPPORTED, "generate_beam: head_dim %d, %d heads over %d KV heads: not a shape of the fused step", m->hd,
+                  m->cfg.n_heads, m->cfg.n_kv_heads);
+        return ATLAS_EUNSUPPORTED;
+    }
+    int rc;
+    try {
+        rc = beam_setup(m);
+        if (!rc) rc = generate_beam(m, prompt, n_prompt, max_new, width, length_penalty, s, out, n_out, scores);
+    } catch (const std::bad_alloc&) {
+        set_error(ATLAS_ENOMEM, "generate_beam: host memory");
+        rc = ATLAS_ENOMEM;
+    }
+    m->pos = 0;
+    const int end = sync_pos(m);
+    if (hipStreamSynchronize(m->st) != hipSuccess && !rc) {
+        set_error(ATLAS_EHIP, "generate_beam: stream synchronisation failed");
+        rc = ATLAS_EHIP;
+    }
+    return rc ? rc : end;
 }

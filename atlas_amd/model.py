@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -375,6 +375,20 @@ class OlmoModel:
         check(load().atlas_model_generate_batch(self._h, _p(flat), _p(lens), len(prompts), max_new,
                                                 C.byref(s), _p(out), _p(nout)))
         return [[int(t) for t in out[i, :nout[i]]] for i in range(len(prompts))]
+
+    def generate_beam(self, prompt: Sequence[int], max_new: int, width: int,
+                      length_penalty: float = 1.0) -> List[Tuple[List[int], float]]:
+        """Beam search (extension): up to ``width`` (of max_batch and 16 at most) hypotheses,
+        best first, as (tokens, sum of log probabilities), ranked by that sum over
+        length ** length_penalty.  The model's stop tokens end a hypothesis."""
+        keep: list = []
+        s = self._sampling(SamplingConfig.greedy(), keep)
+        pr = np.ascontiguousarray(list(prompt) or [0], np.uint32)
+        n = max(width, 1)
+        out, nout, scores = np.zeros((n, max(max_new, 1)), np.uint32), np.zeros(n, np.int32), np.zeros(n)
+        check(load().atlas_model_generate_beam(self._h, _p(pr), len(prompt), max_new, width, length_penalty,
+                                               C.byref(s), _p(out), _p(nout), _p(scores)))
+        return [([int(t) for t in out[i, :nout[i]]], float(scores[i])) for i in range(n) if scores[i] > -np.inf]
 
     def decode_greedy(self, first_token: int, n_steps: int) -> np.ndarray:
         """Replays the captured step n_steps times with no host sync in between."""

@@ -175,6 +175,22 @@ int atlas_model_generate_batch(atlas_model* m, const uint32_t* prompts, const in
                                int n_seqs, int max_new, const atlas_sampling* s, uint32_t* out,
                                int* n_out);
 
+/* Beam search (extension; the reference has none): resets, feeds the prompt (n_prompt >= 1)
+ * and keeps the `width` (up to max_batch and 16) likeliest continuations, each step choosing
+ * among the best of all beams' tokens (atlas_beam_select_f32; the best min(64, width *
+ * (1 + stop tokens)) candidates).  The beams share the prompt's keys and values
+ * (atlas_prefix_attention_f32).  A candidate that ends with one of s's stop tokens (all that is
+ * read of s, which may be NULL) is done if it is among the step's first `width`; at max_new
+ * tokens every beam is.  Hypotheses are ranked by their sum of log probabilities over
+ * length^length_penalty, the length counting the stop token (0: by the sum); the search
+ * ends when no beam can pass the worst of `width` that are done.  out [width][max_new], n_out
+ * and scores (sums of log probabilities) [width], best first; stop tokens are not
+ * emitted; fewer hypotheses (all logits NaN): length 0 and score -inf.  Models whose attention
+ * the fused step does not cover return ATLAS_EUNSUPPORTED.                     */
+int atlas_model_generate_beam(atlas_model* m, const uint32_t* prompt, int n_prompt, int max_new,
+                              int width, float length_penalty, const atlas_sampling* s,
+                              uint32_t* out, int* n_out, double* scores);
+
 /* One token choice of generate_with_sampling's loop on the host
  * (crates/atlas-model/src/lib.rs:1623-1711): step-0 suppression, repetition
  * penalty over the last repetition_window of hist, greedy argmax, or

@@ -126,3 +126,11 @@ def test_host_side_refusals():
         with pytest.raises(AtlasError) as e:
             call()
         assert e.value.code == -1
+
+
+@pytest.mark.parametrize("n", ["0", "17", "x"])
+def test_beams_argument(n):
+    from atlas_amd import cli
+    assert cli.parse_args(["--weights", "/x"]).beams == 1 and cli.parse_args(["--weights", "/x", "--beams", "16"]).beams == 16
+    with pytest.raises(SystemExit):
+        cli.parse_args(["--weights", "/x", "--beams", n])
