@@ -8,6 +8,7 @@
 // instructions.  A row's own tokens go through the same instructions, seen by its
 // columns only.
 #include <algorithm>
+#include <type_traits>
 
 #include "many.hpp"
 
@@ -19,6 +20,9 @@ constexpr float kPfLog2e = 1.4426950408889634f;
 constexpr int kPfWaves = 4;
 constexpr int kPfChunk = 16;           // tokens that a wave takes at a time
 constexpr int kPfMaxSplits = 64;
+
+// waves of a SIMD for the registers of HD and CT, and so blocks of a CU
+constexpr int pf_at_once(int hd, int ct) { return hd == 256 ? 1 : hd * ct <= 64 ? 4 : hd * ct <= 128 ? 3 : hd * ct <= 256 ? 2 : 1; }
 
 struct PfArgs {
     const float *k, *v;
@@ -63,15 +67,6 @@ __device__ __forceinline__ void pf_get(const float* p, float& a, float& b) {
     b = __uint_as_float((uint32_t)(v >> 32));
 }
 
-// What a tile's rows see: the shared tokens [first, last), and `own` tokens of their
-// own in the rows' order, row r's from own_at[r] on.
-template <int CT>
-struct PfRows {
-    int from[16 * CT], to[16 * CT];    // a row sees tokens [from, to)
-    int own_from[16 * CT];             // its first own one that is seen
-    int own_at[16 * CT + 1];
-};
-
 template <int HD, int CT>
 struct PfShared {
     union {
@@ -81,15 +76,111 @@ struct PfShared {
     };
     float m[kPfWaves][16 * CT], l[kPfWaves][16 * CT];
     float sum[16 * CT];                // the columns' sums of weights
-    PfRows<CT> rows;
     int last;
 };
 
 __device__ __forceinline__ bool pf_infinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
+__device__ __forceinline__ int wave_max_int(int v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v = max(v, __shfl_xor(v, d, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// A tile's tokens: the shared ones that any of its rows sees, [first, last), then the
+// rows' own ones one row after the other, each part in whole chunks.  Lane r has what
+// concerns row r.
+struct PfTokens {
+    int n_rows, row0;
+    int from, to;                      // the row sees tokens [from, to)
+    int own_from, own_begin, own_end;  // its first own one that is seen; its places among the own ones
+    int slot;                          // of its own ones, where that is one
+    int shared_len, shared_cell;       // the shared slot's first cell
+    int first, last, own;
+    int shared_chunks, chunks;
+    int lo_all, hi_all;                // tokens [lo_all, hi_all) are seen by all rows
+
+    __device__ __forceinline__ void set(const PfArgs& a, int group, int row0_, int n_rows_, int lane) {
+        row0 = row0_;
+        n_rows = n_rows_;
+        const bool mine = lane < n_rows;
+        const int r = row0 + (mine ? lane : 0), raw = a.lens[r];
+        slot = a.slot_stride ? 0 : a.slots[r];
+        shared_len = __builtin_amdgcn_readfirstlane(max(a.prefix_lens[group], 0));
+        const int shared_slot = __builtin_amdgcn_readfirstlane(a.prefix_slots[group]);
+        const bool cells = a.n_slots > 0 && a.max_seq > 0, there = cells && shared_slot >= 0 && shared_slot < a.n_slots;
+        const int own_cap = cells ? min(a.slot_stride ? a.slot_stride : a.max_seq, max(a.max_seq - shared_len, 0)) : 0;
+        to = mine ? max(raw, 0) : 0;
+        from = a.window > 0 && to > a.window ? to - a.window : 0;
+        own_from = max(from - shared_len, 0);
+        const int n = max(min(to - shared_len, own_cap) - own_from, 0);
+        own_end = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(own_end, d, 64);
+            own_end += lane >= d ? x : 0;
+        }
+        own_begin = own_end - n;
+        own = __builtin_amdgcn_readlane(own_end, 63);
+        const int hi = wave_max_int(to), lo = -wave_max_int(to > from ? -from : -0x7FFFFFFF);
+        lo_all = wave_max_int(mine ? from : 0);
+        hi_all = -wave_max_int(mine ? -to : -0x7FFFFFFF);
+        last = there ? min(min(shared_len, a.max_seq), hi) : 0;
+        first = min(lo, last);
+        shared_cell = there ? shared_slot * a.max_seq : 0;
+        shared_chunks = (last - first + kPfChunk - 1) / kPfChunk;
+        chunks = shared_chunks + (own + kPfChunk - 1) / kPfChunk;
+    }
+};
+
+// A chunk's tokens, token i in the lanes of i.
+struct PfChunk {
+    int row, t;                        // its row (-1: shared) and position (-1: not there)
+    int slot, x;                       // of an own one: its slot, on its way, and place in the row
+    int row_first, row_last;           // of the chunk
+    bool own, live;
+    bool plain;                        // every column sees every token
+
+    // which tokens; the table's entries are asked for
+    __device__ __forceinline__ void find(const PfArgs& a, const PfTokens& k, int chunk, int i) {
+        own = chunk >= k.shared_chunks;
+        plain = false;
+        if (!own) {
+            const int c0 = k.first + chunk * kPfChunk;
+            t = c0 + i;
+            live = t < k.last;
+            row = -1;
+            plain = c0 >= k.lo_all && c0 + kPfChunk <= min(k.hi_all, k.last);
+        } else {
+            const int e0 = (chunk - k.shared_chunks) * kPfChunk, e = e0 + i;
+            row_first = __popcll(__ballot(k.own_end <= e0));
+            row_last = __popcll(__ballot(k.own_end <= min(e0 + kPfChunk, k.own) - 1));
+            row = row_first;
+            for (int r = row_first; r < row_last; ++r) row += e >= __builtin_amdgcn_readlane(k.own_end, r) ? 1 : 0;
+            live = e < k.own;
+            const int begin = __shfl(k.own_begin, row, 64), from = __shfl(k.own_from, row, 64);   // (of every lane)
+            x = live ? e - begin + from : 0;
+            slot = a.slot_stride ? a.slots[(long)(k.row0 + row) * a.slot_stride + x] : __shfl(k.slot, row, 64);
+        }
+    }
+    // the token's cell; of one that is not there some cell that is
+    __device__ __forceinline__ int cell(const PfArgs& a, const PfTokens& k) {
+        int c;
+        if (!own) {
+            c = k.shared_cell + min(t, k.last - 1);
+        } else {
+            live = live & (slot >= 0) & (slot < a.n_slots);
+            t = k.shared_len + x;
+            c = live ? slot * a.max_seq + t : 0;
+        }
+        t = live ? t : -1;
+        return c;
+    }
+};
+
 template <int HD, int CT>
-__global__ __launch_bounds__(kPfWaves * 64) void pf_attention_kernel(PfArgs a) {
-    constexpr int S = HD / 16, H = HD / 64, R = 16 * CT;
+__global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attention_kernel(PfArgs a) {
+    constexpr int S = HD / 16, H = HD / 64;
     __shared__ PfShared<HD, CT> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
@@ -99,8 +190,6 @@ __global__ __launch_bounds__(kPfWaves * 64) void pf_attention_kernel(PfArgs a) {
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, pair = at / a.tiles * 8 + xcd, u = at % a.tiles;
     if (pair >= a.n_kv * a.splits) return;
     const int split = pair / a.n_kv, kvh = pair - split * a.n_kv;
-
-    // ---- the tile's rows
     int grp = 0, row0 = u * a.rows, end = a.n_rows;
     if (a.starts) {
         grp = __builtin_amdgcn_readfirstlane(pf_group(a, u));
@@ -111,63 +200,31 @@ __global__ __launch_bounds__(kPfWaves * 64) void pf_attention_kernel(PfArgs a) {
     }
     row0 = __builtin_amdgcn_readfirstlane(row0);
     const int n_rows = __builtin_amdgcn_readfirstlane(min(a.rows, end - row0)), cols = n_rows * a.group;
-    const int shared_len = max(a.prefix_lens[grp], 0), shared_slot = a.prefix_slots[grp];
-    const bool cells = a.n_slots > 0 && a.max_seq > 0;
-    const int own_cap = cells ? min(a.slot_stride ? a.slot_stride : a.max_seq, max(a.max_seq - shared_len, 0)) : 0;
-    if (wave == 0) {
-        // rows beyond the last see nothing
-        const bool mine = lane < n_rows;
-        const int len = mine ? max(a.lens[row0 + lane], 0) : 0;
-        const int from = a.window > 0 && len > a.window ? len - a.window : 0;
-        const int own_from = max(from - shared_len, 0), own = max(min(len - shared_len, own_cap) - own_from, 0);
-        int sum = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += x;
-        }
-        if (lane < R) {
-            sh.rows.from[lane] = from;
-            sh.rows.to[lane] = len;
-            sh.rows.own_from[lane] = own_from;
-            sh.rows.own_at[lane + 1] = sum;
-        }
-        if (lane == 0) sh.rows.own_at[0] = 0;
-    }
     // the query, scaled for exp2; columns past the last repeat it
-    for (int e = threadIdx.x; e < CT * S * 64; e += kPfWaves * 64) {
+    constexpr int PER = CT * S * 64 / (kPfWaves * 64);
+    f32x4 query[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = threadIdx.x + j * kPfWaves * 64;
         const int l = e & 63, s = e / 64 % S, c = min(e / (64 * S) * 16 + (l & 15), cols - 1), row = c / a.group;
-        const float* p = a.q + (row0 + row) * a.ld_q + ((long)kvh * a.group + c - row * a.group) * HD + s * 16 + (l >> 4) * 4;
-        sh.q[0][0][e] = *reinterpret_cast<const f32x4*>(p) * (a.scale * kPfLog2e);
+        query[j] = *reinterpret_cast<const f32x4*>(a.q + (row0 + row) * a.ld_q + ((long)kvh * a.group + c - row * a.group) * HD +
+                                                   s * 16 + (l >> 4) * 4);
     }
-    __syncthreads();
-    // what every row sees, and what any does
-    int lo = 0x7FFFFFFF, hi = 0, lo_all = 0, hi_all = 0x7FFFFFFF;
-    for (int r = 0; r < n_rows; ++r) {
-        const int f = sh.rows.from[r], t = sh.rows.to[r];
-        if (t > f) lo = min(lo, f);
-        hi = max(hi, t);
-        lo_all = max(lo_all, f);
-        hi_all = min(hi_all, t);
-    }
-    const bool there = cells && shared_slot >= 0 && shared_slot < a.n_slots;
-    const int last = there ? min(min(shared_len, a.max_seq), hi) : 0, first = min(lo, last);
-    const int own = sh.rows.own_at[n_rows];
-    const int shared_chunks = (last - first + kPfChunk - 1) / kPfChunk;
-    const int chunks = __builtin_amdgcn_readfirstlane(shared_chunks + (own + kPfChunk - 1) / kPfChunk);
-    // the block's run
-    const int run = (max((chunks + a.splits - 1) / a.splits, 2 * kPfWaves) + kPfWaves - 1) / kPfWaves * kPfWaves;
-    const int begin = split * run, stop = min(begin + run, chunks);
-    if (split > 0 && begin >= chunks) return;
-    const int runs = max((chunks + run - 1) / run, 1);
+    PfTokens tokens;
+    tokens.set(a, grp, row0, n_rows, lane);
+    // the block's run of the chunks, of which a wave takes every fourth
+    const int run = max((tokens.chunks + a.splits - 1) / a.splits, 2 * kPfWaves);
+    const int begin = split * run, stop = min(begin + run, tokens.chunks);
+    if (split > 0 && begin >= tokens.chunks) return;
+    const int runs = max((tokens.chunks + run - 1) / run, 1);
 
     int col_row[CT], from[CT], to[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-        const int col = 16 * c + i;
-        col_row[c] = col < cols ? col / a.group : -1;
-        from[c] = col < cols ? sh.rows.from[col / a.group] : 0;
-        to[c] = col < cols ? sh.rows.to[col / a.group] : 0;
+        const int col = 16 * c + i, row = col < cols ? col / a.group : 63;
+        from[c] = __shfl(tokens.from, row, 64);
+        to[c] = __shfl(tokens.to, row, 64);
+        col_row[c] = col < cols ? row : -2;
     }
     f32x4 o[CT][H][4];
     float m[CT], l[CT];
@@ -182,90 +239,77 @@ __global__ __launch_bounds__(kPfWaves * 64) void pf_attention_kernel(PfArgs a) {
     }
 
     const long pitch = (long)a.n_kv * HD;
-    const float *const kb = a.k + (long)kvh * HD, *const vb = a.v + (long)kvh * HD;
-#pragma unroll 1
-    for (int chunk = begin + wave; chunk < stop; chunk += kPfWaves) {
-        // Token i of the chunk: its cell (one that is not there: some cell that is, and
-        // `live` says so), and the row that it belongs to (-1: shared).
-        long cell;
-        int row, t;
-        bool live, plain;
-        if (chunk < shared_chunks) {
-            t = first + chunk * kPfChunk + i;
-            live = t < last;
-            cell = (long)shared_slot * a.max_seq + min(t, last - 1);
-            row = -1;
-            const int c0 = first + chunk * kPfChunk;
-            plain = c0 >= lo_all && c0 + kPfChunk <= min(hi_all, last);
-        } else {
-            const int e = (chunk - shared_chunks) * kPfChunk + i;
-            int r = 0, r_end = n_rows;
-            while (r_end - r > 1) {
-                const int mid = (r + r_end) >> 1;
-                if (sh.rows.own_at[mid] <= e) r = mid;
-                else r_end = mid;
-            }
-            row = r;
-            const int x = e - sh.rows.own_at[r] + sh.rows.own_from[r];
-            live = e < own;
-            const int slot = live ? a.slots[(long)(row0 + r) * max(a.slot_stride, 1) + (a.slot_stride ? x : 0)] : -1;
-            live = slot >= 0 && slot < a.n_slots;
-            t = shared_len + x;
-            cell = live ? (long)slot * a.max_seq + t : 0;
-            plain = false;
+    const float *const kb = a.k + (long)kvh * HD + 4 * g, *const vb = a.v + (long)kvh * HD + 4 * i;
+    const int n = begin + wave < stop ? (stop - begin - wave + kPfWaves - 1) / kPfWaves : 0;
+    const auto chunk_of = [&](int t) { return begin + wave + t * kPfWaves; };
+    f32x4 kf[S], vf[4][H];
+    PfChunk cur, next;
+    int cell = 0, next_cell = 0;
+    bool infinite = false;
+    const auto fetch_k = [&](int c) {
+        const float* p = kb + c * pitch;
+#pragma unroll
+        for (int s = 0; s < S; ++s) kf[s] = *reinterpret_cast<const f32x4*>(p + 16 * s);
+    };
+    const auto fetch_v = [&](int c) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float* p = vb + __shfl(c, 4 * g + r, 64) * pitch;
+#pragma unroll
+            for (int h = 0; h < H; ++h) vf[r][h] = *reinterpret_cast<const f32x4*>(p + 64 * h);
         }
-        f32x4 kf[S], vf[4][H];
-        {
-            const float* p = kb + cell * pitch + 4 * g;
+    };
+    if (n > 0) {
+        cur.find(a, tokens, chunk_of(0), i);
+        cell = cur.cell(a, tokens);
+        fetch_k(cell);
+        fetch_v(cell);
+        if (n > 1) next.find(a, tokens, chunk_of(1), i);
+    }
 #pragma unroll
-            for (int s = 0; s < S; ++s) kf[s] = *reinterpret_cast<const f32x4*>(p + 16 * s);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const long vc = __shfl(cell, 4 * g + r, 64);
-                const float* pv = vb + vc * pitch + 4 * i;
-#pragma unroll
-                for (int h = 0; h < H; ++h) vf[r][h] = *reinterpret_cast<const f32x4*>(pv + 64 * h);
-            }
-        }
+    for (int j = 0; j < PER; ++j) sh.q[0][0][threadIdx.x + j * kPfWaves * 64] = query[j] * (a.scale * kPfLog2e);
+    __syncthreads();
+
+    const auto round = [&](int t, auto more) {
+        // the column tiles that see any of the chunk
+        const int c_first = cur.own ? cur.row_first * a.group >> 4 : 0;
+        const int c_last = cur.own ? ((cur.row_last + 1) * a.group - 1) >> 4 : CT - 1;
+        const auto needs = [&](int c) { return CT == 1 || (c >= c_first && c <= c_last); };
         // S: tokens 4g + r of column i
         float sc[CT][4];
-        {
-            f32x4 d[CT];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) d[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < CT; ++c) {
+            f32x4 d[2] = {};
+            if (needs(c))
 #pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
+                for (int s = 0; s < S; ++s) {
                     const f32x4 qf = sh.q[c][s][lane];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) d[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[s][e], qf[e], d[c], 0, 0, 0);
+                    for (int e = 0; e < 4; ++e) d[s & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[s][e], qf[e], d[s & 1], 0, 0, 0);
                 }
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sc[c][r] = d[c][r];
+            for (int r = 0; r < 4; ++r) sc[c][r] = d[0][r] + d[1][r];
         }
-        uint32_t seen[CT];
-        if (!plain) {
+        if constexpr (decltype(more)::value) {
+            next_cell = next.cell(a, tokens);
+            fetch_k(next_cell);
+        }
+        if (!cur.plain) {
             // (without short circuits, which would be branches)
             int tok_row[4], tok[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                tok_row[r] = __shfl(row, 4 * g + r, 64);
-                tok[r] = __shfl(live ? t : -1, 4 * g + r, 64);
+                tok_row[r] = __shfl(cur.row, 4 * g + r, 64);
+                tok[r] = __shfl(cur.t, 4 * g + r, 64);
             }
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                seen[c] = 0;
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t ok = (uint32_t)(tok[r] >= from[c]) & (uint32_t)(tok[r] < to[c]) &
                                         ((uint32_t)(tok_row[r] < 0) | (uint32_t)(tok_row[r] == col_row[c]));
-                    seen[c] |= ok << r;
                     sc[c][r] = ok ? sc[c][r] : -__builtin_inff();
                 }
-            }
         }
         // weights; the maximum is raised only when a score passes it by more than 2^8
         f32x4 p[CT];
@@ -289,54 +333,74 @@ __global__ __launch_bounds__(kPfWaves * 64) void pf_attention_kernel(PfArgs a) {
                 l[c] += p[c][r];
             }
         }
-        if (!plain) {
+        if (!cur.plain) {
             // Infinities and NaN of V are nothing to the columns that do not see their
-            // token: they leave the matrix product and are added where they are seen.
-            bool bad = false;
+            // token: they leave the matrix product, and are seen to at the end.
+            float none = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int h = 0; h < H; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) bad = bad || pf_infinite(vf[r][h][e]);
-            if (__any(bad)) {
-#pragma unroll 1
-                for (int gt = 0; gt < 4; ++gt)
+                    for (int e = 0; e < 4; ++e) none = fmaf(vf[r][h][e], 0.f, none);
+            if (__any(none != 0.f)) {
+                infinite = true;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int c = 0; c < CT; ++c) {
-                            const float w = __shfl(p[c][r], 16 * gt + i, 64);
-                            const bool ok = __shfl((int)(seen[c] >> r & 1u), 16 * gt + i, 64) != 0;
+                    for (int h = 0; h < H; ++h)
 #pragma unroll
-                            for (int h = 0; h < H; ++h)
+                        for (int e = 0; e < 4; ++e) vf[r][h][e] = pf_infinite(vf[r][h][e]) ? 0.f : vf[r][h][e];
+            }
+        }
+        // O^T += V^T P: elements 64 h + 4 (4g + r) + e of column i
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                                    for (int x = 0; x < 4; ++x) {
-                                        const float y = __shfl(vf[r][h][e], 16 * gt + 4 * g + x, 64);
-                                        if (ok && pf_infinite(y)) o[c][h][e][x] += w * y;
-                                    }
-                        }
+        for (int c = 0; c < CT; ++c)
+            if (needs(c))
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int h = 0; h < H; ++h)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (pf_infinite(vf[r][h][e])) vf[r][h][e] = 0.f;
+                            o[c][h][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][h][e], p[c][r], o[c][h][e], 0, 0, 0);
+        if constexpr (decltype(more)::value) {
+            fetch_v(next_cell);
+            cur = next;
+            cell = next_cell;
+            if (t + 2 < n) next.find(a, tokens, chunk_of(t + 2), i);
+        }
+    };
+    int t = 0;
+#pragma unroll 1
+    for (; t + 1 < n; ++t) round(t, std::true_type{});
+    if (t < n) round(t, std::false_type{});
+    // (Rare: the tokens are gone through again.)
+    if (infinite) {
+#pragma unroll 1
+        for (t = 0; t < n; ++t) {
+            cur.find(a, tokens, chunk_of(t), i);
+            cell = cur.cell(a, tokens);
+            if (cur.plain) continue;
+#pragma unroll 1
+            for (int j = 0; j < kPfChunk; ++j) {
+                const int tok = __builtin_amdgcn_readlane(cur.t, j), row = __builtin_amdgcn_readlane(cur.row, j);
+                if (tok < 0) continue;
+                const float* p = vb - 4 * i + __builtin_amdgcn_readlane(cell, j) * pitch + 16 * g;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const f32x4 y = *reinterpret_cast<const f32x4*>(p + 64 * h + 4 * x);
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) {
+                            const bool ok = (tok >= from[c]) & (tok < to[c]) & ((row < 0) | (row == col_row[c]));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[c][h][e][x] += ok & pf_infinite(y[e]) ? y[e] : 0.f;
+                        }
+                    }
             }
         }
-        // O^T += V^T P: elements 64 h + 4 (4g + r) + e of column i
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        o[c][h][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r][h][e], p[c][r], o[c][h][e], 0, 0, 0);
     }
 
     // ---- the waves' sums, a column tile at a time
@@ -450,7 +514,7 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     if (window > 0) own = std::min<int64_t>(own, window);
     const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
     const long units = std::max(1L, (long)s.tiles * c.n_kv);
-    const long want = device_cu_count() * 3L / units, most = (chunks + 2 * kPfWaves - 1) / (2 * kPfWaves);
+    const long want = (long)device_cu_count() * pf_at_once(c.head_dim, s.ct) / units, most = (chunks + 2 * kPfWaves - 1) / (2 * kPfWaves);
     const long fit = (long)((256u << 20) / ((size_t)units * s.cols * (c.head_dim + 2) * sizeof(float)));
     s.splits = (int)std::max(1L, std::min({want, most, fit, (long)kPfMaxSplits}));
     return s;
@@ -470,8 +534,7 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
                   c.head_dim);
     ATLAS_REQUIRE(c.n_slots >= 0 && c.max_seq >= 0 && c.max_seq <= 1 << 24 && c.n_kv > 0 && c.n_kv <= 4096, "%s: %d slots of %d tokens, %d KV heads",
                   who, c.n_slots, c.max_seq, c.n_kv);
-    ATLAS_REQUIRE((long)c.n_slots * c.max_seq <= INT64_MAX / 4 / ((long)c.n_kv * c.head_dim), "%s: %d slots of %d tokens", who,
-                  c.n_slots, c.max_seq);
+    ATLAS_REQUIRE((long)c.n_slots * c.max_seq < 1L << 31, "%s: %d slots of %d tokens", who, c.n_slots, c.max_seq);
     ATLAS_REQUIRE(b.n_groups >= 0 && b.n_rows >= 0 && b.slot_stride >= 0 && b.max_prefix >= 0 && b.max_own >= 0,
                   "%s: %d groups, %d rows, slot stride %d, max_prefix %d, max_own %d", who, b.n_groups, b.n_rows,
                   b.slot_stride, b.max_prefix, b.max_own);
