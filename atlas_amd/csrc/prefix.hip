@@ -8,6 +8,7 @@
 // instructions.  A row's own tokens go through the same instructions, seen by its
 // columns only.
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "many.hpp"
@@ -17,12 +18,12 @@ namespace atlas {
 constexpr float kPfFloor = -3.0e38f;   // running maximum of a column that has seen nothing
 constexpr float kPfLazy = 8.0f;
 constexpr float kPfLog2e = 1.4426950408889634f;
-constexpr int kPfWaves = 4;
 constexpr int kPfChunk = 16;           // tokens that a wave takes at a time
 constexpr int kPfMaxSplits = 64;
 
 // waves of a SIMD for the registers of HD and CT, and so blocks of a CU
-constexpr int pf_at_once(int hd, int ct) { return hd == 256 ? 1 : hd * ct <= 64 ? 4 : hd * ct <= 128 ? 3 : hd * ct <= 256 ? 2 : 1; }
+constexpr int pf_waves(int hd) { return hd == 256 ? 4 : 8; }      // of a block
+constexpr int pf_at_once(int hd, int ct) { return hd * ct <= 64 ? 2 : 1; }
 
 struct PfArgs {
     const float *k, *v;
@@ -69,12 +70,13 @@ __device__ __forceinline__ void pf_get(const float* p, float& a, float& b) {
 
 template <int HD, int CT>
 struct PfShared {
+    static constexpr int W = pf_waves(HD);
     union {
         f32x4 q[CT][HD / 16][64];      // [column tile][step of 16 elements][lane]
-        float o[kPfWaves][16][HD + 4]; // the waves' sums of a column tile
+        float o[W][16][HD + 4]; // the waves' sums of a column tile
         float f[kPfMaxSplits][16 * CT];    // the runs' factors
     };
-    float m[kPfWaves][16 * CT], l[kPfWaves][16 * CT];
+    float m[W][16 * CT], l[W][16 * CT];
     float sum[16 * CT];                // the columns' sums of weights
     int last;
 };
@@ -179,8 +181,8 @@ struct PfChunk {
 };
 
 template <int HD, int CT>
-__global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attention_kernel(PfArgs a) {
-    constexpr int S = HD / 16, H = HD / 64;
+__global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD) / 4) void pf_attention_kernel(PfArgs a) {
+    constexpr int S = HD / 16, H = HD / 64, W = pf_waves(HD);
     __shared__ PfShared<HD, CT> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
@@ -201,22 +203,23 @@ __global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attentio
     row0 = __builtin_amdgcn_readfirstlane(row0);
     const int n_rows = __builtin_amdgcn_readfirstlane(min(a.rows, end - row0)), cols = n_rows * a.group;
     // the query, scaled for exp2; columns past the last repeat it
-    constexpr int PER = CT * S * 64 / (kPfWaves * 64);
+    constexpr int ITEMS = CT * S * 64, PER = (ITEMS + W * 64 - 1) / (W * 64);
     f32x4 query[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int e = threadIdx.x + j * kPfWaves * 64;
+        const int e = threadIdx.x + j * W * 64;
+        if (e >= ITEMS) break;
         const int l = e & 63, s = e / 64 % S, c = min(e / (64 * S) * 16 + (l & 15), cols - 1), row = c / a.group;
         query[j] = *reinterpret_cast<const f32x4*>(a.q + (row0 + row) * a.ld_q + ((long)kvh * a.group + c - row * a.group) * HD +
                                                    s * 16 + (l >> 4) * 4);
     }
     PfTokens tokens;
     tokens.set(a, grp, row0, n_rows, lane);
-    // the block's run of the chunks, of which a wave takes every fourth
-    const int run = max((tokens.chunks + a.splits - 1) / a.splits, 2 * kPfWaves);
-    const int begin = split * run, stop = min(begin + run, tokens.chunks);
-    if (split > 0 && begin >= tokens.chunks) return;
-    const int runs = max((tokens.chunks + run - 1) / run, 1);
+    // Every wave of the tile's blocks takes every so many chunks: shared tokens are more
+    // work than own ones, and each has its share of both.  Two chunks to a wave at least.
+    const int runs = min(max((tokens.chunks + 2 * W - 1) / (2 * W), 1), a.splits);
+    if (split >= runs) return;
+    const int stride = runs * W;
 
     int col_row[CT], from[CT], to[CT];
 #pragma unroll
@@ -240,8 +243,8 @@ __global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attentio
 
     const long pitch = (long)a.n_kv * HD;
     const float *const kb = a.k + (long)kvh * HD + 4 * g, *const vb = a.v + (long)kvh * HD + 4 * i;
-    const int n = begin + wave < stop ? (stop - begin - wave + kPfWaves - 1) / kPfWaves : 0;
-    const auto chunk_of = [&](int t) { return begin + wave + t * kPfWaves; };
+    const int w0 = split * W + wave, n = w0 < tokens.chunks ? (tokens.chunks - w0 + stride - 1) / stride : 0;
+    const auto chunk_of = [&](int t) { return w0 + t * stride; };
     f32x4 kf[S], vf[4][H];
     PfChunk cur, next;
     int cell = 0, next_cell = 0;
@@ -267,7 +270,8 @@ __global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attentio
         if (n > 1) next.find(a, tokens, chunk_of(1), i);
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) sh.q[0][0][threadIdx.x + j * kPfWaves * 64] = query[j] * (a.scale * kPfLog2e);
+    for (int j = 0; j < PER; ++j)
+        if (threadIdx.x + j * W * 64 < ITEMS) sh.q[0][0][threadIdx.x + j * W * 64] = query[j] * (a.scale * kPfLog2e);
     __syncthreads();
 
     const auto round = [&](int t, auto more) {
@@ -430,14 +434,14 @@ __global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attentio
                     f32x4{o[ct][h][0][x], o[ct][h][1][x], o[ct][h][2][x], o[ct][h][3][x]};
         __syncthreads();
         const int here = min(max(cols - 16 * ct, 0), 16);
-        for (int e = threadIdx.x; e < here * (HD / 4); e += kPfWaves * 64) {
+        for (int e = threadIdx.x; e < here * (HD / 4); e += W * 64) {
             const int c = e / (HD / 4), d = e % (HD / 4) * 4, col = 16 * ct + c;
             float top = kPfFloor, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < kPfWaves; ++w) top = fmaxf(top, sh.m[w][col]);
+            for (int w = 0; w < W; ++w) top = fmaxf(top, sh.m[w][col]);
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kPfWaves; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float f = __builtin_amdgcn_exp2f(sh.m[w][col] - top);
                 sum += f * sh.l[w][col];
                 x += f * *reinterpret_cast<const f32x4*>(&sh.o[w][c][d]);
@@ -463,7 +467,7 @@ __global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attentio
     __syncthreads();
     if (!sh.last) return;
     // a run to a lane, a column to a wave
-    for (int c = wave; c < cols; c += kPfWaves) {
+    for (int c = wave; c < cols; c += W) {
         float top = kPfFloor, sum = 0.f;
         if (lane < runs) pf_get(a.part_ml + 2 * (part + (long)lane * a.cols + c), top, sum);
         const float f = __builtin_amdgcn_exp2f(top - wave_max(top));
@@ -472,10 +476,10 @@ __global__ __launch_bounds__(kPfWaves * 64, pf_at_once(HD, CT)) void pf_attentio
         if (lane == 0) sh.sum[c] = sum;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < cols * (HD / 4); e += kPfWaves * 64) {
+    for (int e = threadIdx.x; e < cols * (HD / 4); e += W * 64) {
         const int c = e / (HD / 4), d = e % (HD / 4) * 4;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 16
         for (int r = 0; r < runs; ++r) {
             const float* p = a.part_o + (part + (long)r * a.cols + c) * HD + d;
             float y[4];
@@ -502,6 +506,7 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     // columns of an average group
     const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
     s.ct = wide <= 16 ? 1 : wide <= 32 ? 2 : 4;
+    if (getenv("PFCT")) s.ct = std::min(s.ct, atoi(getenv("PFCT")));
     if (c.head_dim == 256) s.ct = std::min(s.ct, 2);
     s.rows = 16 * s.ct / group;
     s.cols = s.rows * group;
@@ -514,7 +519,7 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     if (window > 0) own = std::min<int64_t>(own, window);
     const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
     const long units = std::max(1L, (long)s.tiles * c.n_kv);
-    const long want = (long)device_cu_count() * pf_at_once(c.head_dim, s.ct) / units, most = (chunks + 2 * kPfWaves - 1) / (2 * kPfWaves);
+    const long want = (long)device_cu_count() * (getenv("PFOCC") ? atoi(getenv("PFOCC")) : pf_at_once(c.head_dim, s.ct)) / units, most = (chunks + 2 * pf_waves(c.head_dim) - 1) / (2 * pf_waves(c.head_dim));
     const long fit = (long)((256u << 20) / ((size_t)units * s.cols * (c.head_dim + 2) * sizeof(float)));
     s.splits = (int)std::max(1L, std::min({want, most, fit, (long)kPfMaxSplits}));
     return s;
@@ -582,7 +587,7 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
         a.part_ml = a.part_o + parts * c.head_dim;
     }
     const dim3 grid((unsigned)(((long)c.n_kv * s.splits + 7) / 8 * 8 * s.tiles));
-#define PF_RUN(HD, CT) hipLaunchKernelGGL((pf_attention_kernel<HD, CT>), grid, dim3(kPfWaves * 64), 0, st, a)
+#define PF_RUN(HD, CT) hipLaunchKernelGGL((pf_attention_kernel<HD, CT>), grid, dim3(pf_waves(HD) * 64), 0, st, a)
     if (c.head_dim == 64) {
         if (s.ct == 1) PF_RUN(64, 1); else if (s.ct == 2) PF_RUN(64, 2); else PF_RUN(64, 4);
     } else if (c.head_dim == 128) {
