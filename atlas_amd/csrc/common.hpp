@@ -39,7 +39,6 @@ enum ScratchSlot {
     SCR_KV4,            // atlas_kv4_attention_f32 split partials
     SCR_KV4_CNT,        // ... its counters of finished blocks (kept at zero by the kernel)
     SCR_PREFIX,         // atlas_prefix_attention_f32 split partials
-    SCR_PREFIX_CNT,     // ... its counters of finished blocks (kept at zero by the kernel)
     SCR_BEAM,           // atlas_beam_select_f32: what the pieces of rows leave
     SCR_LORA,           // atlas_lora_add_f32: the rows' low-rank products
     SCR_N

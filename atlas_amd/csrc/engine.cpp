@@ -1417,26 +1417,14 @@ int beam_setup(atlas_model* m) {
         TRY(dalloc(m, &m->beam_pick.p, bytes));
         m->beam_pick.bytes = bytes;
     }
-    if (!m->beam_attn.counters) {
-        size_t bytes = 256, counters = 1;
+    if (!m->beam_attn.p) {
+        size_t bytes = 256;
         const atlas_slot_cache cache{m->L[0].kc, m->L[0].vc, m->B, c.max_seq, c.n_kv_heads, m->hd};
         for (int n = 1; n <= kMaxRows; ++n)
-            for (const LayerW& L : m->L) {
-                size_t b = 0, k = 0;
-                prefix_attention_workspace(cache, beam_batch(m, n), c.n_heads, L.window, &b, &k);
-                bytes = std::max(bytes, b);
-                counters = std::max(counters, k);
-            }
-        if (!m->beam_attn.p) TRY(dalloc(m, &m->beam_attn.p, bytes));
+            for (const LayerW& L : m->L)
+                bytes = std::max(bytes, prefix_attention_workspace(cache, beam_batch(m, n), c.n_heads, L.window));
+        TRY(dalloc(m, &m->beam_attn.p, bytes));
         m->beam_attn.bytes = bytes;
-        m->beam_attn.n_counters = counters;
-        int* p = nullptr;
-        TRY(dalloc(m, (void**)&p, counters * sizeof(int)));
-        if (hipMemset(p, 0, counters * sizeof(int)) != hipSuccess) {
-            set_error(ATLAS_EHIP, "generate_beam: counter init failed");
-            return ATLAS_EHIP;
-        }
-        m->beam_attn.counters = p;
     }
     return ATLAS_OK;
 }

@@ -10,15 +10,12 @@ namespace atlas {
 struct Workspace {
     void* p = nullptr;
     size_t bytes = 0;
-    int* counters = nullptr;     // zero before the first launch, left at zero
-    size_t n_counters = 0;
 };
 
 int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch& b, const float* q, long ld_q, int n_heads,
                             float scale, int window, float* out, long ld_out, const Workspace& ws, hipStream_t st);
 // what a launch of this shape takes at most
-void prefix_attention_workspace(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window, size_t* bytes,
-                                size_t* counters);
+size_t prefix_attention_workspace(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window);
 
 int beam_select_launch(const float* logits, long ld, int vocab, const double* scores, int n_groups, int width, int n_out,
                        uint32_t* tokens, int* parents, double* out_scores, const Workspace& ws, hipStream_t st);

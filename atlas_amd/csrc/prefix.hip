@@ -8,7 +8,6 @@
 // instructions.  A row's own tokens go through the same instructions, seen by its
 // columns only.
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "many.hpp"
@@ -20,6 +19,12 @@ constexpr float kPfLazy = 8.0f;
 constexpr float kPfLog2e = 1.4426950408889634f;
 constexpr int kPfChunk = 16;           // tokens that a wave takes at a time
 constexpr int kPfMaxSplits = 64;
+constexpr int kPfLeast = 8;            // chunks of a block, where a tile has several
+
+// What a tile and KV head leave for the join.
+struct PfUnit {
+    int runs, cols, row0, pad;         // runs 0 and 1: nothing to join
+};
 
 // waves of a SIMD for the registers of HD and CT, and so blocks of a CU
 constexpr int pf_waves(int hd) { return hd == 256 ? 4 : 8; }      // of a block
@@ -41,7 +46,7 @@ struct PfArgs {
     int window;
     int splits, cols;                  // blocks of a tile and KV head at most; [tiles][n_kv][splits][cols] partial sums
     float *part_o, *part_ml;
-    int* counters;                     // [tiles][n_kv] blocks that are done, zero between calls
+    PfUnit* unit;                      // [tiles][n_kv]
 };
 
 // The group of the batch's tile u.  Tiles of group g begin at starts[g] / rows + g,
@@ -56,37 +61,39 @@ __device__ __forceinline__ int pf_group(const PfArgs& a, int u) {
     return lo;
 }
 
-// partial sums past this XCD's L2 and back (agent scope)
-__device__ __forceinline__ void pf_put(float* p, float a, float b) {
-    const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ void pf_get(const float* p, float& a, float& b) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    a = __uint_as_float((uint32_t)v);
-    b = __uint_as_float((uint32_t)(v >> 32));
-}
-
 template <int HD, int CT>
 struct PfShared {
     static constexpr int W = pf_waves(HD);
     union {
         f32x4 q[CT][HD / 16][64];      // [column tile][step of 16 elements][lane]
         float o[W][16][HD + 4]; // the waves' sums of a column tile
-        float f[kPfMaxSplits][16 * CT];    // the runs' factors
     };
     float m[W][16 * CT], l[W][16 * CT];
-    float sum[16 * CT];                // the columns' sums of weights
-    int last;
+
 };
 
 __device__ __forceinline__ bool pf_infinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
+// all lanes' largest value, and the sum of the lanes up to this one (DPP: rows of 16, then
+// the last lane of one row, and of two, to the next)
 __device__ __forceinline__ int wave_max_int(int v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = max(v, __shfl_xor(v, d, 64));
-    return __builtin_amdgcn_readfirstlane(v);
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+__device__ __forceinline__ int wave_scan_int(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
 }
 
 // A tile's tokens: the shared ones that any of its rows sees, [first, last), then the
@@ -116,12 +123,7 @@ struct PfTokens {
         from = a.window > 0 && to > a.window ? to - a.window : 0;
         own_from = max(from - shared_len, 0);
         const int n = max(min(to - shared_len, own_cap) - own_from, 0);
-        own_end = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(own_end, d, 64);
-            own_end += lane >= d ? x : 0;
-        }
+        own_end = wave_scan_int(n);
         own_begin = own_end - n;
         own = __builtin_amdgcn_readlane(own_end, 63);
         const int hi = wave_max_int(to), lo = -wave_max_int(to > from ? -from : -0x7FFFFFFF);
@@ -197,7 +199,10 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
         grp = __builtin_amdgcn_readfirstlane(pf_group(a, u));
         const int begin = min(max(a.starts[grp], 0), a.n_rows), skip = (u - (a.starts[grp] / a.rows + grp)) * a.rows;
         end = min(a.starts[grp + 1], a.n_rows);
-        if (skip < 0 || skip >= end - begin) return;
+        if (skip < 0 || skip >= end - begin) {
+            if (split == 0 && threadIdx.x == 0 && a.splits > 1) a.unit[u * a.n_kv + kvh] = {0, 0, 0, 0};
+            return;
+        }
         row0 = begin + skip;
     }
     row0 = __builtin_amdgcn_readfirstlane(row0);
@@ -217,8 +222,9 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
     tokens.set(a, grp, row0, n_rows, lane);
     // Every wave of the tile's blocks takes every so many chunks: shared tokens are more
     // work than own ones, and each has its share of both.  Two chunks to a wave at least.
-    const int runs = min(max((tokens.chunks + 2 * W - 1) / (2 * W), 1), a.splits);
+    const int runs = min(max((tokens.chunks + kPfLeast - 1) / kPfLeast, 1), a.splits);
     if (split >= runs) return;
+    if (split == 0 && threadIdx.x == 0 && a.splits > 1) a.unit[u * a.n_kv + kvh] = {runs, cols, row0, 0};
     const int stride = runs * W;
 
     int col_row[CT], from[CT], to[CT];
@@ -450,46 +456,55 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
                 store(col, d, x, sum);
             } else {
                 const long at = part + (long)split * a.cols + col;
-                pf_put(a.part_o + at * HD + d, x.x, x.y);
-                pf_put(a.part_o + at * HD + d + 2, x.z, x.w);
-                if (d == 0) pf_put(a.part_ml + 2 * at, top, sum);
+                *reinterpret_cast<f32x4*>(a.part_o + at * HD + d) = x;
+                if (d == 0) {
+                    a.part_ml[2 * at] = top;
+                    a.part_ml[2 * at + 1] = sum;
+                }
             }
         }
     }
-    if (runs == 1) return;
-    // The block that ends last joins the runs.  Every thread's partial sums have
-    // arrived before its block is counted, so they are there for the last one.
-    __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0)
-    __syncthreads();
-    int* const counter = a.counters + (long)u * a.n_kv + kvh;
-    if (threadIdx.x == 0)
-        sh.last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == runs - 1;
-    __syncthreads();
-    if (!sh.last) return;
-    // a run to a lane, a column to a wave
-    for (int c = wave; c < cols; c += W) {
-        float top = kPfFloor, sum = 0.f;
-        if (lane < runs) pf_get(a.part_ml + 2 * (part + (long)lane * a.cols + c), top, sum);
-        const float f = __builtin_amdgcn_exp2f(top - wave_max(top));
-        sum = wave_sum(lane < runs ? f * sum : 0.f);
-        if (lane < runs) sh.f[lane][c] = f;
-        if (lane == 0) sh.sum[c] = sum;
+}
+
+// The runs' sums of a column: a wave, each of whose lanes has four elements of every so
+// many runs.
+template <int HD>
+__global__ __launch_bounds__(256) void pf_join_kernel(PfArgs a) {
+    constexpr int LANES = HD / 4, RG = 64 / LANES;
+    const int lane = threadIdx.x & 63, unit = blockIdx.x, c = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const PfUnit x = a.unit[unit];
+    if (x.runs <= 1 || c >= x.cols) return;
+    const long part = (long)unit * a.splits * a.cols + c;
+    float top = kPfFloor, sum = 0.f;
+    if (lane < x.runs) {
+        top = a.part_ml[2 * (part + (long)lane * a.cols)];
+        sum = a.part_ml[2 * (part + (long)lane * a.cols) + 1];
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < cols * (HD / 4); e += W * 64) {
-        const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 16
-        for (int r = 0; r < runs; ++r) {
-            const float* p = a.part_o + (part + (long)r * a.cols + c) * HD + d;
-            float y[4];
-            pf_get(p, y[0], y[1]);
-            pf_get(p + 2, y[2], y[3]);
-            x += sh.f[r][c] * f32x4{y[0], y[1], y[2], y[3]};
+    const float f = __builtin_amdgcn_exp2f(top - wave_max(top));
+    sum = wave_sum(lane < x.runs ? f * sum : 0.f);
+    const int rg = lane / LANES, d = lane % LANES * 4;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    // eight loads at a time, without conditions (a last run again, with no weight)
+    for (int r0 = 0; r0 < x.runs; r0 += 8 * RG) {
+        f32x4 y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            y[j] = *reinterpret_cast<const f32x4*>(a.part_o + (part + (long)min(r0 + j * RG + rg, x.runs - 1) * a.cols) * HD + d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = r0 + j * RG + rg;
+            const float fr = __shfl(f, min(r, 63), 64);
+            o += (r < x.runs ? fr : 0.f) * y[j];
         }
-        store(c, d, x, sh.sum[c]);
     }
-    if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int s = LANES; s < 64; s <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], s, 64);
+    if (rg) return;
+    const int row = c / a.group, kvh = unit % a.n_kv;
+    float* p = a.out + (x.row0 + row) * a.ld_out + ((long)kvh * a.group + c - row * a.group) * HD + d;
+    *reinterpret_cast<f32x4*>(p) = o * (sum == 0.f ? 0.f : 1.f / sum);
 }
 
 // ---- launches ---------------------------------------------------------------------
@@ -505,9 +520,7 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     const int group = n_heads / c.n_kv;
     // columns of an average group
     const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
-    s.ct = wide <= 16 ? 1 : wide <= 32 ? 2 : 4;
-    if (getenv("PFCT")) s.ct = std::min(s.ct, atoi(getenv("PFCT")));
-    if (c.head_dim == 256) s.ct = std::min(s.ct, 2);
+    s.ct = wide <= 128 || c.head_dim == 256 ? 1 : 2;
     s.rows = 16 * s.ct / group;
     s.cols = s.rows * group;
     s.tiles = b.group_starts ? b.n_rows / s.rows + b.n_groups : (b.n_rows + s.rows - 1) / s.rows;
@@ -519,17 +532,18 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     if (window > 0) own = std::min<int64_t>(own, window);
     const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
     const long units = std::max(1L, (long)s.tiles * c.n_kv);
-    const long want = (long)device_cu_count() * (getenv("PFOCC") ? atoi(getenv("PFOCC")) : pf_at_once(c.head_dim, s.ct)) / units, most = (chunks + 2 * pf_waves(c.head_dim) - 1) / (2 * pf_waves(c.head_dim));
+    const long want = (long)device_cu_count() * pf_at_once(c.head_dim, s.ct) / units, most = chunks <= 2 * kPfLeast ? 1 : (chunks + kPfLeast - 1) / kPfLeast;
     const long fit = (long)((256u << 20) / ((size_t)units * s.cols * (c.head_dim + 2) * sizeof(float)));
     s.splits = (int)std::max(1L, std::min({want, most, fit, (long)kPfMaxSplits}));
     return s;
 }
 
-void prefix_attention_workspace(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window, size_t* bytes,
-                                size_t* counters) {
-    const PfShape s = pf_shape(c, b, n_heads, window);
-    *bytes = s.splits > 1 ? s.parts() * c.n_kv * (c.head_dim + 2) * sizeof(float) : 0;
-    *counters = s.splits > 1 ? (size_t)s.tiles * c.n_kv : 0;
+static size_t pf_bytes(const PfShape& s, const atlas_slot_cache& c) {
+    return s.splits > 1 ? s.parts() * c.n_kv * (c.head_dim + 2) * sizeof(float) + (size_t)s.tiles * c.n_kv * sizeof(PfUnit) : 0;
+}
+
+size_t prefix_attention_workspace(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window) {
+    return pf_bytes(pf_shape(c, b, n_heads, window), c);
 }
 
 int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch& b, const float* q, long ld_q, int n_heads,
@@ -572,31 +586,34 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
     a.rows = s.rows; a.tiles = s.tiles; a.cols = s.cols; a.splits = s.splits;
     a.scale = scale; a.window = window;
     if (s.splits > 1) {
-        const size_t parts = s.parts() * c.n_kv, bytes = parts * (c.head_dim + 2) * sizeof(float);
-        void *p = ws.p, *cnt = ws.counters;
+        const size_t bytes = pf_bytes(s, c);
+        void* p = ws.p;
         if (p) {
-            ATLAS_REQUIRE(ws.bytes >= bytes && cnt && ws.n_counters >= (size_t)units, "%s: workspace of %zu bytes, %zu needed",
-                          who, ws.bytes, bytes);
+            ATLAS_REQUIRE(ws.bytes >= bytes, "%s: workspace of %zu bytes, %zu needed", who, ws.bytes, bytes);
         } else {
-            int rc;
-            if ((rc = thread_scratch(SCR_PREFIX_CNT, (size_t)units * sizeof(int), &cnt, true))) return rc;
-            if ((rc = thread_scratch(SCR_PREFIX, bytes, &p))) return rc;
+            const int rc = thread_scratch(SCR_PREFIX, bytes, &p);
+            if (rc) return rc;
         }
-        a.counters = static_cast<int*>(cnt);
-        a.part_o = static_cast<float*>(p);
-        a.part_ml = a.part_o + parts * c.head_dim;
+        a.unit = static_cast<PfUnit*>(p);
+        a.part_o = reinterpret_cast<float*>(a.unit + units);
+        a.part_ml = a.part_o + s.parts() * c.n_kv * c.head_dim;
     }
     const dim3 grid((unsigned)(((long)c.n_kv * s.splits + 7) / 8 * 8 * s.tiles));
 #define PF_RUN(HD, CT) hipLaunchKernelGGL((pf_attention_kernel<HD, CT>), grid, dim3(pf_waves(HD) * 64), 0, st, a)
-    if (c.head_dim == 64) {
-        if (s.ct == 1) PF_RUN(64, 1); else if (s.ct == 2) PF_RUN(64, 2); else PF_RUN(64, 4);
-    } else if (c.head_dim == 128) {
-        if (s.ct == 1) PF_RUN(128, 1); else if (s.ct == 2) PF_RUN(128, 2); else PF_RUN(128, 4);
-    } else {
-        if (s.ct == 1) PF_RUN(256, 1); else PF_RUN(256, 2);
-    }
+    if (c.head_dim == 64 && s.ct == 1) PF_RUN(64, 1);
+    else if (c.head_dim == 64) PF_RUN(64, 2);
+    else if (c.head_dim == 128 && s.ct == 1) PF_RUN(128, 1);
+    else if (c.head_dim == 128) PF_RUN(128, 2);
+    else PF_RUN(256, 1);
 #undef PF_RUN
     ATLAS_LAUNCH_CHECK("prefix_attention");
+    if (s.splits > 1) {
+        const dim3 join((unsigned)units, (s.cols + 3) / 4);
+        if (c.head_dim == 64) hipLaunchKernelGGL(pf_join_kernel<64>, join, dim3(256), 0, st, a);
+        else if (c.head_dim == 128) hipLaunchKernelGGL(pf_join_kernel<128>, join, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(pf_join_kernel<256>, join, dim3(256), 0, st, a);
+        ATLAS_LAUNCH_CHECK("prefix_join");
+    }
     return ATLAS_OK;
 }
 
