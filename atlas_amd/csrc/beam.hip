@@ -17,10 +17,13 @@ namespace atlas {
 //   2  a block joins a group's pieces: lse of each row, then the largest scores.
 // The n_out largest of many: each lane's largest first; the n_out-th largest of a wave's
 // 64 is a bound that at least n_out elements reach, so that what lies below it goes, and
-// the few that are left are ranked by counting.
+// the few that are left are ranked by counting.  Where many reach the bound (equal
+// logits), the largest is taken n_out times.
 
 constexpr int kBeamMaxOut = 64;
-constexpr int kBeamPer = 16, kBeamThreads = 256, kBeamPiece = kBeamPer * kBeamThreads;
+constexpr int kBeamThreads = 512;
+constexpr int kBeamWaves = kBeamThreads / 64;
+constexpr int kBeamList = 1024;
 
 // order-preserving: larger logits have larger keys; 0 for what is no candidate
 __device__ __forceinline__ uint32_t beam_order(float z) {
@@ -30,6 +33,8 @@ __device__ __forceinline__ uint32_t beam_order(float z) {
 __device__ __forceinline__ float beam_logit(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
+
+constexpr uint32_t kBeamLowest = 0x00800000u;            // of the lowest finite logit
 
 // larger first; of equal logits the lower token
 __device__ __forceinline__ uint64_t beam_key(float z, uint32_t token) {
@@ -41,24 +46,106 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
     return (uint64_t)hi << 32 | lo;
 }
 
-// the wave's values in descending order of the lanes
-__device__ __forceinline__ uint64_t wave_sort(uint64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            const uint64_t w = shfl_xor64(v, step);
-            const bool large = ((lane & size) == 0) == ((lane & step) == 0);   // the lane keeps the larger
-            v = (v > w) == large ? v : w;
-        }
-    return v;
+// One step of a reduction over the wave's lanes (DPP: quads, rows of 16, then rows to the
+// next); after all six, lane 63 has the result.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp32(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(v, v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    return (uint64_t)dpp32<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp32<CTRL, ROWS>((uint32_t)v);
+}
+template <typename T, int CTRL, int ROWS>
+__device__ __forceinline__ T dpp_of(T v) {
+    if constexpr (sizeof(T) == 8) return dpp64<CTRL, ROWS>(v);
+    else return dpp32<CTRL, ROWS>(v);
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+    return (uint64_t)last_lane((uint32_t)(v >> 32)) << 32 | last_lane((uint32_t)v);
+}
+template <typename T>
+__device__ __forceinline__ T wave_most(T v) {
+    const auto step = [&](T w) { v = w > v ? w : v; };
+    step(dpp_of<T, 0xB1, 0xF>(v));
+    step(dpp_of<T, 0x4E, 0xF>(v));
+    step(dpp_of<T, 0x141, 0xF>(v));
+    step(dpp_of<T, 0x140, 0xF>(v));
+    step(dpp_of<T, 0x142, 0xA>(v));
+    step(dpp_of<T, 0x143, 0xC>(v));
+    return last_lane(v);
 }
 
+// A bound that n or a few more of the wave's 64 keys reach (0: fewer than n are not 0), found
+// between 0 and the largest key `most`.
+template <typename T>
+__device__ __forceinline__ T wave_bound(T key, T most, int n) {
+    if (__popcll(__ballot(key != 0)) < n) return 0;
+    T lo = ~wave_most((T)~(key ? key : most)), hi = most;    // (the smallest key) n keys reach lo
+    if (__popcll(__ballot(key == most)) >= n) return most;
+    while (hi - lo > 1) {
+        const T mid = lo + (hi - lo) / 2;
+        const int reach = __popcll(__ballot(key >= mid));
+        if (reach >= n) {
+            lo = mid;
+            if (reach <= n + n / 4) break;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+__device__ __forceinline__ uint64_t beam_order(double s) {
+    const uint64_t u = (uint64_t)__double_as_longlong(s);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// the wave's sum, in every lane (DPP, as wave_sum)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add64(double v) {
+    const int2 w = __builtin_bit_cast(int2, v);
+    const int2 m = {__builtin_amdgcn_update_dpp(0, w.x, CTRL, ROWS, 0xF, false),
+                    __builtin_amdgcn_update_dpp(0, w.y, CTRL, ROWS, 0xF, false)};
+    return v + __builtin_bit_cast(double, m);
+}
 __device__ __forceinline__ double wave_sum64(double v) {
+    v = dpp_add64<0xB1, 0xF>(v);
+    v = dpp_add64<0x4E, 0xF>(v);
+    v = dpp_add64<0x141, 0xF>(v);
+    v = dpp_add64<0x140, 0xF>(v);
+    v = dpp_add64<0x142, 0xA>(v);
+    v = dpp_add64<0x143, 0xC>(v);
+    const int2 w = __builtin_bit_cast(int2, v);
+    const int2 r = {__builtin_amdgcn_readlane(w.x, 63), __builtin_amdgcn_readlane(w.y, 63)};
+    return __builtin_bit_cast(double, r);
+}
+
+// exp(x) of N values side by side, -708 <= x <= 0: x = n ln 2 + r with |r| <= ln 2 / 2 (ln 2 in
+// two parts, as Cody and Waite have it; n by adding a number whose last place is 1), and
+// exp r by its series, of which the first term left out is 2e-16.
+template <int N>
+__device__ __forceinline__ void beam_exp(double (&x)[N]) {
+    constexpr double ROUND = 0x1.8p52;
+    constexpr double C[13] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0,
+                              1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+    double r[N], p[N];
+    int k[N];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
+    for (int i = 0; i < N; ++i) {
+        const double t = __builtin_fma(x[i], 1.4426950408889634, ROUND), n = t - ROUND;
+        k[i] = (int)__builtin_bit_cast(uint64_t, t);
+        r[i] = __builtin_fma(n, -0x1.62e42fee00000p-1, x[i]);      // the first 32 bits of ln 2
+        r[i] = __builtin_fma(n, -0x1.a39ef35793c76p-33, r[i]);     // and the rest
+        p[i] = C[0];
+    }
+#pragma unroll
+    for (int c = 1; c < 13; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = __builtin_fma(p[i], r[i], C[c]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __builtin_ldexp(p[i], k[i]);
 }
 
 // what a piece of a row leaves
@@ -70,85 +157,132 @@ struct BeamPiece {
 
 __device__ __forceinline__ bool beam_dead(double score) { return !(fabs(score) < __builtin_inf()); }
 
-__global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const float* __restrict__ logits, long ld, int vocab,
-                                                                 const double* __restrict__ scores, int n_out, int vec,
+// PER: logits of a thread
+template <int PER>
+__global__ __launch_bounds__(kBeamThreads, PER > 16 ? 4 : 8) void beam_rows_kernel(const float* __restrict__ logits, long ld, int vocab,
+                                                                 const double* __restrict__ scores, int n_out,
                                                                  BeamPiece* __restrict__ pieces, uint64_t* __restrict__ keys) {
-    constexpr int W = kBeamThreads / 64;
-    __shared__ uint64_t list[kBeamPiece];
-    __shared__ uint64_t bound[W];
+    constexpr int W = kBeamWaves;
+    __shared__ uint64_t list[kBeamList];
+    __shared__ uint64_t largest[W];
+    __shared__ uint32_t bound[W];
     __shared__ float tops[W];
     __shared__ double sums[W];
     __shared__ int count;
     const int row = blockIdx.y, piece = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (beam_dead(scores[row])) return;                  // (the join does not look at its rows' pieces either)
     const float* z = logits + (long)row * ld;
-    const int first = piece * kBeamPiece;
-    float x[kBeamPer];
+    const int first = piece * (PER * kBeamThreads);
+    const bool dead = beam_dead(scores[row]);
+    // Vectors on their boundaries, wherever the row starts; lanes at its ends load a vector
+    // of its middle and then what they have one by one, so that no load waits for another.
+    const int shift = (int)((uintptr_t)z >> 2 & 3);
+    const auto token = [&](int j) { return first + (j / 4 * kBeamThreads + tid) * 4 + j % 4 - shift; };
+    float x[PER];
+    bool edge = vocab < 8;
+    if (!edge) {
 #pragma unroll
-    for (int j = 0; j < kBeamPer / 4; ++j) {
-        const int e = first + (j * kBeamThreads + tid) * 4;
-        if (vec && e + 4 <= vocab) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(z + e);
+        for (int j = 0; j < PER; j += 4) {
+            const int t = token(j);
+            const bool inside = (t >= 0) & (t + 4 <= vocab);
+            const f32x4 v = *reinterpret_cast<const f32x4*>(z + (inside ? t : 4 - shift));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * j + i] = v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * j + i] = e + i < vocab ? z[e + i] : -__builtin_inff();
+            for (int i = 0; i < 4; ++i) x[j + i] = v[i];
+            edge = edge | !inside;
         }
     }
+    if (edge)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int t = token(j);
+            const float v = z[min(max(t, 0), vocab - 1)];
+            x[j] = t >= 0 && t < vocab ? v : -__builtin_inff();
+        }
+    if (dead) return;                                    // (the join does not look at its rows' pieces either)
     if (tid == 0) count = 0;
-    float top = -__builtin_inff();
+    float mine = -__builtin_inff();
     bool nan = false;
-    uint64_t best = 0;
 #pragma unroll
-    for (int j = 0; j < kBeamPer; ++j) {
-        top = fmaxf(top, x[j]);
-        nan = nan || x[j] != x[j];
-        const uint64_t key = beam_key(x[j], first + (j / 4 * kBeamThreads + tid) * 4 + j % 4);
-        best = key > best ? key : best;
+    for (int j = 0; j < PER; ++j) {
+        mine = fmaxf(mine, x[j]);
+        nan = nan | (x[j] != x[j]);
     }
-    top = wave_max(top);
-    const uint64_t sorted = wave_sort(best);
-    if (lane == n_out - 1) bound[wave] = sorted;
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    uint64_t least = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        top = fmaxf(top, tops[w]);
-        least = bound[w] > least ? bound[w] : least;
-    }
-    double sum = nan ? __builtin_nan("") : 0.0;
+    const uint32_t order = mine > -__builtin_inff() ? beam_order(mine + 0.f) : 0, most_order = wave_most(order);
+    const float top = most_order ? beam_logit(most_order) : -__builtin_inff();
+    // relative to the wave's largest; terms below e^-708 are as good as none
+    double sum = 0.0;
     if (top > -__builtin_inff())
 #pragma unroll
-        for (int j = 0; j < kBeamPer; ++j) sum += exp((double)x[j] - (double)top);
-    sum = wave_sum64(sum);
-    if (lane == 0) sums[wave] = sum;
+        for (int j = 0; j < PER; j += 4) {
+            double d[4];
 #pragma unroll
-    for (int j = 0; j < kBeamPer; ++j) {
-        const uint64_t key = beam_key(x[j], first + (j / 4 * kBeamThreads + tid) * 4 + j % 4);
-        if (key && key >= least) list[atomicAdd(&count, 1)] = key;
+            for (int i = 0; i < 4; ++i) d[i] = __builtin_fmax((double)x[j + i] - (double)top, -708.0);
+            beam_exp(d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += d[i];
+        }
+    sum = wave_sum64(nan || top == __builtin_inff() ? __builtin_nan("") : sum);
+    const uint32_t nth = wave_bound(order, most_order, n_out);
+    if (lane == 0) {
+        bound[wave] = nth;
+        tops[wave] = top;
+        sums[wave] = sum;
+    }
+    __syncthreads();
+    uint32_t least = kBeamLowest;
+#pragma unroll
+    for (int w = 0; w < W; ++w) least = max(least, bound[w]);
+    if (order >= least) {
+        const float reach = beam_logit(least);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (x[j] >= reach) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kBeamList) list[at] = beam_key(x[j], token(j));
+            }
     }
     __syncthreads();
     const long at = (long)row * gridDim.x + piece;
-    if (tid == 0) {
-        double all = 0.0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) all += sums[w];
-        pieces[at] = {all, top, 0};
+    if (wave == W - 1) {                                 // (a lane to a wave)
+        const float most = wave_max(tops[min(lane, W - 1)]);
+        double f[1] = {__builtin_fmax((double)tops[min(lane, W - 1)] - (double)most, -708.0)};
+        beam_exp(f);
+        const double part = lane < W ? sums[lane] : 0.0, all = wave_sum64(part == 0.0 ? 0.0 : part * f[0]);
+        if (lane == 0) pieces[at] = {all, most, 0};
     }
-    const int n = count;
     uint64_t* to = keys + at * n_out;
+    const int n = count;
+    if (n > kBeamList) {
+        uint64_t last = ~0ull;
+        for (int k = 0; k < n_out; ++k) {
+            uint64_t best = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const uint64_t key = beam_key(x[j], token(j));
+                best = key < last && key > best ? key : best;
+            }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) {
+                const uint64_t other = shfl_xor64(best, d);
+                best = other > best ? other : best;
+            }
+            __syncthreads();
+            if (lane == 0) largest[wave] = best;
+            __syncthreads();
+            last = 0;
+            for (int w = 0; w < W; ++w) last = largest[w] > last ? largest[w] : last;
+            if (tid == 0) to[k] = last;
+        }
+        return;
+    }
     for (int e = tid; e < n; e += kBeamThreads) {
         const uint64_t key = list[e];
         int rank = 0;
+#pragma unroll 8
         for (int i = 0; i < n; ++i) rank += list[i] > key;
         if (rank < n_out) to[rank] = key;
     }
     for (int e = n + tid; e < n_out; e += kBeamThreads) to[e] = 0;
 }
-
-constexpr int kBeamJoin = 1024, kBeamList = 2048;
 
 // a candidate: larger scores first, of equal ones the lower beam, then its order there
 struct BeamCand {
@@ -164,101 +298,116 @@ __device__ __forceinline__ bool beam_before(const BeamCand& a, const BeamCand& b
 constexpr double kBeamNone = -__builtin_huge_val();
 constexpr BeamCand kBeamNobody = {kBeamNone, 0, 64};
 
-__device__ __forceinline__ BeamCand wave_sort(BeamCand v) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ BeamCand wave_first(BeamCand v) {
 #pragma unroll
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            const BeamCand w = {__shfl_xor(v.score, step, 64), shfl_xor64(v.key, step), __shfl_xor(v.beam, step, 64)};
-            const bool first = ((lane & size) == 0) == ((lane & step) == 0);
-            if (beam_before(w, v) == first) v = w;
-        }
+    for (int d = 32; d > 0; d >>= 1) {
+        const BeamCand w = {__shfl_xor(v.score, d, 64), shfl_xor64(v.key, d), __shfl_xor(v.beam, d, 64)};
+        if (beam_before(w, v)) v = w;
+    }
     return v;
 }
 
-__global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(const double* __restrict__ scores, int vocab, int width,
-                                                              int n_out, int n_pieces, const BeamPiece* __restrict__ pieces,
-                                                              const uint64_t* __restrict__ keys, uint32_t* __restrict__ tokens,
-                                                              int* __restrict__ parents, double* __restrict__ out_scores) {
-    constexpr int W = kBeamJoin / 64;
-    __shared__ double lse[64];                           // NaN: the row has no candidates
-    __shared__ BeamCand bound[W];
-    __shared__ BeamCand list[kBeamList];
+__global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(const double* __restrict__ scores, int vocab, int width,
+                                                                 int n_out, int n_pieces, const BeamPiece* __restrict__ pieces,
+                                                                 const uint64_t* __restrict__ keys, uint32_t* __restrict__ tokens,
+                                                                 int* __restrict__ parents, double* __restrict__ out_scores) {
+    constexpr int W = kBeamWaves, HELD = 4;              // candidates of a thread in registers
+    __shared__ double less[64], given[64];               // a row's lse (NaN: no candidates) and score
+    __shared__ uint64_t bound[W];
+    __shared__ BeamCand first[W];
+    __shared__ double list_score[kBeamList];
+    __shared__ uint64_t list_key[kBeamList];
+    __shared__ int list_beam[kBeamList];
     __shared__ int count;
     const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    scores += (long)group * width;
     const long row0 = (long)group * width;
+    const uint32_t per_row = n_pieces * n_out, all = width * per_row;
+    // (on their way before the rows' sums are known)
+    const uint64_t* const from = keys + row0 * per_row;
+    uint64_t held[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) held[j] = from[min((uint32_t)(tid + j * kBeamThreads), all - 1)];   // (of dead beams: anything)
     if (tid == 0) count = 0;
     for (int r = wave; r < width; r += W) {
+        const double score = scores[row0 + r];
+        const BeamPiece* p = pieces + (row0 + r) * n_pieces;
+        const BeamPiece mine = p[min(lane, n_pieces - 1)];
         double z = __builtin_nan("");
-        if (!beam_dead(scores[r])) {
-            const BeamPiece* p = pieces + (row0 + r) * n_pieces;
-            float top = -__builtin_inff();
-            for (int i = lane; i < n_pieces; i += 64) top = fmaxf(top, p[i].top);
+        if (!beam_dead(score)) {
+            float top = mine.top;
+            for (int i = lane + 64; i < n_pieces; i += 64) top = fmaxf(top, p[i].top);
             top = wave_max(top);
-            double sum = 0.0;
-            for (int i = lane; i < n_pieces; i += 64) {
-                const double s = p[i].sum;               // (a piece of -inf only has sum 0, or NaN)
-                sum += s == 0.0 ? 0.0 : s * exp((double)p[i].top - (double)top);
-            }
-            sum = wave_sum64(sum);
-            z = (double)top + log(sum);
+            // (a piece of -inf only has sum 0, or NaN)
+            const auto part = [&](const BeamPiece& x) {
+                return x.sum == 0.0 ? 0.0 : x.sum * exp((double)x.top - (double)top);
+            };
+            double sum = lane < n_pieces ? part(mine) : 0.0;
+            for (int i = lane + 64; i < n_pieces; i += 64) sum += part(p[i]);
+            z = (double)top + log(wave_sum64(sum));
+            if (!(fabs(z) < __builtin_inf())) z = __builtin_nan("");
         }
-        if (lane == 0) lse[r] = z;
+        if (lane == 0) {
+            less[r] = z;
+            given[r] = score;
+        }
     }
     __syncthreads();
-    const int per_row = n_pieces * n_out;
-    const long all = (long)width * per_row;
-    const auto candidate = [&](long e) {
+    const auto candidate = [&](uint32_t e, uint64_t key) {
         const int r = (int)(e / per_row);
-        BeamCand c = kBeamNobody;
-        const double z = lse[r];
-        if (!(fabs(z) < __builtin_inf())) return c;
-        const uint64_t key = keys[(row0 + r) * per_row + (e - (long)r * per_row)];
-        if (!key) return c;
-        c.score = scores[r] + ((double)beam_logit((uint32_t)(key >> 32)) - z);
-        c.key = key;
-        c.beam = r;
-        return c;
+        const double z = less[r];
+        if (z != z || !key) return kBeamNobody;
+        return BeamCand{given[r] + ((double)beam_logit((uint32_t)(key >> 32)) - z), key, r};
     };
-    BeamCand best = kBeamNobody;
-    for (long e = tid; e < all; e += kBeamJoin) {
-        const BeamCand c = candidate(e);
-        if (beam_before(c, best)) best = c;
-    }
-    const BeamCand sorted = wave_sort(best);
-    if (lane == n_out - 1) bound[wave] = sorted;
-    __syncthreads();
-    BeamCand least = bound[0];
-    for (int w = 1; w < W; ++w)
-        if (beam_before(bound[w], least)) least = bound[w];
-    for (long e = tid; e < all; e += kBeamJoin) {
-        const BeamCand c = candidate(e);
-        if (c.score > kBeamNone && !beam_before(least, c)) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kBeamList) list[at] = c;
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) {
+            const uint32_t e = tid + j * kBeamThreads;
+            if (e < all) f(candidate(e, held[j]));
         }
-    }
+        for (uint32_t e = tid + HELD * kBeamThreads; e < all; e += kBeamThreads) f(candidate(e, from[e]));
+    };
+    uint64_t best = 0;
+    each([&](const BeamCand& c) {
+        const uint64_t order = c.score > kBeamNone ? beam_order(c.score) : 0;
+        best = order > best ? order : best;
+    });
+    const uint64_t nth = wave_bound(best, wave_most(best), n_out);
+    if (lane == 0) bound[wave] = nth;
+    __syncthreads();
+    uint64_t least = 1;
+#pragma unroll
+    for (int w = 0; w < W; ++w) least = bound[w] > least ? bound[w] : least;
+    each([&](const BeamCand& c) {
+        if (c.score > kBeamNone && beam_order(c.score) >= least) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kBeamList) {
+                list_score[at] = c.score;
+                list_key[at] = c.key;
+                list_beam[at] = c.beam;
+            }
+        }
+    });
     __syncthreads();
     int n = count;
     if (n > kBeamList) {
-        // too many reach the bound: the largest one after the other
         BeamCand last = kBeamNobody;
         for (n = 0; n < n_out; ++n) {
+            BeamCand b = kBeamNobody;
+            each([&](const BeamCand& c) {
+                if (beam_before(c, b) && (n == 0 || beam_before(last, c))) b = c;
+            });
+            b = wave_first(b);
             __syncthreads();
-            best = kBeamNobody;
-            for (long e = tid; e < all; e += kBeamJoin) {
-                const BeamCand c = candidate(e);
-                if (beam_before(c, best) && (n == 0 || beam_before(last, c))) best = c;
-            }
-            const BeamCand s = wave_sort(best);
-            if (lane == 0) bound[wave] = s;
+            if (lane == 0) first[wave] = b;
             __syncthreads();
-            last = bound[0];
+            last = first[0];
             for (int w = 1; w < W; ++w)
-                if (beam_before(bound[w], last)) last = bound[w];
-            if (tid == 0) list[n] = last;
+                if (beam_before(first[w], last)) last = first[w];
+            if (tid == 0) {
+                list_score[n] = last.score;
+                list_key[n] = last.key;
+                list_beam[n] = last.beam;
+            }
         }
         __syncthreads();
     }
@@ -269,25 +418,42 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(const double* __re
         parents[to + rank] = some ? c.beam : -1;
         out_scores[to + rank] = some ? c.score : kBeamNone;
     };
-    for (int e = tid; e < n; e += kBeamJoin) {
-        const BeamCand c = list[e];
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += beam_before(list[i], c);
+    for (int e = tid; e < n; e += kBeamThreads) {
+        const BeamCand c = {list_score[e], list_key[e], list_beam[e]};
+        int rank = 0, same = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const double s = list_score[i];
+            rank += s > c.score;
+            same += s == c.score;
+        }
+        if (same > 1)
+            for (int i = 0; i < n; ++i)
+                rank += list_score[i] == c.score && beam_before({list_score[i], list_key[i], list_beam[i]}, c);
         if (rank < n_out) store(rank, c);
     }
-    for (int e = n + tid; e < n_out; e += kBeamJoin) store(e, kBeamNobody);
+    for (int e = n + tid; e < n_out; e += kBeamThreads) store(e, kBeamNobody);
 }
 
-static long beam_pieces(int vocab) { return (vocab + kBeamPiece - 1) / kBeamPiece; }
+// Logits of a thread: as many as leave a block to a CU at least, for what a block does
+// once (bounds, ranks) is as much work as eight exponentials of a thread.
+static int beam_per(int vocab, long rows) {
+    const long all = (long)vocab * rows, chip = (long)device_cu_count() * kBeamThreads;
+    return all >= 32 * chip ? 32 : all >= 16 * chip ? 16 : 8;
+}
+
+// (a row may start up to three logits into its first vector)
+static long beam_pieces(int vocab, int per) { return (vocab + 3L + per * kBeamThreads - 1) / (per * kBeamThreads); }
 
 size_t beam_select_workspace(int vocab, int n_groups, int width, int n_out) {
-    return (size_t)n_groups * width * beam_pieces(vocab) * (sizeof(BeamPiece) + (size_t)n_out * sizeof(uint64_t));
+    const long rows = (long)n_groups * width;
+    return rows * beam_pieces(vocab, beam_per(vocab, rows)) * (sizeof(BeamPiece) + (size_t)n_out * sizeof(uint64_t));
 }
 
 int beam_select_launch(const float* logits, long ld, int vocab, const double* scores, int n_groups, int width, int n_out,
                        uint32_t* tokens, int* parents, double* out_scores, const Workspace& ws, hipStream_t st) {
     const char* who = "beam_select";
-    ATLAS_REQUIRE(vocab > 0 && ld >= vocab, "%s: rows of %d logits, %ld apart", who, vocab, ld);
+    ATLAS_REQUIRE(vocab > 0 && vocab <= 1 << 30 && ld >= vocab, "%s: rows of %d logits, %ld apart", who, vocab, ld);
     ATLAS_REQUIRE(width >= 1 && width <= 64 && n_out >= 1 && n_out <= kBeamMaxOut, "%s: %d beams, %d continuations (1 to 64)", who,
                   width, n_out);
     ATLAS_REQUIRE(n_groups >= 0 && (long)n_groups * width <= 65535, "%s: %d groups of %d beams (65535 beams at most)", who,
@@ -304,14 +470,18 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
         const int rc = thread_scratch(SCR_BEAM, bytes, &p);
         if (rc) return rc;
     }
-    const int n_pieces = (int)beam_pieces(vocab);
+    const int per = beam_per(vocab, (long)n_groups * width), n_pieces = (int)beam_pieces(vocab, per);
     BeamPiece* pieces = static_cast<BeamPiece*>(p);
     uint64_t* keys = reinterpret_cast<uint64_t*>(pieces + (size_t)n_groups * width * n_pieces);
-    const int vec = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
-    hipLaunchKernelGGL(beam_rows_kernel, dim3(n_pieces, n_groups * width), dim3(kBeamThreads), 0, st, logits, ld, vocab, scores,
-                       n_out, vec, pieces, keys);
+#define BEAM_ROWS(PER) \
+    hipLaunchKernelGGL(beam_rows_kernel<PER>, dim3(n_pieces, n_groups * width), dim3(kBeamThreads), 0, st, logits, ld, vocab, \
+                       scores, n_out, pieces, keys)
+    if (per == 32) BEAM_ROWS(32);
+    else if (per == 16) BEAM_ROWS(16);
+    else BEAM_ROWS(8);
+#undef BEAM_ROWS
     ATLAS_LAUNCH_CHECK("beam_rows");
-    hipLaunchKernelGGL(beam_join_kernel, dim3(n_groups), dim3(kBeamJoin), 0, st, scores, vocab, width, n_out, n_pieces, pieces,
+    hipLaunchKernelGGL(beam_join_kernel, dim3(n_groups), dim3(kBeamThreads), 0, st, scores, vocab, width, n_out, n_pieces, pieces,
                        keys, tokens, parents, out_scores);
     ATLAS_LAUNCH_CHECK("beam_join");
     return ATLAS_OK;

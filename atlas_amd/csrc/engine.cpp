@@ -1413,7 +1413,8 @@ int beam_setup(atlas_model* m) {
     if (!m->beam_dev) TRY(dalloc(m, (void**)&m->beam_dev, sizeof(BeamBlock)));
     if (!m->beam_slots) TRY(dalloc(m, (void**)&m->beam_slots, (size_t)kMaxRows * c.max_seq * 4));
     if (!m->beam_pick.p) {
-        const size_t bytes = beam_select_workspace(c.vocab, 1, kMaxRows, kBeamOut);
+        size_t bytes = 0;
+        for (int n = 1; n <= kMaxRows; ++n) bytes = std::max(bytes, beam_select_workspace(c.vocab, 1, n, kBeamOut));
         TRY(dalloc(m, &m->beam_pick.p, bytes));
         m->beam_pick.bytes = bytes;
     }

@@ -417,7 +417,7 @@ int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix
  * group) and out_scores [n_groups][n_out].  A beam whose score is not finite, a row
  * of logits with NaN or +inf or of -inf only, and a logit of -inf give no candidates;
  * where a group has too few, the rest is token 0 of parent -1 and score -inf.
- * width and n_out 1 to 64, n_groups * width up to 65535.                     */
+ * width and n_out 1 to 64, n_groups * width up to 65535, vocab up to 2^30.    */
 int atlas_beam_select_f32(const float* logits, int64_t ld, int vocab, const double* scores,
                           int n_groups, int width, int n_out, uint32_t* tokens, int* parents,
                           double* out_scores);

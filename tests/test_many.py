@@ -56,7 +56,7 @@ def _select(logits=X, ld=100, vocab=100, scores=X, groups=2, width=4, n_out=8, t
 
 
 @pytest.mark.parametrize("kw", [
-    dict(logits=0), dict(scores=0), dict(tokens=0), dict(parents=0), dict(out=0), dict(vocab=0), dict(ld=99), dict(groups=-1),
+    dict(logits=0), dict(scores=0), dict(tokens=0), dict(parents=0), dict(out=0), dict(vocab=0), dict(ld=99), dict(vocab=(1 << 30) + 1, ld=1 << 31), dict(groups=-1),
     dict(width=0), dict(width=65), dict(n_out=0), dict(n_out=65), dict(groups=65536, width=1), dict(groups=20000, width=4),
     dict(scores=X + 4), dict(out=X + 4), dict(logits=X + 2), dict(tokens=X + 1), dict(parents=X + 1)], ids=str)
 def test_beam_select_refusals(kw):
