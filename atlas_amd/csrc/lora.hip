@@ -67,118 +67,167 @@ __device__ __forceinline__ void lora_load(const T* p, int n, float (&to)[N]) {
 // The adapters that a tile's 16 rows name, one bit for the first row of each.  A
 // lane's row is lane % 16; -1: none.
 struct LoraTile {
-    int mine;
+    int mine, lead;                    // the lane's adapter, and the first row that names it
     uint32_t firsts;
 
     __device__ __forceinline__ void set(const LoraArgs& a, int row0, int lane) {
         const int row = row0 + (lane & 15), p = row < a.n ? a.pick[row] : -1;
         mine = p >= 0 && p < a.n_adapters ? p : -1;
-        bool first = mine >= 0;
+        lead = lane & 15;
 #pragma unroll
-        for (int j = 0; j < 15; ++j) {
+        for (int j = 14; j >= 0; --j) {
             const int before = __builtin_amdgcn_readlane(mine, j);
-            first = first & !((j < (lane & 15)) & (before == mine));
+            lead = (j < (lane & 15)) & (before == mine) ? j : lead;
         }
-        firsts = (uint32_t)__ballot(first) & 0xFFFFu;
+        firsts = (uint32_t)__ballot(mine >= 0 && lead == (lane & 15)) & 0xFFFFu;
     }
     // the adapter of the lowest bit of `left`
     __device__ __forceinline__ int adapter(uint32_t left) const {
         return __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
     }
+    // every n-th of them from the z-th on
+    __device__ __forceinline__ uint32_t share(int z, int n) const {
+        if (n == 1) return firsts;
+        uint32_t got = 0;
+        int d = 0;
+        for (uint32_t left = firsts; left; left &= left - 1, ++d)
+            if (d % n == z) got |= left & -left;
+        return got;
+    }
 };
 
 constexpr int kLoraWaves = 4;
+constexpr long kLoraWhole = 16384;     // elements of an adapter's A, up to which a launch is saved
 
+// A wave's part of ranks t .. t + 15 of A_ad x over elements [k0, k1) of k: ranks 4g .. of row
+// i.  A step of 32 elements is eight to a lane; the waves take turns of STEPS steps, whose
+// loads are all on their way before the first product.
+template <typename T, bool VEC>
+__device__ __forceinline__ f32x4 lora_down(const LoraArgs& a, int ad, int t, const float* x, int k0, int k1, int wave, int lane) {
+    constexpr int STEPS = 4;
+    const int i = lane & 15, g = lane >> 4;
+    const T* const w = static_cast<const T*>(a.a) + ((long)ad * a.rank + min(t + i, a.rank - 1)) * a.k;
+    f32x4 acc[2] = {};
+    for (int k = k0 + wave * (32 * STEPS); k < k1; k += kLoraWaves * 32 * STEPS) {
+        float wv[STEPS][8], xv[STEPS][8];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int at = k + 32 * s + 8 * g;
+            if (k + 32 * s >= k1) {                      // (the same in every lane)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) wv[s][e] = xv[s][e] = 0.f;
+                continue;
+            }
+            lora_load<T, 8, VEC>(w + at, k1 - at, wv[s]);
+            lora_load<float, 8, VEC>(x + at, k1 - at, xv[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[s][e], xv[s][e], acc[e & 1], 0, 0, 0);
+    }
+    return acc[0] + acc[1];
+}
+
+// The block's waves' parts of A_ad x summed, in every wave; ranks past the last are zero.
+__device__ __forceinline__ f32x4 lora_joined(const LoraArgs& a, f32x4 (&part)[kLoraWaves][64], f32x4 acc, int t, int wave, int lane) {
+    __syncthreads();
+    part[wave][lane] = acc;
+    __syncthreads();
+    f32x4 sum = part[0][lane];
+#pragma unroll
+    for (int o = 1; o < kLoraWaves; ++o) sum += part[o][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (t + 4 * (lane >> 4) + e >= a.rank) sum[e] = 0.f;
+    return sum;
+}
+
+// Blocks: 16 rows, a piece of k, and of the tile's adapters (x their tiles of rank) every
+// so many.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kLoraWaves * 64) void lora_down_kernel(LoraArgs a) {
     __shared__ f32x4 part[kLoraWaves][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.x * 16, split = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    const int row0 = blockIdx.x * 16, split = blockIdx.y, ranks = a.vr / 16;
+    const int rank_blocks = gridDim.z > 1 ? ranks : 1, rb = blockIdx.z % rank_blocks;
     LoraTile tile;
     tile.set(a, row0, lane);
     const int k0 = split * a.k_piece, k1 = min(k0 + a.k_piece, a.k);
     const float* const x = a.x + min(row0 + i, a.n - 1) * a.ld_x;
-    int d = 0;
-    for (uint32_t left = tile.firsts; left; left &= left - 1, ++d) {
-        if (d % gridDim.z != blockIdx.z) continue;
+    for (uint32_t left = tile.share(blockIdx.z / rank_blocks, gridDim.z / rank_blocks); left; left &= left - 1) {
         const int ad = tile.adapter(left);
-        for (int t = 0; t < a.vr; t += 16) {
-            const T* const w = static_cast<const T*>(a.a) + ((long)ad * a.rank + min(t + i, a.rank - 1)) * a.k;
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            // 32 elements of k a step, eight to a lane
-#pragma unroll 2
-            for (int k = k0 + wave * 32 + 8 * g; k - 8 * g < k1; k += kLoraWaves * 32) {
-                float wv[8], xv[8];
-                lora_load<T, 8, VEC>(w + k, k1 - k, wv);
-                lora_load<float, 8, VEC>(x + k, k1 - k, xv);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[e], xv[e], acc, 0, 0, 0);
-            }
-            __syncthreads();
-            part[wave][lane] = acc;
-            __syncthreads();
+        for (int t = rb * 16; t < a.vr; t += rank_blocks * 16) {
+            const f32x4 sum = lora_joined(a, part, lora_down<T, VEC>(a, ad, t, x, k0, k1, wave, lane), t, wave, lane);
             // lane (row i, ranks 4g ..)
-            if (wave == 0 && tile.mine == ad && row0 + i < a.n) {
-                f32x4 sum = part[0][lane];
-#pragma unroll
-                for (int o = 1; o < kLoraWaves; ++o) sum += part[o][lane];
+            if (wave == 0 && tile.mine == ad)
                 *reinterpret_cast<f32x4*>(a.v + ((long)split * a.n + row0 + i) * a.vr + t + 4 * g) = sum;
-            }
         }
     }
 }
 
-// a wave: 16 rows, and 64 elements of m in four tiles
-template <typename T, bool VEC>
+// A wave: 16 rows, and 16 MT elements of m.  Blocks of z take every so many of the tile's
+// adapters and write these adapters' rows; block 0 also the rows without one.
+// WHOLE: a block forms A x itself.
+template <typename T, bool VX, bool VY, bool WHOLE>
 __global__ __launch_bounds__(kLoraWaves * 64) void lora_up_kernel(LoraArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.y * 16, m0 = (blockIdx.x * kLoraWaves + wave) * 64;
-    if (m0 >= a.m) return;
+    constexpr int MT = 4;
+    __shared__ f32x4 part[kLoraWaves][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    const int row0 = blockIdx.y * 16, row = row0 + i, m0 = (blockIdx.x * kLoraWaves + wave) * (16 * MT);
+    if (!WHOLE && m0 >= a.m) return;
     LoraTile tile;
     tile.set(a, row0, lane);
-    const int row = row0 + i;
-    f32x4 y[4];
+    const uint32_t todo = tile.share(blockIdx.z, gridDim.z);
+    if (todo == 0 && blockIdx.z) return;
+    const bool write = row < a.n && (tile.mine < 0 ? blockIdx.z == 0 : (todo >> tile.lead & 1) != 0);
+    const float* const x = a.x + min(row, a.n - 1) * a.ld_x;
+    f32x4 y[MT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < MT; ++t) {
         const int m = m0 + 16 * t + 4 * g;
-        float b[4];
-        if (row < a.n && m < a.m) lora_load<float, 4, VEC>(a.base + row * a.ld_base + m, a.m - m, b);
-        else b[0] = b[1] = b[2] = b[3] = 0.f;
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (write && m < a.m) lora_load<float, 4, VY>(a.base + row * a.ld_base + m, a.m - m, b);
         y[t] = f32x4{b[0], b[1], b[2], b[3]};
     }
-    for (uint32_t left = tile.firsts; left; left &= left - 1) {
+    for (uint32_t left = todo; left; left &= left - 1) {
         const int ad = tile.adapter(left);
         const float scale = a.scales ? a.scales[ad] : 1.f;
         const bool mine = tile.mine == ad;
-        f32x4 acc[4] = {};
+        f32x4 acc[MT] = {};
         for (int t = 0; t < a.vr; t += 16) {
+            float w[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int m = min(m0 + 16 * mt + i, a.m - 1);
+                lora_load<T, 4, VY>(static_cast<const T*>(a.b) + ((long)ad * a.m + m) * a.rank + t + 4 * g, a.rank - t - 4 * g, w[mt]);
+            }
             // B operand: ranks t + 4g + e of row i at step e
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            if (mine)
-                for (int s = 0; s < a.splits; ++s)
-                    v += *reinterpret_cast<const f32x4*>(a.v + ((long)s * a.n + row) * a.vr + t + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (t + 4 * g + e >= a.rank) v[e] = 0.f;
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                const int m = min(m0 + 16 * mt + i, a.m - 1);
-                float w[4];
-                lora_load<T, 4, VEC>(static_cast<const T*>(a.b) + ((long)ad * a.m + m) * a.rank + t + 4 * g, a.rank - t - 4 * g, w);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], v[e], acc[mt], 0, 0, 0);
+            if constexpr (WHOLE) {
+                v = lora_joined(a, part, lora_down<T, VX>(a, ad, t, x, 0, a.k, wave, lane), t, wave, lane);
+            } else {
+                const float* p = a.v + (long)min(row, a.n - 1) * a.vr + t + 4 * g;
+#pragma unroll 4
+                for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(p + (long)s * a.n * a.vr);
             }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[mt][e], v[e], acc[mt], 0, 0, 0);
         }
-        if (mine)
+        // (other rows' columns hold what their x gives with this adapter: not theirs)
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) y[mt] += scale * acc[mt];
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[mt][e] = mine ? y[mt][e] + scale * acc[mt][e] : y[mt][e];
     }
-    if (row >= a.n) return;
+    if (!write) return;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < MT; ++t) {
         const int m = m0 + 16 * t + 4 * g;
         float* to = a.y + row * a.ld_y + m;
-        if (VEC && m + 4 <= a.m) *reinterpret_cast<f32x4*>(to) = y[t];
+        if (VY && m + 4 <= a.m) *reinterpret_cast<f32x4*>(to) = y[t];
         else
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -208,33 +257,46 @@ int lora_add_launch(const atlas_lora& l, const int* adapters, const float* x, lo
     a.x = x; a.ld_x = ld_x; a.base = base; a.ld_base = ld_base; a.y = y; a.ld_y = ld_y;
     a.n = n;
     a.vr = (l.rank + 15) / 16 * 16;
-    const int tiles = (n + 15) / 16, named = std::min({16, n, std::max(l.n_adapters, 1)});
-    // pieces of k, of 512 elements at least, while the blocks do not fill the chip
-    const int most = std::max(1, (l.k + 511) / 512), want = std::max(1, 2 * device_cu_count() / (tiles * named));
-    a.splits = std::min(most, want);
-    a.k_piece = ((l.k + a.splits - 1) / a.splits + 63) / 64 * 64;
-    a.splits = (l.k + a.k_piece - 1) / a.k_piece;
-    void* p = nullptr;
-    const int rc = thread_scratch(SCR_LORA, (size_t)a.splits * n * a.vr * sizeof(float), &p);
-    if (rc) return rc;
-    a.v = static_cast<float*>(p);
+    const int cus = device_cu_count(), tiles = (n + 15) / 16, named = std::min({16, n, std::max(l.n_adapters, 1)});
+    ATLAS_REQUIRE(tiles <= 65535, "%s: %d rows", who, n);
     // whole vectors of every operand on their boundaries
     const bool vx = (((uintptr_t)x | weights) & 15) == 0 && ld_x % 4 == 0 && l.k % 8 == 0;
     const bool vy = (((uintptr_t)base | (uintptr_t)y | weights) & 15) == 0 && ld_base % 4 == 0 && ld_y % 4 == 0 && l.rank % 4 == 0;
-    const dim3 down(tiles, a.splits, named), up((l.m + 64 * kLoraWaves - 1) / (64 * kLoraWaves), tiles);
-    ATLAS_REQUIRE(tiles <= 65535, "%s: %d rows", who, n);
-#define LORA_RUN(KERNEL, GRID, T, VEC) hipLaunchKernelGGL((KERNEL<T, VEC>), GRID, dim3(kLoraWaves * 64), 0, st, a)
+    // blocks of their own for the adapters of a tile, where the tiles alone leave CUs idle
+    const int wide = (l.m + 64 * kLoraWaves - 1) / (64 * kLoraWaves);
+    const dim3 up(wide, tiles, (long)wide * tiles < 2 * cus ? named : 1);
+#define LORA_RUN(KERNEL, GRID, ...) hipLaunchKernelGGL((KERNEL<__VA_ARGS__>), GRID, dim3(kLoraWaves * 64), 0, st, a)
+    if (l.n_adapters > 0 && (long)l.k * a.vr <= kLoraWhole) {
+        if (size == 2 && vx && vy) LORA_RUN(lora_up_kernel, up, uint16_t, true, true, true);
+        else if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, false, false, true);
+        else if (vx && vy) LORA_RUN(lora_up_kernel, up, float, true, true, true);
+        else LORA_RUN(lora_up_kernel, up, float, false, false, true);
+        ATLAS_LAUNCH_CHECK("lora_up");
+        return ATLAS_OK;
+    }
     if (l.n_adapters > 0) {
+        // pieces of k, of a turn of the waves at least, while the blocks do not fill the chip
+        const bool apart = tiles < cus / 4;
+        const int each = apart ? named * (a.vr / 16) : 1;
+        const int most = (l.k + 511) / 512, want = std::max(1, 4 * cus / (tiles * each));
+        a.splits = std::min(most, want);
+        a.k_piece = ((l.k + a.splits - 1) / a.splits + 127) / 128 * 128;
+        a.splits = (l.k + a.k_piece - 1) / a.k_piece;
+        void* p = nullptr;
+        const int rc = thread_scratch(SCR_LORA, (size_t)a.splits * n * a.vr * sizeof(float), &p);
+        if (rc) return rc;
+        a.v = static_cast<float*>(p);
+        const dim3 down(tiles, a.splits, each);
         if (size == 2 && vx) LORA_RUN(lora_down_kernel, down, uint16_t, true);
         else if (size == 2) LORA_RUN(lora_down_kernel, down, uint16_t, false);
         else if (vx) LORA_RUN(lora_down_kernel, down, float, true);
         else LORA_RUN(lora_down_kernel, down, float, false);
         ATLAS_LAUNCH_CHECK("lora_down");
     }
-    if (size == 2 && vy) LORA_RUN(lora_up_kernel, up, uint16_t, true);
-    else if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, false);
-    else if (vy) LORA_RUN(lora_up_kernel, up, float, true);
-    else LORA_RUN(lora_up_kernel, up, float, false);
+    if (size == 2 && vy) LORA_RUN(lora_up_kernel, up, uint16_t, false, true, false);
+    else if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, false, false, false);
+    else if (vy) LORA_RUN(lora_up_kernel, up, float, false, true, false);
+    else LORA_RUN(lora_up_kernel, up, float, false, false, false);
 #undef LORA_RUN
     ATLAS_LAUNCH_CHECK("lora_up");
     return ATLAS_OK;
