@@ -176,20 +176,21 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_up_kernel(LoraArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int row0 = blockIdx.y * 16, row = row0 + i, m0 = (blockIdx.x * kLoraWaves + wave) * (16 * MT);
     if (!WHOLE && m0 >= a.m) return;
+    // (on their way before the adapters are known)
+    f32x4 y[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = m0 + 16 * t + 4 * g;
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (row < a.n && m < a.m) lora_load<float, 4, VY>(a.base + row * a.ld_base + m, a.m - m, b);
+        y[t] = f32x4{b[0], b[1], b[2], b[3]};
+    }
     LoraTile tile;
     tile.set(a, row0, lane);
     const uint32_t todo = tile.share(blockIdx.z, gridDim.z);
     if (todo == 0 && blockIdx.z) return;
     const bool write = row < a.n && (tile.mine < 0 ? blockIdx.z == 0 : (todo >> tile.lead & 1) != 0);
     const float* const x = a.x + min(row, a.n - 1) * a.ld_x;
-    f32x4 y[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = m0 + 16 * t + 4 * g;
-        float b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (write && m < a.m) lora_load<float, 4, VY>(a.base + row * a.ld_base + m, a.m - m, b);
-        y[t] = f32x4{b[0], b[1], b[2], b[3]};
-    }
     for (uint32_t left = todo; left; left &= left - 1) {
         const int ad = tile.adapter(left);
         const float scale = a.scales ? a.scales[ad] : 1.f;
