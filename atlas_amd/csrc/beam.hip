@@ -489,44 +489,57 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
 
 // ---- reordering -------------------------------------------------------------------
 //
-// A thread has a column of a group's rows: it reads what any of them takes over and
-// then writes, so that a state is reordered in place.
+// A thread has columns of a group's rows: it reads what any of them takes over and then
+// writes, so that a state is reordered in place.
 
-constexpr int kBeamStates = 32;
+constexpr int kBeamStates = 64;
 
 struct BeamStates {
     char* dst[kBeamStates];
     const char* src[kBeamStates];
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void beam_move(const BeamStates& s, int state, long at, long stride, const int* parent, int width) {
-    char* const dst = s.dst[state] + at;
-    const char* const src = s.src[state] + at;
+// One column to a thread in each of U places `apart` columns from each other, as far as
+// there are `columns`; parents are the same in every lane.
+template <typename T, int W, int U>
+__device__ __forceinline__ void beam_move(char* dst, const char* src, long column, long columns, long apart, long stride,
+                                          const int* parents, int width) {
     const bool in_place = dst == src;
-    T v[W];
+    T v[U][W];
+    int parent[W];
+#pragma unroll
+    for (int b = 0; b < W; ++b) {
+        const int p = parents[min(b, width - 1)];
+        parent[b] = b < width && (unsigned)p < (unsigned)width && !(in_place && p == b) ? p : -1;
+    }
 #pragma unroll
     for (int b = 0; b < W; ++b)
-        if (b < width && parent[b] >= 0 && !(in_place && parent[b] == b)) v[b] = *reinterpret_cast<const T*>(src + parent[b] * stride);
+        if (parent[b] >= 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                v[u][b] = reinterpret_cast<const T*>(src + parent[b] * stride)[min(column + u * apart, columns - 1)];
 #pragma unroll
     for (int b = 0; b < W; ++b)
-        if (b < width && parent[b] >= 0 && !(in_place && parent[b] == b)) *reinterpret_cast<T*>(dst + b * stride) = v[b];
+        if (parent[b] >= 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (column + u * apart < columns) reinterpret_cast<T*>(dst + b * stride)[column + u * apart] = v[u][b];
 }
 
-// full: units of T in a row; the bytes after them follow one by one
-template <typename T, int W>
+// full: units of T in a row; the bytes after them follow one by one, in the last block
+template <typename T, int W, int U>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamStates s, long full, int tail, long stride,
                                                            const int* __restrict__ parents, int width) {
-    __shared__ int parent[W];
-    const int group = blockIdx.y;
-    if (threadIdx.x < width) {
-        const int p = parents[group * width + threadIdx.x];
-        parent[threadIdx.x] = p >= 0 && p < width ? p : -1;
+    const long base = (long)blockIdx.y * width * stride;
+    char* const dst = s.dst[blockIdx.z] + base;
+    const char* const src = s.src[blockIdx.z] + base;
+    parents += blockIdx.y * width;
+    const long first = (long)blockIdx.x * (256 * U);
+    if (first < full) {
+        beam_move<T, W, U>(dst, src, first + threadIdx.x, full, 256, stride, parents, width);
+    } else if (threadIdx.x < tail) {
+        beam_move<char, W, 1>(dst + full * sizeof(T), src + full * sizeof(T), threadIdx.x, tail, 0, stride, parents, width);
     }
-    __syncthreads();
-    const long e = (long)blockIdx.x * 256 + threadIdx.x, base = (long)group * width * stride;
-    if (e < full) beam_move<T, W>(s, blockIdx.z, base + e * sizeof(T), stride, parent, width);
-    else if (e < full + tail) beam_move<char, W>(s, blockIdx.z, base + full * sizeof(T) + (e - full), stride, parent, width);
 }
 
 int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, long row_bytes, long row_stride,
@@ -548,7 +561,8 @@ int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, 
         bits |= (uintptr_t)d | (uintptr_t)s;
     }
     const int unit = (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
-    const long full = row_bytes / unit, blocks = (full + row_bytes % unit + 255) / 256;
+    const long full = row_bytes / unit, per = 256L * (width <= 8 ? 4 : width <= 16 ? 2 : 1);
+    const long blocks = (full + per - 1) / per + (row_bytes % unit != 0);
     ATLAS_REQUIRE(blocks <= 0x7FFFFFFF, "%s: rows of %ld bytes", who, row_bytes);
     for (int i = 0; i < n_states; i += kBeamStates) {
         BeamStates s{};
@@ -558,9 +572,9 @@ int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, 
             s.src[j] = static_cast<const char*>(src[i + j]);
         }
         const dim3 grid((unsigned)blocks, n_groups, n);
-#define BEAM_RUN(T, W) \
-    hipLaunchKernelGGL((beam_reorder_kernel<T, W>), grid, dim3(256), 0, st, s, full, (int)(row_bytes % unit), row_stride, parents, width)
-#define BEAM_WIDTH(T) if (width <= 8) BEAM_RUN(T, 8); else if (width <= 16) BEAM_RUN(T, 16); else BEAM_RUN(T, 64)
+#define BEAM_RUN(T, W, U) \
+    hipLaunchKernelGGL((beam_reorder_kernel<T, W, U>), grid, dim3(256), 0, st, s, full, (int)(row_bytes % unit), row_stride, parents, width)
+#define BEAM_WIDTH(T) if (width <= 8) BEAM_RUN(T, 8, 4); else if (width <= 16) BEAM_RUN(T, 16, 2); else BEAM_RUN(T, 64, 1)
         if (unit == 16) { BEAM_WIDTH(u32x4); }
         else if (unit == 4) { BEAM_WIDTH(uint32_t); }
         else { BEAM_WIDTH(char); }
