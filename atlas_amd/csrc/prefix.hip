@@ -250,7 +250,10 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
     const long pitch = (long)a.n_kv * HD;
     const float *const kb = a.k + (long)kvh * HD + 4 * g, *const vb = a.v + (long)kvh * HD + 4 * i;
     const int w0 = split * W + wave, n = w0 < tokens.chunks ? (tokens.chunks - w0 + stride - 1) / stride : 0;
-    const auto chunk_of = [&](int t) { return w0 + t * stride; };
+    // (half of a SIMD's waves from the end, so that shared and own tokens, the ones bound by
+    // products and the others by memory, are under way together)
+    const bool back = wave >= W / 2 && (tokens.chunks - tokens.shared_chunks) * 4 > tokens.chunks;
+    const auto chunk_of = [&](int t) { return w0 + (back ? n - 1 - t : t) * stride; };
     f32x4 kf[S], vf[4][H];
     PfChunk cur, next;
     int cell = 0, next_cell = 0;
@@ -531,8 +534,12 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     if (b.slot_stride > 0) own = std::min<int64_t>(own, b.slot_stride);
     if (window > 0) own = std::min<int64_t>(own, window);
     const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
-    const long units = std::max(1L, (long)s.tiles * c.n_kv);
-    const long want = (long)device_cu_count() * pf_at_once(c.head_dim, s.ct) / units, most = chunks <= 2 * kPfLeast ? 1 : (chunks + kPfLeast - 1) / kPfLeast;
+    // A block to every place of the chip; four to a tile where groups of different lengths
+    // would leave a part of the places empty (16 groups of 1 to 15 rows of 16 heads over 4 of
+    // 128, 700 shared and up to 700 own tokens: 58 us, 96 with one).
+    const long units = std::max(1L, (long)s.tiles * c.n_kv), chip = (long)device_cu_count() * pf_at_once(c.head_dim, s.ct);
+    const long want = chip / units < 2 && units < 2 * chip && b.n_groups > 1 ? 4 : chip / units;
+    const long most = chunks <= 2 * kPfLeast ? 1 : (chunks + kPfLeast - 1) / kPfLeast;
     const long fit = (long)((256u << 20) / ((size_t)units * s.cols * (c.head_dim + 2) * sizeof(float)));
     s.splits = (int)std::max(1L, std::min({want, most, fit, (long)kPfMaxSplits}));
     return s;
