@@ -32,35 +32,34 @@ struct LoraArgs {
     int splits, k_piece;               // k's pieces, multiples of 64
 };
 
-// elements of T at p, p + 1, .. as f32; those from n on are zero
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void lora_load(const T* p, int n, float (&to)[N]) {
-    if (VEC && n >= N) {
-        if constexpr (sizeof(T) == 2) {
-            uint32_t w[N / 2];
-            __builtin_memcpy(w, __builtin_assume_aligned(p, N * 2), N * 2);
+// N elements of T of a row of n from `at` on, as f32.  Rows may start anywhere: the loads
+// need no alignment beyond the elements'.
+template <typename T, int N>
+__device__ __forceinline__ void lora_load(const T* row, int at, float (&to)[N]) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t w[N / 2];
+        __builtin_memcpy(w, row + at, N * 2);
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-                to[2 * i] = bf16_lo(w[i]);
-                to[2 * i + 1] = bf16_hi(w[i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const f32x4 w = reinterpret_cast<const f32x4*>(p)[i];
-                to[4 * i] = w.x; to[4 * i + 1] = w.y; to[4 * i + 2] = w.z; to[4 * i + 3] = w.w;
-            }
+        for (int i = 0; i < N / 2; ++i) {
+            to[2 * i] = bf16_lo(w[i]);
+            to[2 * i + 1] = bf16_hi(w[i]);
         }
     } else {
+        __builtin_memcpy(to, row + at, N * 4);
+    }
+}
+
+// ... at the row's end: those past it are zero.  (One by one, without conditions, so that
+// no load waits for another.)
+template <typename T, int N>
+__device__ __forceinline__ void lora_load_end(const T* row, int at, int n, float (&to)[N]) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i < n) {
-                if constexpr (sizeof(T) == 2) to[i] = __uint_as_float((uint32_t)p[i] << 16);
-                else to[i] = p[i];
-            } else {
-                to[i] = 0.f;
-            }
-        }
+    for (int i = 0; i < N; ++i) {
+        const T v = row[min(at + i, n - 1)];
+        float x;
+        if constexpr (sizeof(T) == 2) x = __uint_as_float((uint32_t)v << 16);
+        else x = v;
+        to[i] = at + i < n ? x : 0.f;
     }
 }
 
@@ -98,28 +97,33 @@ struct LoraTile {
 
 constexpr int kLoraWaves = 4;
 constexpr long kLoraWhole = 16384;     // elements of an adapter's A, up to which a launch is saved
+constexpr int kLoraMaxTiles = 16;      // tiles of rank
 
-// A wave's part of ranks t .. t + 15 of A_ad x over elements [k0, k1) of k: ranks 4g .. of row
-// i.  A step of 32 elements is eight to a lane; the waves take turns of STEPS steps, whose
-// loads are all on their way before the first product.
-template <typename T, bool VEC>
-__device__ __forceinline__ f32x4 lora_down(const LoraArgs& a, int ad, int t, const float* x, int k0, int k1, int wave, int lane) {
+// Ranks t .. t + 15 of A_ad x over elements [k0, k1) of k, every `turns`-th 128 of them from the
+// turn-th on: ranks 4g .. of row i.  A step of 32 elements is eight to a lane; the loads of four
+// are on their way before the first product.
+template <typename T>
+__device__ __forceinline__ f32x4 lora_down(const LoraArgs& a, int ad, int t, const float* x, int k0, int k1, int turn, int turns,
+                                           int lane) {
     constexpr int STEPS = 4;
     const int i = lane & 15, g = lane >> 4;
     const T* const w = static_cast<const T*>(a.a) + ((long)ad * a.rank + min(t + i, a.rank - 1)) * a.k;
     f32x4 acc[2] = {};
-    for (int k = k0 + wave * (32 * STEPS); k < k1; k += kLoraWaves * 32 * STEPS) {
+    for (int k = k0 + turn * (32 * STEPS); k < k1; k += turns * 32 * STEPS) {
         float wv[STEPS][8], xv[STEPS][8];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int at = k + 32 * s + 8 * g;
-            if (k + 32 * s >= k1) {                      // (the same in every lane)
+            if (k + 32 * s + 32 <= k1) {                 // (the same in every lane)
+                lora_load<T, 8>(w, at, wv[s]);
+                lora_load<float, 8>(x, at, xv[s]);
+            } else if (k + 32 * s < k1) {
+                lora_load_end<T, 8>(w, at, k1, wv[s]);
+                lora_load_end<float, 8>(x, at, k1, xv[s]);
+            } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) wv[s][e] = xv[s][e] = 0.f;
-                continue;
             }
-            lora_load<T, 8, VEC>(w + at, k1 - at, wv[s]);
-            lora_load<float, 8, VEC>(x + at, k1 - at, xv[s]);
         }
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
@@ -129,23 +133,9 @@ __device__ __forceinline__ f32x4 lora_down(const LoraArgs& a, int ad, int t, con
     return acc[0] + acc[1];
 }
 
-// The block's waves' parts of A_ad x summed, in every wave; ranks past the last are zero.
-__device__ __forceinline__ f32x4 lora_joined(const LoraArgs& a, f32x4 (&part)[kLoraWaves][64], f32x4 acc, int t, int wave, int lane) {
-    __syncthreads();
-    part[wave][lane] = acc;
-    __syncthreads();
-    f32x4 sum = part[0][lane];
-#pragma unroll
-    for (int o = 1; o < kLoraWaves; ++o) sum += part[o][lane];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (t + 4 * (lane >> 4) + e >= a.rank) sum[e] = 0.f;
-    return sum;
-}
-
 // Blocks: 16 rows, a piece of k, and of the tile's adapters (x their tiles of rank) every
 // so many.
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(kLoraWaves * 64) void lora_down_kernel(LoraArgs a) {
     __shared__ f32x4 part[kLoraWaves][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
@@ -158,31 +148,39 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_down_kernel(LoraArgs a) 
     for (uint32_t left = tile.share(blockIdx.z / rank_blocks, gridDim.z / rank_blocks); left; left &= left - 1) {
         const int ad = tile.adapter(left);
         for (int t = rb * 16; t < a.vr; t += rank_blocks * 16) {
-            const f32x4 sum = lora_joined(a, part, lora_down<T, VEC>(a, ad, t, x, k0, k1, wave, lane), t, wave, lane);
+            const f32x4 acc = lora_down<T>(a, ad, t, x, k0, k1, wave, kLoraWaves, lane);
+            __syncthreads();
+            part[wave][lane] = acc;
+            __syncthreads();
             // lane (row i, ranks 4g ..)
-            if (wave == 0 && tile.mine == ad)
+            if (wave == 0 && tile.mine == ad) {
+                f32x4 sum = part[0][lane];
+#pragma unroll
+                for (int o = 1; o < kLoraWaves; ++o) sum += part[o][lane];
                 *reinterpret_cast<f32x4*>(a.v + ((long)split * a.n + row0 + i) * a.vr + t + 4 * g) = sum;
+            }
         }
     }
 }
 
-// A wave: 16 rows, and 16 MT elements of m.  Blocks of z take every so many of the tile's
+// A wave: 16 rows, and 64 elements of m.  Blocks of z take every so many of the tile's
 // adapters and write these adapters' rows; block 0 also the rows without one.
-// WHOLE: a block forms A x itself.
-template <typename T, bool VX, bool VY, bool WHOLE>
+// WHOLE: a block forms A x itself, a tile of rank (or, of few, a part of k) to a wave.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kLoraWaves * 64) void lora_up_kernel(LoraArgs a) {
     constexpr int MT = 4;
-    __shared__ f32x4 part[kLoraWaves][64];
+    __shared__ f32x4 part[WHOLE ? kLoraMaxTiles : 1][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
-    const int row0 = blockIdx.y * 16, row = row0 + i, m0 = (blockIdx.x * kLoraWaves + wave) * (16 * MT);
+    const int row0 = blockIdx.y * 16, row = row0 + i, here = min(row, a.n - 1), m0 = (blockIdx.x * kLoraWaves + wave) * (16 * MT);
     if (!WHOLE && m0 >= a.m) return;
     // (on their way before the adapters are known)
     f32x4 y[MT];
+    const float* const base = a.base + here * a.ld_base;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        const int m = m0 + 16 * t + 4 * g;
         float b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row < a.n && m < a.m) lora_load<float, 4, VY>(a.base + row * a.ld_base + m, a.m - m, b);
+        if (m0 + 16 * t + 16 <= a.m) lora_load<float, 4>(base, m0 + 16 * t + 4 * g, b);
+        else if (m0 + 16 * t < a.m) lora_load_end<float, 4>(base, m0 + 16 * t + 4 * g, a.m, b);
         y[t] = f32x4{b[0], b[1], b[2], b[3]};
     }
     LoraTile tile;
@@ -190,28 +188,38 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_up_kernel(LoraArgs a) {
     const uint32_t todo = tile.share(blockIdx.z, gridDim.z);
     if (todo == 0 && blockIdx.z) return;
     const bool write = row < a.n && (tile.mine < 0 ? blockIdx.z == 0 : (todo >> tile.lead & 1) != 0);
-    const float* const x = a.x + min(row, a.n - 1) * a.ld_x;
+    const float* const x = a.x + here * a.ld_x;
+    const int ranks = a.vr / 16, parts = WHOLE && ranks < kLoraWaves ? kLoraWaves / ranks : 1;
     for (uint32_t left = todo; left; left &= left - 1) {
         const int ad = tile.adapter(left);
         const float scale = a.scales ? a.scales[ad] : 1.f;
         const bool mine = tile.mine == ad;
+        if constexpr (WHOLE) {
+            __syncthreads();                             // (the adapter before has been read)
+            for (int item = wave; item < ranks * parts; item += kLoraWaves)
+                part[item][lane] = lora_down<T>(a, ad, item / parts * 16, x, 0, a.k, item % parts, parts, lane);
+            __syncthreads();
+        }
         f32x4 acc[MT] = {};
         for (int t = 0; t < a.vr; t += 16) {
             float w[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const int m = min(m0 + 16 * mt + i, a.m - 1);
-                lora_load<T, 4, VY>(static_cast<const T*>(a.b) + ((long)ad * a.m + m) * a.rank + t + 4 * g, a.rank - t - 4 * g, w[mt]);
+                const T* const b = static_cast<const T*>(a.b) + ((long)ad * a.m + min(m0 + 16 * mt + i, a.m - 1)) * a.rank;
+                if (t + 16 <= a.rank) lora_load<T, 4>(b, t + 4 * g, w[mt]);
+                else lora_load_end<T, 4>(b, t + 4 * g, a.rank, w[mt]);
             }
-            // B operand: ranks t + 4g + e of row i at step e
+            // B operand: ranks t + 4g + e of row i at step e; past the last zero
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             if constexpr (WHOLE) {
-                v = lora_joined(a, part, lora_down<T, VX>(a, ad, t, x, 0, a.k, wave, lane), t, wave, lane);
+                for (int p = 0; p < parts; ++p) v += part[t / 16 * parts + p][lane];
             } else {
-                const float* p = a.v + (long)min(row, a.n - 1) * a.vr + t + 4 * g;
+                const float* p = a.v + (long)here * a.vr + t + 4 * g;
 #pragma unroll 4
                 for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(p + (long)s * a.n * a.vr);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = t + 4 * g + e < a.rank ? v[e] : 0.f;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -224,15 +232,15 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_up_kernel(LoraArgs a) {
             for (int e = 0; e < 4; ++e) y[mt][e] = mine ? y[mt][e] + scale * acc[mt][e] : y[mt][e];
     }
     if (!write) return;
+    float* const to = a.y + row * a.ld_y;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int m = m0 + 16 * t + 4 * g;
-        float* to = a.y + row * a.ld_y + m;
-        if (VY && m + 4 <= a.m) *reinterpret_cast<f32x4*>(to) = y[t];
+        if (m + 4 <= a.m) __builtin_memcpy(to + m, &y[t], 16);
         else
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (m + e < a.m) to[e] = y[t][e];
+                if (m + e < a.m) to[m + e] = y[t][e];
     }
 }
 
@@ -247,9 +255,9 @@ int lora_add_launch(const atlas_lora& l, const int* adapters, const float* x, lo
                   l.m, ld_x, ld_base, ld_y);
     if (n == 0) return ATLAS_OK;
     ATLAS_REQUIRE(adapters && x && base && y && (l.n_adapters == 0 || (l.a && l.b)), "%s: null argument", who);
+    const int size = l.fmt == ATLAS_W_F32 ? 4 : 2;
     const uintptr_t floats = (uintptr_t)x | (uintptr_t)base | (uintptr_t)y | (uintptr_t)adapters | (uintptr_t)l.scales;
     const uintptr_t weights = (uintptr_t)l.a | (uintptr_t)l.b;
-    const int size = l.fmt == ATLAS_W_F32 ? 4 : 2;
     ATLAS_REQUIRE((floats & 3) == 0 && weights % size == 0, "%s: misaligned argument", who);
     LoraArgs a{};
     a.a = l.a; a.b = l.b; a.scales = l.scales;
@@ -260,18 +268,13 @@ int lora_add_launch(const atlas_lora& l, const int* adapters, const float* x, lo
     a.vr = (l.rank + 15) / 16 * 16;
     const int cus = device_cu_count(), tiles = (n + 15) / 16, named = std::min({16, n, std::max(l.n_adapters, 1)});
     ATLAS_REQUIRE(tiles <= 65535, "%s: %d rows", who, n);
-    // whole vectors of every operand on their boundaries
-    const bool vx = (((uintptr_t)x | weights) & 15) == 0 && ld_x % 4 == 0 && l.k % 8 == 0;
-    const bool vy = (((uintptr_t)base | (uintptr_t)y | weights) & 15) == 0 && ld_base % 4 == 0 && ld_y % 4 == 0 && l.rank % 4 == 0;
     // blocks of their own for the adapters of a tile, where the tiles alone leave CUs idle
     const int wide = (l.m + 64 * kLoraWaves - 1) / (64 * kLoraWaves);
     const dim3 up(wide, tiles, (long)wide * tiles < 2 * cus ? named : 1);
 #define LORA_RUN(KERNEL, GRID, ...) hipLaunchKernelGGL((KERNEL<__VA_ARGS__>), GRID, dim3(kLoraWaves * 64), 0, st, a)
     if (l.n_adapters > 0 && (long)l.k * a.vr <= kLoraWhole) {
-        if (size == 2 && vx && vy) LORA_RUN(lora_up_kernel, up, uint16_t, true, true, true);
-        else if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, false, false, true);
-        else if (vx && vy) LORA_RUN(lora_up_kernel, up, float, true, true, true);
-        else LORA_RUN(lora_up_kernel, up, float, false, false, true);
+        if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, true);
+        else LORA_RUN(lora_up_kernel, up, float, true);
         ATLAS_LAUNCH_CHECK("lora_up");
         return ATLAS_OK;
     }
@@ -288,16 +291,12 @@ int lora_add_launch(const atlas_lora& l, const int* adapters, const float* x, lo
         if (rc) return rc;
         a.v = static_cast<float*>(p);
         const dim3 down(tiles, a.splits, each);
-        if (size == 2 && vx) LORA_RUN(lora_down_kernel, down, uint16_t, true);
-        else if (size == 2) LORA_RUN(lora_down_kernel, down, uint16_t, false);
-        else if (vx) LORA_RUN(lora_down_kernel, down, float, true);
-        else LORA_RUN(lora_down_kernel, down, float, false);
+        if (size == 2) LORA_RUN(lora_down_kernel, down, uint16_t);
+        else LORA_RUN(lora_down_kernel, down, float);
         ATLAS_LAUNCH_CHECK("lora_down");
     }
-    if (size == 2 && vy) LORA_RUN(lora_up_kernel, up, uint16_t, false, true, false);
-    else if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, false, false, false);
-    else if (vy) LORA_RUN(lora_up_kernel, up, float, false, true, false);
-    else LORA_RUN(lora_up_kernel, up, float, false, false, false);
+    if (size == 2) LORA_RUN(lora_up_kernel, up, uint16_t, false);
+    else LORA_RUN(lora_up_kernel, up, float, false);
 #undef LORA_RUN
     ATLAS_LAUNCH_CHECK("lora_up");
     return ATLAS_OK;

@@ -529,10 +529,13 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     s.tiles = b.group_starts ? b.n_rows / s.rows + b.n_groups : (b.n_rows + s.rows - 1) / s.rows;
     if (b.n_groups == 1) s.tiles = (b.n_rows + s.rows - 1) / s.rows;
     // chunks of a tile, by the caller's hints
-    const int64_t prefix = std::min(b.max_prefix > 0 ? b.max_prefix : c.max_seq, c.max_seq);
+    int64_t prefix = std::min(b.max_prefix > 0 ? b.max_prefix : c.max_seq, c.max_seq);
     int64_t own = std::min(b.max_own > 0 ? b.max_own : c.max_seq, c.max_seq);
     if (b.slot_stride > 0) own = std::min<int64_t>(own, b.slot_stride);
-    if (window > 0) own = std::min<int64_t>(own, window);
+    if (window > 0) {
+        prefix = std::min<int64_t>(prefix, window);
+        own = std::min<int64_t>(own, window);
+    }
     const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
     // A block to every place of the chip; four to a tile where groups of different lengths
     // would leave a part of the places empty (16 groups of 1 to 15 rows of 16 heads over 4 of
