@@ -431,7 +431,7 @@ int atlas_beam_reorder(void* const* dst, const void* const* src, int n_states, i
                        int64_t row_stride, const int* parents, int n_groups, int width);
 
 /* Low-rank adapters of one projection of m x k: a [n_adapters][rank][k] and
- * b [n_adapters][m][rank] without gaps, ATLAS_W_F32 or ATLAS_W_BF16 (an adapter of
+ * b [n_adapters][m][rank] without gaps, up to 4095 of them, ATLAS_W_F32 or ATLAS_W_BF16 (an adapter of
  * lower rank is filled up with zeros); scales [n_adapters] or NULL (1), all on the
  * device.  rank 1 to 256.                                                    */
 typedef struct {

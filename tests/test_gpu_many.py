@@ -486,7 +486,23 @@ def test_lora_sixteen_adapters_in_a_tile_and_no_scales():
     a.check(in_place=True)
 
 
+@pytest.mark.parametrize("m,k", [(40, 64), (70, 2100)])
+@pytest.mark.parametrize("rows,n", [(63, 1), (64, 2), (65, 2), (65, 70), (300, 1), (513, 300), (4096, 3), (4099, 4095), (8200, 17)])
+def test_lora_rows_of_an_adapter_in_any_order(rows, n, m, k):
+    """Rows are gathered by adapter: in one wave's registers up to 64, in spans of 4096."""
+    Adapters(rows, n, 3, m, k, rows, "f32").check(in_place=rows % 2 == 0)
+
+
+def test_lora_one_adapter_for_all_rows_and_rows_without():
+    a = Adapters(9, 3, 16, 64, 2000, 500)
+    a.pick[:] = 1
+    a.check()
+    a.pick[:] = -5
+    a.check()
+
+
 def test_lora_no_adapters():
+    Adapters(5, 0, 8, 64, 64, 200).check()
     Adapters(5, 0, 8, 64, 64, 5).check()
 
 

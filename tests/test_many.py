@@ -93,7 +93,7 @@ def _lora(lora=(), adapters=X, x=X, ld_x=32, base=X, ld_base=64, y=X, ld_y=64, n
 
 
 @pytest.mark.parametrize("kw", [
-    dict(lora=dict(fmt=2)), dict(lora=dict(a=0)), dict(lora=dict(b=0)), dict(lora=dict(n_adapters=-1)), dict(lora=dict(rank=0)),
+    dict(lora=dict(fmt=2)), dict(lora=dict(a=0)), dict(lora=dict(b=0)), dict(lora=dict(n_adapters=-1)), dict(lora=dict(n_adapters=4096)), dict(lora=dict(rank=0)),
     dict(lora=dict(rank=257)), dict(lora=dict(m=0)), dict(lora=dict(k=0)), dict(lora=dict(m=(1 << 24) + 1), ld_base=1 << 25, ld_y=1 << 25),
     dict(lora=dict(a=X + 1)), dict(lora=dict(fmt=0, b=X + 2)), dict(lora=dict(scales=X + 2)), dict(adapters=0), dict(x=0), dict(base=0),
     dict(y=0), dict(ld_x=31), dict(ld_base=63), dict(ld_y=63), dict(n=-1), dict(n=(1 << 20) + 1), dict(x=X + 2), dict(y=X + 1)], ids=str)
