@@ -19,6 +19,12 @@ namespace atlas {
 // 64 is a bound that at least n_out elements reach, so that what lies below it goes, and
 // the few that are left are ranked by counting.  Where many reach the bound (equal
 // logits), the largest is taken n_out times.
+//
+// Bound by what is not the stream of logits: 64 rows of 100278 of them, 25.7 MB and 5 us of
+// bytes, take 24 us, of which the 64-bit exponentials' products are 5, the bounds and ranks
+// of 49 times 64 blocks as much again, each pass over a block's registers a chain of LDS and barriers,
+// and the join 7; 4 rows of 49152, one block to a CU at most, 11, a block's chain (6) and
+// the join's (5).
 
 constexpr int kBeamMaxOut = 64;
 constexpr int kBeamThreads = 512;
@@ -435,11 +441,13 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(const double* _
     for (int e = n + tid; e < n_out; e += kBeamThreads) store(e, kBeamNobody);
 }
 
-// Logits of a thread: as many as leave a block to a CU at least, for what a block does
-// once (bounds, ranks) is as much work as eight exponentials of a thread.
+// Logits of a thread: what a block does once (bounds, ranks) is as much work as eight
+// exponentials of a thread, and what a piece leaves is the join's work; few blocks leave
+// CUs idle.  8, 16 and 32 of them: 4 beams over 49152 tokens 11.1, 12.0 and 13.6 us; 8 over
+// 100278 18.7, 17.1, 18.2; 4 x 8 of them 23.3, 19.4, 20.2; 8 x 8 29.8, 25.2, 23.8.
 static int beam_per(int vocab, long rows) {
     const long all = (long)vocab * rows, chip = (long)device_cu_count() * kBeamThreads;
-    return all >= 32 * chip ? 32 : all >= 16 * chip ? 16 : 8;
+    return all >= 32 * chip ? 32 : all >= 4 * chip ? 16 : 8;
 }
 
 // (a row may start up to three logits into its first vector)
@@ -490,13 +498,21 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
 // ---- reordering -------------------------------------------------------------------
 //
 // A thread has columns of a group's rows: it reads what any of them takes over and then
-// writes, so that a state is reordered in place.
+// writes, so that a state is reordered in place.  Bound by the bytes: 60 caches of 6 beams
+// of 777 x 3 x 64 f32 43 us, 215 MB, 42 at a copy's rate.  A launch has up to 64 states and a
+// thread up to four columns, W rows of each in registers, so that all its loads are under way
+// at once (a column to a thread, and fewer states to a launch: 85 us).
 
 constexpr int kBeamStates = 64;
 
 struct BeamStates {
     char* dst[kBeamStates];
     const char* src[kBeamStates];
+};
+
+struct BeamSpan {
+    uintptr_t at;
+    bool write;
 };
 
 // One column to a thread in each of U places `apart` columns from each other, as far as
@@ -552,6 +568,7 @@ int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, 
     if (n_states == 0 || row_bytes == 0 || n_groups == 0) return ATLAS_OK;
     ATLAS_REQUIRE(dst && src && parents, "%s: null argument", who);
     ATLAS_REQUIRE(((uintptr_t)parents & 3) == 0, "%s: misaligned parents", who);
+    ATLAS_REQUIRE(row_stride < 1L << 40, "%s: rows %ld bytes apart", who, row_stride);
     const long span = (((long)n_groups * width) - 1) * row_stride + row_bytes;
     uintptr_t bits = (uintptr_t)row_stride;
     for (int i = 0; i < n_states; ++i) {
@@ -563,7 +580,26 @@ int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, 
     const int unit = (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
     const long full = row_bytes / unit, per = 256L * (width <= 8 ? 4 : width <= 16 ? 2 : 1);
     const long blocks = (full + per - 1) / per + (row_bytes % unit != 0);
-    ATLAS_REQUIRE(blocks <= 0x7FFFFFFF, "%s: rows of %ld bytes", who, row_bytes);
+    ATLAS_REQUIRE(blocks < 1 << 24, "%s: rows of %ld bytes", who, row_bytes);
+    // states of one launch are moved at once: none may be written that another reads or writes
+    // (their rows may lie between another's)
+    const auto meet = [&](uintptr_t p, uintptr_t q) {
+        const uintptr_t apart = p < q ? q - p : p - q, at = apart % std::max(row_stride, 1L);
+        return apart < (uintptr_t)span && ((long)at < row_bytes || row_stride - (long)at < row_bytes);
+    };
+    for (int i = 0; i < n_states; i += kBeamStates) {
+        const int n = std::min(kBeamStates, n_states - i);
+        BeamSpan all[2 * kBeamStates];
+        int m = 0;
+        for (int j = i; j < i + n; ++j) {
+            all[m++] = {(uintptr_t)dst[j], true};
+            if (src[j] != dst[j]) all[m++] = {(uintptr_t)src[j], false};
+        }
+        std::sort(all, all + m, [](const BeamSpan& a, const BeamSpan& b) { return a.at < b.at; });
+        for (int j = 0; j < m; ++j)
+            for (int o = j + 1; o < m && all[o].at - all[j].at < (uintptr_t)span; ++o)
+                ATLAS_REQUIRE(!(all[j].write || all[o].write) || !meet(all[j].at, all[o].at), "%s: states overlap", who);
+    }
     for (int i = 0; i < n_states; i += kBeamStates) {
         BeamStates s{};
         const int n = std::min(kBeamStates, n_states - i);

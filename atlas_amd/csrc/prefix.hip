@@ -7,6 +7,20 @@
 // the shared tokens are read once for all of them, and their products are matrix
 // instructions.  A row's own tokens go through the same instructions, seen by its
 // columns only.
+//
+// With scores in powers of two (s = q.k scale log2 e), a wave keeps for each column
+//   m >= max s - 8,  l = sum 2^(s - m),  O = sum 2^(s - m) v
+// over its chunks of 16 tokens; waves and then blocks are joined by their maxima.
+// S = K Q^T and O^T += V^T P are f32 products of 16 x 16 x 4, in which a lane's scores are
+// just what its next product's B operand wants: P stays in registers, K and V pass from
+// memory to registers in whole 64-byte pieces and through no LDS.
+//
+// Bound by the cache's stream where a group has few columns: 8 beams of 32 heads of 128
+// over 4000 shared tokens and up to 96 of each 34 us, 135 MB, 26 at a copy's rate; and
+// by the f32 products (60 us of 134) and what stands between them, masks, exponentials and
+// loads of K and V that 32 columns share, where groups are wide: 64 requests of
+// 32 heads over 8 of 128.  The smallest, 4 beams of 9 heads over 3 of 64, are a launch and the chain of
+// its loads: 4.9 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,15 +33,18 @@ constexpr float kPfLazy = 8.0f;
 constexpr float kPfLog2e = 1.4426950408889634f;
 constexpr int kPfChunk = 16;           // tokens that a wave takes at a time
 constexpr int kPfMaxSplits = 64;
-constexpr int kPfLeast = 8;            // chunks of a block, where a tile has several
+// Chunks of a block, where a tile has several: a wave of eight then has one.  A chunk's
+// chain of loads, products and exponentials is as long as what a block costs by itself.
+constexpr int kPfLeast = 8;
 
 // What a tile and KV head leave for the join.
 struct PfUnit {
     int runs, cols, row0, pad;         // runs 0 and 1: nothing to join
 };
 
-// waves of a SIMD for the registers of HD and CT, and so blocks of a CU
-constexpr int pf_waves(int hd) { return hd == 256 ? 4 : 8; }      // of a block
+// Waves of a block, and blocks of a CU by their registers.  (Head dimension 128: eight waves 34
+// us for 8 beams of 32 heads, four in blocks of their own 36, twelve 42.)
+constexpr int pf_waves(int hd) { return hd == 256 ? 4 : 8; }
 constexpr int pf_at_once(int hd, int ct) { return hd * ct <= 64 ? 2 : 1; }
 
 struct PfArgs {
@@ -221,7 +238,7 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
     PfTokens tokens;
     tokens.set(a, grp, row0, n_rows, lane);
     // Every wave of the tile's blocks takes every so many chunks: shared tokens are more
-    // work than own ones, and each has its share of both.  Two chunks to a wave at least.
+    // work than own ones, and each has its share of both.
     const int runs = min(max((tokens.chunks + kPfLeast - 1) / kPfLeast, 1), a.splits);
     if (split >= runs) return;
     if (split == 0 && threadIdx.x == 0 && a.splits > 1) a.unit[u * a.n_kv + kvh] = {runs, cols, row0, 0};
@@ -521,7 +538,9 @@ struct PfShape {
 static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window) {
     PfShape s{};
     const int group = n_heads / c.n_kv;
-    // columns of an average group
+    // Columns of an average group: a second tile of columns halves the loads of K and V for
+    // wide groups (64 requests of 32 heads over 8: 134 us, 165 with one), and leaves half of
+    // a narrow one's products empty.
     const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
     s.ct = wide <= 128 || c.head_dim == 256 ? 1 : 2;
     s.rows = 16 * s.ct / group;
@@ -584,7 +603,8 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
                   ld_q, ld_out);
     const PfShape s = pf_shape(c, b, n_heads, window);
     const long units = (long)s.tiles * c.n_kv;
-    ATLAS_REQUIRE(units <= 1 << 23, "%s: %d tiles of rows and %d KV heads", who, s.tiles, c.n_kv);
+    const long blocks = ((long)c.n_kv * s.splits + 7) / 8 * 8 * s.tiles;
+    ATLAS_REQUIRE(blocks < 1 << 23, "%s: %d tiles of rows and %d KV heads", who, s.tiles, c.n_kv);   // 2^32 threads
     PfArgs a{};
     a.k = c.k; a.v = c.v;
     a.n_slots = c.n_slots; a.max_seq = c.max_seq; a.n_kv = c.n_kv;
@@ -608,7 +628,7 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
         a.part_o = reinterpret_cast<float*>(a.unit + units);
         a.part_ml = a.part_o + s.parts() * c.n_kv * c.head_dim;
     }
-    const dim3 grid((unsigned)(((long)c.n_kv * s.splits + 7) / 8 * 8 * s.tiles));
+    const dim3 grid((unsigned)blocks);
 #define PF_RUN(HD, CT) hipLaunchKernelGGL((pf_attention_kernel<HD, CT>), grid, dim3(pf_waves(HD) * 64), 0, st, a)
     if (c.head_dim == 64 && s.ct == 1) PF_RUN(64, 1);
     else if (c.head_dim == 64) PF_RUN(64, 2);

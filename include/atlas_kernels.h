@@ -401,10 +401,15 @@ typedef struct {
 
 /* Attention of one query row ([n_rows][n_heads * head_dim] f32, ld_q elements
  * apart) over its tokens, the last `window` of them (0: all), scores times scale, in
- * f32.  A group's shared tokens are read once for up to 64 of its rows' heads.
- * n_heads / n_kv in 1 .. 16.  A row without tokens gives zeros, whatever its q.  A
- * token of infinities or NaN is nothing to the rows that do not see it.
- * out may be q, with ld_out = ld_q.                                          */
+ * f32.  A group's shared tokens are read once for 16 columns, a row and one of a KV
+ * head's heads each (32 where a group has more than 128 on average and head_dim is below
+ * 256).  n_heads / n_kv in 1 .. 16; n_slots * max_seq below 2^31; n_kv in whole eights times
+ * the tiles of columns (n_groups, and one to each full tile of rows) below 2^23.  A row
+ * without tokens, or whose scores are all -inf, gives zeros, whatever its q.  A
+ * token of infinities or NaN is nothing to the rows that do not see it.  (A score times
+ * 1.45 scale has to be below 2^127 in magnitude, and 2^8 times an element of V, summed over
+ * the tokens that a row sees, likewise: weights are kept up to 2^8 before they are divided
+ * by their sum.)  out may be q, with ld_out = ld_q.                          */
 int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix_batch* batch,
                                const float* q, int64_t ld_q, int n_heads, float scale, int window,
                                float* out, int64_t ld_out);
@@ -424,8 +429,8 @@ int atlas_beam_select_f32(const float* logits, int64_t ld, int vocab, const doub
 /* Beams take over the states of the beams they continue: row g * width + b of each
  * of n_states states (dst[i], src[i]: arrays on the host of device pointers, read during the call)
  * becomes row g * width + parents[g * width + b]; rows of row_bytes, row_stride bytes
- * apart.  dst[i] may be src[i] (rows that stay are then left alone) and must not
- * overlap it otherwise.  A parent that is no beam leaves its row of dst as it is.
+ * apart (below 2^40).  dst[i] may be src[i] (rows that stay are then left alone); no state that
+ * is written may overlap another otherwise.  A parent that is no beam leaves its row of dst as it is.
  * width up to 64, n_groups up to 65535.                                      */
 int atlas_beam_reorder(void* const* dst, const void* const* src, int n_states, int64_t row_bytes,
                        int64_t row_stride, const int* parents, int n_groups, int width);

@@ -1,6 +1,7 @@
 """Attention over shared prefixes, beam selection, reordering of states and low-rank adapters on the
 device, against 64 bits."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -419,6 +420,19 @@ def test_reorder_part_of_a_row_and_many_states(off):
         assert (y.get() == want).all()
 
 
+def test_reorder_states_whose_rows_lie_between_each_other():
+    rng = np.random.default_rng(4)
+    x = rng.integers(0, 256, (6, 400)).astype(np.uint8)
+    parents = np.array([5, 5, 0, 3, 3, 1], np.int32)
+    d, p = Dev(x), Dev(parents)
+    ptrs = (C.c_void_p * 3)(d.ptr + 296, d.ptr, d.ptr + 96)
+    check(lib().atlas_beam_reorder(ptrs, ptrs, 3, 96, 400, p.ptr, 1, 6))
+    want = x.copy()
+    for at in (0, 96, 296):
+        want[:, at:at + 96] = x[parents, at:at + 96]
+    assert (d.get() == want).all()
+
+
 # ---- adapters ----------------------------------------------------------------------
 
 
@@ -655,3 +669,43 @@ def test_beam_reorder_gpu():
                 if p[i, b] >= 0:
                     want[i, b] = v[i, p[i, b]]
         assert (g.download().reshape(v.shape) == want).all()
+
+
+def test_two_threads_on_streams_of_their_own_at_once():
+    """Scratch is each thread's: both run all kinds of calls with other sizes, together."""
+    failed = []
+
+    def worker(seed, ready):
+        def work(hip):
+            b = Batch(seed, [8, 5], [700 + 300 * seed, 40], [20] * 13, group=4, hd=128, n_kv=2).upload()
+            out = Dev(np.full((13, b.heads * b.hd), 7, np.float32))
+            want, want_off = b.want()
+            a = Adapters(seed, 5, 16, 256 + seed, 2100, 70 * seed)
+            d = [Dev(v) for v in (*a.raw, a.x, a.base, a.pick, a.scales)]
+            y = Dev(np.zeros((70 * seed, 256 + seed), np.float32))
+            c = LoraC(1, d[0].ptr, d[1].ptr, d[5].ptr, 5, 16, 256 + seed, 2100)
+            sum_want, off = many_ref.lora(a.base, a.x, a.a, a.b, a.scales, a.pick)
+            rng = np.random.default_rng(seed)
+            logits, scores = rng.standard_normal((2, 4, 5000 * seed)).astype(np.float32), np.zeros((2, 4))
+            with Stream(hip) as s:
+                ready.wait(60)
+                for _ in range(10):
+                    b.call(out)
+                    check(lib().atlas_lora_add_f32(C.byref(c), d[4].ptr, d[2].ptr, 2100, d[3].ptr, 256 + seed, y.ptr, 256 + seed,
+                                                   70 * seed))
+                    _check_select(logits, scores, 6)
+                    s.sync()
+                    _near(out.get().reshape(want.shape), want, want_off[..., None])
+                    _near(y.get(), sum_want, off)
+        try:
+            on_thread(work)
+        except BaseException as e:     # (of a thread)
+            failed.append(e)
+
+    ready = threading.Barrier(2)
+    threads = [threading.Thread(target=worker, args=(seed, ready)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

@@ -37,6 +37,8 @@ def _attention(cache=(), batch=(), q=X, ld_q=256, heads=4, window=0, out=X, ld_o
     dict(batch=dict(n_groups=(1 << 20) + 1)), dict(heads=3), dict(heads=0), dict(heads=34, ld_q=4096, ld_out=4096), dict(window=-1),
     dict(q=0), dict(out=0), dict(q=X + 4), dict(out=X + 8), dict(ld_q=252), dict(ld_out=255), dict(ld_q=258),
     dict(cache=dict(n_kv=4096, n_slots=1), heads=4096, ld_q=1 << 20, ld_out=1 << 20, batch=dict(n_rows=1 << 20)),
+    dict(cache=dict(n_slots=1 << 10, max_seq=1 << 21)), dict(cache=dict(n_kv=1, head_dim=256), heads=16, ld_q=4096, ld_out=4096,
+                                                             batch=dict(n_rows=1 << 20, n_groups=1, group_starts=0)),
 ], ids=str)
 def test_prefix_attention_refusals(kw):
     assert "prefix_attention" in _refused(_attention(**kw))
@@ -75,7 +77,10 @@ def _reorder(dst=(X, 2 * X), src=(X, 2 * X), n=2, row=64, stride=128, parents=X,
 @pytest.mark.parametrize("kw", [
     dict(dst=None), dict(src=None), dict(dst=(X, 0)), dict(src=(0, X)), dict(n=-1), dict(row=-1), dict(row=129), dict(parents=0),
     dict(parents=X + 1), dict(groups=-1), dict(groups=65536), dict(width=0), dict(width=65),
-    dict(dst=(X + 64, 2 * X)), dict(dst=(X, 2 * X - 3 * 128 - 63))], ids=str)
+    dict(dst=(X + 64, 2 * X)), dict(dst=(X, 2 * X - 3 * 128 - 63)), dict(stride=1 << 40),
+    # a state twice, and states whose rows meet, in place or not
+    dict(dst=(X, X), src=(X, X)), dict(dst=(X, X + 65), src=(X, X + 65)), dict(dst=(X, X + 3 * 128 + 63), src=(X, X + 3 * 128 + 63)),
+    dict(dst=(X, 2 * X), src=(3 * X, X)), dict(dst=(X, X + 32), src=(3 * X, 3 * X))], ids=str)
 def test_beam_reorder_refusals(kw):
     assert "beam_reorder" in _refused(_reorder(**kw))
 
