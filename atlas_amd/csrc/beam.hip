@@ -21,9 +21,9 @@ namespace atlas {
 // logits), the largest is taken n_out times.
 //
 // Bound by what is not the stream of logits: 64 rows of 100278 of them, 25.7 MB and 5 us of
-// bytes, take 24 us, of which the 64-bit exponentials' products are 5, the bounds and ranks
-// of 49 times 64 blocks as much again, each pass over a block's registers a chain of LDS and barriers,
-// and the join 7; 4 rows of 49152, one block to a CU at most, 11, a block's chain (6) and
+// bytes, take 24 us: the loads and 64-bit exponentials (5 us of the VALU) of 448 pieces, then
+// their bounds and ranks, each pass over a block's registers a chain of LDS and barriers,
+// and the join (7).  4 rows of 49152, less than a block to a CU, take 11: a block's chain (6) and
 // the join's (5).
 
 constexpr int kBeamMaxOut = 64;
