@@ -120,7 +120,6 @@ struct PfTokens {
     int n_rows, row0;
     int from, to;                      // the row sees tokens [from, to)
     int own_from, own_begin, own_end;  // its first own one that is seen; its places among the own ones
-    int slot;                          // of its own ones, where that is one
     int shared_len, shared_cell;       // the shared slot's first cell
     int first, last, own;
     int shared_chunks, chunks;
@@ -131,7 +130,6 @@ struct PfTokens {
         n_rows = n_rows_;
         const bool mine = lane < n_rows;
         const int r = row0 + (mine ? lane : 0), raw = a.lens[r];
-        slot = a.slot_stride ? 0 : a.slots[r];
         shared_len = __builtin_amdgcn_readfirstlane(max(a.prefix_lens[group], 0));
         const int shared_slot = __builtin_amdgcn_readfirstlane(a.prefix_slots[group]);
         const bool cells = a.n_slots > 0 && a.max_seq > 0, there = cells && shared_slot >= 0 && shared_slot < a.n_slots;
@@ -181,7 +179,7 @@ struct PfChunk {
             live = e < k.own;
             const int begin = __shfl(k.own_begin, row, 64), from = __shfl(k.own_from, row, 64);   // (of every lane)
             x = live ? e - begin + from : 0;
-            slot = a.slot_stride ? a.slots[(long)(k.row0 + row) * a.slot_stride + x] : __shfl(k.slot, row, 64);
+            slot = a.slots[(long)(k.row0 + row) * max(a.slot_stride, 1) + (a.slot_stride ? x : 0)];
         }
     }
     // the token's cell; of one that is not there some cell that is
@@ -273,7 +271,7 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
     const auto chunk_of = [&](int t) { return w0 + (back ? n - 1 - t : t) * stride; };
     f32x4 kf[S], vf[4][H];
     PfChunk cur, next;
-    int cell = 0, next_cell = 0;
+    int next_cell = 0;
     bool infinite = false;
     const auto fetch_k = [&](int c) {
         const float* p = kb + c * pitch;
@@ -290,17 +288,24 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
     };
     if (n > 0) {
         cur.find(a, tokens, chunk_of(0), i);
-        cell = cur.cell(a, tokens);
+        next.find(a, tokens, chunk_of(min(1, n - 1)), i);
+        const int cell = cur.cell(a, tokens);
         fetch_k(cell);
         fetch_v(cell);
-        if (n > 1) next.find(a, tokens, chunk_of(1), i);
+        next_cell = next.cell(a, tokens);
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j)
         if (threadIdx.x + j * W * 64 < ITEMS) sh.q[0][0][threadIdx.x + j * W * 64] = query[j] * (a.scale * kPfLog2e);
     __syncthreads();
 
+    // Loads return in order, and what is copied from one step to the next is waited for: the
+    // table's entry for the chunk after the next is asked for before the next one's K and V,
+    // and used before its own are.
     const auto round = [&](int t, auto more) {
+        PfChunk after;
+        int after_cell = 0;
+        if constexpr (decltype(more)::value) after.find(a, tokens, chunk_of(min(t + 2, n - 1)), i);
         // the column tiles that see any of the chunk
         const int c_first = cur.own ? cur.row_first * a.group >> 4 : 0;
         const int c_last = cur.own ? ((cur.row_last + 1) * a.group - 1) >> 4 : CT - 1;
@@ -320,10 +325,7 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[c][r] = d[0][r] + d[1][r];
         }
-        if constexpr (decltype(more)::value) {
-            next_cell = next.cell(a, tokens);
-            fetch_k(next_cell);
-        }
+        if constexpr (decltype(more)::value) fetch_k(next_cell);
         if (!cur.plain) {
             // (without short circuits, which would be branches)
             int tok_row[4], tok[4];
@@ -383,6 +385,7 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
                         for (int e = 0; e < 4; ++e) vf[r][h][e] = pf_infinite(vf[r][h][e]) ? 0.f : vf[r][h][e];
             }
         }
+        if constexpr (decltype(more)::value) after_cell = after.cell(a, tokens);
         // O^T += V^T P: elements 64 h + 4 (4g + r) + e of column i
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -397,8 +400,8 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
         if constexpr (decltype(more)::value) {
             fetch_v(next_cell);
             cur = next;
-            cell = next_cell;
-            if (t + 2 < n) next.find(a, tokens, chunk_of(t + 2), i);
+            next = after;
+            next_cell = after_cell;
         }
     };
     int t = 0;
@@ -410,7 +413,7 @@ __global__ __launch_bounds__(pf_waves(HD) * 64, pf_at_once(HD, CT) * pf_waves(HD
 #pragma unroll 1
         for (t = 0; t < n; ++t) {
             cur.find(a, tokens, chunk_of(t), i);
-            cell = cur.cell(a, tokens);
+            const int cell = cur.cell(a, tokens);
             if (cur.plain) continue;
 #pragma unroll 1
             for (int j = 0; j < kPfChunk; ++j) {
