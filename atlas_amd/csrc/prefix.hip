@@ -16,10 +16,10 @@
 // memory to registers in whole 64-byte pieces and through no LDS.
 //
 // Bound by the cache's stream where a group has few columns: 8 beams of 32 heads of 128
-// over 4000 shared tokens and up to 96 of each 34 us, 135 MB, 26 at a copy's rate; and
-// by the f32 products (60 us of 134) and what stands between them, masks, exponentials and
-// loads of K and V that 32 columns share, where groups are wide: 64 requests of
-// 32 heads over 8 of 128.  The smallest, 4 beams of 9 heads over 3 of 64, are a launch and the chain of
+// over 4001 shared tokens and up to 97 of each 32 us, 135 MB, 26 at a copy's rate; and
+// by the f32 products where groups are wide (64 requests of 32 heads over 8 of 128, 8191 tokens
+// and up to 1023 of each: 69 of 124 us; shared tokens alone go at 114 TFLOP/s of 155), with
+// masks and exponentials between them that a SIMD's two waves do not quite cover.  The smallest, 4 beams of 9 heads over 3 of 64, are a launch and the chain of
 // its loads: 4.9 us.
 #include <algorithm>
 #include <type_traits>
@@ -35,6 +35,7 @@ constexpr int kPfChunk = 16;           // tokens that a wave takes at a time
 constexpr int kPfMaxSplits = 64;
 // Chunks of a block, where a tile has several: a wave of eight then has one.  A chunk's
 // chain of loads, products and exponentials is as long as what a block costs by itself.
+// (4 beams of 9 heads over 700 tokens: 9.7 us, 10.6 with 16.)
 constexpr int kPfLeast = 8;
 
 // What a tile and KV head leave for the join.
@@ -42,8 +43,9 @@ struct PfUnit {
     int runs, cols, row0, pad;         // runs 0 and 1: nothing to join
 };
 
-// Waves of a block, and blocks of a CU by their registers.  (Head dimension 128: eight waves 34
-// us for 8 beams of 32 heads, four in blocks of their own 36, twelve 42.)
+// Waves of a block, and blocks of a CU by their registers.  (Head dimension 128, 8 beams of 32
+// heads and 64 requests of 32 over 8: four waves 33.3 and 152 us, eight 32.4 and 124, twelve 35.7
+// and, with what does not fit the registers in memory, 151.)
 constexpr int pf_waves(int hd) { return hd == 256 ? 4 : 8; }
 constexpr int pf_at_once(int hd, int ct) { return hd * ct <= 64 ? 2 : 1; }
 
@@ -560,8 +562,10 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
     PfShape s{};
     const int group = n_heads / c.n_kv;
     // Columns of an average group: a second tile of columns halves the loads of K and V for
-    // wide groups (64 requests of 32 heads over 8: 134 us, 165 with one), and leaves half of
-    // a narrow one's products empty.
+    // wide groups (64 requests of 32 heads over 8, 256 columns: 124 us, 148 with one; 40 of
+    // groups of 32 columns: 40 with two, 27 with one).  At 128 columns it is the prefix: 61 us
+    // with one and 55 with two over 8191 tokens, 27 and 28 over 2047; eight such groups 275 and 251,
+    // 120 and 141.
     const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
     s.ct = wide <= 128 || c.head_dim == 256 ? 1 : 2;
     s.rows = 16 * s.ct / group;
