@@ -470,6 +470,10 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
     ATLAS_REQUIRE(logits && scores && tokens && parents && out_scores, "%s: null argument", who);
     ATLAS_REQUIRE((((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)parents) & 3) == 0 &&
                       (((uintptr_t)scores | (uintptr_t)out_scores) & 7) == 0, "%s: misaligned argument", who);
+    // a group's results are written while others' scores are read
+    const long n_in = (long)n_groups * width, n_best = (long)n_groups * n_out;
+    const uintptr_t in0 = (uintptr_t)scores, to0 = (uintptr_t)out_scores;
+    ATLAS_REQUIRE(in0 + n_in * 8 <= to0 || to0 + n_best * 8 <= in0, "%s: out_scores overlaps scores", who);
     const size_t bytes = beam_select_workspace(vocab, n_groups, width, n_out);
     void* p = ws.p;
     if (p) {

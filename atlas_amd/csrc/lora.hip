@@ -443,6 +443,15 @@ int lora_add_launch(const atlas_lora& l, const int* adapters, const float* x, lo
     const uintptr_t floats = (uintptr_t)x | (uintptr_t)base | (uintptr_t)y | (uintptr_t)adapters | (uintptr_t)l.scales;
     const uintptr_t weights = (uintptr_t)l.a | (uintptr_t)l.b;
     ATLAS_REQUIRE((floats & 3) == 0 && weights % size == 0, "%s: misaligned argument", who);
+    ATLAS_REQUIRE(std::max({ld_x, ld_base, ld_y}) < 1L << 40, "%s: rows %ld, %ld and %ld elements apart", who, ld_x, ld_base, ld_y);
+    // y's rows and p's of w elements (which may lie between them) have nothing in common
+    const auto apart = [&](const float* p, long w, long ld) {
+        const uintptr_t y0 = (uintptr_t)y, p0 = (uintptr_t)p;
+        if (y0 + ((n - 1) * ld_y + l.m) * 4 <= p0 || p0 + ((n - 1) * ld + w) * 4 <= y0) return true;
+        const long at = ((((long)p0 - (long)y0) / 4) % ld_y + ld_y) % ld_y;
+        return ld == ld_y && at >= l.m && at + w <= ld_y;
+    };
+    ATLAS_REQUIRE(apart(x, l.k, ld_x) && ((base == y && ld_base == ld_y) || apart(base, l.m, ld_base)), "%s: y overlaps x or base", who);
     LoraArgs a{};
     a.a = l.a; a.b = l.b; a.scales = l.scales;
     a.n_adapters = l.n_adapters; a.rank = l.rank; a.m = l.m; a.k = l.k;

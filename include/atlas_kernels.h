@@ -409,7 +409,7 @@ typedef struct {
  * token of infinities or NaN is nothing to the rows that do not see it.  (A score times
  * 1.45 scale has to be below 2^127 in magnitude, and 2^8 times an element of V, summed over
  * the tokens that a row sees, likewise: weights are kept up to 2^8 before they are divided
- * by their sum.)  out may be q, with ld_out = ld_q.                          */
+ * by their sum.)  out may be q, with ld_out = ld_q, and overlaps nothing else.  */
 int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix_batch* batch,
                                const float* q, int64_t ld_q, int n_heads, float scale, int window,
                                float* out, int64_t ld_out);
@@ -419,7 +419,7 @@ int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix
  * 64 bits, the n_out largest of each group in descending order (equal scores: the lower beam,
  * then the larger logit, then the lower token).  logits [n_groups * width] rows of
  * vocab, ld apart; scores [n_groups * width]; tokens, parents (the beam within its
- * group) and out_scores [n_groups][n_out].  A beam whose score is not finite, a row
+ * group) and out_scores [n_groups][n_out], none of which overlaps the scores.  A beam whose score is not finite, a row
  * of logits with NaN or +inf or of -inf only, and a logit of -inf give no candidates;
  * where a group has too few, the rest is token 0 of parent -1 and score -inf.
  * width and n_out 1 to 64, n_groups * width up to 65535, vocab up to 2^30.    */
@@ -449,8 +449,8 @@ typedef struct {
 
 /* y_r = base_r + scales[p] b_p (a_p x_r), p = adapters[r], for n rows (up to 2^20) of x (k
  * elements, ld_x apart), base and y (m elements); a row whose p is no adapter is its
- * base.  base is the shared projection's product and may be y (with ld_y = ld_base), but must not
- * overlap it otherwise.  f32 sums of exact products.                          */
+ * base.  base is the shared projection's product and may be y (with ld_y = ld_base), but neither it
+ * nor x must overlap y otherwise; rows of one may lie between another's, if they are as far apart.  f32 sums of exact products.                          */
 int atlas_lora_add_f32(const atlas_lora* lora, const int* adapters, const float* x, int64_t ld_x,
                        const float* base, int64_t ld_base, float* y, int64_t ld_y, int n);
 

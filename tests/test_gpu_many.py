@@ -548,6 +548,57 @@ def test_lora_infinities_and_nan_stay_with_their_rows(rank):
     assert np.isfinite(got[2]).sum() == 99 and not np.isfinite(got[2, 7])
 
 
+def test_lora_rows_between_each_other():
+    # x, base and y are columns of one matrix
+    a = Adapters(10, 3, 16, 100, 60, 40, "f32")
+    a.pick = (np.arange(40) % 5 - 1).astype(np.int32)
+    d = Dev(np.concatenate([a.x, a.base, np.full((40, 104), 7, np.float32)], 1))
+    w = [Dev(v) for v in (a.a, a.b, a.pick, a.scales)]
+    c = LoraC(0, w[0].ptr, w[1].ptr, w[3].ptr, 3, 16, 100, 60)
+    check(lib().atlas_lora_add_f32(C.byref(c), w[2].ptr, d.ptr, 264, d.ptr + 4 * 60, 264, d.ptr + 4 * 160, 264, 40))
+    got = d.get()
+    want, off = many_ref.lora(a.base, a.x, a.a, a.b, a.scales, a.pick)
+    _near(got[:, 160:260], want, off)
+    assert (got[:, 260:] == 7).all() and (got[:, :60] == a.x).all() and (got[:, 60:160] == a.base).all()
+
+
+def test_scratch_refused_in_a_capture_or_short_of_memory_then_there():
+    def work(hip):
+        a = Adapters(11, 3, 16, 64, 2000, 9)
+        d = [Dev(v) for v in (*a.raw, a.x, a.base, a.pick, a.scales)]
+        y = Dev(np.zeros((9, 64), np.float32))
+        c = LoraC(1, d[0].ptr, d[1].ptr, d[5].ptr, 3, 16, 64, 2000)
+        z, s = Dev(np.tile(np.arange(10, dtype=np.float32), 2)), Dev(np.zeros(2))
+        out = [Dev(np.zeros(2, t)) for t in (np.uint32, np.int32, np.float64)]
+        b = Batch(12, [4], [3000], [30] * 4, hd=128, junk=False).upload()
+        to = Dev(np.zeros((4, b.heads * b.hd), np.float32))
+        calls = [lambda: check(lib().atlas_lora_add_f32(C.byref(c), d[4].ptr, d[2].ptr, 2000, d[3].ptr, 64, y.ptr, 64, 9)),
+                 lambda: check(lib().atlas_beam_select_f32(z.ptr, 10, 10, s.ptr, 1, 2, 2, *(x.ptr for x in out))),
+                 lambda: b.call(to)]
+
+        def refused(call, code):
+            with pytest.raises(AtlasError) as e:
+                call()
+            assert e.value.code == code
+        with Stream(hip) as st:
+            for call in calls:
+                st.capture(lambda: refused(call, -4))
+                check(lib().atlas_debug_fail_allocations(0, 1))
+                refused(call, -3)
+                check(lib().atlas_debug_fail_allocations(0, 0))
+                call()
+                st.sync()
+            exe, _ = st.capture(lambda: [call() for call in calls])
+            for _ in range(3):
+                st.launch(exe)
+                st.sync()
+        _near(y.get(), *many_ref.lora(a.base, a.x, a.a, a.b, a.scales, a.pick))
+        assert out[0].get().tolist() == [9, 9] and out[1].get().tolist() == [0, 1]
+        want, off = b.want()
+        _near(to.get().reshape(want.shape), want, off[..., None])
+    on_thread(work)
+
+
 def test_lora_captured():
     def work(hip):
         a = Adapters(8, 5, 16, 256, 1024, 9)

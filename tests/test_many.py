@@ -53,13 +53,14 @@ def test_prefix_attention_null_and_nothing_to_do():
     check(_attention(batch=dict(n_groups=0, group_starts=0)))
 
 
-def _select(logits=X, ld=100, vocab=100, scores=X, groups=2, width=4, n_out=8, tokens=X, parents=X, out=X):
+def _select(logits=X, ld=100, vocab=100, scores=X, groups=2, width=4, n_out=8, tokens=X, parents=X, out=1 << 20):
     return load().atlas_beam_select_f32(logits, ld, vocab, scores, groups, width, n_out, tokens, parents, out)
 
 
 @pytest.mark.parametrize("kw", [
     dict(logits=0), dict(scores=0), dict(tokens=0), dict(parents=0), dict(out=0), dict(vocab=0), dict(ld=99), dict(vocab=(1 << 30) + 1, ld=1 << 31), dict(groups=-1),
     dict(width=0), dict(width=65), dict(n_out=0), dict(n_out=65), dict(groups=65536, width=1), dict(groups=20000, width=4),
+    dict(out=X), dict(out=X + 56), dict(out=X - 120),
     dict(scores=X + 4), dict(out=X + 4), dict(logits=X + 2), dict(tokens=X + 1), dict(parents=X + 1)], ids=str)
 def test_beam_select_refusals(kw):
     assert "beam_select" in _refused(_select(**kw))
@@ -93,7 +94,10 @@ def test_beam_reorder_nothing_to_do():
 LORA = dict(fmt=1, a=X, b=X, scales=X, n_adapters=3, rank=8, m=64, k=32)
 
 
-def _lora(lora=(), adapters=X, x=X, ld_x=32, base=X, ld_base=64, y=X, ld_y=64, n=4):
+Y = 1 << 20
+
+
+def _lora(lora=(), adapters=X, x=X, ld_x=32, base=Y, ld_base=64, y=Y, ld_y=64, n=4):
     return load().atlas_lora_add_f32(C.byref(LoraC(**{**LORA, **dict(lora)})), adapters, x, ld_x, base, ld_base, y, ld_y, n)
 
 
@@ -101,7 +105,9 @@ def _lora(lora=(), adapters=X, x=X, ld_x=32, base=X, ld_base=64, y=X, ld_y=64, n
     dict(lora=dict(fmt=2)), dict(lora=dict(a=0)), dict(lora=dict(b=0)), dict(lora=dict(n_adapters=-1)), dict(lora=dict(n_adapters=4096)), dict(lora=dict(rank=0)),
     dict(lora=dict(rank=257)), dict(lora=dict(m=0)), dict(lora=dict(k=0)), dict(lora=dict(m=(1 << 24) + 1), ld_base=1 << 25, ld_y=1 << 25),
     dict(lora=dict(a=X + 1)), dict(lora=dict(fmt=0, b=X + 2)), dict(lora=dict(scales=X + 2)), dict(adapters=0), dict(x=0), dict(base=0),
-    dict(y=0), dict(ld_x=31), dict(ld_base=63), dict(ld_y=63), dict(n=-1), dict(n=(1 << 20) + 1), dict(x=X + 2), dict(y=X + 1)], ids=str)
+    dict(y=0), dict(ld_x=31), dict(ld_base=63), dict(ld_y=63), dict(n=-1), dict(n=(1 << 20) + 1), dict(x=X + 2), dict(y=X + 1),
+    dict(ld_x=1 << 40), dict(x=Y + 4 * 255), dict(x=Y - 4 * 127), dict(base=Y + 4), dict(base=Y, ld_base=65), dict(x=Y + 4 * 63, ld_x=64),
+    dict(x=Y + 4 * 64, ld_x=96, ld_y=95)], ids=str)
 def test_lora_refusals(kw):
     assert "lora_add" in _refused(_lora(**kw))
 
