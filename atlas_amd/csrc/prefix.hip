@@ -527,7 +527,7 @@ __global__ __launch_bounds__(256) void pf_join_kernel(PfArgs a) {
     sum = wave_sum(lane < x.runs ? f * sum : 0.f);
     const int rg = lane / LANES, d = lane % LANES * 4;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    // eight loads at a time, without conditions (a last run again, with no weight)
+    // eight loads at a time, without conditions (past the last run it again, for nothing)
     for (int r0 = 0; r0 < x.runs; r0 += 8 * RG) {
         f32x4 y[8];
 #pragma unroll
@@ -537,7 +537,8 @@ __global__ __launch_bounds__(256) void pf_join_kernel(PfArgs a) {
         for (int j = 0; j < 8; ++j) {
             const int r = r0 + j * RG + rg;
             const float fr = __shfl(f, min(r, 63), 64);
-            o += (r < x.runs ? fr : 0.f) * y[j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += r < x.runs ? fr * y[j][e] : 0.f;   // (not 0 times an infinity)
         }
     }
 #pragma unroll
@@ -561,18 +562,7 @@ struct PfShape {
 static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, int n_heads, int window) {
     PfShape s{};
     const int group = n_heads / c.n_kv;
-    // Columns of an average group: a second tile of columns halves the loads of K and V for
-    // wide groups (64 requests of 32 heads over 8, 256 columns: 124 us, 148 with one; 40 of
-    // groups of 32 columns: 40 with two, 27 with one).  At 128 columns it is the prefix: 61 us
-    // with one and 55 with two over 8191 tokens, 27 and 28 over 2047; eight such groups 275 and 251,
-    // 120 and 141.
-    const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
-    s.ct = wide <= 128 || c.head_dim == 256 ? 1 : 2;
-    s.rows = 16 * s.ct / group;
-    s.cols = s.rows * group;
-    s.tiles = b.group_starts ? b.n_rows / s.rows + b.n_groups : (b.n_rows + s.rows - 1) / s.rows;
-    if (b.n_groups == 1) s.tiles = (b.n_rows + s.rows - 1) / s.rows;
-    // chunks of a tile, by the caller's hints
+    // the caller's hints
     int64_t prefix = std::min(b.max_prefix > 0 ? b.max_prefix : c.max_seq, c.max_seq);
     int64_t own = std::min(b.max_own > 0 ? b.max_own : c.max_seq, c.max_seq);
     if (b.slot_stride > 0) own = std::min<int64_t>(own, b.slot_stride);
@@ -580,6 +570,19 @@ static PfShape pf_shape(const atlas_slot_cache& c, const atlas_prefix_batch& b, 
         prefix = std::min<int64_t>(prefix, window);
         own = std::min<int64_t>(own, window);
     }
+    // A second tile of columns halves the loads of K and V and the masks and exponentials' share,
+    // where an average group is wide and its prefix long, and halves the blocks elsewhere.  With one
+    // tile and two, 8 KV heads of 128: 64 columns over 8191 tokens 35.0 and 34.3 us, 96 columns 49.6
+    // and 46.8, 128 columns 61.5 and 54.6, 256 columns over 4095 66.6 and 60.9; 128 columns over
+    // 2047 28.0 and 28.3, eight such groups 120 and 141; 512 columns over 511 48 and 53.  Heads
+    // of 64, 256 columns over 4095 tokens: 36.0 and 37.8; of 256 have no registers for it.
+    const long wide = (long)b.n_rows * group / std::max(b.n_groups, 1);
+    s.ct = c.head_dim == 128 && wide > 64 && prefix > 2048 ? 2 : 1;
+    s.rows = 16 * s.ct / group;
+    s.cols = s.rows * group;
+    s.tiles = b.group_starts ? b.n_rows / s.rows + b.n_groups : (b.n_rows + s.rows - 1) / s.rows;
+    if (b.n_groups == 1) s.tiles = (b.n_rows + s.rows - 1) / s.rows;
+    // chunks of a tile
     const int64_t chunks = (prefix + kPfChunk - 1) / kPfChunk + (own * s.rows + kPfChunk - 1) / kPfChunk;
     // A block to every place of the chip; four to a tile where groups of different lengths
     // would leave a part of the places empty (16 groups of 1 to 15 rows of 16 heads over 4 of
@@ -655,8 +658,7 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
     }
     const dim3 grid((unsigned)blocks);
 #define PF_RUN(HD, CT) hipLaunchKernelGGL((pf_attention_kernel<HD, CT>), grid, dim3(pf_waves(HD) * 64), 0, st, a)
-    if (c.head_dim == 64 && s.ct == 1) PF_RUN(64, 1);
-    else if (c.head_dim == 64) PF_RUN(64, 2);
+    if (c.head_dim == 64) PF_RUN(64, 1);
     else if (c.head_dim == 128 && s.ct == 1) PF_RUN(128, 1);
     else if (c.head_dim == 128) PF_RUN(128, 2);
     else PF_RUN(256, 1);

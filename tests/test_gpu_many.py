@@ -134,6 +134,43 @@ def test_prefix_attention_long(hd, n_kv, group, hints):
     b.upload(hints=hints).check()
 
 
+@pytest.mark.parametrize("rows,group", [(65, 1), (100, 1), (17, 4), (33, 4), (40, 2), (14, 5), (23, 3), (5, 16)])
+@pytest.mark.parametrize("window", [0, 2060])
+def test_prefix_attention_wide_groups_of_long_caches(rows, group, window):
+    # two tiles of columns to a block, by what the cache can hold; then by the prefix
+    own = np.random.default_rng(3).integers(0, 25, rows)
+    Batch(3, [rows], [70], own, n_kv=1, group=group, hd=128, slack=2100, table=rows % 2 == 0).upload(hints=False).check(window=window)
+
+
+def test_prefix_attention_wide_groups_over_long_prefixes():
+    own = np.random.default_rng(5).integers(0, 60, 40)
+    b = Batch(15, [23, 0, 17], [2100, 30, 700], own, n_kv=1, group=6, hd=128, extra_rows=2).upload()
+    b.check()
+    b.check(window=2080)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prefix_attention_infinities_in_the_last_of_several_runs(hd):
+    b = Batch(17, [4], [1300], [9, 9, 0, 9], n_kv=1, group=3, hd=hd, table=False, junk=False)
+    b.v[b.slots[3], 1308] = np.inf
+    b.v[b.slots[1], 1300, 0, 2] = -np.inf
+    got = b.upload().check().reshape(4, 3, hd)
+    assert (got[3] == np.inf).all() and (got[1, :, 2] == -np.inf).all() and np.isfinite(got[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("window", [0, 2080])
+def test_prefix_attention_wide_groups_with_infinities_and_nan(window):
+    b = Batch(16, [20, 12], [2090, 18], [12, 3, 12, 0] * 8, n_kv=2, group=5, hd=128, table=False, junk=False)
+    own = b.slots
+    b.v[own[0], 2091, :, 3] = np.nan
+    b.v[own[2], 2100, 1, :] = np.inf
+    b.k[own[4], 2094, 0, 5] = np.nan
+    b.v[b.prefix_slots[0], 4, 0, 7] = -np.inf       # the rows whose window begins after it do not see it
+    b.v[b.prefix_slots[1], 2, 1, 0] = np.nan
+    b.q[3] = np.nan
+    b.upload().check(window=window)
+
+
 def test_prefix_attention_short_lengths():
     # rows whose length ends inside the prefix, is zero or below
     b = Batch(6, [7], [60], [0] * 7, hd=128, junk=False)
