@@ -471,9 +471,10 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
     ATLAS_REQUIRE((((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)parents) & 3) == 0 &&
                       (((uintptr_t)scores | (uintptr_t)out_scores) & 7) == 0, "%s: misaligned argument", who);
     // a group's results are written while others' scores are read
-    const long n_in = (long)n_groups * width, n_best = (long)n_groups * n_out;
-    const uintptr_t in0 = (uintptr_t)scores, to0 = (uintptr_t)out_scores;
-    ATLAS_REQUIRE(in0 + n_in * 8 <= to0 || to0 + n_best * 8 <= in0, "%s: out_scores overlaps scores", who);
+    const ByteRows given(scores, (long)n_groups * width * 8);
+    const long n_best = (long)n_groups * n_out;
+    ATLAS_REQUIRE(rows_apart(given, ByteRows(out_scores, n_best * 8)) && rows_apart(given, ByteRows(tokens, n_best * 4)) &&
+                      rows_apart(given, ByteRows(parents, n_best * 4)), "%s: a result overlaps scores", who);
     const size_t bytes = beam_select_workspace(vocab, n_groups, width, n_out);
     void* p = ws.p;
     if (p) {

@@ -145,3 +145,11 @@ def test_beams_argument(n):
     assert cli.parse_args(["--weights", "/x"]).beams == 1 and cli.parse_args(["--weights", "/x", "--beams", "16"]).beams == 16
     with pytest.raises(SystemExit):
         cli.parse_args(["--weights", "/x", "--beams", n])
+
+
+@pytest.mark.parametrize("kw", [
+    # each result where another group's scores are read: from the first to the last, and up to their ends
+    dict(tokens=X), dict(tokens=X + 60), dict(tokens=X - 60), dict(parents=X), dict(parents=X + 60), dict(parents=X - 60)], ids=str)
+def test_beam_select_results_apart_from_scores(kw):
+    """Scores [2 x 4] f64 at X; results [2 x 8], 64 bytes of tokens and of parents."""
+    assert "overlap" in _refused(_select(**{**dict(logits=1 << 21, tokens=2 * X, parents=3 * X), **kw}))
