@@ -1,6 +1,8 @@
 // beam.hip -- beam search: the choice of a group's best continuations over its beams
 // and the vocabulary, and the reordering of the beams' states.
 #include <algorithm>
+#include <memory>
+#include <new>
 
 #include "many.hpp"
 
@@ -515,10 +517,35 @@ struct BeamStates {
     const char* src[kBeamStates];
 };
 
+// a state's rows, read or written
 struct BeamSpan {
     uintptr_t at;
+    long phase;                        // in the stride
     bool write;
 };
+
+// No rows that are written meet others, which may lie between them: m states of the same rows.
+// Of those whose spans hang together only neighbours within the stride are looked at, so
+// that the time is a sort's.
+static bool beam_apart(BeamSpan* all, long m, long span, long row_bytes, long stride) {
+    const auto same = [](const BeamSpan& a, const BeamSpan& b) { return a.at == b.at && !a.write && !b.write; };
+    std::sort(all, all + m, [](const BeamSpan& a, const BeamSpan& b) { return a.at != b.at ? a.at < b.at : a.write > b.write; });
+    m = std::unique(all, all + m, same) - all;           // (many may read one)
+    for (long lo = 0, hi; lo < m; lo = hi) {
+        for (hi = lo + 1; hi < m && all[hi].at - all[hi - 1].at < (uintptr_t)span;) ++hi;
+        BeamSpan* const c = all + lo;
+        const long n = hi - lo;
+        std::sort(c, c + n, [](const BeamSpan& a, const BeamSpan& b) { return a.phase < b.phase; });
+        for (long j = 0; j < n; ++j)
+            for (long k = 1; k < n; ++k) {
+                const BeamSpan& o = c[(j + k) % n];
+                if (o.phase - c[j].phase + (j + k >= n ? stride : 0) >= row_bytes) break;
+                const uintptr_t apart = o.at > c[j].at ? o.at - c[j].at : c[j].at - o.at;
+                if ((o.write || c[j].write) && apart < (uintptr_t)span) return false;
+            }
+    }
+    return true;
+}
 
 // One column to a thread in each of U places `apart` columns from each other, as far as
 // there are `columns`; parents are the same in every lane.
@@ -586,24 +613,25 @@ int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, 
     const long full = row_bytes / unit, per = 256L * (width <= 8 ? 4 : width <= 16 ? 2 : 1);
     const long blocks = (full + per - 1) / per + (row_bytes % unit != 0);
     ATLAS_REQUIRE(blocks < 1 << 24, "%s: rows of %ld bytes", who, row_bytes);
-    // states of one launch are moved at once: none may be written that another reads or writes
-    // (their rows may lie between another's)
-    const auto meet = [&](uintptr_t p, uintptr_t q) {
-        const uintptr_t apart = p < q ? q - p : p - q, at = apart % std::max(row_stride, 1L);
-        return apart < (uintptr_t)span && ((long)at < row_bytes || row_stride - (long)at < row_bytes);
-    };
-    for (int i = 0; i < n_states; i += kBeamStates) {
-        const int n = std::min(kBeamStates, n_states - i);
-        BeamSpan all[2 * kBeamStates];
-        int m = 0;
-        for (int j = i; j < i + n; ++j) {
-            all[m++] = {(uintptr_t)dst[j], true};
-            if (src[j] != dst[j]) all[m++] = {(uintptr_t)src[j], false};
+    // states are moved side by side: none may be written that another reads or writes
+    {
+        BeamSpan few[2 * kBeamStates];
+        std::unique_ptr<BeamSpan[]> many;
+        if (n_states > kBeamStates) {
+            many.reset(new (std::nothrow) BeamSpan[2 * (size_t)n_states]);
+            if (!many) {
+                set_error(ATLAS_ENOMEM, "%s: no host memory for %d states", who, n_states);
+                return ATLAS_ENOMEM;
+            }
         }
-        std::sort(all, all + m, [](const BeamSpan& a, const BeamSpan& b) { return a.at < b.at; });
-        for (int j = 0; j < m; ++j)
-            for (int o = j + 1; o < m && all[o].at - all[j].at < (uintptr_t)span; ++o)
-                ATLAS_REQUIRE(!(all[j].write || all[o].write) || !meet(all[j].at, all[o].at), "%s: states overlap", who);
+        BeamSpan* const all = many ? many.get() : few;
+        long m = 0;
+        const auto add = [&](const void* p, bool write) { all[m++] = {(uintptr_t)p, (long)((uintptr_t)p % (uintptr_t)row_stride), write}; };
+        for (int i = 0; i < n_states; ++i) {
+            add(dst[i], true);
+            if (src[i] != dst[i]) add(src[i], false);
+        }
+        ATLAS_REQUIRE(beam_apart(all, m, span, row_bytes, row_stride), "%s: states overlap", who);
     }
     for (int i = 0; i < n_states; i += kBeamStates) {
         BeamStates s{};

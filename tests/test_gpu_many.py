@@ -470,6 +470,26 @@ def test_reorder_states_whose_rows_lie_between_each_other():
     assert (d.get() == want).all()
 
 
+def test_reorder_many_states_whose_rows_lie_between_each_other():
+    # 150 columns of one matrix, each a state, moved in place, then into another matrix
+    rng = np.random.default_rng(5)
+    x = rng.integers(0, 1 << 30, (6, 150, 12)).astype(np.int32)
+    parents = np.array([4, 0, 2, 2, -1, 5], np.int32)
+    d, p = Dev(x), Dev(parents)
+    ptrs = (C.c_void_p * 150)(*(d.ptr + 48 * i for i in range(150)))
+    check(lib().atlas_beam_reorder(ptrs, ptrs, 150, 48, 7200, p.ptr, 1, 6))
+    want = x.copy()
+    for b in (0, 1, 3):
+        want[b] = x[parents[b]]
+    assert (d.get() == want).all()
+    e = Dev(x)
+    check(lib().atlas_beam_reorder((C.c_void_p * 150)(*(e.ptr + 48 * i for i in range(150))), ptrs, 150, 48, 7200, p.ptr, 1, 6))
+    moved = x.copy()
+    for b in (0, 1, 2, 3, 5):
+        moved[b] = want[parents[b]]
+    assert (e.get() == moved).all()
+
+
 # ---- adapters ----------------------------------------------------------------------
 
 

@@ -153,3 +153,31 @@ def test_beams_argument(n):
 def test_beam_select_results_apart_from_scores(kw):
     """Scores [2 x 4] f64 at X; results [2 x 8], 64 bytes of tokens and of parents."""
     assert "overlap" in _refused(_select(**{**dict(logits=1 << 21, tokens=2 * X, parents=3 * X), **kw}))
+
+
+def _reorder_many(dst, src, n=None, row=64, stride=128, groups=1, width=4):
+    d, s = ((C.c_void_p * len(x))(*x) for x in (dst, src))
+    return load().atlas_beam_reorder(d, s, len(dst) if n is None else n, row, stride, X, groups, width)
+
+
+@pytest.mark.parametrize("first,second", [(3, 70), (0, 199), (63, 64), (130, 131)])
+@pytest.mark.parametrize("off", [0, 65, 3 * 128 + 63, -63])
+def test_beam_reorder_states_that_meet_among_many(first, second, off):
+    """States of one call are apart, however many they are: rows of 64 bytes, 128 apart, 4 to a state."""
+    at = [(1 << 20) + 4096 * i for i in range(200)]
+    at[second] = at[first] + off
+    assert "overlap" in _refused(_reorder_many(at, at))
+    # what one state reads is not what another writes
+    src = [(1 << 30) + 4096 * i for i in range(200)]
+    src[first] = at[second]
+    assert "overlap" in _refused(_reorder_many(at, src))
+
+
+def test_beam_reorder_states_that_meet_between_others():
+    # 150 states whose rows lie between each other's, one of them a byte into the next one's
+    at = [(1 << 20) + 64 * i for i in range(150)]
+    at[97] += 1
+    assert "overlap" in _refused(_reorder_many(at, at, row=64, stride=64 * 150))
+    # the row before that of the first state, as far on as the stride is
+    at = [(1 << 20) + 64 * i for i in range(149)] + [(1 << 20) + 64 * 150 * 3 - 63]
+    assert "overlap" in _refused(_reorder_many(at, at, row=64, stride=64 * 150))
