@@ -601,12 +601,14 @@ int beam_reorder_launch(void* const* dst, const void* const* src, int n_states, 
     ATLAS_REQUIRE(dst && src && parents, "%s: null argument", who);
     ATLAS_REQUIRE(((uintptr_t)parents & 3) == 0, "%s: misaligned parents", who);
     ATLAS_REQUIRE(row_stride < 1L << 40, "%s: rows %ld bytes apart", who, row_stride);
-    const long span = (((long)n_groups * width) - 1) * row_stride + row_bytes;
+    const long n_rows = (long)n_groups * width, span = (n_rows - 1) * row_stride + row_bytes;
+    const ByteRows given(parents, n_rows * 4);
     uintptr_t bits = (uintptr_t)row_stride;
     for (int i = 0; i < n_states; ++i) {
         ATLAS_REQUIRE(dst[i] && src[i], "%s: null state %d", who, i);
         const char *d = static_cast<const char*>(dst[i]), *s = static_cast<const char*>(src[i]);
         ATLAS_REQUIRE(d == s || d + span <= s || s + span <= d, "%s: state %d overlaps its new place", who, i);
+        ATLAS_REQUIRE(rows_apart(given, ByteRows(d, n_rows, row_bytes, row_stride)), "%s: state %d overlaps parents", who, i);
         bits |= (uintptr_t)d | (uintptr_t)s;
     }
     const int unit = (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;

@@ -429,9 +429,10 @@ int atlas_beam_select_f32(const float* logits, int64_t ld, int vocab, const doub
 /* Beams take over the states of the beams they continue: row g * width + b of each
  * of n_states states (dst[i], src[i]: arrays on the host of device pointers, read during the call)
  * becomes row g * width + parents[g * width + b]; rows of row_bytes, row_stride bytes
- * apart (below 2^40).  dst[i] may be src[i] (rows that stay are then left alone); no state that
- * is written may overlap another otherwise.  A parent that is no beam leaves its row of dst as it is.
- * width up to 64, n_groups up to 65535.                                      */
+ * apart (below 2^40).  dst[i] may be src[i] (rows that stay are then left alone), or lies
+ * before or behind it as a whole; no row that is written may overlap a row of another state
+ * otherwise, or parents.  Rows of one state may lie between another's.  A parent that is no beam
+ * leaves its row of dst as it is.  width up to 64, n_groups up to 65535.     */
 int atlas_beam_reorder(void* const* dst, const void* const* src, int n_states, int64_t row_bytes,
                        int64_t row_stride, const int* parents, int n_groups, int width);
 

@@ -181,3 +181,12 @@ def test_beam_reorder_states_that_meet_between_others():
     # the row before that of the first state, as far on as the stride is
     at = [(1 << 20) + 64 * i for i in range(149)] + [(1 << 20) + 64 * 150 * 3 - 63]
     assert "overlap" in _refused(_reorder_many(at, at, row=64, stride=64 * 150))
+
+
+@pytest.mark.parametrize("off", [0, 60, 128, 3 * 128 + 60, -12])
+@pytest.mark.parametrize("state", [0, 70])
+def test_beam_reorder_parents_in_a_state(off, state):
+    """Blocks read the parents while others write: they are in no row that is written (4 of them, 16 bytes)."""
+    at = [(1 << 20) + 4096 * i for i in range(80)]
+    d = (C.c_void_p * 80)(*at)
+    assert "parents" in _refused(load().atlas_beam_reorder(d, d, 80, 64, 128, at[state] + off, 1, 4))
