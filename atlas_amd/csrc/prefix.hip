@@ -629,6 +629,17 @@ int prefix_attention_launch(const atlas_slot_cache& c, const atlas_prefix_batch&
                       ld_out % 4 == 0 && ld_q >= wide && ld_out >= wide,
                   "%s: the cache and rows start on 16 bytes, rows at least %ld elements apart (strides %ld and %ld)", who, wide,
                   ld_q, ld_out);
+    // a block writes its rows while others read
+    const ByteRows to(out, b.n_rows, wide * 4, ld_out * 4);
+    const long cells = (long)c.n_slots * c.max_seq * c.n_kv * c.head_dim * 4, ints = sizeof(int);
+    ATLAS_REQUIRE((out == q && (ld_out == ld_q || b.n_rows == 1)) || rows_apart(to, ByteRows(q, b.n_rows, wide * 4, ld_q * 4)),
+                  "%s: out overlaps q", who);
+    ATLAS_REQUIRE(rows_apart(ByteRows(c.k, cells), to) && rows_apart(ByteRows(c.v, cells), to), "%s: out overlaps the cache", who);
+    ATLAS_REQUIRE((!b.group_starts || rows_apart(ByteRows(b.group_starts, (b.n_groups + 1) * ints), to)) &&
+                      rows_apart(ByteRows(b.prefix_slots, b.n_groups * ints), to) &&
+                      rows_apart(ByteRows(b.prefix_lens, b.n_groups * ints), to) && rows_apart(ByteRows(b.kv_lens, b.n_rows * ints), to) &&
+                      rows_apart(ByteRows(b.slots, (long)b.n_rows * std::max(b.slot_stride, 1) * ints), to),
+                  "%s: out overlaps the batch", who);
     const PfShape s = pf_shape(c, b, n_heads, window);
     const long units = (long)s.tiles * c.n_kv;
     const long blocks = ((long)c.n_kv * s.splits + 7) / 8 * 8 * s.tiles;

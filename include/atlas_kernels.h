@@ -409,7 +409,8 @@ typedef struct {
  * token of infinities or NaN is nothing to the rows that do not see it.  (A score times
  * 1.45 scale has to be below 2^127 in magnitude, and 2^8 times an element of V, summed over
  * the tokens that a row sees, likewise: weights are kept up to 2^8 before they are divided
- * by their sum.)  out may be q, with ld_out = ld_q, and overlaps nothing else.  */
+ * by their sum.)  out may be q, with ld_out = ld_q; its rows may lie between q's, and overlap nothing
+ * else of what is read.                                                      */
 int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix_batch* batch,
                                const float* q, int64_t ld_q, int n_heads, float scale, int window,
                                float* out, int64_t ld_out);

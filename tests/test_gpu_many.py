@@ -223,6 +223,22 @@ def test_prefix_attention_strides_one_group_and_in_place():
     b.upload(one_group=True).check(out=b.d["q"])
 
 
+@pytest.mark.parametrize("one_row", [False, True])
+def test_prefix_attention_rows_of_q_and_out_between_each_other(one_row):
+    # both are columns of one matrix, with something behind them; a single row may be written in place at any stride
+    rows, wide = 1 if one_row else 6, 4 * 64
+    b = Batch(20, [rows], [45], [3, 8, 8, 0, 1, 30][:rows], pad_q=wide + 12)
+    b.q[:, wide:] = 7
+    b.upload()
+    at = 0 if one_row else 4 * wide
+    check(lib().atlas_prefix_attention_f32(C.byref(b.c), C.byref(b.b), b.d["q"].ptr, b.q.shape[1], 4, b.hd ** -0.5, 0, b.d["q"].ptr + at,
+                                           wide if one_row else b.q.shape[1]))
+    got, (want, off) = b.d["q"].get(), b.want()
+    _near(got[:, at // 4:at // 4 + wide].reshape(want.shape), want, off[..., None])
+    assert (got[:, 2 * wide:] == 7).all() and (got[:, wide:2 * wide] == 7).all() == one_row
+    assert one_row or (got[:, :wide] == b.q[:, :wide]).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
 def test_prefix_attention_scales(scale):
     Batch(11, [5], [100], [9, 2, 0, 1, 40], hd=64).upload().check(scale=scale)

@@ -190,3 +190,26 @@ def test_beam_reorder_parents_in_a_state(off, state):
     at = [(1 << 20) + 4096 * i for i in range(80)]
     d = (C.c_void_p * 80)(*at)
     assert "parents" in _refused(load().atlas_beam_reorder(d, d, 80, 64, 128, at[state] + off, 1, 4))
+
+
+# K and V of 4 x 64 tokens of 2 heads of 64 (128 KB each), a batch of 4 rows in 2 groups, a table of 8 slots for each, rows of
+# 4 heads of 64 (1 KB)
+K, V, Q, OUT, TABLE = (i << 24 for i in range(1, 6))
+FAR = dict(cache=dict(k=K, v=V), q=Q, out=OUT,
+           batch=dict(group_starts=TABLE, prefix_slots=TABLE + 64, prefix_lens=TABLE + 128, kv_lens=TABLE + 192, slots=TABLE + 256))
+
+
+@pytest.mark.parametrize("kw", [
+    # a part of q's rows, from before and behind, and q with rows further apart or closer than its own
+    dict(out=Q + 16), dict(out=Q - 16), dict(out=Q + 4 * 1024 - 16), dict(out=Q - 4 * 1024 + 16), dict(out=Q, ld_out=260),
+    dict(out=Q, ld_q=260), dict(out=Q + 1024, ld_q=512, ld_out=260), dict(out=Q + 1008, ld_q=512, ld_out=512),
+    dict(out=Q - 2048 + 16, ld_q=512, ld_out=512), dict(out=Q + 3 * 2048 - 16, ld_q=512, ld_out=256),
+    # K, V and what describes the batch
+    dict(out=K), dict(out=K - 4096 + 16), dict(out=K + (1 << 17) - 16), dict(out=V), dict(out=V + (1 << 17) - 16), dict(out=V - 16),
+    dict(out=TABLE - 4096 + 16), dict(out=TABLE + 64 + 16 - 1024), dict(out=TABLE + 256 + 112), dict(out=TABLE + 192, ld_out=1024),
+    dict(out=TABLE + 112, batch=dict(group_starts=0, n_groups=1))],
+    ids=str)
+def test_prefix_attention_out_apart_from_what_is_read(kw):
+    args = {**FAR, **kw}
+    args["batch"] = {**FAR["batch"], **kw.get("batch", {})}
+    assert "overlaps" in _refused(_attention(**args))
