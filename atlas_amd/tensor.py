@@ -637,15 +637,30 @@ class GpuSlotCache:
     def __init__(self, keys: GpuVec, values: GpuVec, n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int):
         self.keys, self.values = keys, values
         self.n_slots, self.max_seq, self.n_kv_heads, self.head_dim = n_slots, max_seq, n_kv_heads, head_dim
-        self.c = SlotCacheC(keys.gpu_ptr(), values.gpu_ptr(), n_slots, max_seq, n_kv_heads, head_dim)
+        self.c                         # (refuses what does not fit)
+
+    @staticmethod
+    def _total(n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int) -> int:
+        if min(n_slots, max_seq, n_kv_heads, head_dim) < 0:
+            raise AtlasError(-1, f"GpuSlotCache: {n_slots} slots of {max_seq} tokens, {n_kv_heads} heads of {head_dim}")
+        return n_slots * max_seq * n_kv_heads * head_dim
+
+    @property
+    def c(self) -> SlotCacheC:
+        """The cache as its vectors are now: an op may have given them other buffers."""
+        shape = self.n_slots, self.max_seq, self.n_kv_heads, self.head_dim
+        total = self._total(*shape)
+        for x in (self.keys, self.values):
+            x._need()
+            if min(x.len, x.buf.len) < total:
+                raise AtlasError(-1, f"GpuSlotCache: {min(x.len, x.buf.len)} elements, {total} expected")
+        return SlotCacheC(self.keys.buf.ptr, self.values.buf.ptr, *shape)
 
     @staticmethod
     def new(n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int) -> Optional["GpuSlotCache"]:
-        if min(n_slots, max_seq, n_kv_heads, head_dim) < 0:
-            raise AtlasError(-1, f"GpuSlotCache: {n_slots} slots of {max_seq} tokens, {n_kv_heads} heads of {head_dim}")
+        total = GpuSlotCache._total(n_slots, max_seq, n_kv_heads, head_dim)
         if not cuda_available():
             return None
-        total = n_slots * max_seq * n_kv_heads * head_dim
         keys, values = GpuVec.zeros(total), GpuVec.zeros(total)
         if keys.buf is None or values.buf is None:
             return None
@@ -657,19 +672,20 @@ class GpuSlotCache:
         n = new_k.len // max(wide, 1)
         if new_k.len != n * wide or new_v.len != new_k.len or not 0 <= slot < self.n_slots or not 0 <= pos <= self.max_seq - n:
             raise AtlasError(-1, f"GpuSlotCache.write: {new_k.len} and {new_v.len} elements at slot {slot}, position {pos}")
-        self.keys._need(self.values, new_k, new_v)
-        for cache, new in ((self.keys, new_k), (self.values, new_v)):
-            check(load().atlas_memcpy_d2d(cache.buf.ptr + 4 * wide * (slot * self.max_seq + pos), new.buf.ptr, 4 * new.len))
+        new_k._need(new_v)
+        c = self.c
+        for at, new in ((c.k, new_k), (c.v, new_v)):
+            check(load().atlas_memcpy_d2d(at + 4 * wide * (slot * self.max_seq + pos), new.buf.ptr, 4 * new.len))
 
     def attention(self, batch: PrefixBatch, q: GpuVec, n_heads: int, scale: float, window_size: int = 0) -> GpuVec:
         """Attention of the batch's query rows [n_rows x n_heads x head_dim]."""
-        wide = n_heads * self.head_dim
+        c, wide = self.c, n_heads * self.head_dim
         if q.buf is None or q.len < batch.n_rows * wide:
             raise AtlasError(-1, f"GpuSlotCache: {batch.n_rows} rows of {wide} elements expected on the GPU")
         out = GpuBuf.alloc(batch.n_rows * wide)
         if out is None:
             raise AtlasError(-3, f"GpuSlotCache: no device memory for {batch.n_rows} rows of {wide} elements")
-        check(load().atlas_prefix_attention_f32(C.byref(self.c), C.byref(batch.c), q.buf.ptr, wide, n_heads, scale,
+        check(load().atlas_prefix_attention_f32(C.byref(c), C.byref(batch.c), q.buf.ptr, wide, n_heads, scale,
                                                 window_size, out.ptr, wide))
         return GpuVec(out, np.zeros(out.len, np.float32), out.len)
 
@@ -681,9 +697,8 @@ class GpuSlotCache:
         wide = 4 * self.n_kv_heads * self.head_dim
         if p.ndim != 2 or p.size > self.n_slots or not 0 <= begin <= end <= self.max_seq:
             raise AtlasError(-1, f"GpuSlotCache.reorder: parents of shape {p.shape}, positions {begin} to {end}")
-        self.keys._need(self.values)
-        _reorder([self.keys.buf.ptr + wide * begin, self.values.buf.ptr + wide * begin], wide * (end - begin),
-                 wide * self.max_seq, p)
+        c = self.c
+        _reorder([c.k + wide * begin, c.v + wide * begin], wide * (end - begin), wide * self.max_seq, p)
 
 
 def _reorder(ptrs, row_bytes: int, stride: int, parents: np.ndarray) -> None:

@@ -761,6 +761,26 @@ def test_slot_cache_steps_of_a_beam_search():
     assert len({tuple(b) for b in beams}) == width
 
 
+def test_slot_cache_after_an_op_on_its_vectors():
+    # add_inplace gives keys and values buffers of their own: attention, write and reorder use those
+    rng = np.random.default_rng(3)
+    k, v, dk, dv = (rng.standard_normal((3, 16, 2, 64)).astype(np.float32) for _ in range(4))
+    cache = T.GpuSlotCache(T.GpuVec.from_slice(k), T.GpuVec.from_slice(v), 3, 16, 2, 64)
+    cache.keys.add_inplace(T.GpuVec.from_slice(dk))
+    cache.values.add_inplace(T.GpuVec.from_slice(dv))
+    k, v = k + dk, v + dv
+    new = rng.standard_normal((2, 2, 64)).astype(np.float32)
+    cache.write(1, 9, T.GpuVec.from_slice(new[0]), T.GpuVec.from_slice(new[1]))
+    k[1, 9], v[1, 9] = new
+    cache.reorder([0, 1, 1], 9, 10)
+    k[2, 9], v[2, 9] = k[1, 9], v[1, 9]
+    q = rng.standard_normal((2, 4, 64)).astype(np.float32)
+    lens, slots = [10, 10], np.array([1, 2])
+    got = cache.attention(T.PrefixBatch(lens, [0], [9], slots), T.GpuVec.from_slice(q), 4, 0.125).download().reshape(q.shape)
+    want, off = many_ref.attention(k, v, q, lens, [0, 2], [0], [9], slots, 0.125)
+    _near(got, want, off[..., None])
+
+
 def test_sgemm_rows_with_adapters():
     rng = np.random.default_rng(2)
     m, k, rows = 192, 256, 7

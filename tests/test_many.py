@@ -213,3 +213,63 @@ def test_prefix_attention_out_apart_from_what_is_read(kw):
     args = {**FAR, **kw}
     args["batch"] = {**FAR["batch"], **kw.get("batch", {})}
     assert "overlaps" in _refused(_attention(**args))
+
+
+class _Mem:
+    """An allocation that nothing follows."""
+
+    def __init__(self, ptr):
+        self.ptr = ptr
+
+    free = staticmethod(lambda: None)
+
+
+def _vec(n, ptr=X):
+    return T.GpuVec(T.GpuBuf(_Mem(ptr), n), np.zeros(0, np.float32), n)
+
+
+@pytest.mark.parametrize("keys,values", [(4, 4), (8191, 8192), (8192, 8191), (0, 8192)])
+def test_slot_cache_of_vectors_that_are_too_short(keys, values):
+    with pytest.raises(AtlasError) as e:
+        T.GpuSlotCache(_vec(keys), _vec(values), 2, 32, 2, 64)
+    assert e.value.code == -1
+    T.GpuSlotCache(_vec(8192), _vec(8193), 2, 32, 2, 64)
+
+
+def test_slot_cache_of_vectors_that_are_not_there():
+    off = T.GpuVec(None, np.zeros(8192, np.float32), 8192)
+    for args in ((off, _vec(8192), 2, 32, 2, 64), (_vec(8192), off, 2, 32, 2, 64), (_vec(8192), _vec(8192), -2, -32, 2, 64)):
+        with pytest.raises(AtlasError) as e:
+            T.GpuSlotCache(*args)
+        assert e.value.code == -1
+
+
+def test_slot_cache_follows_its_vectors(monkeypatch):
+    # an op that swaps a vector's buffer (add_inplace) leaves the cache with the new one, a shorter one is refused
+    cache, at = T.GpuSlotCache(_vec(8192, X), _vec(8192, 2 * X), 2, 32, 2, 64), []
+    batch = T.PrefixBatch.__new__(T.PrefixBatch)
+    batch.n_rows, batch.n_groups, batch.c = 1, 1, PrefixBatchC()
+
+    class Lib:
+        @staticmethod
+        def atlas_prefix_attention_f32(c, *_):
+            at.append((c._obj.k, c._obj.v))
+            return 0
+
+        @staticmethod
+        def atlas_memcpy_d2d(to, *_):
+            at.append(to)
+            return 0
+    monkeypatch.setattr(T, "load", lambda: Lib)
+    monkeypatch.setattr(T.GpuBuf, "alloc", staticmethod(lambda n: _vec(n).buf))
+    cache.attention(batch, _vec(256), 4, 1.0)
+    cache.keys.buf, cache.values = _vec(8192, 3 * X).buf, _vec(8192, 4 * X)
+    cache.attention(batch, _vec(256), 4, 1.0)
+    cache.write(0, 0, _vec(128), _vec(128))
+    assert at == [(X, 2 * X), (3 * X, 4 * X), 3 * X, 4 * X] and (cache.c.k, cache.c.v) == (3 * X, 4 * X)
+    cache.values = _vec(8191)
+    for call in (lambda: cache.attention(batch, _vec(256), 4, 1.0), lambda: cache.write(0, 0, _vec(128), _vec(128)),
+                 lambda: cache.reorder([0, 1])):
+        with pytest.raises(AtlasError) as e:
+            call()
+        assert e.value.code == -1
