@@ -286,13 +286,16 @@ class GpuMatrix:
         """Ragged micro-batch: x holds n activation rows [n x cols]; returns
         [n x rows] (extension, skinny MFMA GEMM).  With ``lora`` each row r gets the product
         of its adapter ``adapters[r]`` (-1: none) on top."""
+        if (lora is None) != (adapters is None):
+            raise AtlasError(-1, "sgemm_rows: lora and adapters go together")
         if lora is not None and (lora.rows, lora.cols) != (self.rows, self.cols):
             raise AtlasError(-1, f"sgemm_rows: adapters of {lora.rows}x{lora.cols} beside {self.rows}x{self.cols}")
         if lora is not None and np.size(adapters) != n:
             raise AtlasError(-1, f"sgemm_rows: {np.size(adapters)} adapters for {n} rows")
+        pick = None if lora is None else _ints("sgemm_rows", adapters)
         out = self._sgemm_rows(x, n)
         if lora is not None:
-            lora.add(out, x, adapters)
+            lora.add(out, x, pick)
         return out
 
     def _sgemm_rows(self, x: "GpuVec", n: int) -> "GpuVec":

@@ -273,3 +273,25 @@ def test_slot_cache_follows_its_vectors(monkeypatch):
         with pytest.raises(AtlasError) as e:
             call()
         assert e.value.code == -1
+
+
+def _lora_of(n, rank, rows, cols):
+    lora = T.GpuLora.__new__(T.GpuLora)
+    lora.n, lora.rank, lora.rows, lora.cols, lora.c = n, rank, rows, cols, LoraC()
+    return lora
+
+
+@pytest.mark.parametrize("n,kw", [
+    (1, dict(lora=True)), (3, dict(lora=True)), (1, dict(adapters=[0])), (3, dict(adapters=[0, 1, -1])), (1, dict(lora=True, adapters=[])),
+    (3, dict(lora=True, adapters=[0, 1])), (1, dict(lora=True, adapters=[1 << 31])), (1, dict(lora=True, adapters=[-(1 << 31) - 1]))], ids=str)
+def test_sgemm_rows_adapters_that_do_not_belong(monkeypatch, n, kw):
+    """Adapters without their matrices, or the other way round, are refused before the shared product runs."""
+    mat, ran = T.GpuMatrix(T.GpuBufKind.BF16, object(), 8, 16), []
+    monkeypatch.setattr(T.GpuMatrix, "_sgemm_rows", lambda *a: ran.append(a))
+    monkeypatch.setattr(T.GpuLora, "add", lambda *a: ran.append(a))
+    with pytest.raises(AtlasError) as e:
+        mat.sgemm_rows(_vec(16 * n), n, **{**kw, **(dict(lora=_lora_of(2, 4, 8, 16)) if "lora" in kw else {})})
+    assert e.value.code == -1 and not ran
+    mat.sgemm_rows(_vec(16 * n), n)
+    mat.sgemm_rows(_vec(16 * n), n, _lora_of(2, 4, 8, 16), [0] * n)
+    assert len(ran) == 3
