@@ -301,7 +301,7 @@ class GpuMatrix:
     def _sgemm_rows(self, x: "GpuVec", n: int) -> "GpuVec":
         if self.buf is None or x.buf is None:
             raise AtlasError(-1, "sgemm_rows: operands are not on the GPU")
-        if self.kind is GpuBufKind.MXFP4 and x.len < n * self.cols:
+        if x.len < n * self.cols:
             raise AtlasError(-1, f"sgemm_rows: {n} rows of {self.cols} elements expected")
         out = GpuBuf.alloc(self.rows * n)
         if out is None:

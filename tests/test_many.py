@@ -295,3 +295,14 @@ def test_sgemm_rows_adapters_that_do_not_belong(monkeypatch, n, kw):
     mat.sgemm_rows(_vec(16 * n), n)
     mat.sgemm_rows(_vec(16 * n), n, _lora_of(2, 4, 8, 16), [0] * n)
     assert len(ran) == 3
+
+
+@pytest.mark.parametrize("with_lora", [False, True])
+def test_sgemm_rows_of_a_vector_that_is_too_short(monkeypatch, with_lora):
+    """Nothing runs that would read past the rows there are."""
+    mat, ran = T.GpuMatrix(T.GpuBufKind.BF16, _vec(128).buf, 8, 16), []
+    monkeypatch.setattr(T.GpuBuf, "alloc", staticmethod(lambda n: ran.append(n) or _vec(n).buf))
+    monkeypatch.setattr(T, "load", lambda: ran.append("load"))
+    with pytest.raises(AtlasError) as e:
+        mat.sgemm_rows(_vec(47), 3, *((_lora_of(2, 4, 8, 16), [0, 1, 0]) if with_lora else ()))
+    assert e.value.code == -1 and not ran
