@@ -717,6 +717,7 @@ def beam_reorder_gpu(states, parents) -> None:
     p = np.atleast_2d(_ints("beam_reorder_gpu", parents))
     if p.ndim != 2 or p.size == 0:
         raise AtlasError(-1, f"beam_reorder_gpu: parents of shape {p.shape}")
+    states = list(states)
     for x in states:
         x._need()
         if x.len % p.size:

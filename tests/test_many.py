@@ -306,3 +306,11 @@ def test_sgemm_rows_of_a_vector_that_is_too_short(monkeypatch, with_lora):
     with pytest.raises(AtlasError) as e:
         mat.sgemm_rows(_vec(47), 3, *((_lora_of(2, 4, 8, 16), [0, 1, 0]) if with_lora else ()))
     assert e.value.code == -1 and not ran
+
+
+def test_beam_reorder_of_states_that_come_once(monkeypatch):
+    """States may be any iterable, also one that can be gone through once."""
+    done = []
+    monkeypatch.setattr(T, "_reorder", lambda ptrs, row, stride, p: done.append((ptrs, row)))
+    T.beam_reorder_gpu((_vec(n, X * n) for n in (6, 12, 6)), [1, 0])
+    assert done == [([6 * X, 6 * X], 12), ([12 * X], 24)]
