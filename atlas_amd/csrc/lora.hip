@@ -452,6 +452,11 @@ int lora_add_launch(const atlas_lora& l, const int* adapters, const float* x, lo
         return ld == ld_y && at >= l.m && at + w <= ld_y;
     };
     ATLAS_REQUIRE(apart(x, l.k, ld_x) && ((base == y && ld_base == ld_y) || apart(base, l.m, ld_base)), "%s: y overlaps x or base", who);
+    const ByteRows to(y, n, l.m * 4L, ld_y * 4);
+    const long each = (long)l.n_adapters * l.rank * size;
+    ATLAS_REQUIRE(rows_apart(ByteRows(adapters, n * 4L), to) && (!l.scales || rows_apart(ByteRows(l.scales, l.n_adapters * 4L), to)) &&
+                      rows_apart(ByteRows(l.a, each * l.k), to) && rows_apart(ByteRows(l.b, each * l.m), to),
+                  "%s: y overlaps adapters", who);
     LoraArgs a{};
     a.a = l.a; a.b = l.b; a.scales = l.scales;
     a.n_adapters = l.n_adapters; a.rank = l.rank; a.m = l.m; a.k = l.k;

@@ -452,7 +452,8 @@ typedef struct {
 /* y_r = base_r + scales[p] b_p (a_p x_r), p = adapters[r], for n rows (up to 2^20) of x (k
  * elements, ld_x apart), base and y (m elements); a row whose p is no adapter is its
  * base.  base is the shared projection's product and may be y (with ld_y = ld_base), but neither it
- * nor x must overlap y otherwise; rows of one may lie between another's, if they are as far apart.  f32 sums of exact products.                          */
+ * nor x must overlap y otherwise (rows of one may lie between another's, if they are as far apart),
+ * nor do adapters and what lora points to.  f32 sums of exact products.      */
 int atlas_lora_add_f32(const atlas_lora* lora, const int* adapters, const float* x, int64_t ld_x,
                        const float* base, int64_t ld_base, float* y, int64_t ld_y, int n);
 

@@ -314,3 +314,12 @@ def test_beam_reorder_of_states_that_come_once(monkeypatch):
     monkeypatch.setattr(T, "_reorder", lambda ptrs, row, stride, p: done.append((ptrs, row)))
     T.beam_reorder_gpu((_vec(n, X * n) for n in (6, 12, 6)), [1, 0])
     assert done == [([6 * X, 6 * X], 12), ([12 * X], 24)]
+
+
+@pytest.mark.parametrize("kw", [
+    # y: 4 rows of 256 bytes.  16 bytes of adapters, 12 of scales, A 3 x 8 x 32 and B 3 x 64 x 8 bf16
+    dict(adapters=Y), dict(adapters=Y + 1020), dict(adapters=Y - 12), dict(lora=dict(scales=Y + 1020)), dict(lora=dict(scales=Y - 8)),
+    dict(lora=dict(a=Y + 1022)), dict(lora=dict(a=Y - 1534)), dict(lora=dict(b=Y + 512)), dict(lora=dict(b=Y - 3070)),
+    dict(lora=dict(fmt=0, b=Y - 6140)), dict(adapters=Y + 1524, ld_y=128, ld_base=128)], ids=str)
+def test_lora_result_apart_from_adapters(kw):
+    assert "overlaps" in _refused(_lora(**{**dict(x=1 << 22, base=1 << 23, adapters=1 << 24), **kw}))
