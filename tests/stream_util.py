@@ -7,6 +7,7 @@ from atlas_amd._lib import check, load
 
 def hip_runtime():
     """The HIP runtime that the library uses (the copy loaded in this process)."""
+    load()
     with open("/proc/self/maps") as f:
         path = next(line.split()[-1] for line in f if "libamdhip64.so" in line)
     hip = C.CDLL(path)
