@@ -171,7 +171,7 @@ def run_infer(args: argparse.Namespace,
     out(f"\n  Generating {args.max_tokens} tokens (temperature={args.temperature}) ...")
     t0 = time.perf_counter()
     if args.beams > 1:
-        hyps = m.generate_beam(prompt, args.max_tokens, args.beams)
+        hyps = m.generate_beam(prompt, args.max_tokens, args.beams) if args.max_tokens else []
         new = hyps[0][0] if hyps else []
     else:
         new = m.generate(prompt, args.max_tokens, args.temperature)

@@ -323,3 +323,21 @@ def test_beam_reorder_of_states_that_come_once(monkeypatch):
     dict(lora=dict(fmt=0, b=Y - 6140)), dict(adapters=Y + 1524, ld_y=128, ld_base=128)], ids=str)
 def test_lora_result_apart_from_adapters(kw):
     assert "overlaps" in _refused(_lora(**{**dict(x=1 << 22, base=1 << 23, adapters=1 << 24), **kw}))
+
+
+@pytest.mark.parametrize("beams", ["1", "3"])
+def test_infer_without_tokens(monkeypatch, tmp_path, beams):
+    """--max-tokens 0 prints the prompt's logits, with beams too: a search of no tokens is nothing to ask the model for."""
+    from atlas_amd import cli
+
+    class Model:
+        weight_bytes = reset = close = prefill = staticmethod(lambda *_: 0)
+        forward_one = staticmethod(lambda t: np.arange(50, dtype=np.float32))
+        generate = staticmethod(lambda prompt, n, temperature: [])
+
+        @staticmethod
+        def generate_beam(prompt, n, width):
+            raise AtlasError(-1, "generate_beam: 0 new tokens")
+    monkeypatch.setattr(cli.loader, "load_model_from_dir", lambda *a, **kw: Model())
+    args = cli.parse_args(["--weights", str(tmp_path), "--model", "olmo3-1b", "--max-tokens", "0", "--beams", beams])
+    assert cli.run_infer(args, out=lambda x: None)["tokens"] == []
