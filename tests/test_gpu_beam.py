@@ -142,6 +142,25 @@ def test_beam_search_without_memory():
     assert m.generate_beam(prompt, 6, 4) == want
 
 
+def test_beam_search_refuses_what_it_has_no_memory_for():
+    """A first search allocates a block on the host and four on the device, in turn.  Each fails once, and the search with it:
+    the first at once, each other after the one before it; then there is nothing left to allocate."""
+    W, prompt = _weights("olmo", 2), _prompt(2, 9)
+    want = _model(W, 4).generate_beam(prompt, 6, 4)
+    m, codes, got = _model(W, 4), [], None
+    for skip in [0] + [1] * 20:
+        check(load().atlas_debug_fail_allocations(skip, 1))
+        try:
+            got = m.generate_beam(prompt, 6, 4)
+            break
+        except AtlasError as e:
+            codes.append(e.code)
+        finally:
+            check(load().atlas_debug_fail_allocations(0, 0))
+    assert len(codes) >= 5 and set(codes) == {-3} and got == want
+    assert m.generate_beam(prompt, 6, 4) == want
+
+
 def test_infer_command_with_beams(tmp_path):
     from atlas_amd import cli
     from tests import ckptgen

@@ -280,6 +280,30 @@ def test_prefix_attention_far_slots():
             assert np.abs(got[r, h] - (p / p.sum()) @ vv).max() <= off
 
 
+def test_prefix_attention_far_slots_of_rows_that_differ():
+    # cells past 4 GB, rows whose windows begin in the prefix and behind it, one of them a token before the others'
+    n_kv, hd, max_seq, n_slots, first = 8, 128, 32768, 34, 32763
+    total = n_slots * max_seq * n_kv * hd
+    mem = [T._DevMem(4 * total, sync_alloc=True) for _ in range(2)]
+    rng = np.random.default_rng(23)
+    host = rng.standard_normal((2, n_slots, max_seq - first, n_kv, hd)).astype(np.float32)
+    for s in range(n_slots):
+        for x, m in enumerate(mem):
+            row = np.ascontiguousarray(host[x, s])
+            check(lib().atlas_memcpy_h2d(m.ptr + 4 * n_kv * hd * (s * max_seq + first), row.ctypes.data_as(C.c_void_p), row.nbytes))
+    heads, window = 8, 4
+    lens, slots = np.array([32768, 32768, 32767, 32768], np.int32), np.array([33, 31, 2, 0], np.int32)
+    q = rng.standard_normal((4, heads, hd)).astype(np.float32)
+    d = [Dev(x) for x in (np.array([32], np.int32), np.array([32766], np.int32), lens, slots)]
+    dq, out = Dev(q), Dev(np.full((4, heads * hd), 7, np.float32))
+    c = SlotCacheC(mem[0].ptr, mem[1].ptr, n_slots, max_seq, n_kv, hd)
+    b = PrefixBatchC(None, d[0].ptr, d[1].ptr, d[2].ptr, d[3].ptr, 0, 1, 4, 0, 0)
+    check(lib().atlas_prefix_attention_f32(C.byref(c), C.byref(b), dq.ptr, heads * hd, heads, 0.09, window, out.ptr, heads * hd))
+    # (the cells from `first` on, as a cache of their own)
+    want, off = many_ref.attention(host[0], host[1], q, lens - first, [0, 4], [32], [32766 - first], slots, 0.09, window)
+    _near(out.get().reshape(want.shape), want, off[..., None])
+
+
 def test_prefix_attention_captured():
     # a captured call follows the batch's contents; eager calls between the replays
     def work(hip):
@@ -669,6 +693,46 @@ def test_scratch_refused_in_a_capture_or_short_of_memory_then_there():
         assert out[0].get().tolist() == [9, 9] and out[1].get().tolist() == [0, 1]
         want, off = b.want()
         _near(to.get().reshape(want.shape), want, off[..., None])
+    on_thread(work)
+
+
+def test_one_graph_of_all_kinds_of_calls_writes_its_results():
+    """Replays over results that were cleared and inputs that were changed: adapters, selection and attention."""
+    def work(hip):
+        a = Adapters(21, 3, 16, 64, 2000, 9)
+        d = [Dev(v) for v in (*a.raw, a.x, a.base, a.pick, a.scales)]
+        c = LoraC(1, d[0].ptr, d[1].ptr, d[5].ptr, 3, 16, 64, 2000)
+        b = Batch(22, [4], [3000], [30] * 4, hd=128, junk=False).upload()
+        z, s = Dev(np.zeros((2, 500), np.float32)), Dev(np.zeros(2))
+        shapes = ((9, 64), np.float32), (2, np.uint32), (2, np.int32), (2, np.float64), (b.q.shape, np.float32)
+        y, tokens, parents, best, out = outs = [Dev(np.full(n, 77, t)) for n, t in shapes]
+
+        def put(dev, x):
+            x = np.ascontiguousarray(x)
+            check(lib().atlas_memcpy_h2d(dev.ptr, x.ctypes.data_as(C.c_void_p), x.nbytes))
+
+        def calls():
+            check(lib().atlas_lora_add_f32(C.byref(c), d[4].ptr, d[2].ptr, 2000, d[3].ptr, 64, y.ptr, 64, 9))
+            check(lib().atlas_beam_select_f32(z.ptr, 500, 500, s.ptr, 1, 2, 2, tokens.ptr, parents.ptr, best.ptr))
+            b.call(out)
+        with Stream(hip) as st:
+            calls()
+            exe, _ = st.capture(calls)
+            for turn in range(4):
+                a.x, b.q = (b.rng.standard_normal(v.shape).astype(np.float32) for v in (a.x, b.q))
+                logits, scores = b.rng.standard_normal((1, 2, 500)).astype(np.float32), -b.rng.random((1, 2))
+                for dev, v in ((d[2], a.x), (b.d["q"], b.q), (z, logits), (s, scores), *((o, o.a) for o in outs)):
+                    put(dev, v)
+                st.launch(exe)
+                st.sync()
+                _near(y.get(), *many_ref.lora(a.base, a.x, a.a, a.b, a.scales, a.pick))
+                want = many_ref.select(logits, scores, 2)
+                assert (tokens.get() == want[0][0]).all() and (parents.get() == want[1][0]).all()
+                assert np.abs(best.get() - want[2][0]).max() <= 1e-12 * (1 + np.abs(want[2]).max())
+                want, off = b.want()
+                _near(out.get().reshape(want.shape), want, off[..., None])
+                calls()
+                st.sync()
     on_thread(work)
 
 
