@@ -473,10 +473,11 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
     ATLAS_REQUIRE((((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)parents) & 3) == 0 &&
                       (((uintptr_t)scores | (uintptr_t)out_scores) & 7) == 0, "%s: misaligned argument", who);
     // a group's results are written while others' scores are read
-    const ByteRows given(scores, (long)n_groups * width * 8);
     const long n_best = (long)n_groups * n_out;
-    ATLAS_REQUIRE(rows_apart(given, ByteRows(out_scores, n_best * 8)) && rows_apart(given, ByteRows(tokens, n_best * 4)) &&
-                      rows_apart(given, ByteRows(parents, n_best * 4)), "%s: a result overlaps scores", who);
+    const ByteRows given(scores, (long)n_groups * width * 8), best(out_scores, n_best * 8), toks(tokens, n_best * 4),
+        beams(parents, n_best * 4);
+    ATLAS_REQUIRE(rows_apart(given, best) && rows_apart(given, toks) && rows_apart(given, beams), "%s: a result overlaps scores", who);
+    ATLAS_REQUIRE(rows_apart(toks, beams) && rows_apart(toks, best) && rows_apart(beams, best), "%s: results overlap each other", who);
     const size_t bytes = beam_select_workspace(vocab, n_groups, width, n_out);
     void* p = ws.p;
     if (p) {

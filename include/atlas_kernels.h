@@ -420,9 +420,10 @@ int atlas_prefix_attention_f32(const atlas_slot_cache* cache, const atlas_prefix
  * 64 bits, the n_out largest of each group in descending order (equal scores: the lower beam,
  * then the larger logit, then the lower token).  logits [n_groups * width] rows of
  * vocab, ld apart; scores [n_groups * width]; tokens, parents (the beam within its
- * group) and out_scores [n_groups][n_out], none of which overlaps the scores.  A beam whose score is not finite, a row
- * of logits with NaN or +inf or of -inf only, and a logit of -inf give no candidates;
- * where a group has too few, the rest is token 0 of parent -1 and score -inf.
+ * group) and out_scores [n_groups][n_out], which overlap neither the scores nor each
+ * other.  A beam whose score is not finite, a row of logits with NaN or +inf or of -inf
+ * only, and a logit of -inf give no candidates; where a group has too few, the rest is
+ * token 0 of parent -1 and score -inf.
  * width and n_out 1 to 64, n_groups * width up to 65535, vocab up to 2^30.    */
 int atlas_beam_select_f32(const float* logits, int64_t ld, int vocab, const double* scores,
                           int n_groups, int width, int n_out, uint32_t* tokens, int* parents,

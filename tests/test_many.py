@@ -341,3 +341,8 @@ def test_infer_without_tokens(monkeypatch, tmp_path, beams):
     monkeypatch.setattr(cli.loader, "load_model_from_dir", lambda *a, **kw: Model())
     args = cli.parse_args(["--weights", str(tmp_path), "--model", "olmo3-1b", "--max-tokens", "0", "--beams", beams])
     assert cli.run_infer(args, out=lambda x: None)["tokens"] == []
+
+
+@pytest.mark.parametrize("kw", [dict(parents=2 * X), dict(parents=2 * X + 60), dict(out=2 * X - 120), dict(out=3 * X + 56)], ids=str)
+def test_beam_select_results_apart_from_each_other(kw):
+    assert "each other" in _refused(_select(**{**dict(logits=1 << 21, scores=X, tokens=2 * X, parents=3 * X), **kw}))
