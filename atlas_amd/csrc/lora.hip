@@ -225,7 +225,9 @@ struct LoraTile {
 
 // Elements of an adapter's A up to which every block forms A x itself, which saves a launch
 // (rank 16, 13 rows of 1024 x 1024: 7.4 us, 8.9 in two; 2048 x 2048: 9.8 and 8.9; 4096 x
-// 4096: 14.5 and 9.2).
+// 4096: 14.5 and 9.2; 70 rows of 4096 x 1024 9.7 and 10.6).  Blocks of one tile form it anew
+// each, and count its rows, which many rows make longer than a launch: 500 rows of 1024 x 1024
+// 11.3 and 12.0, but of 4096 x 1024 16.1 and 14.6, 2000 rows 45 and 32.
 constexpr long kLoraWhole = 16384;
 constexpr int kLoraUp = 4;             // blocks of a CU (2047 rows: 65 us, 71 with a block to each 256 of m)
 constexpr int kLoraMaxTiles = 16;      // tiles of rank
@@ -398,7 +400,7 @@ __global__ __launch_bounds__(kLoraWaves * 64) void lora_up_kernel(LoraArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(this_w[mt][e], v[e], acc[mt], 0, 0, 0);
             }
-            load(m0 + gridDim.x * WIDE); 
+            load(m0 + gridDim.x * WIDE);
             // from columns to rows, in the wave's own part of LDS
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<f32x4*>(&turn[wave][i][16 * mt + 4 * g]) = scale * acc[mt];

@@ -19,8 +19,11 @@
 // over 4001 shared tokens and up to 97 of each 32 us, 135 MB, 26 at a copy's rate; and
 // by the f32 products where groups are wide (64 requests of 32 heads over 8 of 128, 8191 tokens
 // and up to 1023 of each: 69 of 124 us; shared tokens alone go at 114 TFLOP/s of 155), with
-// masks and exponentials between them that a SIMD's two waves do not quite cover.  The smallest, 4 beams of 9 heads over 3 of 64, are a launch and the chain of
-// its loads: 4.9 us.
+// masks and exponentials between them that a SIMD's two waves do not quite cover.  Heads
+// of 256 leave a wave to a SIMD: 8 rows of 16 heads over 8, 4001 shared tokens and up to 97
+// of each, 27 to 29 us, 68 MB, 13 at a copy's rate; the first shape with a window of 1024
+// tokens 17 us, 35 MB, 7 at that rate.  The smallest, 4 beams of 9 heads over 3 of 64, are a
+// launch and the chain of its loads: 4.9 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -45,7 +48,9 @@ struct PfUnit {
 
 // Waves of a block, and blocks of a CU by their registers.  (Head dimension 128, 8 beams of 32
 // heads and 64 requests of 32 over 8: four waves 33.3 and 152 us, eight 32.4 and 124, twelve 35.7
-// and, with what does not fit the registers in memory, 151.)
+// and, with what does not fit the registers in memory, 151.  256, four waves of 314
+// registers and eight of 250: 4 rows over 300 tokens 15.2 and 16.1, 8 over 4001 28.7 and 35.1, 40
+// of five groups 35.0 and 39.4; 64 rows of 32 heads over 8 149 and 144.)
 constexpr int pf_waves(int hd) { return hd == 256 ? 4 : 8; }
 constexpr int pf_at_once(int hd, int ct) { return hd * ct <= 64 ? 2 : 1; }
 

@@ -403,8 +403,9 @@ typedef struct {
  * apart) over its tokens, the last `window` of them (0: all), scores times scale, in
  * f32.  A group's shared tokens are read once for 16 columns, a row and one of a KV
  * head's heads each (32 where a group has more than 64 on average, its prefix may be
- * longer than 2048 tokens and head_dim is 128).  n_heads / n_kv in 1 .. 16; n_slots * max_seq below 2^31; n_kv in whole eights times
- * the tiles of columns (n_groups, and one to each full tile of rows) below 2^23.  A row
+ * longer than 2048 tokens and head_dim is 128).  n_heads / n_kv in 1 .. 16; n_slots *
+ * max_seq below 2^31; n_kv in whole eights times the tiles of columns (n_groups, and one
+ * to each full tile of rows) below 2^23.  A row
  * without tokens, or whose scores are all -inf, gives zeros, whatever its q.  A
  * token of infinities or NaN is nothing to the rows that do not see it.  (A score times
  * 1.45 scale has to be below 2^127 in magnitude, and 2^8 times an element of V, summed over
