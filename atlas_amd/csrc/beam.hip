@@ -507,7 +507,7 @@ int beam_select_launch(const float* logits, long ld, int vocab, const double* sc
 //
 // A thread has columns of a group's rows: it reads what any of them takes over and then
 // writes, so that a state is reordered in place.  Bound by the bytes: 60 caches of 6 beams
-// of 777 x 3 x 64 f32 42 to 45 us, 215 MB, 42 at a copy's rate; as many bytes of 12 beams 45,
+// of 777 x 3 x 64 f32 40 to 45 us, 215 MB, 42 at a copy's rate; as many bytes of 12 beams 45,
 // of 32 and 64, whose rows leave a wave to a SIMD, 54.  A launch has up to 64 states and a
 // thread up to four columns, W rows of each in registers, so that all its loads are under way
 // at once (a column to a thread, and fewer states to a launch: 85 us).
